@@ -140,8 +140,8 @@ def prepare(case, seed):
     if c["kind"] == "pages":
         shape = (c["layers"], c["pages"], c["kv"], c["page"], c["dim"])
         s["k"], s["v"] = _rows(g, shape, cache, True), _rows(g, shape, cache, False)
-        p = np.random.RandomState(seed % (1 << 31)).permutation(c["pages"])
-        s["src"], s["dst"] = [int(x) for x in p[: c["moved"]]], [int(x) for x in p[c["moved"]: 2 * c["moved"]]]
+        p = np.random.RandomState(seed % (1 << 31)).permutation(c["pages"]).astype(np.int32)
+        s["src"], s["dst"] = p[: c["moved"]].copy(), p[c["moved"]: 2 * c["moved"]].copy()
         return s
     total, fresh = _lengths(c, seed)
     page = c["page"]
@@ -231,7 +231,7 @@ def _kv(s):
 
 def _workspace(s, nbytes):
     if "ws" not in s:
-        s["ws"] = torch.empty(max(nbytes, 16), dtype=torch.uint8, device="cuda")
+        s["ws"] = torch.empty(max(nbytes(), 16), dtype=torch.uint8, device="cuda")
     return s["ws"].data_ptr(), s["ws"].numel()
 
 
@@ -247,10 +247,10 @@ def _own_run(s):
         return [s["k"], s["v"]]
     t, scale = TYPES[c["q"]][1], c["dim"] ** -0.5
     if c["kind"] == "decode":
-        ws = _workspace(s, L.attn_decode_workspace(kv, c["seqs"], c["heads"]))
+        ws = _workspace(s, lambda: L.attn_decode_workspace(kv, c["seqs"], c["heads"]))
         L.attn_decode_dev(kv, c["seqs"], c["heads"], t, s["q"].data_ptr(), 0, scale, c["window"], s["out"].data_ptr(), 0, *ws)
     else:
-        ws = _workspace(s, L.attn_prompt_workspace(kv, c["seqs"], ntok, c["heads"], t))
+        ws = _workspace(s, lambda: L.attn_prompt_workspace(kv, c["seqs"], ntok, c["heads"], t))
         L.attn_prompt_dev(kv, c["seqs"], s["start"].data_ptr(), ntok, c["heads"], t, s["q"].data_ptr(), 0, scale, c["window"],
                           s["out"].data_ptr(), 0, *ws)
     return s["out"]
@@ -287,7 +287,7 @@ def exact(case, seed):
         got = []
         for x in (s["k"], s["v"]):
             y = x.double()
-            for a, b in zip(s["src"], s["dst"]):
+            for a, b in zip(s["src"].tolist(), s["dst"].tolist()):
                 y[:, b] = x[:, a].double()
             got.append(y)
         return got
