@@ -43,6 +43,8 @@ enum {
     ES_HIP_Q4_0 = 2, ES_HIP_Q5_0 = 6, ES_HIP_Q8_0 = 8, ES_HIP_Q2_K = 10, ES_HIP_Q3_K = 11, ES_HIP_Q4_K = 12, ES_HIP_Q5_K = 13,
     ES_HIP_Q6_K = 14
 };
+/* GGML type ids of the unquantized types that the key-value cache and its attention take (not weight formats) */
+enum { ES_HIP_F32 = 0, ES_HIP_F16 = 1, ES_HIP_BF16 = 30 };
 
 /* fp32 epilogue order, see the header comment */
 enum { ES_HIP_ORDER_X86_CONTRACT = 0, ES_HIP_ORDER_X86_STRICT = 1, ES_HIP_ORDER_SCALAR = 2 };
@@ -437,6 +439,97 @@ int  es_hip_cache_acquire(es_hip_cache *c, int layer, const int *sel, int k, con
 int  es_hip_cache_prefetch(es_hip_cache *c, int layer, int expert, const es_hip_expert_src *src, void *stream, int *slot);
 int  es_hip_cache_slot_info(const es_hip_cache *c, int slot, es_hip_slot_info *out);
 int  es_hip_cache_get_stats(const es_hip_cache *c, es_hip_cache_stats *out);
+
+/* ---- paged key-value cache and attention ---------------------------------------------------------------------------------
+ * What lies between a layer's q/k/v products and its output projection, on the device: K and V rows go into pages, and
+ * attention reads them there, for prompts and for one new token per sequence. The reference keeps its cache in host memory
+ * (attention_n, src/es_engine.c:975); here no row leaves the device, and the fp32 rows that the products write go in as they
+ * are. Sums, maxima and softmax statistics are fp32. Outputs are within rounding of the formula, not bit-identical to a CPU
+ * loop's, and the same from call to call.
+ *
+ * One layer's cache. The pools hold npages pages each; element e of token i of head h in page p is at
+ * ((p * heads + h) * page + i) * dim + e. Sequence row r's token j is token j % page of page table[r * max_pages + j / page].
+ * The arrays on the device are read when the work runs, so a captured call follows their later contents; the struct itself is
+ * read at the call. Whatever they hold, no access leaves the pools: len is taken as at least 0 and at most max_pages * page,
+ * a sequence whose row is outside [0, rows) has no tokens, and the tokens of a page outside [0, npages) take no part (nothing
+ * is written for them, no query sees them), so that padded batches and tables with holes are in order. */
+typedef struct {
+    uint32_t type;      /* ES_HIP_F16 or ES_HIP_BF16 */
+    int heads, dim;     /* K/V heads; elements per head, a multiple of 8 up to 256 */
+    int page, npages;   /* tokens per page, a power of two from 16 to 1024; pages in the pools */
+    void *k, *v;        /* device, 16-byte aligned */
+    const int *table;   /* device */
+    const int *len;     /* device: row r's tokens in the cache, those of the call included */
+    const int *seq;     /* device: the call's sequence b is row seq[b]; NULL: row b */
+    int rows;           /* rows of table and entries of len */
+    int max_pages;      /* entries of a table row */
+} es_hip_kv;
+/* The rows of ntok new tokens into their pages, rounded to the cache's type (nearest even; fp16 overflows to infinity). The
+ * call's sequence b brings rows start[b] to start[b + 1] - 1 of k and v, which are its last tokens: those at len - n to len - 1
+ * (start: device, nseq + 1 entries, not decreasing; NULL: one token per sequence, ntok = nseq). Rows from start[nseq] on are
+ * not read, as are rows whose token would lie before the first or in no page. src_type: ES_HIP_F32 or the cache's own type; token t's heads *
+ * dim elements at k + t * kstride elements (0: packed), the same for v; aligned to their type. A page that several rows of
+ * the table share is written through whichever asks: see es_hip_kv_seq_extend for private copies. */
+int es_hip_kv_append_dev(const es_hip_kv *kv, int nseq, const int *start, int ntok, uint32_t src_type, const void *k,
+                         size_t kstride, const void *v, size_t vstride, void *stream);
+/* Attention of one new token per sequence, the last in its cache (append it first):
+ *   out[b][h] = sum over j of p[j] * v[j],  p = softmax over j of scale * (q[b][h] . k[j]),  len - window <= j < len
+ * (window 0: all), with head h reading K/V head h / (heads / kv->heads). heads: a multiple of kv->heads. type: q's and out's,
+ * ES_HIP_F32 (with either cache) or the cache's own; head h of sequence b at q + b * qstride + h * dim elements (0: packed), the
+ * same for out; aligned to their type. scale is positive and finite. A sequence without tokens gets zeros. Tokens that
+ * a query does not see have no influence, whatever their rows hold. fp32 q is carried to 22 bits or more through the matrix
+ * products, as are the weights p; with a 16-bit q, p is rounded to the cache's type.
+ * ws: the caller's device workspace of at least es_hip_attn_decode_workspace bytes (16-byte aligned; 0 bytes: may be NULL); its
+ * contents need no setup and nothing is kept in it between calls, but calls that may overlap need one each. Nothing is
+ * allocated, copied or waited for: the call can be captured. */
+size_t es_hip_attn_decode_workspace(const es_hip_kv *kv, int nseq, int heads);
+int es_hip_attn_decode_dev(const es_hip_kv *kv, int nseq, int heads, uint32_t type, const void *q, size_t qstride, float scale,
+                           int window, void *out, size_t ostride, void *ws, size_t ws_bytes, void *stream);
+/* Causal attention of prompts, or of the next piece of them: sequence b's queries are rows start[b] to start[b + 1] - 1 of q
+ * (start as in es_hip_kv_append_dev; required), its last tokens in the cache (append them first); query i of n sees tokens j with
+ * pos - window < j <= pos, pos = len - n + i (window 0: from the first). Rows from start[nseq] on of out are left as they
+ * were; a query that sees no token (pos < 0, no pages) gets zeros. ntok: rows of q and out. Otherwise as
+ * es_hip_attn_decode_dev, which gives what this gives for one query per sequence, up to rounding. */
+size_t es_hip_attn_prompt_workspace(const es_hip_kv *kv, int nseq, int ntok, int heads, uint32_t type);
+int es_hip_attn_prompt_dev(const es_hip_kv *kv, int nseq, const int *start, int ntok, int heads, uint32_t type, const void *q,
+                           size_t qstride, float scale, int window, void *out, size_t ostride, void *ws, size_t ws_bytes,
+                           void *stream);
+/* Page src[i] copied over page dst[i], for i < n, in the K and V pools of nlayers layers, layer l's pools at kv->k and kv->v +
+ * l * layer_bytes (0: packed). src and dst are host arrays, read at the call; no page is a destination twice, or a
+ * source and a destination. table, len and seq are not used. */
+int es_hip_kv_copy_pages_dev(const es_hip_kv *kv, int nlayers, size_t layer_bytes, const int *src, const int *dst, int n,
+                             void *stream);
+
+/* The bookkeeping of such a cache: which sequence holds which pages, on the host, with the tables on the device kept in step.
+ * Sequences share pages after a fork, and a shared page is copied before the first of them writes to it. Pages are given out lowest
+ * number first. Calls take effect on the device in stream order: use one stream, or order them. A call that fails changes
+ * nothing, unless the device itself failed (ES_HIP_ERUNTIME). They cannot be captured (what they send is fixed at the call): a
+ * capturing stream is refused with ES_HIP_EINVAL. nlayers = 0 makes a pool of bookkeeping alone (no device memory, no GPU
+ * needed). One pool is used from one host thread at a time. */
+typedef struct es_hip_kv_pool es_hip_kv_pool;
+/* nlayers layers of npages pages each, for up to max_seqs sequences of max_pages pages */
+int  es_hip_kv_pool_create(es_hip_kv_pool **out, uint32_t type, int nlayers, int heads, int dim, int page, int npages,
+                           int max_seqs, int max_pages);
+void es_hip_kv_pool_destroy(es_hip_kv_pool *p);   /* waits for nothing: let the device finish first */
+/* a layer's cache for the calls above: table row = sequence number, seq NULL (set it to a device list of a batch's numbers) */
+int  es_hip_kv_pool_view(const es_hip_kv_pool *p, int layer, es_hip_kv *out);
+int  es_hip_kv_pool_free_pages(const es_hip_kv_pool *p);
+/* a new sequence without tokens: its number, the lowest unused; ES_HIP_EBUSY if there are max_seqs */
+int  es_hip_kv_seq_create(es_hip_kv_pool *p, void *stream);
+/* room for n[i] >= 0 more tokens at the end of sequence seqs[i], i < count (no sequence twice), their lengths counting them from now on:
+ * append then writes them. A partly filled last page that is shared is replaced by a copy. ES_HIP_EBUSY if too few pages are
+ * free (free or truncate a sequence first), ES_HIP_EINVAL past max_pages pages. */
+int  es_hip_kv_seq_extend(es_hip_kv_pool *p, const int *seqs, const int *n, int count, void *stream);
+/* a new sequence with the tokens of seq, sharing its pages: its number, or ES_HIP_EBUSY */
+int  es_hip_kv_seq_fork(es_hip_kv_pool *p, int seq, void *stream);
+/* seq cut to its first len tokens, pages that no sequence needs any more freed */
+int  es_hip_kv_seq_truncate(es_hip_kv_pool *p, int seq, int len, void *stream);
+int  es_hip_kv_seq_free(es_hip_kv_pool *p, int seq, void *stream);
+int  es_hip_kv_seq_len(const es_hip_kv_pool *p, int seq);
+/* the sequence's page numbers into out (up to cap of them; out may be NULL if cap is 0): how many it has */
+int  es_hip_kv_seq_pages(const es_hip_kv_pool *p, int seq, int *out, int cap);
+/* pages moved down so that those in use are 0 to N - 1; returns N */
+int  es_hip_kv_pool_compact(es_hip_kv_pool *p, void *stream);
 
 #ifdef __cplusplus
 }

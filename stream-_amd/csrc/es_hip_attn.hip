@@ -1,0 +1,857 @@
+// Attention over the paged key-value cache (attention_n of the reference, src/es_engine.c:975, whose loops over a host cache
+// this replaces): out = softmax(scale q k^T) v with one pass over the keys, keeping per query the running maximum m, the sum
+// l of 2^(s - m) and the weighted sum of v rows, all in fp32; a growing maximum scales l and the sum by 2^(m_old - m_new).
+//
+// Rows. The G = heads / kv heads query heads that share a K/V head are rows of one product, for every token of a tile: row r
+// of a sequence is query r / G, head r % G. A prompt's tile is then 128 rows of few tokens (little lost to causality) and a decode
+// tile the G heads of the one token, and each K or V element that is read serves all of them.
+//
+// Orientation. Both products run transposed, S^T = K q^T and O^T = V^T P^T: a query is a column, so that its m, l and scale live in
+// the lanes of that column, and the layout in which the matrix cores leave S^T is the one in which they take P^T as the second
+// operand, up to an order of the keys that V^T is given too: the weights never leave their registers.
+//
+// fp32 queries. q is split into as many terms of the cache's type as carry fp32's 24 bits (two of fp16 after scaling the row to
+// 2^14, 22 bits; three of bf16), one product each into the same sums, and so are the weights. K and V are exact as they are.
+// fp16 weights are 2^15 p, so that keys down to 2^-29 of the largest keep all their bits.
+#include <hip/hip_runtime.h>
+
+#include <algorithm>
+#include <cmath>
+
+#include "es_hip_attn.h"
+#include "es_hip_host.h"
+
+namespace {
+
+using namespace esq;
+
+struct AttnArgs {
+    KvView c;
+    const int *start;          // null: one query per sequence
+    const uint8_t *q;
+    uint8_t *out;
+    float *po;                 // parts' sums: [part][row of the tile][dim]
+    float2 *pml;               // parts' m and l: [part][row of the tile]
+    size_t qstride, ostride;   // bytes
+    int nseq, ntok, G, window;
+    float c2;                  // scale * log2(e)
+    int target;                // parts aimed for per K/V head; 0: every tile is one part
+    int items;                 // parts per K/V head that there is room for
+};
+
+// ---- which work a workgroup takes ------------------------------------------------------------------------------------------
+// A tile is BM rows of one sequence and K/V head; a part is a tile's chunk of keys. Chunks have one length for the whole call, from
+// the lengths on the device: the least that leaves about `target` parts, so that ragged batches split evenly and a captured call
+// adapts to later lengths. Every wave finds its part by a scan over the sequences, 64 at a time.
+struct Seq {
+    int t0, n, len;      // first query row, queries, tokens
+    int base, tiles;     // first key of the first chunk (a multiple of 64), tiles of BM rows
+};
+__device__ Seq seq_of(const AttnArgs &a, int b, int bm) {
+    Seq s;
+    if (a.start) {
+        s.t0 = min(max(a.start[b], 0), a.ntok);
+        s.n = min(max(a.start[b + 1], s.t0), a.ntok) - s.t0;
+    } else {
+        s.t0 = b;
+        s.n = 1;
+    }
+    s.len = a.c.tokens(b);
+    s.base = a.window ? max(0, s.len - s.n - a.window + 1) & ~63 : 0;
+    s.tiles = (int)(((long long)s.n * a.G + bm - 1) / bm);
+    return s;
+}
+
+constexpr int CHUNK_MIN = 128;   // keys
+
+__device__ int chunk_of(const AttnArgs &a, int bm) {
+    if (!a.target) return 1 << 30;
+    const int lane = threadIdx.x & 63;
+    unsigned long long all = 0;
+    for (int b = lane; b < a.nseq; b += 64) {
+        const Seq s = seq_of(a, b, bm);
+        all += (unsigned long long)s.tiles * (unsigned)(s.len - s.base);
+    }
+#pragma unroll
+    for (int d = 32; d; d >>= 1) all += __shfl_xor(all, d);
+    const unsigned long long per = (all + a.target - 1) / a.target;
+    const unsigned long long chunk = (per + CHUNK_MIN - 1) / CHUNK_MIN * CHUNK_MIN;
+    return __builtin_amdgcn_readfirstlane((int)min(max(chunk, (unsigned long long)CHUNK_MIN), 1ull << 30));
+}
+__device__ int chunks_of(const Seq &s, int chunk) { return max(1, (int)(((long long)(s.len - s.base) + chunk - 1) / chunk)); }
+
+struct Part {
+    int b, tile, chunk, chunks;   // chunks: of the tile
+    Seq s;
+};
+// the part with number `item` (within one K/V head); false if there is none
+__device__ bool part_of(const AttnArgs &a, int item, int chunk, int bm, Part &p) {
+    const int lane = threadIdx.x & 63;
+    uint32_t before = 0;   // (starts that are out of order may give any number of parts: counted modulo 2^32)
+    for (int g = 0; g < a.nseq; g += 64) {
+        Seq s{};
+        int chunks = 1;
+        uint32_t mine = 0;
+        if (g + lane < a.nseq) {
+            s = seq_of(a, g + lane, bm);
+            chunks = chunks_of(s, chunk);
+            mine = (uint32_t)s.tiles * (uint32_t)chunks;
+        }
+        uint32_t upto = mine;
+#pragma unroll
+        for (int d = 1; d < 64; d <<= 1) {
+            const uint32_t o = __shfl_up(upto, d);
+            if (lane >= d) upto += o;
+        }
+        const unsigned long long past = __ballot((uint32_t)item < before + upto);
+        if (past) {
+            const int w = __builtin_ctzll(past);
+            p.b = g + w;
+            p.s.t0 = __builtin_amdgcn_readlane(s.t0, w);
+            p.s.n = __builtin_amdgcn_readlane(s.n, w);
+            p.s.len = __builtin_amdgcn_readlane(s.len, w);
+            p.s.base = __builtin_amdgcn_readlane(s.base, w);
+            p.s.tiles = __builtin_amdgcn_readlane(s.tiles, w);
+            p.chunks = __builtin_amdgcn_readlane(chunks, w);
+            const int i = (int)((uint32_t)item - before - (uint32_t)__builtin_amdgcn_readlane((int)(upto - mine), w));
+            p.tile = i / p.chunks;
+            p.chunk = i - p.tile * p.chunks;
+            return i >= 0 && p.tile < p.s.tiles;
+        }
+        before += (uint32_t)__builtin_amdgcn_readlane((int)upto, 63);
+    }
+    return false;
+}
+// the number of the first part of sequence b
+__device__ uint32_t parts_before(const AttnArgs &a, int b, int chunk, int bm) {
+    const int lane = threadIdx.x & 63;
+    uint32_t n = 0;
+    for (int g = lane; g < b; g += 64) {
+        const Seq s = seq_of(a, g, bm);
+        n += (uint32_t)s.tiles * (uint32_t)chunks_of(s, chunk);
+    }
+#pragma unroll
+    for (int d = 32; d; d >>= 1) n += __shfl_xor(n, d);
+    return (uint32_t)__builtin_amdgcn_readfirstlane((int)n);
+}
+
+// ---- arithmetic --------------------------------------------------------------------------------------------------------------
+template <bool BF> __device__ f4 mfma16(u4 x, u4 y, f4 c) {
+    if constexpr (BF) return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(b8, x), __builtin_bit_cast(b8, y), c, 0, 0, 0);
+    else return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(h8, x), __builtin_bit_cast(h8, y), c, 0, 0, 0);
+}
+template <bool BF> __device__ f16v mfma32(u4 x, u4 y, f16v c) {
+    if constexpr (BF) return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(b8, x), __builtin_bit_cast(b8, y), c, 0, 0, 0);
+    else return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(h8, x), __builtin_bit_cast(h8, y), c, 0, 0, 0);
+}
+
+// x as the sum of N values of the cache's type, each the nearest to what is left
+template <bool BF, int N> __device__ void split(const float (&x)[8], u4 (&y)[N]) {
+    using T = std::conditional_t<BF, __bf16, _Float16>;
+    using V = T __attribute__((ext_vector_type(8)));
+    float r[8];
+#pragma unroll
+    for (int i = 0; i < 8; i++) r[i] = x[i];
+#pragma unroll
+    for (int t = 0; t < N; t++) {
+        V v;
+#pragma unroll
+        for (int i = 0; i < 8; i++) {
+            v[i] = static_cast<T>(r[i]);
+            if (t + 1 < N) r[i] -= static_cast<float>(v[i]);
+        }
+        y[t] = __builtin_bit_cast(u4, v);
+    }
+}
+
+constexpr float LOWEST = -INFINITY;
+template <bool BF> constexpr float SHIFT = BF ? 0.0f : 15.0f;   // weights are 2^SHIFT p
+// the exponent that weights are taken relative to: a row that has seen no key (or only minus infinity) keeps zeros, not NaN
+__device__ float reference(float m) { return m == LOWEST ? 0.0f : m; }
+
+// Eight elements of a query row, from d on (zeros past dim): fp32 or 16 bits.
+__device__ void load8(const uint8_t *row, int d, int dim, float (&x)[8]) {
+    struct __attribute__((packed, aligned(4))) F8 { float x[8]; };
+    if (d < dim) {
+        const F8 f = *reinterpret_cast<const F8 *>(row + (size_t)d * 4);
+#pragma unroll
+        for (int i = 0; i < 8; i++) x[i] = f.x[i];
+    } else {
+#pragma unroll
+        for (int i = 0; i < 8; i++) x[i] = 0.0f;
+    }
+}
+__device__ u4 load8(const uint8_t *row, int d, int dim) {
+    struct __attribute__((packed, aligned(2))) H8 { uint32_t x[4]; };
+    u4 y = {0, 0, 0, 0};
+    if (d < dim) {
+        const H8 f = *reinterpret_cast<const H8 *>(row + (size_t)d * 2);
+#pragma unroll
+        for (int i = 0; i < 4; i++) y[i] = f.x[i];
+    }
+    return y;
+}
+
+// A query row's terms for the K steps of a product of KS * KL elements a step (lane group g of the row holds elements g * 8 of
+// each), and what the row's scores are multiplied by. xor_lanes: the lanes, apart by that and up, that share a row.
+template <bool BF, int NQ, int KS, int KL, int XOR>
+__device__ float load_query(const uint8_t *row, bool valid, int g, int dim, float c2, u4 (&q)[KS][NQ]) {
+    if constexpr (NQ == 1) {
+#pragma unroll
+        for (int s = 0; s < KS; s++) q[s][0] = valid ? load8(row, s * KL + g * 8, dim) : u4{0, 0, 0, 0};
+        return c2;
+    } else {
+        float x[KS][8];
+        float big = 0.0f;
+#pragma unroll
+        for (int s = 0; s < KS; s++) {
+            load8(row, valid ? s * KL + g * 8 : dim, dim, x[s]);
+#pragma unroll
+            for (int i = 0; i < 8; i++) big = fmaxf(big, fabsf(x[s][i]));
+        }
+        int e = 0;
+        if constexpr (!BF) {   // to 2^14 <= the largest < 2^15: both terms far from fp16's limits
+#pragma unroll
+            for (int d = XOR; d < 64; d <<= 1) big = fmaxf(big, __shfl_xor(big, d));
+            if (big > 0.0f && big < INFINITY) e = 14 - (static_cast<int>(__float_as_uint(big) >> 23) - 127);
+            e = min(e, 126);
+        }
+#pragma unroll
+        for (int s = 0; s < KS; s++) {
+            if constexpr (!BF) {
+#pragma unroll
+                for (int i = 0; i < 8; i++) x[s][i] = ldexpf(x[s][i], e);
+            }
+            split<BF, NQ>(x[s], q[s]);
+        }
+        return fmaxf(ldexpf(c2, -e), 1.17549435e-38f);   // (never 0, which would turn a hidden key's score into NaN)
+    }
+}
+
+template <bool F32, bool BF> __device__ void store4(uint8_t *row, int d, const float (&x)[4]) {
+    if constexpr (F32) {
+        struct __attribute__((packed, aligned(4))) F4 { float x[4]; };
+        F4 f;
+#pragma unroll
+        for (int i = 0; i < 4; i++) f.x[i] = x[i];
+        *reinterpret_cast<F4 *>(row + (size_t)d * 4) = f;
+    } else {
+        using T = std::conditional_t<BF, __bf16, _Float16>;
+        struct __attribute__((packed, aligned(2))) H4 { T x[4]; };
+        H4 f;
+#pragma unroll
+        for (int i = 0; i < 4; i++) f.x[i] = static_cast<T>(x[i]);
+        *reinterpret_cast<H4 *>(row + (size_t)d * 2) = f;
+    }
+}
+
+// two rows' elements j of 2 packed elements, as a pair
+template <int J> __device__ uint32_t pair(uint32_t first, uint32_t second) {
+    return __builtin_amdgcn_perm(second, first, J & 1 ? 0x07060302u : 0x05040100u);
+}
+
+// ---- one query per sequence ----------------------------------------------------------------------------------------------------
+// A workgroup of four waves takes a part: up to 16 heads of one K/V head against a chunk of keys, each wave 32 keys at a time in
+// turn, joined in LDS at the end. Nothing is staged: a lane loads its K fragments as the matrix cores take them (key lane % 16,
+// 8 elements) and, of V, the DP / 16 elements from (lane % 16) * DP / 16 on of the 8 keys whose weights it holds, which
+// it turns into 8 keys of one element each with byte permutes. Bound by HBM where the caches are long.
+template <bool BF, int NQ, int DP> __global__ __launch_bounds__(256) void attn_decode_kernel(AttnArgs a) {
+    constexpr int KS = DP / 32, DL = DP / 16, BM = 16;
+    constexpr bool F32 = NQ > 1;
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int col = lane & 15, g = lane >> 4;
+    const int head = blockIdx.x % a.c.heads, item = blockIdx.x / a.c.heads;
+    const int chunk = chunk_of(a, BM);
+    Part p;
+    if (!part_of(a, item, chunk, BM, p)) return;
+    const int lo = max(a.window ? p.s.len - a.window : 0, 0), hi = p.s.len;
+    const int first = p.s.base + p.chunk * (chunk < 1 << 30 ? chunk : 0);
+    const int last = chunk < 1 << 30 ? min(hi, first + chunk) : hi;
+    const int r = p.tile * BM + col, rows = a.G;
+    const int shift16 = a.c.shift - 4;
+    const int *table = a.c.table + (size_t)max(a.c.row(p.b), 0) * a.c.max_pages;
+    const size_t pagestep = (size_t)a.c.heads << a.c.shift;   // token rows per page
+
+    u4 q[KS][NQ];
+    const float cs = load_query<BF, NQ, KS, 32, 16>(a.q + (size_t)p.s.t0 * a.qstride + (size_t)(head * a.G + r) * a.c.dim * (F32 ? 4 : 2),
+                                                    r < rows, g, a.c.dim, a.c2, q);
+    f4 acc[DL];
+#pragma unroll
+    for (int j = 0; j < DL; j++) acc[j] = f4{0, 0, 0, 0};
+    float m = LOWEST, l = 0.0f;
+
+    for (int t0 = first + wave * 32; t0 < last; t0 += 128) {
+        // the two pages; one that there is not: no keys, and page 0 in its place
+        bool ok[2];
+        const uint8_t *kp[2], *vp[2];
+#pragma unroll
+        for (int h = 0; h < 2; h++) {
+            const int u = (t0 >> 4) + h;
+            int page = u * 16 < last ? table[u >> shift16] : -1;
+            ok[h] = page >= 0 && page < a.c.npages;
+            page = ok[h] ? page : 0;
+            const size_t at = ((size_t)page * pagestep + ((size_t)head << a.c.shift) + (u & ((1 << shift16) - 1)) * 16) * a.c.dim * 2;
+            kp[h] = a.c.k + at;
+            vp[h] = a.c.v + at;
+        }
+        u4 kf[2][KS];
+#pragma unroll
+        for (int h = 0; h < 2; h++)
+#pragma unroll
+            for (int s = 0; s < KS; s++) {
+                const int d = s * 32 + g * 8;
+                kf[h][s] = d < a.c.dim ? *reinterpret_cast<const u4 *>(kp[h] + ((size_t)col * a.c.dim + d) * 2) : u4{0, 0, 0, 0};
+            }
+        uint32_t vr[8][DL / 2];
+#pragma unroll
+        for (int i = 0; i < 8; i++) {
+            const int d = col * DL;   // dim is a multiple of 8: DL = 4 may end inside the row's last 8, DL = 16 may begin there
+            const uint8_t *src = vp[i >> 2] + ((size_t)(g * 4 + (i & 3)) * a.c.dim + d) * 2;
+#pragma unroll
+            for (int w = 0; w < DL / 2; w += (DL == 4 ? 2 : 4)) {
+                const bool in = d + w * 2 < a.c.dim;
+                if constexpr (DL == 4) {
+                    const u2 x = in ? *reinterpret_cast<const u2 *>(src) : u2{0, 0};
+                    vr[i][0] = x[0];
+                    vr[i][1] = x[1];
+                } else {
+                    const u4 x = in ? *reinterpret_cast<const u4 *>(src + w * 4) : u4{0, 0, 0, 0};
+#pragma unroll
+                    for (int k = 0; k < 4; k++) vr[i][w + k] = x[k];
+                }
+            }
+        }
+        f4 s[2] = {f4{0, 0, 0, 0}, f4{0, 0, 0, 0}};
+#pragma unroll
+        for (int t = 0; t < NQ; t++)
+#pragma unroll
+            for (int k = 0; k < KS; k++)
+#pragma unroll
+                for (int h = 0; h < 2; h++) s[h] = mfma16<BF>(kf[h][k], q[k][t], s[h]);
+        if (t0 < lo || t0 + 32 > last || !ok[0] || !ok[1]) {   // what is not to be seen: no score, and zeros for whatever V holds
+#pragma unroll
+            for (int i = 0; i < 8; i++) {
+                const int t = t0 + (i >> 2) * 16 + g * 4 + (i & 3);
+                if (t < lo || t >= last || !ok[i >> 2]) {
+                    s[i >> 2][i & 3] = LOWEST;
+#pragma unroll
+                    for (int w = 0; w < DL / 2; w++) vr[i][w] = 0;
+                }
+            }
+        }
+        float big = LOWEST;
+#pragma unroll
+        for (int i = 0; i < 8; i++) big = fmaxf(big, s[i >> 2][i & 3]);
+        big = fmaxf(big, __shfl_xor(big, 16));
+        big = fmaxf(big, __shfl_xor(big, 32)) * cs;
+        if (__any(big > m)) {
+            const float now = fmaxf(m, big), f = __builtin_amdgcn_exp2f(m - reference(now));
+            m = now;
+            l *= f;
+#pragma unroll
+            for (int j = 0; j < DL; j++)
+#pragma unroll
+                for (int i = 0; i < 4; i++) acc[j][i] *= f;
+        }
+        const float ref = SHIFT<BF> - reference(m);
+        float w8[8];
+#pragma unroll
+        for (int i = 0; i < 8; i++) {
+            w8[i] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[i >> 2][i & 3], cs, ref));
+            l += w8[i];
+        }
+        u4 pt[NQ];
+        split<BF, NQ>(w8, pt);
+#pragma unroll
+        for (int j = 0; j < DL; j += 2) {
+            u4 v0, v1;
+#pragma unroll
+            for (int k = 0; k < 4; k++) {
+                v0[k] = pair<0>(vr[2 * k][j / 2], vr[2 * k + 1][j / 2]);
+                v1[k] = pair<1>(vr[2 * k][j / 2], vr[2 * k + 1][j / 2]);
+            }
+#pragma unroll
+            for (int t = 0; t < NQ; t++) {
+                acc[j] = mfma16<BF>(v0, pt[t], acc[j]);
+                acc[j + 1] = mfma16<BF>(v1, pt[t], acc[j + 1]);
+            }
+        }
+    }
+    l += __shfl_xor(l, 16);
+    l += __shfl_xor(l, 32);
+
+    // the four waves' m, l and sums; lane (g, col) holds elements (g * 4 + i) * DL + j of head col
+    __shared__ float lm[4][BM], ll[4][BM];
+    __shared__ __attribute__((aligned(16))) float lo_acc[4][BM][DP + 4];
+    if (g == 0) {
+        lm[wave][col] = m;
+        ll[wave][col] = l;
+    }
+#pragma unroll
+    for (int i = 0; i < 4; i++)
+#pragma unroll
+        for (int j = 0; j < DL; j += 4)
+            *reinterpret_cast<f4 *>(&lo_acc[wave][col][(g * 4 + i) * DL + j]) = f4{acc[j][i], acc[j + 1][i], acc[j + 2][i], acc[j + 3][i]};
+    __syncthreads();
+    const size_t slot = (size_t)item * a.c.heads + head;
+    for (int e = threadIdx.x; e < BM * (DP / 4); e += 256) {
+        const int row = e / (DP / 4), d = e % (DP / 4) * 4;
+        if (p.tile * BM + row >= rows || d >= a.c.dim) continue;
+        float mm = LOWEST;
+#pragma unroll
+        for (int w = 0; w < 4; w++) mm = fmaxf(mm, lm[w][row]);
+        float sum = 0.0f, x[4] = {0, 0, 0, 0};
+#pragma unroll
+        for (int w = 0; w < 4; w++) {
+            const float f = __builtin_amdgcn_exp2f(lm[w][row] - reference(mm));
+            sum += f * ll[w][row];
+#pragma unroll
+            for (int i = 0; i < 4; i++) x[i] += f * lo_acc[w][row][d + i];
+        }
+        if (p.chunks == 1) {
+            const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
+#pragma unroll
+            for (int i = 0; i < 4; i++) x[i] = sum == 0.0f ? 0.0f : x[i] * inv;
+            store4<F32, BF>(a.out + (size_t)p.s.t0 * a.ostride + (size_t)(head * a.G + p.tile * BM + row) * a.c.dim * (F32 ? 4 : 2), d, x);
+        } else {
+            if (d == 0) a.pml[slot * BM + row] = float2{mm, sum};
+            *reinterpret_cast<f4 *>(a.po + (slot * BM + row) * a.c.dim + d) = f4{x[0], x[1], x[2], x[3]};
+        }
+    }
+}
+
+// ---- a tile of prompt rows -------------------------------------------------------------------------------------------------------
+// A workgroup of four waves takes 128 rows, 32 a wave, against its keys, 64 at a time through LDS: K as it is, V turned to [element][key]
+// on its way from registers, its keys in the order in which the lanes hold the weights. The next keys' loads run under the
+// products. Keys that a row does not see have weight 0; V rows that no row sees are staged as zeros, and a V row with an infinity or NaN that
+// only some rows see is kept out of the product and added to those alone (0 times infinity is not 0).
+constexpr int PM = 128, PN = 64;
+
+template <bool BF, int NQ, int DP> __global__ __launch_bounds__(256) void attn_prompt_kernel(AttnArgs a) {
+    constexpr int KS = DP / 16, DT = DP / 32, KC = DP / 8;
+    constexpr int KP = DP + 8, VP = PN + 8;   // LDS pitches, elements
+    constexpr int NK = PN * KC / 256, NV = (PN / 4 * KC + 255) / 256;
+    constexpr bool F32 = NQ > 1;
+    __shared__ __attribute__((aligned(16))) uint16_t lk[PN * KP], lv[DP * VP];
+    __shared__ uint32_t odd[2][2];   // keys whose V row is not finite, by step
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int col = lane & 31, half = lane >> 5;
+    const int head = blockIdx.x % a.c.heads, item = blockIdx.x / a.c.heads;
+    const int chunk = chunk_of(a, PM);
+    Part p;
+    if (!part_of(a, item, chunk, PM, p)) return;
+    const bool whole = chunk == 1 << 30;
+    const int tile = p.s.tiles - 1 - p.tile;   // the tiles that see most keys first
+    const int rows = min(PM, p.s.n * a.G - tile * PM);
+    const int back = p.s.len - p.s.n;          // query i stands at back + i
+    const int pos_lo = back + tile * PM / a.G, pos_hi = back + (tile * PM + rows - 1) / a.G;
+    const int see_lo = a.window ? max(0, pos_lo - a.window + 1) : 0, see_hi = pos_hi + 1;   // keys that some row sees
+    int first = p.s.base + (whole ? 0 : p.chunk * chunk), last = whole ? see_hi : min(see_hi, first + chunk);
+    first = max(first, see_lo & ~(PN - 1));
+    const int shift16 = a.c.shift - 4;
+    const int *table = a.c.table + (size_t)max(a.c.row(p.b), 0) * a.c.max_pages;
+    const size_t pagestep = (size_t)a.c.heads << a.c.shift;
+
+    const int r = min(tile * PM + wave * 32 + col, tile * PM + rows - 1);   // lanes past the last row repeat it
+    const int query = r / a.G, pos = back + query, from = a.window ? pos - a.window + 1 : 0;
+    const size_t qoff = (size_t)(head * a.G + r - query * a.G) * a.c.dim * (F32 ? 4 : 2);
+    u4 q[KS][NQ];
+    const float cs = load_query<BF, NQ, KS, 16, 32>(a.q + (size_t)(p.s.t0 + query) * a.qstride + qoff, true, half, a.c.dim, a.c2, q);
+    const int wpos_lo = __builtin_amdgcn_readlane(pos, 0), wpos_hi = __builtin_amdgcn_readlane(pos, 31);
+    const bool idle = wave * 32 >= rows;
+
+    f16v acc[DT];
+#pragma unroll
+    for (int j = 0; j < DT; j++)
+#pragma unroll
+        for (int i = 0; i < 16; i++) acc[j][i] = 0.0f;
+    float m = LOWEST, l = 0.0f;
+
+    u4 kr[NK], vr[NV][4];
+    // page of 16 keys u * 16.., or -1
+    auto page_of = [&](int u) {
+        const int g = u * 16 < last ? table[u >> shift16] : -1;
+        return g < a.c.npages ? g : -1;
+    };
+    auto row_at = [&](int page, int t) {
+        return ((size_t)max(page, 0) * pagestep + ((size_t)head << a.c.shift) + (t & ((1 << a.c.shift) - 1))) * a.c.dim * 2;
+    };
+    auto load = [&](int t0) {
+#pragma unroll
+        for (int i = 0; i < NK; i++) {
+            const int c = tid + i * 256, t = t0 + c / KC, d = c % KC * 8;
+            const int page = page_of(t >> 4);
+            kr[i] = page >= 0 && d < a.c.dim ? *reinterpret_cast<const u4 *>(a.c.k + row_at(page, t) + d * 2) : u4{0, 0, 0, 0};
+        }
+#pragma unroll
+        for (int i = 0; i < NV; i++) {
+            const int c = tid + i * 256, t = t0 + c / KC * 4, d = c % KC * 8;
+            const int page = c < PN / 4 * KC ? page_of(t >> 4) : -1;
+#pragma unroll
+            for (int k = 0; k < 4; k++)
+                vr[i][k] = page >= 0 && d < a.c.dim && t + k >= see_lo && t + k < last
+                               ? *reinterpret_cast<const u4 *>(a.c.v + row_at(page, t + k) + d * 2) : u4{0, 0, 0, 0};
+        }
+    };
+    if (tid < 4) odd[tid >> 1][tid & 1] = 0;
+    if (first < last) load(first);
+    int step = 0;
+    for (int t0 = first; t0 < last; t0 += PN, step ^= 1) {
+        __syncthreads();
+        const bool edge = t0 + PN > pos_lo + 1 || t0 < (a.window ? pos_hi - a.window + 1 : 0);   // some row does not see all keys
+#pragma unroll
+        for (int i = 0; i < NK; i++) {
+            const int c = tid + i * 256;
+            *reinterpret_cast<u4 *>(&lk[c / KC * KP + c % KC * 8]) = kr[i];
+        }
+#pragma unroll
+        for (int i = 0; i < NV; i++) {
+            const int c = tid + i * 256;
+            if (c < PN / 4 * KC) {
+                const int t = c / KC * 4, d = c % KC * 8;
+                const int at = (t & ~15) + (t & 4 ? 8 : 0) + (t & 8 ? 4 : 0);   // keys t..t+3 among the 64 as the weights lie
+#pragma unroll
+                for (int k = 0; k < 4; k++) {
+                    u2 x = {pair<0>(vr[i][0][k], vr[i][1][k]), pair<0>(vr[i][2][k], vr[i][3][k])};
+                    u2 y = {pair<1>(vr[i][0][k], vr[i][1][k]), pair<1>(vr[i][2][k], vr[i][3][k])};
+                    *reinterpret_cast<u2 *>(&lv[(d + 2 * k) * VP + at]) = x;
+                    *reinterpret_cast<u2 *>(&lv[(d + 2 * k + 1) * VP + at]) = y;
+                }
+                if (edge) {
+                    constexpr uint32_t E = BF ? 0x7f80u : 0x7c00u;   // an exponent of ones
+#pragma unroll
+                    for (int k = 0; k < 4; k++) {
+                        bool bad = false;
+#pragma unroll
+                        for (int w = 0; w < 4; w++)
+                            bad |= (vr[i][k][w] & E) == E || (vr[i][k][w] >> 16 & E) == E;
+                        if (bad) atomicOr(&odd[step][t >> 5], 1u << ((t + k) & 31));
+                    }
+                }
+            }
+        }
+        __syncthreads();
+        if (t0 + PN < last) load(t0 + PN);
+        if (tid < 2) odd[step ^ 1][tid] = 0;
+        if (idle || t0 > wpos_hi || (a.window && t0 + PN <= wpos_lo - a.window + 1)) continue;
+        int holes = 0;
+#pragma unroll
+        for (int u = 0; u < PN / 16; u++) holes |= page_of((t0 >> 4) + u) < 0 ? 1 << u : 0;
+
+        f16v s[2];
+#pragma unroll
+        for (int h = 0; h < 2; h++)
+#pragma unroll
+            for (int i = 0; i < 16; i++) s[h][i] = 0.0f;
+#pragma unroll
+        for (int k = 0; k < KS; k++)
+#pragma unroll
+            for (int h = 0; h < 2; h++) {
+                const u4 kf = *reinterpret_cast<const u4 *>(&lk[(h * 32 + col) * KP + k * 16 + half * 8]);
+#pragma unroll
+                for (int t = 0; t < NQ; t++) s[h] = mfma32<BF>(kf, q[k][t], s[h]);
+            }
+        if (t0 + PN > wpos_lo + 1 || holes || (a.window && t0 < wpos_hi - a.window + 1)) {
+#pragma unroll
+            for (int h = 0; h < 2; h++)
+#pragma unroll
+                for (int i = 0; i < 16; i++) {
+                    const int t = t0 + h * 32 + i / 4 * 8 + half * 4 + (i & 3);
+                    if (t > pos || t < from || t >= last || (holes >> (h * 2 + i / 8) & 1)) s[h][i] = LOWEST;
+                }
+        }
+        float big = LOWEST;
+#pragma unroll
+        for (int h = 0; h < 2; h++)
+#pragma unroll
+            for (int i = 0; i < 16; i++) big = fmaxf(big, s[h][i]);
+        big = fmaxf(big, __shfl_xor(big, 32)) * cs;
+        if (__any(big > m)) {
+            const float now = fmaxf(m, big), f = __builtin_amdgcn_exp2f(m - reference(now));
+            m = now;
+            l *= f;
+#pragma unroll
+            for (int j = 0; j < DT; j++)
+#pragma unroll
+                for (int i = 0; i < 16; i++) acc[j][i] *= f;
+        }
+        const float ref = SHIFT<BF> - reference(m);
+        u4 pt[4][NQ];
+#pragma unroll
+        for (int u = 0; u < 4; u++) {
+            float w8[8];
+#pragma unroll
+            for (int i = 0; i < 8; i++) {
+                w8[i] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[u >> 1][(u & 1) * 8 + i], cs, ref));
+                l += w8[i];
+            }
+            split<BF, NQ>(w8, pt[u]);
+        }
+        const uint32_t odd0 = edge ? odd[step][0] : 0, odd1 = edge ? odd[step][1] : 0;
+        if (!__builtin_amdgcn_readfirstlane(odd0 | odd1)) {
+#pragma unroll
+            for (int u = 0; u < 4; u++)
+#pragma unroll
+                for (int j = 0; j < DT; j++) {
+                    const u4 vf = *reinterpret_cast<const u4 *>(&lv[(j * 32 + col) * VP + u * 16 + half * 8]);
+#pragma unroll
+                    for (int t = 0; t < NQ; t++) acc[j] = mfma32<BF>(vf, pt[u][t], acc[j]);
+                }
+        } else {
+            // the lane's keys of step u: u * 16 + half * 4 + {0..3, 8..11}
+            auto only = [&](u4 v, uint32_t keys, int u) {   // V with the keys that are not in the mask (of 32) as zeros
+                const uint32_t k = keys >> ((u & 1) * 16 + half * 4);
+#pragma unroll
+                for (int w = 0; w < 4; w++) {
+                    const int b = (w >> 1) * 8 + (w & 1) * 2;
+                    v[w] &= (k >> b & 1 ? 0xffffu : 0) | (k >> (b + 1) & 1 ? 0xffff0000u : 0);
+                }
+                return v;
+            };
+#pragma unroll
+            for (int u = 0; u < 4; u++)
+#pragma unroll
+                for (int j = 0; j < DT; j++) {
+                    const u4 vf = only(*reinterpret_cast<const u4 *>(&lv[(j * 32 + col) * VP + u * 16 + half * 8]), ~(u < 2 ? odd0 : odd1), u);
+#pragma unroll
+                    for (int t = 0; t < NQ; t++) acc[j] = mfma32<BF>(vf, pt[u][t], acc[j]);
+                }
+#pragma unroll
+            for (int u = 0; u < 4; u++) {
+                uint32_t keys = __builtin_amdgcn_readfirstlane((u < 2 ? odd0 : odd1) & 0xffffu << (u & 1) * 16);
+                while (keys) {
+                    const int b = __builtin_ctz(keys);
+                    keys &= keys - 1;
+                    const int t = t0 + (u >> 1) * 32 + b;
+                    const bool seen = t <= pos && t >= from;
+#pragma unroll
+                    for (int j = 0; j < DT; j++) {
+                        const u4 vf = only(*reinterpret_cast<const u4 *>(&lv[(j * 32 + col) * VP + u * 16 + half * 8]), 1u << b, u);
+                        f16v x;
+#pragma unroll
+                        for (int i = 0; i < 16; i++) x[i] = 0.0f;
+#pragma unroll
+                        for (int n = 0; n < NQ; n++) x = mfma32<BF>(vf, pt[u][n], x);
+#pragma unroll
+                        for (int i = 0; i < 16; i++) acc[j][i] = seen ? acc[j][i] + x[i] : acc[j][i];
+                    }
+                }
+            }
+        }
+    }
+    l += __shfl_xor(l, 32);
+
+    if (wave * 32 + col >= rows) return;
+    if (p.chunks == 1) {
+        uint8_t *row = a.out + (size_t)(p.s.t0 + query) * a.ostride + qoff;
+        const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+#pragma unroll
+        for (int j = 0; j < DT; j++)
+#pragma unroll
+            for (int i = 0; i < 16; i += 4) {
+                const int d = j * 32 + i * 2 + half * 4;
+                float x[4];
+#pragma unroll
+                for (int k = 0; k < 4; k++) x[k] = l == 0.0f ? 0.0f : acc[j][i + k] * inv;
+                if (d < a.c.dim) store4<F32, BF>(row, d, x);
+            }
+    } else {
+        const size_t at = ((size_t)item * a.c.heads + head) * PM + wave * 32 + col;
+        if (half == 0) a.pml[at] = float2{m, l};
+#pragma unroll
+        for (int j = 0; j < DT; j++)
+#pragma unroll
+            for (int i = 0; i < 16; i += 4) {
+                const int d = j * 32 + i * 2 + half * 4;
+                if (d < a.c.dim) *reinterpret_cast<f4 *>(a.po + at * a.c.dim + d) = f4{acc[j][i], acc[j][i + 1], acc[j][i + 2], acc[j][i + 3]};
+            }
+    }
+}
+
+// ---- parts joined ------------------------------------------------------------------------------------------------------------
+// One workgroup per row (query, head): the parts' sums, each scaled by 2^(m of the part - the largest m), in the order of the parts.
+template <bool F32, bool BF, int BM> __global__ __launch_bounds__(256) void attn_join_kernel(AttnArgs a) {
+    const int heads = a.c.heads * a.G;
+    const int t = blockIdx.x / heads, hq = blockIdx.x % heads, head = hq / a.G;
+    int b = t;
+    if (a.start) {
+        int lo = 0, hi = a.nseq;
+        while (hi - lo > 1) {
+            const int mid = (lo + hi) >> 1;
+            if (a.start[mid] <= t) lo = mid; else hi = mid;
+        }
+        b = lo;
+    }
+    const Seq s = seq_of(a, b, BM);
+    if (t < s.t0 || t >= s.t0 + s.n) return;
+    const int chunk = chunk_of(a, BM), chunks = chunks_of(s, chunk);
+    if (chunks == 1) return;   // written already
+    const int r = (t - s.t0) * a.G + hq - head * a.G;
+    int tile = r / BM;
+    const int row = r - tile * BM;
+    if (a.start) tile = s.tiles - 1 - tile;
+    const size_t part = (size_t)parts_before(a, b, chunk, BM) + (size_t)tile * chunks;
+    if (part + chunks > (size_t)a.items) return;   // (starts out of order)
+    const int quads = a.c.dim / 4, w = quads <= 16 ? 16 : quads <= 32 ? 32 : 64;   // threads per part
+    const int d = threadIdx.x % w, k = threadIdx.x / w, n = 256 / w;
+    float m = LOWEST, l = 0.0f;
+    f4 x = {0, 0, 0, 0};
+    for (int c = k; c < chunks; c += n) {
+        const size_t at = ((part + c) * a.c.heads + head) * BM + row;
+        const float2 ml = a.pml[at];
+        if (ml.y == 0.0f) continue;
+        f4 y = {0, 0, 0, 0};
+        if (d < quads) y = *reinterpret_cast<const f4 *>(a.po + at * a.c.dim + d * 4);
+        const float now = fmaxf(m, ml.x), f = __builtin_amdgcn_exp2f(m - reference(now)), f2 = __builtin_amdgcn_exp2f(ml.x - reference(now));
+        m = now;
+        l = l * f + ml.y * f2;
+#pragma unroll
+        for (int i = 0; i < 4; i++) x[i] = x[i] * f + y[i] * f2;
+    }
+    __shared__ float sm[16], sl[16];
+    __shared__ f4 sx[256];
+    if (d == 0) {
+        sm[k] = m;
+        sl[k] = l;
+    }
+    sx[threadIdx.x] = x;
+    __syncthreads();
+    if (k || d >= quads) return;
+    for (int c = 1; c < n; c++) {
+        if (sl[c] == 0.0f) continue;
+        const f4 y = sx[c * w + d];
+        const float now = fmaxf(m, sm[c]), f = __builtin_amdgcn_exp2f(m - reference(now)), f2 = __builtin_amdgcn_exp2f(sm[c] - reference(now));
+        m = now;
+        l = l * f + sl[c] * f2;
+#pragma unroll
+        for (int i = 0; i < 4; i++) x[i] = x[i] * f + y[i] * f2;
+    }
+    float o[4];
+    const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+#pragma unroll
+    for (int i = 0; i < 4; i++) o[i] = l == 0.0f ? 0.0f : x[i] * inv;
+    store4<F32, BF>(a.out + (size_t)t * a.ostride + (size_t)hq * a.c.dim * (F32 ? 4 : 2), d * 4, o);
+}
+
+// ---- host ------------------------------------------------------------------------------------------------------------------------
+constexpr int DECODE_M = 16;
+constexpr int DECODE_PARTS = 512, PROMPT_PARTS = 512;   // workgroups that a call is split into, about: two per CU
+
+struct Shape {
+    size_t tiles;   // the most tiles per K/V head that the call's lengths can give
+    int target;     // AttnArgs::target
+    int bm;
+    size_t items() const { return tiles + (size_t)target; }   // sum of tiles * ceil(span / chunk) <= target + tiles
+    size_t workspace(const es_hip_kv *kv) const { return target ? items() * kv->heads * bm * (kv->dim + 2) * sizeof(float) : 0; }
+};
+Shape shape_of(const es_hip_kv *kv, int nseq, int ntok, int heads, bool prompt) {
+    const int G = heads / kv->heads;
+    Shape s;
+    s.bm = prompt ? PM : DECODE_M;
+    s.tiles = prompt ? (size_t)ntok * G / PM + nseq : (size_t)nseq * ((G + DECODE_M - 1) / DECODE_M);
+    const int parts = (prompt ? PROMPT_PARTS : DECODE_PARTS) / kv->heads;
+    const bool many = prompt && s.tiles >= (size_t)std::max(parts, 1);
+    s.target = many || (long long)kv->max_pages * kv->page <= CHUNK_MIN ? 0 : std::max(parts, 1);
+    return s;
+}
+
+int check_heads(const es_hip_kv *kv, int nseq, int ntok, int heads, KvView &v) {
+    if (int rc = kv_check(kv, nseq, v, true)) return rc;
+    if (heads < 1 || heads % kv->heads || heads > 65536) return host_fail(ES_HIP_EINVAL, "heads: a multiple of the cache's, up to 65536");
+    if (ntok < 0) return host_fail(ES_HIP_EINVAL, "negative number of tokens");
+    // (a launch holds 2^24 workgroups of 256)
+    if ((long long)ntok * heads > 1 << 29 || (long long)nseq * heads > 1 << 23)
+        return host_fail(ES_HIP_EINVAL, "more than 2^29 query rows, or 2^23 sequences times heads");
+    return ES_HIP_OK;
+}
+
+template <bool BF, int NQ> hipError_t launch(const AttnArgs &a, const Shape &s, bool prompt, hipStream_t st) {
+    const size_t grid = s.items() * a.c.heads;
+    if (prompt) {
+        auto f = a.c.dim <= 64 ? attn_prompt_kernel<BF, NQ, 64> : a.c.dim <= 128 ? attn_prompt_kernel<BF, NQ, 128> : attn_prompt_kernel<BF, NQ, 256>;
+        f<<<(unsigned)grid, 256, 0, st>>>(a);
+    } else {
+        auto f = a.c.dim <= 64 ? attn_decode_kernel<BF, NQ, 64> : a.c.dim <= 128 ? attn_decode_kernel<BF, NQ, 128> : attn_decode_kernel<BF, NQ, 256>;
+        f<<<(unsigned)grid, 256, 0, st>>>(a);
+    }
+    hipError_t e = hipGetLastError();
+    if (e != hipSuccess || !s.target) return e;
+    auto f = prompt ? attn_join_kernel<(NQ > 1), BF, PM> : attn_join_kernel<(NQ > 1), BF, DECODE_M>;
+    f<<<(unsigned)((size_t)a.ntok * a.c.heads * a.G), 256, 0, st>>>(a);
+    return hipGetLastError();
+}
+
+int attention(const es_hip_kv *kv, int nseq, const int *start, int ntok, int heads, uint32_t type, const void *q, size_t qstride,
+              float scale, int window, void *out, size_t ostride, void *ws, size_t ws_bytes, void *stream) {
+    if (int rc = host_need_device()) return rc;
+    AttnArgs a;
+    const bool prompt = start != nullptr;
+    if (int rc = check_heads(kv, nseq, ntok, heads, a.c)) return rc;
+    if (type != ES_HIP_F32 && type != kv->type) return host_fail(ES_HIP_EINVAL, "q and out are F32 or of the cache's type");
+    if (!(scale > 0.0f) || !std::isfinite(scale * 1.5f)) return host_fail(ES_HIP_EINVAL, "scale is positive and finite");
+    if (window < 0) return host_fail(ES_HIP_EINVAL, "negative window");
+    if (nseq == 0 || ntok == 0) return ES_HIP_OK;
+    const size_t es = type == ES_HIP_F32 ? 4 : 2, row = (size_t)heads * kv->dim;
+    if (!q || !out || ((reinterpret_cast<uintptr_t>(q) | reinterpret_cast<uintptr_t>(out)) & (es - 1)) || (reinterpret_cast<uintptr_t>(start) & 3))
+        return host_fail(ES_HIP_EINVAL, "null or misaligned q, out or start");
+    if (!qstride) qstride = row;
+    if (!ostride) ostride = row;
+    if (ntok > 1 && (qstride < row || ostride < row)) return host_fail(ES_HIP_EINVAL, "rows overlap (stride below heads * dim)");
+    const Shape s = shape_of(kv, nseq, ntok, heads, prompt);
+    const size_t need = s.workspace(kv);
+    if (need && (!ws || ws_bytes < need || (reinterpret_cast<uintptr_t>(ws) & 15)))
+        return host_fail(ES_HIP_EINVAL, "workspace missing, too small or misaligned (16 bytes)");
+    a.start = start;
+    a.q = static_cast<const uint8_t *>(q);
+    a.out = static_cast<uint8_t *>(out);
+    a.po = static_cast<float *>(ws);
+    a.pml = reinterpret_cast<float2 *>(a.po + (need ? s.items() * kv->heads * s.bm * (size_t)kv->dim : 0));
+    a.qstride = qstride * es;
+    a.ostride = ostride * es;
+    a.nseq = nseq;
+    a.ntok = ntok;
+    a.G = heads / kv->heads;
+    a.window = window;
+    a.c2 = std::max(scale * 1.44269504088896340736f, 1.17549435e-38f);
+    a.target = s.target;
+    a.items = (int)s.items();
+    const hipStream_t st = static_cast<hipStream_t>(stream);
+    hipError_t e;
+    if (kv->type == ES_HIP_BF16) e = type == ES_HIP_F32 ? launch<true, 3>(a, s, prompt, st) : launch<true, 1>(a, s, prompt, st);
+    else e = type == ES_HIP_F32 ? launch<false, 2>(a, s, prompt, st) : launch<false, 1>(a, s, prompt, st);
+    return e == hipSuccess ? ES_HIP_OK : host_hip_fail(e, "attention launch");
+}
+
+}  // namespace
+
+extern "C" {
+
+size_t es_hip_attn_decode_workspace(const es_hip_kv *kv, int nseq, int heads) {
+    KvView v;
+    if (check_heads(kv, nseq, nseq, heads, v) || !nseq) return 0;
+    return shape_of(kv, nseq, nseq, heads, false).workspace(kv);
+}
+
+size_t es_hip_attn_prompt_workspace(const es_hip_kv *kv, int nseq, int ntok, int heads, uint32_t type) {
+    KvView v;
+    (void)type;
+    if (check_heads(kv, nseq, ntok, heads, v) || !nseq || !ntok) return 0;
+    return shape_of(kv, nseq, ntok, heads, true).workspace(kv);
+}
+
+int es_hip_attn_decode_dev(const es_hip_kv *kv, int nseq, int heads, uint32_t type, const void *q, size_t qstride, float scale,
+                           int window, void *out, size_t ostride, void *ws, size_t ws_bytes, void *stream) {
+    return attention(kv, nseq, nullptr, nseq, heads, type, q, qstride, scale, window, out, ostride, ws, ws_bytes, stream);
+}
+
+int es_hip_attn_prompt_dev(const es_hip_kv *kv, int nseq, const int *start, int ntok, int heads, uint32_t type, const void *q,
+                           size_t qstride, float scale, int window, void *out, size_t ostride, void *ws, size_t ws_bytes,
+                           void *stream) {
+    if (!start && ntok > 0 && nseq > 0) {
+        if (int rc = host_need_device()) return rc;
+        return host_fail(ES_HIP_EINVAL, "null start");
+    }
+    return attention(kv, nseq, start, ntok, heads, type, q, qstride, scale, window, out, ostride, ws, ws_bytes, stream);
+}
+
+}  // extern "C"

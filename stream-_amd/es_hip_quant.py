@@ -21,6 +21,7 @@ Q4_0, Q5_0, Q8_0, Q2_K, Q3_K, Q4_K, Q5_K, Q6_K = 2, 6, 8, 10, 11, 12, 13, 14
 TYPES = {"Q4_0": Q4_0, "Q5_0": Q5_0, "Q8_0": Q8_0, "Q2_K": Q2_K, "Q3_K": Q3_K, "Q4_K": Q4_K, "Q5_K": Q5_K, "Q6_K": Q6_K}
 ORDER_X86_CONTRACT, ORDER_X86_STRICT, ORDER_SCALAR = 0, 1, 2
 NOALLOC_SCRATCH_BYTES = 32 << 20   # ES_HIP_NOALLOC_SCRATCH_BYTES
+F32, F16, BF16 = 0, 1, 30          # the key-value cache's and its attention's types
 BLOCK_ELEMS = {Q4_0: 32, Q5_0: 32, Q8_0: 32, Q2_K: 256, Q3_K: 256, Q4_K: 256, Q5_K: 256, Q6_K: 256}
 BLOCK_BYTES = {Q4_0: 18, Q5_0: 22, Q8_0: 34, Q2_K: 84, Q3_K: 110, Q4_K: 144, Q5_K: 176, Q6_K: 210}
 ACT_BYTES = {Q4_0: 36, Q5_0: 36, Q8_0: 36, Q2_K: 292, Q3_K: 292, Q4_K: 292, Q5_K: 292, Q6_K: 292}
@@ -35,6 +36,12 @@ class EsHipError(RuntimeError):
 class Job(C.Structure):   # es_hip_job
     _fields_ = [("type", C.c_uint32), ("rows", C.c_int), ("cols", C.c_int), ("W", C.c_void_p), ("act", C.c_void_p),
                 ("astride", C.c_size_t), ("nb", C.c_int), ("y", C.c_void_p), ("ystride", C.c_size_t)]
+
+
+class Kv(C.Structure):   # es_hip_kv
+    _fields_ = [("type", C.c_uint32), ("heads", C.c_int), ("dim", C.c_int), ("page", C.c_int), ("npages", C.c_int),
+                ("k", C.c_void_p), ("v", C.c_void_p), ("table", C.c_void_p), ("len", C.c_void_p), ("seq", C.c_void_p),
+                ("rows", C.c_int), ("max_pages", C.c_int)]
 
 
 class Moe(C.Structure):   # es_hip_moe
@@ -212,6 +219,64 @@ class ExpertCache:
         return res, slots, stats
 
 
+class KvPool:
+    """es_hip_kv_pool: sequences and pages of a paged key-value cache (nlayers = 0: bookkeeping only)"""
+
+    def __init__(self, lib, t, nlayers, heads, dim, page, npages, max_seqs, max_pages):
+        self.lib, self.h = lib, None
+        h = C.c_void_p()
+        lib._check(lib._L.es_hip_kv_pool_create(C.byref(h), t, nlayers, heads, dim, page, npages, max_seqs, max_pages))
+        self.h = h.value
+
+    def close(self):
+        if self.h:
+            self.lib._L.es_hip_kv_pool_destroy(self.h)
+            self.h = None
+
+    def __del__(self):
+        self.close()
+
+    def view(self, layer, seq=None) -> Kv:
+        """the layer's Kv; seq: a device list of a batch's sequence numbers"""
+        kv = Kv()
+        self.lib._check(self.lib._L.es_hip_kv_pool_view(self.h, layer, C.byref(kv)))
+        kv.seq = None if seq is None else int(seq)
+        return kv
+
+    def free_pages(self):
+        return self.lib._check(self.lib._L.es_hip_kv_pool_free_pages(self.h))
+
+    def create(self, stream=None):
+        return self.lib._check(self.lib._L.es_hip_kv_seq_create(self.h, stream))
+
+    def extend(self, seqs, n, stream=None):
+        s, n = np.ascontiguousarray(seqs, np.int32), np.ascontiguousarray(n, np.int32)
+        if s.shape != n.shape:
+            raise ValueError("seqs and n have different lengths")
+        self.lib._check(self.lib._L.es_hip_kv_seq_extend(self.h, s.ctypes.data, n.ctypes.data, s.size, stream))
+
+    def fork(self, seq, stream=None):
+        return self.lib._check(self.lib._L.es_hip_kv_seq_fork(self.h, seq, stream))
+
+    def truncate(self, seq, n, stream=None):
+        self.lib._check(self.lib._L.es_hip_kv_seq_truncate(self.h, seq, n, stream))
+
+    def free(self, seq, stream=None):
+        self.lib._check(self.lib._L.es_hip_kv_seq_free(self.h, seq, stream))
+
+    def len(self, seq):
+        return self.lib._check(self.lib._L.es_hip_kv_seq_len(self.h, seq))
+
+    def pages(self, seq):
+        n = self.lib._check(self.lib._L.es_hip_kv_seq_pages(self.h, seq, None, 0))
+        out = np.zeros(n, np.int32)
+        self.lib._check(self.lib._L.es_hip_kv_seq_pages(self.h, seq, out.ctypes.data, n))
+        return out.tolist()
+
+    def compact(self, stream=None):
+        return self.lib._check(self.lib._L.es_hip_kv_pool_compact(self.h, stream))
+
+
 class Lib:
     def __init__(self, path: str | None = None):
         path = path or LIB_PATH
@@ -263,6 +328,17 @@ class Lib:
             ("es_hip_cache_find", i, [vp, i, i]), ("es_hip_cache_claim", i, [vp, i, i]),
             ("es_hip_cache_slot_ptr", vp, [vp, i]), ("es_hip_cache_load", i, [vp, i, sz, vp, sz, vp]),
             ("es_hip_cache_wait", i, [vp, i]), ("es_hip_cache_step", i, [vp]),
+            ("es_hip_kv_append_dev", i, [vp, i, vp, i, u32, vp, sz, vp, sz, vp]),
+            ("es_hip_attn_decode_workspace", sz, [vp, i, i]), ("es_hip_attn_prompt_workspace", sz, [vp, i, i, i, u32]),
+            ("es_hip_attn_decode_dev", i, [vp, i, i, u32, vp, sz, C.c_float, i, vp, sz, vp, sz, vp]),
+            ("es_hip_attn_prompt_dev", i, [vp, i, vp, i, i, u32, vp, sz, C.c_float, i, vp, sz, vp, sz, vp]),
+            ("es_hip_kv_copy_pages_dev", i, [vp, i, sz, vp, vp, i, vp]),
+            ("es_hip_kv_pool_create", i, [vp, u32, i, i, i, i, i, i, i]), ("es_hip_kv_pool_destroy", None, [vp]),
+            ("es_hip_kv_pool_view", i, [vp, i, vp]), ("es_hip_kv_pool_free_pages", i, [vp]),
+            ("es_hip_kv_pool_compact", i, [vp, vp]), ("es_hip_kv_seq_create", i, [vp, vp]),
+            ("es_hip_kv_seq_extend", i, [vp, vp, vp, i, vp]), ("es_hip_kv_seq_fork", i, [vp, i, vp]),
+            ("es_hip_kv_seq_truncate", i, [vp, i, i, vp]), ("es_hip_kv_seq_free", i, [vp, i, vp]),
+            ("es_hip_kv_seq_len", i, [vp, i]), ("es_hip_kv_seq_pages", i, [vp, i, vp, i]),
             ("es_hip_cache_acquire", i, [vp, i, vp, i, vp, vp, vp]), ("es_hip_cache_prefetch", i, [vp, i, i, vp, vp, vp]),
             ("es_hip_cache_slot_info", i, [vp, i, vp]), ("es_hip_cache_get_stats", i, [vp, vp]),
         ]:
@@ -473,6 +549,33 @@ class Lib:
     def route_softmax_dev(self, logits, lstride, ntok, n_exp, k, norm_topk, sel, w, kmax, stream=None):
         self._check(self._L.es_hip_route_softmax_dev(int(logits), lstride, ntok, n_exp, k, int(norm_topk), int(sel), int(w),
                                                      kmax, stream))
+
+    # ---- paged key-value cache and attention (kv: a Kv; device pointers as DevBuf / ints) ----
+    def kv_append_dev(self, kv, nseq, start, ntok, src_type, k, kstride, v, vstride, stream=None):
+        """start None: one token per sequence"""
+        self._check(self._L.es_hip_kv_append_dev(C.byref(kv), nseq, self._ptr(start), ntok, src_type, self._ptr(k), kstride,
+                                                 self._ptr(v), vstride, stream))
+
+    def attn_decode_workspace(self, kv, nseq, heads) -> int:
+        return self._L.es_hip_attn_decode_workspace(C.byref(kv), nseq, heads)
+
+    def attn_prompt_workspace(self, kv, nseq, ntok, heads, t) -> int:
+        return self._L.es_hip_attn_prompt_workspace(C.byref(kv), nseq, ntok, heads, t)
+
+    def attn_decode_dev(self, kv, nseq, heads, t, q, qstride, scale, window, out, ostride, ws, ws_bytes, stream=None):
+        self._check(self._L.es_hip_attn_decode_dev(C.byref(kv), nseq, heads, t, self._ptr(q), qstride, scale, window,
+                                                   self._ptr(out), ostride, self._ptr(ws), ws_bytes, stream))
+
+    def attn_prompt_dev(self, kv, nseq, start, ntok, heads, t, q, qstride, scale, window, out, ostride, ws, ws_bytes, stream=None):
+        self._check(self._L.es_hip_attn_prompt_dev(C.byref(kv), nseq, self._ptr(start), ntok, heads, t, self._ptr(q), qstride,
+                                                   scale, window, self._ptr(out), ostride, self._ptr(ws), ws_bytes, stream))
+
+    def kv_copy_pages_dev(self, kv, nlayers, layer_bytes, src, dst, stream=None):
+        """src, dst: page numbers on the host"""
+        if len(src) != len(dst):
+            raise ValueError("src and dst have different lengths")
+        s, d = np.ascontiguousarray(src, np.int32), np.ascontiguousarray(dst, np.int32)
+        self._check(self._L.es_hip_kv_copy_pages_dev(C.byref(kv), nlayers, layer_bytes, s.ctypes.data, d.ctypes.data, len(s), stream))
 
     # ---- activation preparation on the device (device pointers as DevBuf / ints; None for an output not wanted) ----
     @staticmethod
