@@ -422,19 +422,24 @@ template <bool BF, int NQ, int DP> __global__ __launch_bounds__(256) void attn_d
 
 // ---- a tile of prompt rows -------------------------------------------------------------------------------------------------------
 // A workgroup of four waves takes 128 rows, 32 a wave, against its keys, 64 at a time through LDS: K as it is, V turned to [element][key]
-// on its way from registers, its keys in the order in which the lanes hold the weights. The next keys' loads run under the
-// products. Keys that a row does not see have weight 0; V rows that no row sees are staged as zeros, and a V row with an infinity or NaN that
-// only some rows see is kept out of the product and added to those alone (0 times infinity is not 0).
+// on its way from registers, its keys in the order in which the lanes hold the weights. The keys after next are on their way into registers
+// and the next are in the other half of LDS while these are multiplied.
+// V's element d is row (d % VE) * 16 + d / VE of its LDS tile and of O^T, VE = DP / 16: the 16 threads that hold a key's elements then write
+// consecutive rows, whose pitch of 36 words spreads them over the banks (and the eight lanes of a read), and a lane ends with runs of VE elements.
+// Keys that a row does not see have weight 0, and 0 times an infinity or NaN is not 0: V rows that no row sees are staged as zeros, and
+// so are such elements of keys that only some rows see; where there were any, they are added to those rows at the end.
 constexpr int PM = 128, PN = 64;
 
-template <bool BF, int NQ, int DP> __global__ __launch_bounds__(256) void attn_prompt_kernel(AttnArgs a) {
+template <bool BF, int NQ, int DP> __global__ __launch_bounds__(256, DP == 256 || NQ == 3 ? 1 : 2) void attn_prompt_kernel(AttnArgs a) {
     constexpr int KS = DP / 16, DT = DP / 32, KC = DP / 8;
-    constexpr int KP = DP + 8, VP = PN + 8;   // LDS pitches, elements
-    constexpr int NK = PN * KC / 256, NV = (PN / 4 * KC + 255) / 256;
+    constexpr int KP = DP + 8;            // LDS pitch of K, elements
+    constexpr int NK = PN * KC / 256;     // 16-byte pieces of K per thread
+    constexpr int VE = DP / 16;           // elements of V per thread, of 4 keys
     constexpr bool F32 = NQ > 1;
-    __shared__ __attribute__((aligned(16))) uint16_t lk[PN * KP], lv[DP * VP];
-    __shared__ uint32_t odd[2][2];   // keys whose V row is not finite, by step
-    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    constexpr int VP = PN + 8;            // and of V
+    __shared__ __attribute__((aligned(16))) uint16_t lk[2][PN * KP], lv[2][DP * VP];
+    __shared__ int odd;                   // elements of V were left out
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int col = lane & 31, half = lane >> 5;
     const int head = blockIdx.x % a.c.heads, item = blockIdx.x / a.c.heads;
     const int chunk = chunk_of(a, PM);
@@ -446,18 +451,21 @@ template <bool BF, int NQ, int DP> __global__ __launch_bounds__(256) void attn_p
     const int back = p.s.len - p.s.n;          // query i stands at back + i
     const int pos_lo = back + tile * PM / a.G, pos_hi = back + (tile * PM + rows - 1) / a.G;
     const int see_lo = a.window ? max(0, pos_lo - a.window + 1) : 0, see_hi = pos_hi + 1;   // keys that some row sees
-    int first = p.s.base + (whole ? 0 : p.chunk * chunk), last = whole ? see_hi : min(see_hi, first + chunk);
+    int first = p.s.base + (whole ? 0 : p.chunk * chunk);
+    const int last = whole ? see_hi : min(see_hi, first + chunk);
     first = max(first, see_lo & ~(PN - 1));
     const int shift16 = a.c.shift - 4;
     const int *table = a.c.table + (size_t)max(a.c.row(p.b), 0) * a.c.max_pages;
-    const size_t pagestep = (size_t)a.c.heads << a.c.shift;
+    const int dim = a.c.dim;
+    const bool padded = dim < DP;
 
     const int r = min(tile * PM + wave * 32 + col, tile * PM + rows - 1);   // lanes past the last row repeat it
     const int query = r / a.G, pos = back + query, from = a.window ? pos - a.window + 1 : 0;
-    const size_t qoff = (size_t)(head * a.G + r - query * a.G) * a.c.dim * (F32 ? 4 : 2);
+    const size_t qoff = (size_t)(head * a.G + r - query * a.G) * dim * (F32 ? 4 : 2);
     u4 q[KS][NQ];
-    const float cs = load_query<BF, NQ, KS, 16, 32>(a.q + (size_t)(p.s.t0 + query) * a.qstride + qoff, true, half, a.c.dim, a.c2, q);
+    const float cs = load_query<BF, NQ, KS, 16, 32>(a.q + (size_t)(p.s.t0 + query) * a.qstride + qoff, true, half, dim, a.c2, q);
     const int wpos_lo = __builtin_amdgcn_readlane(pos, 0), wpos_hi = __builtin_amdgcn_readlane(pos, 31);
+    const int from_hi = a.window ? pos_hi - a.window + 1 : 0, wfrom_hi = a.window ? wpos_hi - a.window + 1 : 0;
     const bool idle = wave * 32 >= rows;
 
     f16v acc[DT];
@@ -467,204 +475,229 @@ template <bool BF, int NQ, int DP> __global__ __launch_bounds__(256) void attn_p
         for (int i = 0; i < 16; i++) acc[j][i] = 0.0f;
     float m = LOWEST, l = 0.0f;
 
-    u4 kr[NK], vr[NV][4];
-    // page of 16 keys u * 16.., or -1
-    auto page_of = [&](int u) {
+    // the pages of 64 runs of 16 keys from run `pb` on, one per lane (-1: none), and of the 64 after them
+    auto fetch = [&](int u) {
         const int g = u * 16 < last ? table[u >> shift16] : -1;
         return g < a.c.npages ? g : -1;
     };
-    auto row_at = [&](int page, int t) {
-        return ((size_t)max(page, 0) * pagestep + ((size_t)head << a.c.shift) + (t & ((1 << a.c.shift) - 1))) * a.c.dim * 2;
-    };
+    int pb = first >> 4, pg = fetch(pb + lane), pgn = fetch(pb + 64 + lane);
+
+    u4 kr[NK];
+    uint32_t vr[4][VE / 2];
+    const int kt = tid / KC, kd = min(tid % KC * 8, dim - 8);   // this thread's first piece of K: token (of 64) and element
+    const int vt = tid / 16 * 4, vd = tid % 16 * VE;            // its 4 keys of V and their elements
+    const uint32_t rowb = (uint32_t)dim * 2;
+    const uint32_t k_off = (kt & 15) * rowb + kd * 2, v_off = (vt & 15) * rowb;
+    // loads the keys from t0 on into registers; which of their four runs are in no page
     auto load = [&](int t0) {
+        int u0 = (t0 >> 4) - pb;
+        if (u0 >= 64) {
+            pb += 64;
+            u0 -= 64;
+            pg = pgn;
+            pgn = fetch(pb + 64 + lane);
+        }
+        int holes = 0;
+        auto run = [&](int sub) {   // bytes from the pool's start to a run's rows; one that is in no page: page 0 in its place
+            const int page = __builtin_amdgcn_readlane(pg, u0 + sub);
+            const int token = ((t0 >> 4) + sub & ((1 << shift16) - 1)) << 4;
+            return a.c.at(max(page, 0), head, token);
+        };
 #pragma unroll
-        for (int i = 0; i < NK; i++) {
-            const int c = tid + i * 256, t = t0 + c / KC, d = c % KC * 8;
-            const int page = page_of(t >> 4);
-            kr[i] = page >= 0 && d < a.c.dim ? *reinterpret_cast<const u4 *>(a.c.k + row_at(page, t) + d * 2) : u4{0, 0, 0, 0};
+        for (int u = 0; u < 4; u++) holes |= __builtin_amdgcn_readlane(pg, u0 + u) < 0 ? 1 << u : 0;
+#pragma unroll
+        for (int i = 0; i < NK; i++)   // pieces i: tokens kt + i * (256 / KC)
+            kr[i] = *reinterpret_cast<const u4 *>(a.c.k + run(KC == 8 ? (wave >> 1) + 2 * i : KC == 16 ? i : i >> 1) +
+                                                  k_off + (KC == 32 ? (i & 1) * 8 * rowb : 0));
+        const uint8_t *vp = a.c.v + run(wave) + v_off;
+#pragma unroll
+        for (int k = 0; k < 4; k++) {   // (elements past dim: others' in their place, in rows of O^T that are not written)
+            if constexpr (VE == 4) {
+                const u2 x = *reinterpret_cast<const u2 *>(vp + k * rowb + min(vd, dim - 4) * 2);
+                vr[k][0] = x[0];
+                vr[k][1] = x[1];
+            } else {
+#pragma unroll
+                for (int w = 0; w < VE / 2; w += 4) {
+                    const u4 x = *reinterpret_cast<const u4 *>(vp + k * rowb + min(vd + w * 2, dim - 8) * 2);
+#pragma unroll
+                    for (int n = 0; n < 4; n++) vr[k][w + n] = x[n];
+                }
+            }
+        }
+        return holes;
+    };
+    // registers to LDS: the keys from t0 on, loaded last
+    auto stage = [&](int t0, int buf, int holes) {
+        if (padded && tid % KC * 8 >= dim) {   // elements past dim: zeros, which the query's zeros keep
+#pragma unroll
+            for (int i = 0; i < NK; i++) kr[i] = u4{0, 0, 0, 0};
         }
 #pragma unroll
-        for (int i = 0; i < NV; i++) {
-            const int c = tid + i * 256, t = t0 + c / KC * 4, d = c % KC * 8;
-            const int page = c < PN / 4 * KC ? page_of(t >> 4) : -1;
+        for (int i = 0; i < NK; i++)
+            *reinterpret_cast<u4 *>(&lk[buf][(kt + i * (256 / KC)) * KP + tid % KC * 8]) = kr[i];
+        if (t0 < see_lo || t0 + PN > last || holes) {
 #pragma unroll
             for (int k = 0; k < 4; k++)
-                vr[i][k] = page >= 0 && d < a.c.dim && t + k >= see_lo && t + k < last
-                               ? *reinterpret_cast<const u4 *>(a.c.v + row_at(page, t + k) + d * 2) : u4{0, 0, 0, 0};
+                if (t0 + vt + k < see_lo || t0 + vt + k >= last || (holes >> wave & 1)) {
+#pragma unroll
+                    for (int w = 0; w < VE / 2; w++) vr[k][w] = 0;
+                }
+        }
+        if (t0 + PN > pos_lo + 1 || t0 < from_hi) {   // some row does not see all of them
+            constexpr uint32_t E = BF ? 0x7f80u : 0x7c00u;   // an exponent of ones
+            bool left = false;
+#pragma unroll
+            for (int k = 0; k < 4; k++)
+#pragma unroll
+                for (int w = 0; w < VE / 2; w++) {
+                    const uint32_t x = vr[k][w], bad = ((x & E) == E ? 0xffffu : 0) | ((x >> 16 & E) == E ? 0xffff0000u : 0);
+                    vr[k][w] = x & ~bad;
+                    left |= bad != 0;
+                }
+            if (left) odd = 1;
+        }
+        const int at = wave * 16 + (vt >> 2 & 1) * 8 + (vt >> 3 & 1) * 4;   // keys vt..vt+3 as the weights lie
+#pragma unroll
+        for (int e = 0; e < VE; e += 2) {
+            const int w = e / 2;
+            const u2 x = {pair<0>(vr[0][w], vr[1][w]), pair<0>(vr[2][w], vr[3][w])};
+            const u2 y = {pair<1>(vr[0][w], vr[1][w]), pair<1>(vr[2][w], vr[3][w])};
+            *reinterpret_cast<u2 *>(&lv[buf][(e * 16 + tid % 16) * VP + at]) = x;
+            *reinterpret_cast<u2 *>(&lv[buf][(e * 16 + 16 + tid % 16) * VP + at]) = y;
         }
     };
-    if (tid < 4) odd[tid >> 1][tid & 1] = 0;
-    if (first < last) load(first);
-    int step = 0;
-    for (int t0 = first; t0 < last; t0 += PN, step ^= 1) {
-        __syncthreads();
-        const bool edge = t0 + PN > pos_lo + 1 || t0 < (a.window ? pos_hi - a.window + 1 : 0);   // some row does not see all keys
-#pragma unroll
-        for (int i = 0; i < NK; i++) {
-            const int c = tid + i * 256;
-            *reinterpret_cast<u4 *>(&lk[c / KC * KP + c % KC * 8]) = kr[i];
-        }
-#pragma unroll
-        for (int i = 0; i < NV; i++) {
-            const int c = tid + i * 256;
-            if (c < PN / 4 * KC) {
-                const int t = c / KC * 4, d = c % KC * 8;
-                const int at = (t & ~15) + (t & 4 ? 8 : 0) + (t & 8 ? 4 : 0);   // keys t..t+3 among the 64 as the weights lie
-#pragma unroll
-                for (int k = 0; k < 4; k++) {
-                    u2 x = {pair<0>(vr[i][0][k], vr[i][1][k]), pair<0>(vr[i][2][k], vr[i][3][k])};
-                    u2 y = {pair<1>(vr[i][0][k], vr[i][1][k]), pair<1>(vr[i][2][k], vr[i][3][k])};
-                    *reinterpret_cast<u2 *>(&lv[(d + 2 * k) * VP + at]) = x;
-                    *reinterpret_cast<u2 *>(&lv[(d + 2 * k + 1) * VP + at]) = y;
-                }
-                if (edge) {
-                    constexpr uint32_t E = BF ? 0x7f80u : 0x7c00u;   // an exponent of ones
-#pragma unroll
-                    for (int k = 0; k < 4; k++) {
-                        bool bad = false;
-#pragma unroll
-                        for (int w = 0; w < 4; w++)
-                            bad |= (vr[i][k][w] & E) == E || (vr[i][k][w] >> 16 & E) == E;
-                        if (bad) atomicOr(&odd[step][t >> 5], 1u << ((t + k) & 31));
-                    }
-                }
-            }
-        }
-        __syncthreads();
-        if (t0 + PN < last) load(t0 + PN);
-        if (tid < 2) odd[step ^ 1][tid] = 0;
-        if (idle || t0 > wpos_hi || (a.window && t0 + PN <= wpos_lo - a.window + 1)) continue;
-        int holes = 0;
-#pragma unroll
-        for (int u = 0; u < PN / 16; u++) holes |= page_of((t0 >> 4) + u) < 0 ? 1 << u : 0;
-
-        f16v s[2];
-#pragma unroll
-        for (int h = 0; h < 2; h++)
-#pragma unroll
-            for (int i = 0; i < 16; i++) s[h][i] = 0.0f;
-#pragma unroll
-        for (int k = 0; k < KS; k++)
-#pragma unroll
-            for (int h = 0; h < 2; h++) {
-                const u4 kf = *reinterpret_cast<const u4 *>(&lk[(h * 32 + col) * KP + k * 16 + half * 8]);
-#pragma unroll
-                for (int t = 0; t < NQ; t++) s[h] = mfma32<BF>(kf, q[k][t], s[h]);
-            }
-        if (t0 + PN > wpos_lo + 1 || holes || (a.window && t0 < wpos_hi - a.window + 1)) {
+    if (tid == 0) odd = 0;
+    __syncthreads();
+    int holes = 0, next = 0;
+    if (first < last) {
+        holes = load(first);
+        stage(first, 0, holes);
+        if (first + PN < last) next = load(first + PN);
+    }
+    __syncthreads();
+    int buf = 0;
+    for (int t0 = first; t0 < last; t0 += PN) {
+        if (!(idle || t0 > wpos_hi || (a.window && t0 + PN <= wpos_lo - a.window + 1))) {
+            f16v s[2];
 #pragma unroll
             for (int h = 0; h < 2; h++)
 #pragma unroll
-                for (int i = 0; i < 16; i++) {
-                    const int t = t0 + h * 32 + i / 4 * 8 + half * 4 + (i & 3);
-                    if (t > pos || t < from || t >= last || (holes >> (h * 2 + i / 8) & 1)) s[h][i] = LOWEST;
+                for (int i = 0; i < 16; i++) s[h][i] = 0.0f;
+#pragma unroll
+            for (int k = 0; k < KS; k++)
+#pragma unroll
+                for (int h = 0; h < 2; h++) {
+                    const u4 kf = *reinterpret_cast<const u4 *>(&lk[buf][(h * 32 + col) * KP + k * 16 + half * 8]);
+#pragma unroll
+                    for (int t = 0; t < NQ; t++) s[h] = mfma32<BF>(kf, q[k][t], s[h]);
                 }
-        }
-        float big = LOWEST;
+            if (t0 + PN > wpos_lo + 1 || t0 < wfrom_hi) {
+                const int to = pos - t0 - half * 4, since = from - t0 - half * 4;
 #pragma unroll
-        for (int h = 0; h < 2; h++)
+                for (int h = 0; h < 2; h++)
 #pragma unroll
-            for (int i = 0; i < 16; i++) big = fmaxf(big, s[h][i]);
-        big = fmaxf(big, __shfl_xor(big, 32)) * cs;
-        if (__any(big > m)) {
-            const float now = fmaxf(m, big), f = __builtin_amdgcn_exp2f(m - reference(now));
-            m = now;
-            l *= f;
-#pragma unroll
-            for (int j = 0; j < DT; j++)
-#pragma unroll
-                for (int i = 0; i < 16; i++) acc[j][i] *= f;
-        }
-        const float ref = SHIFT<BF> - reference(m);
-        u4 pt[4][NQ];
-#pragma unroll
-        for (int u = 0; u < 4; u++) {
-            float w8[8];
-#pragma unroll
-            for (int i = 0; i < 8; i++) {
-                w8[i] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[u >> 1][(u & 1) * 8 + i], cs, ref));
-                l += w8[i];
+                    for (int i = 0; i < 16; i++) {
+                        const int t = h * 32 + i / 4 * 8 + (i & 3);
+                        if (t > to || t < since) s[h][i] = LOWEST;
+                    }
             }
-            split<BF, NQ>(w8, pt[u]);
-        }
-        const uint32_t odd0 = edge ? odd[step][0] : 0, odd1 = edge ? odd[step][1] : 0;
-        if (!__builtin_amdgcn_readfirstlane(odd0 | odd1)) {
+            if (holes) {
 #pragma unroll
-            for (int u = 0; u < 4; u++)
+                for (int h = 0; h < 2; h++)
 #pragma unroll
-                for (int j = 0; j < DT; j++) {
-                    const u4 vf = *reinterpret_cast<const u4 *>(&lv[(j * 32 + col) * VP + u * 16 + half * 8]);
+                    for (int i = 0; i < 16; i++)
+                        if (holes >> (h * 2 + i / 8) & 1) s[h][i] = LOWEST;
+            }
+            float big = LOWEST;
 #pragma unroll
-                    for (int t = 0; t < NQ; t++) acc[j] = mfma32<BF>(vf, pt[u][t], acc[j]);
-                }
-        } else {
-            // the lane's keys of step u: u * 16 + half * 4 + {0..3, 8..11}
-            auto only = [&](u4 v, uint32_t keys, int u) {   // V with the keys that are not in the mask (of 32) as zeros
-                const uint32_t k = keys >> ((u & 1) * 16 + half * 4);
+            for (int h = 0; h < 2; h++)
 #pragma unroll
-                for (int w = 0; w < 4; w++) {
-                    const int b = (w >> 1) * 8 + (w & 1) * 2;
-                    v[w] &= (k >> b & 1 ? 0xffffu : 0) | (k >> (b + 1) & 1 ? 0xffff0000u : 0);
-                }
-                return v;
-            };
+                for (int i = 0; i < 16; i++) big = fmaxf(big, s[h][i]);
+            big = fmaxf(big, __shfl_xor(big, 32)) * cs;
+            if (__any(big > m)) {
+                const float now = fmaxf(m, big), f = __builtin_amdgcn_exp2f(m - reference(now));
+                m = now;
+                l *= f;
 #pragma unroll
-            for (int u = 0; u < 4; u++)
+                for (int j = 0; j < DT; j++)
 #pragma unroll
-                for (int j = 0; j < DT; j++) {
-                    const u4 vf = only(*reinterpret_cast<const u4 *>(&lv[(j * 32 + col) * VP + u * 16 + half * 8]), ~(u < 2 ? odd0 : odd1), u);
-#pragma unroll
-                    for (int t = 0; t < NQ; t++) acc[j] = mfma32<BF>(vf, pt[u][t], acc[j]);
-                }
+                    for (int i = 0; i < 16; i++) acc[j][i] *= f;
+            }
+            const float ref = SHIFT<BF> - reference(m);
+            u4 pt[4][NQ];
 #pragma unroll
             for (int u = 0; u < 4; u++) {
-                uint32_t keys = __builtin_amdgcn_readfirstlane((u < 2 ? odd0 : odd1) & 0xffffu << (u & 1) * 16);
-                while (keys) {
-                    const int b = __builtin_ctz(keys);
-                    keys &= keys - 1;
-                    const int t = t0 + (u >> 1) * 32 + b;
-                    const bool seen = t <= pos && t >= from;
+                float w8[8];
 #pragma unroll
-                    for (int j = 0; j < DT; j++) {
-                        const u4 vf = only(*reinterpret_cast<const u4 *>(&lv[(j * 32 + col) * VP + u * 16 + half * 8]), 1u << b, u);
-                        f16v x;
-#pragma unroll
-                        for (int i = 0; i < 16; i++) x[i] = 0.0f;
-#pragma unroll
-                        for (int n = 0; n < NQ; n++) x = mfma32<BF>(vf, pt[u][n], x);
-#pragma unroll
-                        for (int i = 0; i < 16; i++) acc[j][i] = seen ? acc[j][i] + x[i] : acc[j][i];
-                    }
+                for (int i = 0; i < 8; i++) {
+                    w8[i] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[u >> 1][(u & 1) * 8 + i], cs, ref));
+                    l += w8[i];
                 }
+                split<BF, NQ>(w8, pt[u]);
             }
+#pragma unroll
+            for (int u = 0; u < 4; u++)
+#pragma unroll
+                for (int j = 0; j < DT; j++) {
+                    const u4 vf = *reinterpret_cast<const u4 *>(&lv[buf][(j * 32 + col) * VP + u * 16 + half * 8]);
+#pragma unroll
+                    for (int t = 0; t < NQ; t++) acc[j] = mfma32<BF>(vf, pt[u][t], acc[j]);
+                }
         }
+        holes = next;
+        if (t0 + PN < last) {
+            stage(t0 + PN, buf ^ 1, next);
+            if (t0 + 2 * PN < last) next = load(t0 + 2 * PN);
+        }
+        buf ^= 1;
+        __syncthreads();
     }
     l += __shfl_xor(l, 32);
 
     if (wave * 32 + col >= rows) return;
-    if (p.chunks == 1) {
-        uint8_t *row = a.out + (size_t)(p.s.t0 + query) * a.ostride + qoff;
-        const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+    // acc[j][i] is row j * 32 + i / 4 * 8 + half * 4 + i % 4 of O^T: element c * VE + j * 2 + i / 8, c = i / 4 % 2 * 8 + half * 4 + i % 4
+    if (odd) {   // what was left out, for the keys of the steps that were looked through (an infinity or NaN, whatever its weight)
+        for (int t = max(first, see_lo); t < last; t++) {
+            const int t0 = t & ~(PN - 1);
+            if (!(t0 + PN > pos_lo + 1 || t0 < from_hi) || t > pos || t < from) continue;
+            const int page = table[t >> a.c.shift];
+            if (page < 0 || page >= a.c.npages) continue;
+            const uint8_t *row = a.c.v + a.c.at(page, head, t & ((1 << a.c.shift) - 1));
 #pragma unroll
-        for (int j = 0; j < DT; j++)
+            for (int i = 0; i < 8; i++) {
+                const int c = i / 4 * 8 + half * 4 + (i & 3);
+                if (c * VE >= dim) continue;
 #pragma unroll
-            for (int i = 0; i < 16; i += 4) {
-                const int d = j * 32 + i * 2 + half * 4;
-                float x[4];
-#pragma unroll
-                for (int k = 0; k < 4; k++) x[k] = l == 0.0f ? 0.0f : acc[j][i + k] * inv;
-                if (d < a.c.dim) store4<F32, BF>(row, d, x);
+                for (int e = 0; e < VE; e++) {
+                    using T = std::conditional_t<BF, __bf16, _Float16>;
+                    const float v = c * VE + e < dim ? static_cast<float>(*reinterpret_cast<const T *>(row + (c * VE + e) * 2)) : 0.0f;
+                    if (!(fabsf(v) < INFINITY)) acc[e / 2][e % 2 * 8 + i] += v;
+                }
             }
-    } else {
-        const size_t at = ((size_t)item * a.c.heads + head) * PM + wave * 32 + col;
-        if (half == 0) a.pml[at] = float2{m, l};
+        }
+    }
+    const bool done = p.chunks == 1;
+    const size_t at = ((size_t)item * a.c.heads + head) * PM + wave * 32 + col;
+    const float inv = !done ? 1.0f : l == 0.0f ? 0.0f : 1.0f / l;
+    if (!done && half == 0) a.pml[at] = float2{m, l};
+    uint8_t *row = a.out + (size_t)(p.s.t0 + query) * a.ostride + qoff;
 #pragma unroll
-        for (int j = 0; j < DT; j++)
+    for (int i = 0; i < 8; i++) {
+        const int c = i / 4 * 8 + half * 4 + (i & 3);
 #pragma unroll
-            for (int i = 0; i < 16; i += 4) {
-                const int d = j * 32 + i * 2 + half * 4;
-                if (d < a.c.dim) *reinterpret_cast<f4 *>(a.po + at * a.c.dim + d) = f4{acc[j][i], acc[j][i + 1], acc[j][i + 2], acc[j][i + 3]};
+        for (int e = 0; e < VE; e += 4) {
+            const int d = c * VE + e;
+            float x[4];
+#pragma unroll
+            for (int k = 0; k < 4; k++) {
+                x[k] = acc[(e + k) / 2][(e + k) % 2 * 8 + i] * inv;
+                if (done && l == 0.0f) x[k] = 0.0f;
             }
+            if (d >= dim) continue;
+            if (done) store4<F32, BF>(row, d, x);
+            else *reinterpret_cast<f4 *>(a.po + at * dim + d) = f4{x[0], x[1], x[2], x[3]};
+        }
     }
 }
 
