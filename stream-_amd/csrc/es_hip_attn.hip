@@ -66,73 +66,82 @@ constexpr int CHUNK_MIN = 128;   // keys
 
 __device__ int chunk_of(const AttnArgs &a, int bm) {
     if (!a.target) return 1 << 30;
-    const int lane = threadIdx.x & 63;
     unsigned long long all = 0;
-    for (int b = lane; b < a.nseq; b += 64) {
-        const Seq s = seq_of(a, b, bm);
-        all += (unsigned long long)s.tiles * (unsigned)(s.len - s.base);
-    }
+    if (a.nseq == 1) {
+        const Seq s = seq_of(a, 0, bm);
+        all = (unsigned long long)s.tiles * (unsigned)(s.len - s.base);
+    } else {
+        for (int b = threadIdx.x & 63; b < a.nseq; b += 64) {
+            const Seq s = seq_of(a, b, bm);
+            all += (unsigned long long)s.tiles * (unsigned)(s.len - s.base);
+        }
 #pragma unroll
-    for (int d = 32; d; d >>= 1) all += __shfl_xor(all, d);
+        for (int d = 32; d; d >>= 1) all += __shfl_xor(all, d);
+    }
     const unsigned long long per = (all + a.target - 1) / a.target;
     const unsigned long long chunk = (per + CHUNK_MIN - 1) / CHUNK_MIN * CHUNK_MIN;
     return __builtin_amdgcn_readfirstlane((int)min(max(chunk, (unsigned long long)CHUNK_MIN), 1ull << 30));
 }
-__device__ int chunks_of(const Seq &s, int chunk) { return max(1, (int)(((long long)(s.len - s.base) + chunk - 1) / chunk)); }
+__device__ int chunks_of(const Seq &s, int chunk) { return max(1, (s.len - s.base + chunk - 1) / chunk); }
 
 struct Part {
     int b, tile, chunk, chunks;   // chunks: of the tile
+    uint32_t first;               // number of the sequence's first part
     Seq s;
 };
-// the part with number `item` (within one K/V head); false if there is none
-__device__ bool part_of(const AttnArgs &a, int item, int chunk, int bm, Part &p) {
+__device__ uint32_t sum_up_to(uint32_t x) {   // over the lanes up to this one
     const int lane = threadIdx.x & 63;
-    uint32_t before = 0;   // (starts that are out of order may give any number of parts: counted modulo 2^32)
-    for (int g = 0; g < a.nseq; g += 64) {
-        Seq s{};
-        int chunks = 1;
-        uint32_t mine = 0;
-        if (g + lane < a.nseq) {
-            s = seq_of(a, g + lane, bm);
-            chunks = chunks_of(s, chunk);
-            mine = (uint32_t)s.tiles * (uint32_t)chunks;
-        }
-        uint32_t upto = mine;
 #pragma unroll
-        for (int d = 1; d < 64; d <<= 1) {
-            const uint32_t o = __shfl_up(upto, d);
-            if (lane >= d) upto += o;
-        }
-        const unsigned long long past = __ballot((uint32_t)item < before + upto);
-        if (past) {
-            const int w = __builtin_ctzll(past);
-            p.b = g + w;
-            p.s.t0 = __builtin_amdgcn_readlane(s.t0, w);
-            p.s.n = __builtin_amdgcn_readlane(s.n, w);
-            p.s.len = __builtin_amdgcn_readlane(s.len, w);
-            p.s.base = __builtin_amdgcn_readlane(s.base, w);
-            p.s.tiles = __builtin_amdgcn_readlane(s.tiles, w);
-            p.chunks = __builtin_amdgcn_readlane(chunks, w);
-            const int i = (int)((uint32_t)item - before - (uint32_t)__builtin_amdgcn_readlane((int)(upto - mine), w));
-            p.tile = i / p.chunks;
-            p.chunk = i - p.tile * p.chunks;
-            return i >= 0 && p.tile < p.s.tiles;
-        }
-        before += (uint32_t)__builtin_amdgcn_readlane((int)upto, 63);
+    for (int d = 1; d < 64; d <<= 1) {
+        const uint32_t o = __shfl_up(x, d);
+        if (lane >= d) x += o;
     }
-    return false;
+    return x;
 }
-// the number of the first part of sequence b
-__device__ uint32_t parts_before(const AttnArgs &a, int b, int chunk, int bm) {
+// The part with number `item` (within one K/V head), or, TILES, the tile with that number and `chunk` 0; false if there is none. Starts that
+// are out of order may give any number of parts: they are counted modulo 2^32.
+template <bool TILES = false> __device__ bool part_of(const AttnArgs &a, int item, int chunk, int bm, Part &p) {
     const int lane = threadIdx.x & 63;
-    uint32_t n = 0;
-    for (int g = lane; g < b; g += 64) {
-        const Seq s = seq_of(a, g, bm);
-        n += (uint32_t)s.tiles * (uint32_t)chunks_of(s, chunk);
+    uint32_t tiles_before = 0, parts_before = 0;
+    if (a.nseq == 1) {
+        p.b = 0;
+        p.s = seq_of(a, 0, bm);
+        p.chunks = chunks_of(p.s, chunk);
+        p.first = 0;
+    } else {
+        for (int g = 0;; g += 64) {
+            if (g >= a.nseq) return false;
+            Seq s{};
+            int chunks = 1;
+            uint32_t parts = 0;
+            if (g + lane < a.nseq) {
+                s = seq_of(a, g + lane, bm);
+                chunks = chunks_of(s, chunk);
+                parts = (uint32_t)s.tiles * (uint32_t)chunks;
+            }
+            const uint32_t mine = TILES ? (uint32_t)s.tiles : parts, upto = sum_up_to(mine), parts_upto = TILES ? sum_up_to(parts) : upto;
+            uint32_t &before = TILES ? tiles_before : parts_before;
+            const unsigned long long past = __ballot((uint32_t)item < before + upto);
+            if (past) {
+                const int w = __builtin_ctzll(past);
+                p.b = g + w;
+                p.s.t0 = __builtin_amdgcn_readlane(s.t0, w);
+                p.s.n = __builtin_amdgcn_readlane(s.n, w);
+                p.s.len = __builtin_amdgcn_readlane(s.len, w);
+                p.s.base = __builtin_amdgcn_readlane(s.base, w);
+                p.s.tiles = __builtin_amdgcn_readlane(s.tiles, w);
+                p.chunks = __builtin_amdgcn_readlane(chunks, w);
+                p.first = parts_before + (uint32_t)__builtin_amdgcn_readlane((int)(parts_upto - parts), w);
+                item = (int)((uint32_t)item - before - (uint32_t)__builtin_amdgcn_readlane((int)(upto - mine), w));
+                break;
+            }
+            tiles_before += TILES ? (uint32_t)__builtin_amdgcn_readlane((int)upto, 63) : 0;
+            parts_before += (uint32_t)__builtin_amdgcn_readlane((int)parts_upto, 63);
+        }
     }
-#pragma unroll
-    for (int d = 32; d; d >>= 1) n += __shfl_xor(n, d);
-    return (uint32_t)__builtin_amdgcn_readfirstlane((int)n);
+    p.tile = TILES ? item : item / p.chunks;
+    p.chunk = TILES ? 0 : item - p.tile * p.chunks;
+    return item >= 0 && p.tile < p.s.tiles;
 }
 
 // ---- arithmetic --------------------------------------------------------------------------------------------------------------
@@ -702,73 +711,83 @@ template <bool BF, int NQ, int DP> __global__ __launch_bounds__(256, DP == 256 |
 }
 
 // ---- parts joined ------------------------------------------------------------------------------------------------------------
-// One workgroup per row (query, head): the parts' sums, each scaled by 2^(m of the part - the largest m), in the order of the parts.
-template <bool F32, bool BF, int BM> __global__ __launch_bounds__(256) void attn_join_kernel(AttnArgs a) {
-    const int heads = a.c.heads * a.G;
-    const int t = blockIdx.x / heads, hq = blockIdx.x % heads, head = hq / a.G;
-    int b = t;
-    if (a.start) {
-        int lo = 0, hi = a.nseq;
-        while (hi - lo > 1) {
-            const int mid = (lo + hi) >> 1;
-            if (a.start[mid] <= t) lo = mid; else hi = mid;
-        }
-        b = lo;
-    }
-    const Seq s = seq_of(a, b, BM);
-    if (t < s.t0 || t >= s.t0 + s.n) return;
-    const int chunk = chunk_of(a, BM), chunks = chunks_of(s, chunk);
-    if (chunks == 1) return;   // written already
-    const int r = (t - s.t0) * a.G + hq - head * a.G;
-    int tile = r / BM;
-    const int row = r - tile * BM;
-    if (a.start) tile = s.tiles - 1 - tile;
-    const size_t part = (size_t)parts_before(a, b, chunk, BM) + (size_t)tile * chunks;
-    if (part + chunks > (size_t)a.items) return;   // (starts out of order)
-    const int quads = a.c.dim / 4, w = quads <= 16 ? 16 : quads <= 32 ? 32 : 64;   // threads per part
-    const int d = threadIdx.x % w, k = threadIdx.x / w, n = 256 / w;
-    float m = LOWEST, l = 0.0f;
-    f4 x = {0, 0, 0, 0};
-    for (int c = k; c < chunks; c += n) {
-        const size_t at = ((part + c) * a.c.heads + head) * BM + row;
-        const float2 ml = a.pml[at];
-        if (ml.y == 0.0f) continue;
-        f4 y = {0, 0, 0, 0};
-        if (d < quads) y = *reinterpret_cast<const f4 *>(a.po + at * a.c.dim + d * 4);
-        const float now = fmaxf(m, ml.x), f = __builtin_amdgcn_exp2f(m - reference(now)), f2 = __builtin_amdgcn_exp2f(ml.x - reference(now));
-        m = now;
-        l = l * f + ml.y * f2;
-#pragma unroll
-        for (int i = 0; i < 4; i++) x[i] = x[i] * f + y[i] * f2;
-    }
-    __shared__ float sm[16], sl[16];
+// out of a row = sum over its parts of 2^(m of the part - the largest m) * (the part's sum), over the same of l: the weights first, in LDS,
+// then the sums in the order of the parts, dim / 4 threads (rounded up to 16, 32 or 64) a row. One query per sequence has few rows of many
+// parts: a workgroup then takes one row and each of its groups a share of the parts (ONE); a prompt's takes as many rows as it has groups.
+constexpr int PARTS = 512;   // workgroups that a call is split into, about: two per CU
+template <bool F32, bool BF, int BM, bool ONE> __global__ __launch_bounds__(256) void attn_join_kernel(AttnArgs a) {
+    const int quads = a.c.dim / 4, w = quads <= 16 ? 16 : quads <= 32 ? 32 : 64;   // threads per row
+    const int d = threadIdx.x % w, k = threadIdx.x / w, groups = 256 / w;
+    const int blocks = ONE ? min(BM, a.G) : BM / groups;   // workgroups per tile
+    const int head = blockIdx.x % a.c.heads, block = blockIdx.x / a.c.heads % blocks;
+    const int chunk = chunk_of(a, BM);
+    Part p;
+    if (!part_of<true>(a, blockIdx.x / a.c.heads / blocks, chunk, BM, p) || p.chunks == 1) return;   // (one part: written already)
+    const uint32_t first = p.first + (uint32_t)p.tile * (uint32_t)p.chunks;
+    const int tile = a.start ? p.s.tiles - 1 - p.tile : p.tile;
+    const int rows = min(BM, p.s.n * a.G - tile * BM), row = ONE ? block : block * groups + k;
+    if ((ONE ? row : block * groups) >= rows || p.chunks > PARTS + 1 || (size_t)first + p.chunks > (size_t)a.items) return;   // (the latter two: starts out of order)
+    const size_t at = ((size_t)first * a.c.heads + head) * BM + min(row, rows - 1), step = (size_t)a.c.heads * BM;
+
+    __shared__ float wt[ONE ? 1 : 16][PARTS + 1];
+    __shared__ float sm[4], sl[4];
     __shared__ f4 sx[256];
-    if (d == 0) {
-        sm[k] = m;
-        sl[k] = l;
+    float *f = wt[ONE ? 0 : k];
+    const int lanes = ONE ? 256 : w, t = ONE ? threadIdx.x : d;
+    float m = LOWEST;
+    for (int c = t; c < p.chunks; c += lanes) {
+        const float2 ml = a.pml[at + c * step];
+        if (ml.y != 0.0f) m = fmaxf(m, ml.x);
     }
-    sx[threadIdx.x] = x;
+    for (int o = (ONE ? 64 : w) / 2; o; o >>= 1) m = fmaxf(m, __shfl_xor(m, o));
+    if constexpr (ONE) {
+        if ((threadIdx.x & 63) == 0) sm[threadIdx.x >> 6] = m;
+        __syncthreads();
+        m = fmaxf(fmaxf(sm[0], sm[1]), fmaxf(sm[2], sm[3]));
+    }
+    float l = 0.0f;
+    for (int c = t; c < p.chunks; c += lanes) {
+        const float2 ml = a.pml[at + c * step];
+        const float x = ml.y != 0.0f ? __builtin_amdgcn_exp2f(ml.x - reference(m)) : 0.0f;
+        f[c] = x;
+        l += x * ml.y;
+    }
+    for (int o = (ONE ? 64 : w) / 2; o; o >>= 1) l += __shfl_xor(l, o);
+    if constexpr (ONE) {
+        if ((threadIdx.x & 63) == 0) sl[threadIdx.x >> 6] = l;
+    }
     __syncthreads();
-    if (k || d >= quads) return;
-    for (int c = 1; c < n; c++) {
-        if (sl[c] == 0.0f) continue;
-        const f4 y = sx[c * w + d];
-        const float now = fmaxf(m, sm[c]), f = __builtin_amdgcn_exp2f(m - reference(now)), f2 = __builtin_amdgcn_exp2f(sm[c] - reference(now));
-        m = now;
-        l = l * f + sl[c] * f2;
+    if constexpr (ONE) l = (sl[0] + sl[1]) + (sl[2] + sl[3]);
+    f4 x = {0, 0, 0, 0};
+    if (d < quads) {
+        const float *y = a.po + at * a.c.dim + d * 4;
+        const size_t pitch = step * a.c.dim;
+#pragma unroll 8
+        for (int c = ONE ? k : 0; c < p.chunks; c += ONE ? groups : 1) {
+            const f4 v = *reinterpret_cast<const f4 *>(y + c * pitch);
 #pragma unroll
-        for (int i = 0; i < 4; i++) x[i] = x[i] * f + y[i] * f2;
+            for (int i = 0; i < 4; i++) x[i] = __builtin_fmaf(f[c], v[i], x[i]);
+        }
     }
+    if constexpr (ONE) {
+        sx[threadIdx.x] = x;
+        __syncthreads();
+        if (k) return;
+        for (int g = 1; g < groups; g++)
+#pragma unroll
+            for (int i = 0; i < 4; i++) x[i] += sx[g * w + d][i];
+    }
+    if (d >= quads || row >= rows) return;
+    const int r = tile * BM + row, query = r / a.G;
     float o[4];
     const float inv = l == 0.0f ? 0.0f : 1.0f / l;
 #pragma unroll
     for (int i = 0; i < 4; i++) o[i] = l == 0.0f ? 0.0f : x[i] * inv;
-    store4<F32, BF>(a.out + (size_t)t * a.ostride + (size_t)hq * a.c.dim * (F32 ? 4 : 2), d * 4, o);
+    store4<F32, BF>(a.out + (size_t)(p.s.t0 + query) * a.ostride + (size_t)(head * a.G + r - query * a.G) * a.c.dim * (F32 ? 4 : 2), d * 4, o);
 }
 
 // ---- host ------------------------------------------------------------------------------------------------------------------------
 constexpr int DECODE_M = 16;
-constexpr int DECODE_PARTS = 512, PROMPT_PARTS = 512;   // workgroups that a call is split into, about: two per CU
 
 struct Shape {
     size_t tiles;   // the most tiles per K/V head that the call's lengths can give
@@ -782,9 +801,9 @@ Shape shape_of(const es_hip_kv *kv, int nseq, int ntok, int heads, bool prompt) 
     Shape s;
     s.bm = prompt ? PM : DECODE_M;
     s.tiles = prompt ? (size_t)ntok * G / PM + nseq : (size_t)nseq * ((G + DECODE_M - 1) / DECODE_M);
-    const int parts = (prompt ? PROMPT_PARTS : DECODE_PARTS) / kv->heads;
-    const bool many = prompt && s.tiles >= (size_t)std::max(parts, 1);
-    s.target = many || (long long)kv->max_pages * kv->page <= CHUNK_MIN ? 0 : std::max(parts, 1);
+    const int parts = std::max(PARTS / kv->heads, 1);
+    const bool many = prompt && s.tiles >= (size_t)parts;
+    s.target = many || (long long)kv->max_pages * kv->page <= CHUNK_MIN ? 0 : parts;
     return s;
 }
 
@@ -809,8 +828,9 @@ template <bool BF, int NQ> hipError_t launch(const AttnArgs &a, const Shape &s, 
     }
     hipError_t e = hipGetLastError();
     if (e != hipSuccess || !s.target) return e;
-    auto f = prompt ? attn_join_kernel<(NQ > 1), BF, PM> : attn_join_kernel<(NQ > 1), BF, DECODE_M>;
-    f<<<(unsigned)((size_t)a.ntok * a.c.heads * a.G), 256, 0, st>>>(a);
+    const int groups = a.c.dim <= 64 ? 16 : a.c.dim <= 128 ? 8 : 4;   // rows that a workgroup joins
+    auto f = prompt ? attn_join_kernel<(NQ > 1), BF, PM, false> : attn_join_kernel<(NQ > 1), BF, DECODE_M, true>;
+    f<<<(unsigned)(s.tiles * a.c.heads * (prompt ? PM / groups : std::min(DECODE_M, a.G))), 256, 0, st>>>(a);
     return hipGetLastError();
 }
 
