@@ -254,6 +254,22 @@ template <bool F32, bool BF> __device__ void store4(uint8_t *row, int d, const f
     }
 }
 
+// A run of 16 keys of one page, or as many of them as there are, for loads whose offsets count from its first row: what lies past its end reads as
+// zeros, and all of a run that is in no page (the bounds are the loads' own; no address needs a lane's registers but its offset).
+struct Run {
+    __amdgpu_buffer_rsrc_t r;
+    __device__ Run(const KvView &c, const uint8_t *pool, int page, int head, int token, int keys) {
+        const uint8_t *at = pool + c.at(max(page, 0), head, token);
+        r = __builtin_amdgcn_make_buffer_rsrc(const_cast<uint8_t *>(at), (short)0, page < 0 ? 0 : min(keys, 16) * c.dim * 2, 0x00020000);
+    }
+    __device__ u4 load16(int lane_offset, int offset) const {
+        return __builtin_bit_cast(u4, __builtin_amdgcn_raw_buffer_load_b128(r, lane_offset, offset, 0));
+    }
+    __device__ u2 load8(int lane_offset, int offset) const {
+        return __builtin_bit_cast(u2, __builtin_amdgcn_raw_buffer_load_b64(r, lane_offset, offset, 0));
+    }
+};
+
 // two rows' elements j of 2 packed elements, as a pair
 template <int J> __device__ uint32_t pair(uint32_t first, uint32_t second) {
     return __builtin_amdgcn_perm(second, first, J & 1 ? 0x07060302u : 0x05040100u);
@@ -264,7 +280,7 @@ template <int J> __device__ uint32_t pair(uint32_t first, uint32_t second) {
 // turn, joined in LDS at the end. Nothing is staged: a lane loads its K fragments as the matrix cores take them (key lane % 16,
 // 8 elements) and, of V, the DP / 16 elements from (lane % 16) * DP / 16 on of the 8 keys whose weights it holds, which
 // it turns into 8 keys of one element each with byte permutes. Bound by HBM where the caches are long.
-template <bool BF, int NQ, int DP> __global__ __launch_bounds__(256) void attn_decode_kernel(AttnArgs a) {
+template <bool BF, int NQ, int DP> __global__ __launch_bounds__(256, DP == 256 ? 1 : 2) void attn_decode_kernel(AttnArgs a) {
     constexpr int KS = DP / 32, DL = DP / 16, BM = 16;
     constexpr bool F32 = NQ > 1;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -279,7 +295,6 @@ template <bool BF, int NQ, int DP> __global__ __launch_bounds__(256) void attn_d
     const int r = p.tile * BM + col, rows = a.G;
     const int shift16 = a.c.shift - 4;
     const int *table = a.c.table + (size_t)max(a.c.row(p.b), 0) * a.c.max_pages;
-    const size_t pagestep = (size_t)a.c.heads << a.c.shift;   // token rows per page
 
     u4 q[KS][NQ];
     const float cs = load_query<BF, NQ, KS, 32, 16>(a.q + (size_t)p.s.t0 * a.qstride + (size_t)(head * a.G + r) * a.c.dim * (F32 ? 4 : 2),
@@ -289,60 +304,93 @@ template <bool BF, int NQ, int DP> __global__ __launch_bounds__(256) void attn_d
     for (int j = 0; j < DL; j++) acc[j] = f4{0, 0, 0, 0};
     float m = LOWEST, l = 0.0f;
 
-    for (int t0 = first + wave * 32; t0 < last; t0 += 128) {
-        // the two pages; one that there is not: no keys, and page 0 in its place
-        bool ok[2];
-        const uint8_t *kp[2], *vp[2];
+    // This wave's keys of step n: 32 from first + (4 n + wave) * 32 on, two runs of 16. Lane 2 i + h holds the page of run h of step
+    // 32 s + i (-1: none), of the 32 steps at hand and of the 32 after them.
+    const int dim = a.c.dim;
+    auto fetch = [&](int n) {
+        const int u = (first >> 4) + ((n + (lane >> 1)) * 4 + wave) * 2 + (lane & 1);
+        const int page = u * 16 < last ? table[u >> shift16] : -1;
+        return page < a.c.npages ? page : -1;
+    };
+    int pg = fetch(0), pgn = fetch(32);
+    const int kd = (col * dim + g * 8) * 2, vd = (g * 4 * dim + col * DL) * 2;
+    u4 kr[2][KS];             // run h, elements s * 32 + g * 8 of key col
+    uint32_t vr[8][DL / 2];   // DL elements of the keys g * 4 + i (first four) and 16 + g * 4 + i
+    auto page_of = [&](int n, int h) { return __builtin_amdgcn_readlane(pg, (n & 31) * 2 + h); };
+    auto run = [&](const uint8_t *pool, int n, int h) {
+        const int u = (first >> 4) + (n * 4 + wave) * 2 + h;
+        return Run(a.c, pool, page_of(n, h), head, (u & ((1 << shift16) - 1)) << 4, last - u * 16);
+    };
+    auto load_k = [&](int n) {
 #pragma unroll
         for (int h = 0; h < 2; h++) {
-            const int u = (t0 >> 4) + h;
-            int page = u * 16 < last ? table[u >> shift16] : -1;
-            ok[h] = page >= 0 && page < a.c.npages;
-            page = ok[h] ? page : 0;
-            const size_t at = ((size_t)page * pagestep + ((size_t)head << a.c.shift) + (u & ((1 << shift16) - 1)) * 16) * a.c.dim * 2;
-            kp[h] = a.c.k + at;
-            vp[h] = a.c.v + at;
+            const Run r = run(a.c.k, n, h);
+#pragma unroll
+            for (int s = 0; s < KS; s++) kr[h][s] = r.load16(kd + s * 64, 0);
         }
-        u4 kf[2][KS];
+    };
+    auto load_v = [&](int n) {
 #pragma unroll
-        for (int h = 0; h < 2; h++)
+        for (int h = 0; h < 2; h++) {
+            const Run r = run(a.c.v, n, h);
 #pragma unroll
-            for (int s = 0; s < KS; s++) {
-                const int d = s * 32 + g * 8;
-                kf[h][s] = d < a.c.dim ? *reinterpret_cast<const u4 *>(kp[h] + ((size_t)col * a.c.dim + d) * 2) : u4{0, 0, 0, 0};
-            }
-        uint32_t vr[8][DL / 2];
-#pragma unroll
-        for (int i = 0; i < 8; i++) {
-            const int d = col * DL;   // dim is a multiple of 8: DL = 4 may end inside the row's last 8, DL = 16 may begin there
-            const uint8_t *src = vp[i >> 2] + ((size_t)(g * 4 + (i & 3)) * a.c.dim + d) * 2;
-#pragma unroll
-            for (int w = 0; w < DL / 2; w += (DL == 4 ? 2 : 4)) {
-                const bool in = d + w * 2 < a.c.dim;
+            for (int i = 0; i < 4; i++) {   // (elements past dim: others' in their place, in sums that are not written)
                 if constexpr (DL == 4) {
-                    const u2 x = in ? *reinterpret_cast<const u2 *>(src) : u2{0, 0};
-                    vr[i][0] = x[0];
-                    vr[i][1] = x[1];
+                    const u2 y = r.load8(vd, i * dim * 2);
+                    vr[h * 4 + i][0] = y[0];
+                    vr[h * 4 + i][1] = y[1];
                 } else {
-                    const u4 x = in ? *reinterpret_cast<const u4 *>(src + w * 4) : u4{0, 0, 0, 0};
 #pragma unroll
-                    for (int k = 0; k < 4; k++) vr[i][w + k] = x[k];
+                    for (int w = 0; w < DL / 2; w += 4) {
+                        const u4 y = r.load16(vd + w * 4, i * dim * 2);
+#pragma unroll
+                        for (int k = 0; k < 4; k++) vr[h * 4 + i][w + k] = y[k];
+                    }
                 }
             }
         }
+    };
+    // The next step's K is loaded once this one's scores are there and its V once this one's is summed, into the same registers.
+    const int mine = first + wave * 32, steps = mine < last ? (last - mine + 127) / 128 : 0;
+    bool ok[2] = {false, false};
+    if (steps > 0) {
+        ok[0] = page_of(0, 0) >= 0;
+        ok[1] = page_of(0, 1) >= 0;
+        load_k(0);
+        load_v(0);
+    }
+    for (int n = 0; n < steps; n++) {
+        const int t0 = mine + n * 128;
         f4 s[2] = {f4{0, 0, 0, 0}, f4{0, 0, 0, 0}};
+        if (dim < DP) {   // elements past dim: zeros, which the query's zeros keep
+#pragma unroll
+            for (int h = 0; h < 2; h++)
+#pragma unroll
+                for (int k = 0; k < KS; k++)
+                    if (k * 32 + g * 8 >= dim) kr[h][k] = u4{0, 0, 0, 0};
+        }
 #pragma unroll
         for (int t = 0; t < NQ; t++)
 #pragma unroll
             for (int k = 0; k < KS; k++)
 #pragma unroll
-                for (int h = 0; h < 2; h++) s[h] = mfma16<BF>(kf[h][k], q[k][t], s[h]);
-        if (t0 < lo || t0 + 32 > last || !ok[0] || !ok[1]) {   // what is not to be seen: no score, and zeros for whatever V holds
+                for (int h = 0; h < 2; h++) s[h] = mfma16<BF>(kr[h][k], q[k][t], s[h]);
+        const bool ok0 = ok[0], ok1 = ok[1], more = n + 1 < steps;
+        if (more) {
+            if (((n + 1) & 31) == 0) {
+                pg = pgn;
+                pgn = fetch(n + 33);
+            }
+            ok[0] = page_of(n + 1, 0) >= 0;
+            ok[1] = page_of(n + 1, 1) >= 0;
+            load_k(n + 1);
+        }
+        if (t0 < lo || t0 + 32 > last || !ok0 || !ok1) {   // what is not to be seen: no score, and zeros for whatever V holds
 #pragma unroll
             for (int i = 0; i < 8; i++) {
                 const int t = t0 + (i >> 2) * 16 + g * 4 + (i & 3);
-                if (t < lo || t >= last || !ok[i >> 2]) {
-                    s[i >> 2][i & 3] = LOWEST;
+                if (t < lo || t >= last || !(i < 4 ? ok0 : ok1)) s[i >> 2][i & 3] = LOWEST;
+                if (t < lo) {
 #pragma unroll
                     for (int w = 0; w < DL / 2; w++) vr[i][w] = 0;
                 }
@@ -385,6 +433,7 @@ template <bool BF, int NQ, int DP> __global__ __launch_bounds__(256) void attn_d
                 acc[j + 1] = mfma16<BF>(v1, pt[t], acc[j + 1]);
             }
         }
+        if (more) load_v(n + 1);
     }
     l += __shfl_xor(l, 16);
     l += __shfl_xor(l, 32);
@@ -493,10 +542,9 @@ template <bool BF, int NQ, int DP> __global__ __launch_bounds__(256, DP == 256 |
 
     u4 kr[NK];
     uint32_t vr[4][VE / 2];
-    const int kt = tid / KC, kd = min(tid % KC * 8, dim - 8);   // this thread's first piece of K: token (of 64) and element
-    const int vt = tid / 16 * 4, vd = tid % 16 * VE;            // its 4 keys of V and their elements
-    const uint32_t rowb = (uint32_t)dim * 2;
-    const uint32_t k_off = (kt & 15) * rowb + kd * 2, v_off = (vt & 15) * rowb;
+    const int kt = tid / KC, kd = tid % KC * 8;        // this thread's first piece of K: token (of 64) and element
+    const int vt = tid / 16 * 4, vd = tid % 16 * VE;   // its 4 keys of V and their elements
+    const int k_off = ((kt & 15) * dim + kd) * 2, v_off = ((vt & 15) * dim + vd) * 2;
     // loads the keys from t0 on into registers; which of their four runs are in no page
     auto load = [&](int t0) {
         int u0 = (t0 >> 4) - pb;
@@ -507,28 +555,26 @@ template <bool BF, int NQ, int DP> __global__ __launch_bounds__(256, DP == 256 |
             pgn = fetch(pb + 64 + lane);
         }
         int holes = 0;
-        auto run = [&](int sub) {   // bytes from the pool's start to a run's rows; one that is in no page: page 0 in its place
-            const int page = __builtin_amdgcn_readlane(pg, u0 + sub);
-            const int token = ((t0 >> 4) + sub & ((1 << shift16) - 1)) << 4;
-            return a.c.at(max(page, 0), head, token);
+        auto run = [&](const uint8_t *pool, int sub) {
+            const int u = (t0 >> 4) + sub;
+            return Run(a.c, pool, __builtin_amdgcn_readlane(pg, u0 + sub), head, (u & ((1 << shift16) - 1)) << 4, last - u * 16);
         };
 #pragma unroll
         for (int u = 0; u < 4; u++) holes |= __builtin_amdgcn_readlane(pg, u0 + u) < 0 ? 1 << u : 0;
 #pragma unroll
         for (int i = 0; i < NK; i++)   // pieces i: tokens kt + i * (256 / KC)
-            kr[i] = *reinterpret_cast<const u4 *>(a.c.k + run(KC == 8 ? (wave >> 1) + 2 * i : KC == 16 ? i : i >> 1) +
-                                                  k_off + (KC == 32 ? (i & 1) * 8 * rowb : 0));
-        const uint8_t *vp = a.c.v + run(wave) + v_off;
+            kr[i] = run(a.c.k, KC == 8 ? (wave >> 1) + 2 * i : KC == 16 ? i : i >> 1).load16(k_off, KC == 32 ? (i & 1) * 16 * dim : 0);
+        const Run v = run(a.c.v, wave);
 #pragma unroll
         for (int k = 0; k < 4; k++) {   // (elements past dim: others' in their place, in rows of O^T that are not written)
             if constexpr (VE == 4) {
-                const u2 x = *reinterpret_cast<const u2 *>(vp + k * rowb + min(vd, dim - 4) * 2);
+                const u2 x = v.load8(v_off, k * dim * 2);
                 vr[k][0] = x[0];
                 vr[k][1] = x[1];
             } else {
 #pragma unroll
                 for (int w = 0; w < VE / 2; w += 4) {
-                    const u4 x = *reinterpret_cast<const u4 *>(vp + k * rowb + min(vd + w * 2, dim - 8) * 2);
+                    const u4 x = v.load16(v_off + w * 4, k * dim * 2);
 #pragma unroll
                     for (int n = 0; n < 4; n++) vr[k][w + n] = x[n];
                 }
@@ -537,18 +583,18 @@ template <bool BF, int NQ, int DP> __global__ __launch_bounds__(256, DP == 256 |
         return holes;
     };
     // registers to LDS: the keys from t0 on, loaded last
-    auto stage = [&](int t0, int buf, int holes) {
-        if (padded && tid % KC * 8 >= dim) {   // elements past dim: zeros, which the query's zeros keep
+    auto stage = [&](int t0, int buf) {
+        if (padded && kd >= dim) {   // elements past dim: zeros, which the query's zeros keep
 #pragma unroll
             for (int i = 0; i < NK; i++) kr[i] = u4{0, 0, 0, 0};
         }
 #pragma unroll
         for (int i = 0; i < NK; i++)
-            *reinterpret_cast<u4 *>(&lk[buf][(kt + i * (256 / KC)) * KP + tid % KC * 8]) = kr[i];
-        if (t0 < see_lo || t0 + PN > last || holes) {
+            *reinterpret_cast<u4 *>(&lk[buf][(kt + i * (256 / KC)) * KP + kd]) = kr[i];
+        if (t0 < see_lo) {
 #pragma unroll
             for (int k = 0; k < 4; k++)
-                if (t0 + vt + k < see_lo || t0 + vt + k >= last || (holes >> wave & 1)) {
+                if (t0 + vt + k < see_lo) {
 #pragma unroll
                     for (int w = 0; w < VE / 2; w++) vr[k][w] = 0;
                 }
@@ -581,7 +627,7 @@ template <bool BF, int NQ, int DP> __global__ __launch_bounds__(256, DP == 256 |
     int holes = 0, next = 0;
     if (first < last) {
         holes = load(first);
-        stage(first, 0, holes);
+        stage(first, 0);
         if (first + PN < last) next = load(first + PN);
     }
     __syncthreads();
@@ -656,7 +702,7 @@ template <bool BF, int NQ, int DP> __global__ __launch_bounds__(256, DP == 256 |
         }
         holes = next;
         if (t0 + PN < last) {
-            stage(t0 + PN, buf ^ 1, next);
+            stage(t0 + PN, buf ^ 1);
             if (t0 + 2 * PN < last) next = load(t0 + 2 * PN);
         }
         buf ^= 1;
