@@ -30,49 +30,47 @@ struct AttnArgs {
     const int *start;          // null: one query per sequence
     const uint8_t *q;
     uint8_t *out;
-    float *po;                 // parts' sums: [part][row of the tile][dim]
-    float2 *pml;               // parts' m and l: [part][row of the tile]
+    float *po;                 // parts' sums: the same of [dim]
+    float2 *pml;               // parts' m and l: [part][row of the tile] (one query per sequence: [head][row][part], two parts a workgroup)
     size_t qstride, ostride;   // bytes
     int nseq, ntok, G, window;
     float c2;                  // scale * log2(e)
-    int target;                // parts aimed for per K/V head; 0: every tile is one part
+    int target;                // parts aimed for per K/V head; 0: every tile is one part. One query per sequence: workgroups
+    int block;                 // one query per sequence: log2 of the keys of a block
     int items;                 // parts per K/V head that there is room for
 };
 
-// ---- which work a workgroup takes ------------------------------------------------------------------------------------------
-// A tile is BM rows of one sequence and K/V head; a part is a tile's chunk of keys. Chunks have one length for the whole call, from
-// the lengths on the device: the least that leaves about `target` parts, so that ragged batches split evenly and a captured call
+// ---- which work a prompt's workgroup takes ---------------------------------------------------------------------------------------
+// A tile is PM rows of one sequence and K/V head; a part is a tile's chunk of keys. Chunks have one length for the whole call, from the
+// lengths on the device: the least that leaves about `target` parts, so that few rows over many keys fill the device and a captured call
 // adapts to later lengths. Every wave finds its part by a scan over the sequences, 64 at a time.
+constexpr int PM = 128, PN = 64;   // rows of a tile, keys of a step
+
 struct Seq {
     int t0, n, len;      // first query row, queries, tokens
-    int base, tiles;     // first key of the first chunk (a multiple of 64), tiles of BM rows
+    int base, tiles;     // first key of the first chunk (a multiple of 64), tiles of PM rows
 };
-__device__ Seq seq_of(const AttnArgs &a, int b, int bm) {
+__device__ Seq seq_of(const AttnArgs &a, int b) {
     Seq s;
-    if (a.start) {
-        s.t0 = min(max(a.start[b], 0), a.ntok);
-        s.n = min(max(a.start[b + 1], s.t0), a.ntok) - s.t0;
-    } else {
-        s.t0 = b;
-        s.n = 1;
-    }
+    s.t0 = min(max(a.start[b], 0), a.ntok);
+    s.n = min(max(a.start[b + 1], s.t0), a.ntok) - s.t0;
     s.len = a.c.tokens(b);
     s.base = a.window ? max(0, s.len - s.n - a.window + 1) & ~63 : 0;
-    s.tiles = (int)(((long long)s.n * a.G + bm - 1) / bm);
+    s.tiles = (int)(((long long)s.n * a.G + PM - 1) / PM);
     return s;
 }
 
 constexpr int CHUNK_MIN = 128;   // keys
 
-__device__ int chunk_of(const AttnArgs &a, int bm) {
+__device__ int chunk_of(const AttnArgs &a) {
     if (!a.target) return 1 << 30;
     unsigned long long all = 0;
     if (a.nseq == 1) {
-        const Seq s = seq_of(a, 0, bm);
+        const Seq s = seq_of(a, 0);
         all = (unsigned long long)s.tiles * (unsigned)(s.len - s.base);
     } else {
         for (int b = threadIdx.x & 63; b < a.nseq; b += 64) {
-            const Seq s = seq_of(a, b, bm);
+            const Seq s = seq_of(a, b);
             all += (unsigned long long)s.tiles * (unsigned)(s.len - s.base);
         }
 #pragma unroll
@@ -100,12 +98,12 @@ __device__ uint32_t sum_up_to(uint32_t x) {   // over the lanes up to this one
 }
 // The part with number `item` (within one K/V head), or, TILES, the tile with that number and `chunk` 0; false if there is none. Starts that
 // are out of order may give any number of parts: they are counted modulo 2^32.
-template <bool TILES = false> __device__ bool part_of(const AttnArgs &a, int item, int chunk, int bm, Part &p) {
+template <bool TILES = false> __device__ bool part_of(const AttnArgs &a, int item, int chunk, Part &p) {
     const int lane = threadIdx.x & 63;
     uint32_t tiles_before = 0, parts_before = 0;
     if (a.nseq == 1) {
         p.b = 0;
-        p.s = seq_of(a, 0, bm);
+        p.s = seq_of(a, 0);
         p.chunks = chunks_of(p.s, chunk);
         p.first = 0;
     } else {
@@ -115,7 +113,7 @@ template <bool TILES = false> __device__ bool part_of(const AttnArgs &a, int ite
             int chunks = 1;
             uint32_t parts = 0;
             if (g + lane < a.nseq) {
-                s = seq_of(a, g + lane, bm);
+                s = seq_of(a, g + lane);
                 chunks = chunks_of(s, chunk);
                 parts = (uint32_t)s.tiles * (uint32_t)chunks;
             }
@@ -255,18 +253,19 @@ template <bool F32, bool BF> __device__ void store4(uint8_t *row, int d, const f
 }
 
 // A run of 16 keys of one page, or as many of them as there are, for loads whose offsets count from its first row: what lies past its end reads as
-// zeros, and all of a run that is in no page (the bounds are the loads' own; no address needs a lane's registers but its offset).
-struct Run {
+// zeros, and all of a run that is in no page (the bounds are the loads' own; no address needs a lane's registers but its offset). ONCE: nobody else
+// reads them soon (a non-temporal load).
+template <bool ONCE> struct Run {
     __amdgpu_buffer_rsrc_t r;
     __device__ Run(const KvView &c, const uint8_t *pool, int page, int head, int token, int keys) {
         const uint8_t *at = pool + c.at(max(page, 0), head, token);
         r = __builtin_amdgcn_make_buffer_rsrc(const_cast<uint8_t *>(at), (short)0, page < 0 ? 0 : min(keys, 16) * c.dim * 2, 0x00020000);
     }
     __device__ u4 load16(int lane_offset, int offset) const {
-        return __builtin_bit_cast(u4, __builtin_amdgcn_raw_buffer_load_b128(r, lane_offset, offset, 0));
+        return __builtin_bit_cast(u4, __builtin_amdgcn_raw_buffer_load_b128(r, lane_offset, offset, ONCE ? 2 : 0));
     }
     __device__ u2 load8(int lane_offset, int offset) const {
-        return __builtin_bit_cast(u2, __builtin_amdgcn_raw_buffer_load_b64(r, lane_offset, offset, 0));
+        return __builtin_bit_cast(u2, __builtin_amdgcn_raw_buffer_load_b64(r, lane_offset, offset, ONCE ? 2 : 0));
     }
 };
 
@@ -276,206 +275,342 @@ template <int J> __device__ uint32_t pair(uint32_t first, uint32_t second) {
 }
 
 // ---- one query per sequence ----------------------------------------------------------------------------------------------------
-// A workgroup of four waves takes a part: up to 16 heads of one K/V head against a chunk of keys, each wave 32 keys at a time in
-// turn, joined in LDS at the end. Nothing is staged: a lane loads its K fragments as the matrix cores take them (key lane % 16,
-// 8 elements) and, of V, the DP / 16 elements from (lane % 16) * DP / 16 on of the 8 keys whose weights it holds, which
-// it turns into 8 keys of one element each with byte permutes. Bound by HBM where the caches are long.
-template <bool BF, int NQ, int DP> __global__ __launch_bounds__(256, DP == 256 ? 1 : 2) void attn_decode_kernel(AttnArgs a) {
-    constexpr int KS = DP / 32, DL = DP / 16, BM = 16;
+// A tile is the G query heads of a sequence's K/V head (16 of them, where there are more), its keys blocks of 128. The tiles' blocks, one
+// after another, are dealt out evenly: workgroup w of a K/V head takes blocks [w * each, (w + 1) * each) of them, whatever sequences they are of,
+// so that a ragged batch keeps every workgroup busy to the end. What a workgroup has of a tile that others have parts of goes to the workspace,
+// and a second launch joins them. (The last workgroup of a tile to arrive could do that in the same launch, but 128 of them counting in one word and
+// one CU reading all their sums took 78 us for one sequence of 131072 tokens, where the two launches take TWO.)
+//
+// Inside: four waves, each 32 keys at a time in turn, joined in LDS at the end. Nothing is staged: a lane loads its K fragments as the matrix
+// cores take them (key lane % 16, 8 elements) and, of V, the DP / 16 elements from (lane % 16) * DP / 16 on of the 8 keys whose weights it
+// holds, which it turns into 8 keys of one element each with byte permutes. Bound by HBM where the caches are long.
+constexpr int BLOCK = 7, BLOCK_WHOLE = 9, DECODE_M = 16;   // (log2)
+// workgroups, all heads together: as many as fit the device at once, and no more than bring it to the memory's rate
+constexpr int decode_groups(int dim) { return dim <= 128 ? 512 : 256; }
+
+// the sequences' blocks: lane i has those of sequence g + i
+struct Blocks {
+    int len;
+    uint32_t mine, upto;   // of the sequence; of the group's sequences up to it
+};
+__device__ int blocks_of(const AttnArgs &a, int len, int &base) {   // of one tile; an empty one has a block too: somebody writes its zeros
+    base = a.window ? max(0, len - a.window) & ~63 : 0;
+    return max(1, (len - base + (1 << a.block) - 1) >> a.block);
+}
+__device__ Blocks blocks_from(const AttnArgs &a, int g, int tiles) {
+    Blocks x{0, 0, 0};
+    const int b = g + (threadIdx.x & 63);
+    int base;
+    if (b < a.nseq) {
+        x.len = a.c.tokens(b);
+        x.mine = (uint32_t)tiles * (uint32_t)blocks_of(a, x.len, base);
+    }
+    x.upto = a.nseq == 1 ? (uint32_t)__builtin_amdgcn_readfirstlane((int)x.mine) : sum_up_to(x.mine);
+    return x;
+}
+
+// Every workgroup's way to its blocks: lane i holds those of the sequences `group` + i, of which there are `before` before.
+struct Deal {
+    Blocks bl;
+    uint32_t total, each, before = 0;
+    int group = 0;
+    __device__ Deal(const AttnArgs &a, int tiles) : bl(blocks_from(a, 0, tiles)) {
+        total = (uint32_t)__builtin_amdgcn_readlane((int)bl.upto, 63);
+        for (int g = 64; g < a.nseq; g += 64) total += (uint32_t)__builtin_amdgcn_readlane((int)blocks_from(a, g, tiles).upto, 63);
+        each = (total + a.target - 1) / a.target;
+    }
+    // on to the sequences from g on (a multiple of 64)
+    __device__ void next(const AttnArgs &a, int tiles) {
+        before += (uint32_t)__builtin_amdgcn_readlane((int)bl.upto, 63);
+        group += 64;
+        bl = blocks_from(a, group, tiles);
+    }
+    __device__ uint32_t first_of(int in) const { return before + (uint32_t)__builtin_amdgcn_readlane((int)(bl.upto - bl.mine), in); }
+};
+
+template <bool BF, int NQ, int DP> __global__ __launch_bounds__(256, DP == 64 && NQ < 3 ? 3 : DP <= 128 ? 2 : 1) void attn_decode_kernel(AttnArgs a) {
+    constexpr int KS = DP / 32, DL = DP / 16, BM = DECODE_M;
     constexpr bool F32 = NQ > 1;
+    __shared__ float lm[4][BM], ll[4][BM];
+    __shared__ __attribute__((aligned(16))) float lo_acc[4][BM][DP + 4];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int col = lane & 15, g = lane >> 4;
-    const int head = blockIdx.x % a.c.heads, item = blockIdx.x / a.c.heads;
-    const int chunk = chunk_of(a, BM);
-    Part p;
-    if (!part_of(a, item, chunk, BM, p)) return;
-    const int lo = max(a.window ? p.s.len - a.window : 0, 0), hi = p.s.len;
-    const int first = p.s.base + p.chunk * (chunk < 1 << 30 ? chunk : 0);
-    const int last = chunk < 1 << 30 ? min(hi, first + chunk) : hi;
-    const int r = p.tile * BM + col, rows = a.G;
+    const int head = blockIdx.x % a.c.heads, group = blockIdx.x / a.c.heads;
+    const int rows = a.G, tiles = (a.G + BM - 1) / BM, dim = a.c.dim;
     const int shift16 = a.c.shift - 4;
-    const int *table = a.c.table + (size_t)max(a.c.row(p.b), 0) * a.c.max_pages;
 
-    u4 q[KS][NQ];
-    const float cs = load_query<BF, NQ, KS, 32, 16>(a.q + (size_t)p.s.t0 * a.qstride + (size_t)(head * a.G + r) * a.c.dim * (F32 ? 4 : 2),
-                                                    r < rows, g, a.c.dim, a.c2, q);
-    f4 acc[DL];
-#pragma unroll
-    for (int j = 0; j < DL; j++) acc[j] = f4{0, 0, 0, 0};
-    float m = LOWEST, l = 0.0f;
-
-    // This wave's keys of step n: 32 from first + (4 n + wave) * 32 on, two runs of 16. Lane 2 i + h holds the page of run h of step
-    // 32 s + i (-1: none), of the 32 steps at hand and of the 32 after them.
-    const int dim = a.c.dim;
-    auto fetch = [&](int n) {
-        const int u = (first >> 4) + ((n + (lane >> 1)) * 4 + wave) * 2 + (lane & 1);
-        const int page = u * 16 < last ? table[u >> shift16] : -1;
-        return page < a.c.npages ? page : -1;
-    };
-    int pg = fetch(0), pgn = fetch(32);
-    const int kd = (col * dim + g * 8) * 2, vd = (g * 4 * dim + col * DL) * 2;
-    u4 kr[2][KS];             // run h, elements s * 32 + g * 8 of key col
-    uint32_t vr[8][DL / 2];   // DL elements of the keys g * 4 + i (first four) and 16 + g * 4 + i
-    auto page_of = [&](int n, int h) { return __builtin_amdgcn_readlane(pg, (n & 31) * 2 + h); };
-    auto run = [&](const uint8_t *pool, int n, int h) {
-        const int u = (first >> 4) + (n * 4 + wave) * 2 + h;
-        return Run(a.c, pool, page_of(n, h), head, (u & ((1 << shift16) - 1)) << 4, last - u * 16);
-    };
-    auto load_k = [&](int n) {
-#pragma unroll
-        for (int h = 0; h < 2; h++) {
-            const Run r = run(a.c.k, n, h);
-#pragma unroll
-            for (int s = 0; s < KS; s++) kr[h][s] = r.load16(kd + s * 64, 0);
+    Deal deal(a, tiles);
+    const uint32_t each = deal.each, end = min(deal.total, (group + 1) * each);
+    for (uint32_t pos = group * each; pos < end;) {
+        unsigned long long past;
+        while (!(past = __ballot(pos < deal.before + deal.bl.upto))) {
+            deal.next(a, tiles);
+            if (deal.group >= a.nseq) return;   // (not while the lengths stay)
         }
-    };
-    auto load_v = [&](int n) {
+        const int in = __builtin_ctzll(past), seq = deal.group + in;
+        const int hi = __builtin_amdgcn_readlane(deal.bl.len, in);
+        const uint32_t s0 = deal.first_of(in);
+        int base;
+        const int blocks = blocks_of(a, hi, base);
+        const int tile = (int)((pos - s0) / blocks), block = (int)((pos - s0) - (uint32_t)tile * blocks);
+        const int here = (int)min((uint32_t)(blocks - block), end - pos);
+        const uint32_t tile_at = pos - block;   // the tile's first block among all
+        pos += here;
+        const int lo = max(a.window ? hi - a.window : 0, 0), first = base + (block << a.block), last = min(hi, first + (here << a.block));
+        const int r = tile * BM + col;
+        const int *table = a.c.table + (size_t)max(a.c.row(seq), 0) * a.c.max_pages;
+
+        u4 q[KS][NQ];
+        const float cs = load_query<BF, NQ, KS, 32, 16>(a.q + (size_t)seq * a.qstride + (size_t)(head * a.G + r) * dim * (F32 ? 4 : 2),
+                                                        r < rows, g, dim, a.c2, q);
+        f4 acc[DL];
 #pragma unroll
-        for (int h = 0; h < 2; h++) {
-            const Run r = run(a.c.v, n, h);
+        for (int j = 0; j < DL; j++) acc[j] = f4{0, 0, 0, 0};
+        float m = LOWEST, l = 0.0f;
+
+        // This wave's keys of step n: 32 from first + (4 n + wave) * 32 on, two runs of 16. Lane 2 i + h holds the page of run h of step
+        // 32 s + i (-1: none), of the 32 steps at hand and of the 32 after them.
+        auto fetch = [&](int n) {
+            const int u = (first >> 4) + ((n + (lane >> 1)) * 4 + wave) * 2 + (lane & 1);
+            const int page = u * 16 < last ? table[u >> shift16] : -1;
+            return page < a.c.npages ? page : -1;
+        };
+        int pg = fetch(0), pgn = fetch(32);
+        const int kd = (col * dim + g * 8) * 2, vd = (g * 4 * dim + col * DL) * 2;
+        u4 kr[2][KS];             // run h, elements s * 32 + g * 8 of key col
+        uint32_t vr[8][DL / 2];   // DL elements of the keys g * 4 + i (first four) and 16 + g * 4 + i
+        auto page_of = [&](int n, int h) { return __builtin_amdgcn_readlane(pg, (n & 31) * 2 + h); };
+        auto run = [&](const uint8_t *pool, int n, int h) {
+            const int u = (first >> 4) + (n * 4 + wave) * 2 + h;
+            return Run<true>(a.c, pool, page_of(n, h), head, (u & ((1 << shift16) - 1)) << 4, last - u * 16);
+        };
+        auto load_k = [&](int n) {
 #pragma unroll
-            for (int i = 0; i < 4; i++) {   // (elements past dim: others' in their place, in sums that are not written)
-                if constexpr (DL == 4) {
-                    const u2 y = r.load8(vd, i * dim * 2);
-                    vr[h * 4 + i][0] = y[0];
-                    vr[h * 4 + i][1] = y[1];
-                } else {
+            for (int h = 0; h < 2; h++) {
+                const Run<true> r = run(a.c.k, n, h);
 #pragma unroll
-                    for (int w = 0; w < DL / 2; w += 4) {
-                        const u4 y = r.load16(vd + w * 4, i * dim * 2);
+                for (int s = 0; s < KS; s++) kr[h][s] = r.load16(kd + s * 64, 0);
+            }
+        };
+        auto load_v = [&](int n) {
 #pragma unroll
-                        for (int k = 0; k < 4; k++) vr[h * 4 + i][w + k] = y[k];
+            for (int h = 0; h < 2; h++) {
+                const Run<true> r = run(a.c.v, n, h);
+#pragma unroll
+                for (int i = 0; i < 4; i++) {   // (elements past dim: others' in their place, in sums that are not written)
+                    if constexpr (DL == 4) {
+                        const u2 y = r.load8(vd, i * dim * 2);
+                        vr[h * 4 + i][0] = y[0];
+                        vr[h * 4 + i][1] = y[1];
+                    } else {
+#pragma unroll
+                        for (int w = 0; w < DL / 2; w += 4) {
+                            const u4 y = r.load16(vd + w * 4, i * dim * 2);
+#pragma unroll
+                            for (int k = 0; k < 4; k++) vr[h * 4 + i][w + k] = y[k];
+                        }
                     }
                 }
             }
+        };
+        // The next step's K is loaded once this one's scores are there and its V once this one's is summed, into the same registers.
+        const int mine = first + wave * 32, steps = mine < last ? (last - mine + 127) / 128 : 0;
+        bool ok[2] = {false, false};
+        if (steps > 0) {
+            ok[0] = page_of(0, 0) >= 0;
+            ok[1] = page_of(0, 1) >= 0;
+            load_k(0);
+            load_v(0);
         }
-    };
-    // The next step's K is loaded once this one's scores are there and its V once this one's is summed, into the same registers.
-    const int mine = first + wave * 32, steps = mine < last ? (last - mine + 127) / 128 : 0;
-    bool ok[2] = {false, false};
-    if (steps > 0) {
-        ok[0] = page_of(0, 0) >= 0;
-        ok[1] = page_of(0, 1) >= 0;
-        load_k(0);
-        load_v(0);
-    }
-    for (int n = 0; n < steps; n++) {
-        const int t0 = mine + n * 128;
-        f4 s[2] = {f4{0, 0, 0, 0}, f4{0, 0, 0, 0}};
-        if (dim < DP) {   // elements past dim: zeros, which the query's zeros keep
+        for (int n = 0; n < steps; n++) {
+            const int t0 = mine + n * 128;
+            f4 s[2] = {f4{0, 0, 0, 0}, f4{0, 0, 0, 0}};
+            if (dim < DP) {   // elements past dim: zeros, which the query's zeros keep
 #pragma unroll
-            for (int h = 0; h < 2; h++)
+                for (int h = 0; h < 2; h++)
+#pragma unroll
+                    for (int k = 0; k < KS; k++)
+                        if (k * 32 + g * 8 >= dim) kr[h][k] = u4{0, 0, 0, 0};
+            }
+#pragma unroll
+            for (int t = 0; t < NQ; t++)
 #pragma unroll
                 for (int k = 0; k < KS; k++)
-                    if (k * 32 + g * 8 >= dim) kr[h][k] = u4{0, 0, 0, 0};
-        }
 #pragma unroll
-        for (int t = 0; t < NQ; t++)
-#pragma unroll
-            for (int k = 0; k < KS; k++)
-#pragma unroll
-                for (int h = 0; h < 2; h++) s[h] = mfma16<BF>(kr[h][k], q[k][t], s[h]);
-        const bool ok0 = ok[0], ok1 = ok[1], more = n + 1 < steps;
-        if (more) {
-            if (((n + 1) & 31) == 0) {
-                pg = pgn;
-                pgn = fetch(n + 33);
+                    for (int h = 0; h < 2; h++) s[h] = mfma16<BF>(kr[h][k], q[k][t], s[h]);
+            const bool ok0 = ok[0], ok1 = ok[1], more = n + 1 < steps;
+            if (more) {
+                if (((n + 1) & 31) == 0) {
+                    pg = pgn;
+                    pgn = fetch(n + 33);
+                }
+                ok[0] = page_of(n + 1, 0) >= 0;
+                ok[1] = page_of(n + 1, 1) >= 0;
+                load_k(n + 1);
             }
-            ok[0] = page_of(n + 1, 0) >= 0;
-            ok[1] = page_of(n + 1, 1) >= 0;
-            load_k(n + 1);
-        }
-        if (t0 < lo || t0 + 32 > last || !ok0 || !ok1) {   // what is not to be seen: no score, and zeros for whatever V holds
+            if (t0 < lo || t0 + 32 > last || !ok0 || !ok1) {   // what is not to be seen: no score, and zeros for whatever V holds
 #pragma unroll
-            for (int i = 0; i < 8; i++) {
-                const int t = t0 + (i >> 2) * 16 + g * 4 + (i & 3);
-                if (t < lo || t >= last || !(i < 4 ? ok0 : ok1)) s[i >> 2][i & 3] = LOWEST;
-                if (t < lo) {
+                for (int i = 0; i < 8; i++) {
+                    const int t = t0 + (i >> 2) * 16 + g * 4 + (i & 3);
+                    if (t < lo || t >= last || !(i < 4 ? ok0 : ok1)) s[i >> 2][i & 3] = LOWEST;
+                    if (t < lo) {
 #pragma unroll
-                    for (int w = 0; w < DL / 2; w++) vr[i][w] = 0;
+                        for (int w = 0; w < DL / 2; w++) vr[i][w] = 0;
+                    }
                 }
             }
-        }
-        float big = LOWEST;
+            float big = LOWEST;
 #pragma unroll
-        for (int i = 0; i < 8; i++) big = fmaxf(big, s[i >> 2][i & 3]);
-        big = fmaxf(big, __shfl_xor(big, 16));
-        big = fmaxf(big, __shfl_xor(big, 32)) * cs;
-        if (__any(big > m)) {
-            const float now = fmaxf(m, big), f = __builtin_amdgcn_exp2f(m - reference(now));
-            m = now;
-            l *= f;
+            for (int i = 0; i < 8; i++) big = fmaxf(big, s[i >> 2][i & 3]);
+            big = fmaxf(big, __shfl_xor(big, 16));
+            big = fmaxf(big, __shfl_xor(big, 32)) * cs;
+            if (__any(big > m)) {
+                const float now = fmaxf(m, big), f = __builtin_amdgcn_exp2f(m - reference(now));
+                m = now;
+                l *= f;
 #pragma unroll
-            for (int j = 0; j < DL; j++)
+                for (int j = 0; j < DL; j++)
 #pragma unroll
-                for (int i = 0; i < 4; i++) acc[j][i] *= f;
-        }
-        const float ref = SHIFT<BF> - reference(m);
-        float w8[8];
-#pragma unroll
-        for (int i = 0; i < 8; i++) {
-            w8[i] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[i >> 2][i & 3], cs, ref));
-            l += w8[i];
-        }
-        u4 pt[NQ];
-        split<BF, NQ>(w8, pt);
-#pragma unroll
-        for (int j = 0; j < DL; j += 2) {
-            u4 v0, v1;
-#pragma unroll
-            for (int k = 0; k < 4; k++) {
-                v0[k] = pair<0>(vr[2 * k][j / 2], vr[2 * k + 1][j / 2]);
-                v1[k] = pair<1>(vr[2 * k][j / 2], vr[2 * k + 1][j / 2]);
+                    for (int i = 0; i < 4; i++) acc[j][i] *= f;
             }
+            const float ref = SHIFT<BF> - reference(m);
+            float w8[8];
 #pragma unroll
-            for (int t = 0; t < NQ; t++) {
-                acc[j] = mfma16<BF>(v0, pt[t], acc[j]);
-                acc[j + 1] = mfma16<BF>(v1, pt[t], acc[j + 1]);
+            for (int i = 0; i < 8; i++) {
+                w8[i] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[i >> 2][i & 3], cs, ref));
+                l += w8[i];
             }
+            u4 pt[NQ];
+            split<BF, NQ>(w8, pt);
+#pragma unroll
+            for (int j = 0; j < DL; j += 2) {
+                u4 v0, v1;
+#pragma unroll
+                for (int k = 0; k < 4; k++) {
+                    v0[k] = pair<0>(vr[2 * k][j / 2], vr[2 * k + 1][j / 2]);
+                    v1[k] = pair<1>(vr[2 * k][j / 2], vr[2 * k + 1][j / 2]);
+                }
+#pragma unroll
+                for (int t = 0; t < NQ; t++) {
+                    acc[j] = mfma16<BF>(v0, pt[t], acc[j]);
+                    acc[j + 1] = mfma16<BF>(v1, pt[t], acc[j + 1]);
+                }
+            }
+            if (more) load_v(n + 1);
         }
-        if (more) load_v(n + 1);
-    }
-    l += __shfl_xor(l, 16);
-    l += __shfl_xor(l, 32);
+        l += __shfl_xor(l, 16);
+        l += __shfl_xor(l, 32);
 
-    // the four waves' m, l and sums; lane (g, col) holds elements (g * 4 + i) * DL + j of head col
-    __shared__ float lm[4][BM], ll[4][BM];
-    __shared__ __attribute__((aligned(16))) float lo_acc[4][BM][DP + 4];
-    if (g == 0) {
-        lm[wave][col] = m;
-        ll[wave][col] = l;
+        // the four waves' m, l and sums; lane (g, col) holds elements (g * 4 + i) * DL + j of head col
+        if (g == 0) {
+            lm[wave][col] = m;
+            ll[wave][col] = l;
+        }
+#pragma unroll
+        for (int i = 0; i < 4; i++)
+#pragma unroll
+            for (int j = 0; j < DL; j += 4)
+                *reinterpret_cast<f4 *>(&lo_acc[wave][col][(g * 4 + i) * DL + j]) = f4{acc[j][i], acc[j + 1][i], acc[j + 2][i], acc[j + 3][i]};
+        __syncthreads();
+        const bool whole = here == blocks;
+        // a group's part of a tile that it begins is its second in the workspace, of one that it goes on with its first
+        const size_t part = (size_t)head * BM * 2 * a.target + (size_t)group * 2 + (group == (int)(tile_at / each) ? 1 : 0);
+        uint8_t *out = a.out + (size_t)seq * a.ostride + (size_t)(head * a.G + tile * BM) * dim * (F32 ? 4 : 2);
+        for (int e = threadIdx.x; e < BM * (DP / 4); e += 256) {
+            const int row = e / (DP / 4), d = e % (DP / 4) * 4;
+            if (tile * BM + row >= rows || d >= dim) continue;
+            float mm = LOWEST;
+#pragma unroll
+            for (int w = 0; w < 4; w++) mm = fmaxf(mm, lm[w][row]);
+            float sum = 0.0f, x[4] = {0, 0, 0, 0};
+#pragma unroll
+            for (int w = 0; w < 4; w++) {
+                const float f = __builtin_amdgcn_exp2f(lm[w][row] - reference(mm));
+                sum += f * ll[w][row];
+#pragma unroll
+                for (int i = 0; i < 4; i++) x[i] += f * lo_acc[w][row][d + i];
+            }
+            if (whole) {
+                const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
+#pragma unroll
+                for (int i = 0; i < 4; i++) x[i] = sum == 0.0f ? 0.0f : x[i] * inv;
+                store4<F32, BF>(out + (size_t)row * dim * (F32 ? 4 : 2), d, x);
+            } else {
+                const size_t at = part + (size_t)row * 2 * a.target;
+                if (d == 0) a.pml[at] = float2{mm, sum};
+                *reinterpret_cast<f4 *>(a.po + at * dim + d) = f4{x[0], x[1], x[2], x[3]};
+            }
+        }
+        __syncthreads();   // the next tile's sums go where these were
     }
+}
+
+// The parts of `together` rows of a tile a workgroup (a power of two), dim / 4 threads (rounded up to 16, 32 or 64) to a row and the 256 / that /
+// together such groups of a row sharing its parts: each group finds the weights 2^(m - the largest m) for itself, in LDS. The sums' first loads, which
+// need no weights, go out before them; what order they are added in, the lengths alone give.
+template <bool F32, bool BF> __global__ __launch_bounds__(256) void attn_decode_join_kernel(AttnArgs a, int together) {
+    constexpr int BM = DECODE_M, AHEAD = 16, MOST = 512;
+    const int tiles = (a.G + BM - 1) / BM, dim = a.c.dim, quads = dim / 4;
+    const int w = quads <= 16 ? 16 : quads <= 32 ? 32 : 64, d = threadIdx.x % w, k = threadIdx.x / w, shares = 256 / w / together;
+    const int blocks_per_head = (a.G + together - 1) / together;
+    const int seq = blockIdx.x / (a.c.heads * blocks_per_head), rest = blockIdx.x - seq * (a.c.heads * blocks_per_head);
+    const int head = rest / blocks_per_head, r0 = (rest - head * blocks_per_head) * together;   // (together divides 16: rows of one tile)
+    Deal deal(a, tiles);
+    while (seq >= deal.group + 64) deal.next(a, tiles);
+    int base;
+    const int blocks = blocks_of(a, __builtin_amdgcn_readlane(deal.bl.len, seq - deal.group), base);
+    const uint32_t at = deal.first_of(seq - deal.group) + (uint32_t)(r0 / BM) * blocks;
+    const uint32_t from = at / deal.each, parts = (at + blocks - 1) / deal.each - from + 1;
+    if (parts == 1 || parts > MOST || from + parts > (uint32_t)a.target) return;   // (one: written already; the others cannot be while the lengths stay)
+    const int r = r0 + k % together, share = k / together;
+    // the row's part in group from + n: the first is its group's second
+    const size_t part0 = ((size_t)head * BM + min(r, a.G - 1) % BM) * 2 * a.target + (size_t)from * 2;
+    auto part = [&](uint32_t n) { return part0 + (n ? n * 2 : 1); };
+    const float *sums = a.po + min(d, quads - 1) * 4;
+    f4 v[AHEAD];   // (a part that there is not: the last again, at weight 0)
 #pragma unroll
-    for (int i = 0; i < 4; i++)
-#pragma unroll
-        for (int j = 0; j < DL; j += 4)
-            *reinterpret_cast<f4 *>(&lo_acc[wave][col][(g * 4 + i) * DL + j]) = f4{acc[j][i], acc[j + 1][i], acc[j + 2][i], acc[j + 3][i]};
+    for (int i = 0; i < AHEAD; i++) v[i] = *reinterpret_cast<const f4 *>(sums + part(min((uint32_t)(share + i * shares), parts - 1)) * dim);
+
+    __shared__ float wt[16][MOST];
+    __shared__ f4 sx[256];
+    float m = LOWEST, l = 0.0f;
+    for (uint32_t n = d; n < parts; n += w) {
+        const float2 ml = a.pml[part(n)];
+        if (ml.y != 0.0f) m = fmaxf(m, ml.x);
+    }
+    for (int o = w / 2; o; o >>= 1) m = fmaxf(m, __shfl_xor(m, o));
+    for (uint32_t n = d; n < parts; n += w) {
+        const float2 ml = a.pml[part(n)];
+        const float f = ml.y != 0.0f ? __builtin_amdgcn_exp2f(ml.x - reference(m)) : 0.0f;
+        wt[k][n] = f;
+        l += f * ml.y;
+    }
+    for (int o = w / 2; o; o >>= 1) l += __shfl_xor(l, o);
     __syncthreads();
-    const size_t slot = (size_t)item * a.c.heads + head;
-    for (int e = threadIdx.x; e < BM * (DP / 4); e += 256) {
-        const int row = e / (DP / 4), d = e % (DP / 4) * 4;
-        if (p.tile * BM + row >= rows || d >= a.c.dim) continue;
-        float mm = LOWEST;
+    f4 x = {0, 0, 0, 0};
 #pragma unroll
-        for (int w = 0; w < 4; w++) mm = fmaxf(mm, lm[w][row]);
-        float sum = 0.0f, x[4] = {0, 0, 0, 0};
+    for (int n = 0; n < AHEAD; n++) {
+        const int i = share + n * shares;
+        const float f = i < (int)parts ? wt[k][i] : 0.0f;
 #pragma unroll
-        for (int w = 0; w < 4; w++) {
-            const float f = __builtin_amdgcn_exp2f(lm[w][row] - reference(mm));
-            sum += f * ll[w][row];
-#pragma unroll
-            for (int i = 0; i < 4; i++) x[i] += f * lo_acc[w][row][d + i];
-        }
-        if (p.chunks == 1) {
-            const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
-#pragma unroll
-            for (int i = 0; i < 4; i++) x[i] = sum == 0.0f ? 0.0f : x[i] * inv;
-            store4<F32, BF>(a.out + (size_t)p.s.t0 * a.ostride + (size_t)(head * a.G + p.tile * BM + row) * a.c.dim * (F32 ? 4 : 2), d, x);
-        } else {
-            if (d == 0) a.pml[slot * BM + row] = float2{mm, sum};
-            *reinterpret_cast<f4 *>(a.po + (slot * BM + row) * a.c.dim + d) = f4{x[0], x[1], x[2], x[3]};
-        }
+        for (int j = 0; j < 4; j++) x[j] = __builtin_fmaf(f, v[n][j], x[j]);
     }
+    for (uint32_t n = share + AHEAD * shares; n < parts; n += shares) {
+        const f4 y = *reinterpret_cast<const f4 *>(sums + part(n) * dim);
+#pragma unroll
+        for (int j = 0; j < 4; j++) x[j] = __builtin_fmaf(wt[k][n], y[j], x[j]);
+    }
+    sx[threadIdx.x] = x;
+    __syncthreads();
+    if (share || d >= quads || r >= a.G) return;
+    for (int g = 1; g < shares; g++)
+#pragma unroll
+        for (int j = 0; j < 4; j++) x[j] += sx[(g * together + k) * w + d][j];
+    float o[4];
+    const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+#pragma unroll
+    for (int j = 0; j < 4; j++) o[j] = l == 0.0f ? 0.0f : x[j] * inv;
+    store4<F32, BF>(a.out + (size_t)seq * a.ostride + (size_t)(head * a.G + r) * dim * (F32 ? 4 : 2), d * 4, o);
 }
 
 // ---- a tile of prompt rows -------------------------------------------------------------------------------------------------------
@@ -486,8 +621,6 @@ template <bool BF, int NQ, int DP> __global__ __launch_bounds__(256, DP == 256 ?
 // consecutive rows, whose pitch of 36 words spreads them over the banks (and the eight lanes of a read), and a lane ends with runs of VE elements.
 // Keys that a row does not see have weight 0, and 0 times an infinity or NaN is not 0: V rows that no row sees are staged as zeros, and
 // so are such elements of keys that only some rows see; where there were any, they are added to those rows at the end.
-constexpr int PM = 128, PN = 64;
-
 template <bool BF, int NQ, int DP> __global__ __launch_bounds__(256, DP == 256 || NQ == 3 ? 1 : 2) void attn_prompt_kernel(AttnArgs a) {
     constexpr int KS = DP / 16, DT = DP / 32, KC = DP / 8;
     constexpr int KP = DP + 8;            // LDS pitch of K, elements
@@ -500,9 +633,9 @@ template <bool BF, int NQ, int DP> __global__ __launch_bounds__(256, DP == 256 |
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int col = lane & 31, half = lane >> 5;
     const int head = blockIdx.x % a.c.heads, item = blockIdx.x / a.c.heads;
-    const int chunk = chunk_of(a, PM);
+    const int chunk = chunk_of(a);
     Part p;
-    if (!part_of(a, item, chunk, PM, p)) return;
+    if (!part_of(a, item, chunk, p)) return;
     const bool whole = chunk == 1 << 30;
     const int tile = p.s.tiles - 1 - p.tile;   // the tiles that see most keys first
     const int rows = min(PM, p.s.n * a.G - tile * PM);
@@ -557,14 +690,14 @@ template <bool BF, int NQ, int DP> __global__ __launch_bounds__(256, DP == 256 |
         int holes = 0;
         auto run = [&](const uint8_t *pool, int sub) {
             const int u = (t0 >> 4) + sub;
-            return Run(a.c, pool, __builtin_amdgcn_readlane(pg, u0 + sub), head, (u & ((1 << shift16) - 1)) << 4, last - u * 16);
+            return Run<false>(a.c, pool, __builtin_amdgcn_readlane(pg, u0 + sub), head, (u & ((1 << shift16) - 1)) << 4, last - u * 16);
         };
 #pragma unroll
         for (int u = 0; u < 4; u++) holes |= __builtin_amdgcn_readlane(pg, u0 + u) < 0 ? 1 << u : 0;
 #pragma unroll
         for (int i = 0; i < NK; i++)   // pieces i: tokens kt + i * (256 / KC)
             kr[i] = run(a.c.k, KC == 8 ? (wave >> 1) + 2 * i : KC == 16 ? i : i >> 1).load16(k_off, KC == 32 ? (i & 1) * 16 * dim : 0);
-        const Run v = run(a.c.v, wave);
+        const Run<false> v = run(a.c.v, wave);
 #pragma unroll
         for (int k = 0; k < 4; k++) {   // (elements past dim: others' in their place, in rows of O^T that are not written)
             if constexpr (VE == 4) {
@@ -757,74 +890,51 @@ template <bool BF, int NQ, int DP> __global__ __launch_bounds__(256, DP == 256 |
 }
 
 // ---- parts joined ------------------------------------------------------------------------------------------------------------
-// out of a row = sum over its parts of 2^(m of the part - the largest m) * (the part's sum), over the same of l: the weights first, in LDS,
-// then the sums in the order of the parts, dim / 4 threads (rounded up to 16, 32 or 64) a row. One query per sequence has few rows of many
-// parts: a workgroup then takes one row and each of its groups a share of the parts (ONE); a prompt's takes as many rows as it has groups.
+// out of a prompt's row = sum over its parts of 2^(m of the part - the largest m) * (the part's sum), over the same of l: the weights first,
+// in LDS, then the sums in the order of the parts, dim / 4 threads (rounded up to 16, 32 or 64) a row, as many rows as that gives a workgroup.
 constexpr int PARTS = 512;   // workgroups that a call is split into, about: two per CU
-template <bool F32, bool BF, int BM, bool ONE> __global__ __launch_bounds__(256) void attn_join_kernel(AttnArgs a) {
+template <bool F32, bool BF> __global__ __launch_bounds__(256) void attn_join_kernel(AttnArgs a) {
     const int quads = a.c.dim / 4, w = quads <= 16 ? 16 : quads <= 32 ? 32 : 64;   // threads per row
     const int d = threadIdx.x % w, k = threadIdx.x / w, groups = 256 / w;
-    const int blocks = ONE ? min(BM, a.G) : BM / groups;   // workgroups per tile
+    const int blocks = PM / groups;   // workgroups per tile
     const int head = blockIdx.x % a.c.heads, block = blockIdx.x / a.c.heads % blocks;
-    const int chunk = chunk_of(a, BM);
+    const int chunk = chunk_of(a);
     Part p;
-    if (!part_of<true>(a, blockIdx.x / a.c.heads / blocks, chunk, BM, p) || p.chunks == 1) return;   // (one part: written already)
+    if (!part_of<true>(a, blockIdx.x / a.c.heads / blocks, chunk, p) || p.chunks == 1) return;   // (one part: written already)
     const uint32_t first = p.first + (uint32_t)p.tile * (uint32_t)p.chunks;
-    const int tile = a.start ? p.s.tiles - 1 - p.tile : p.tile;
-    const int rows = min(BM, p.s.n * a.G - tile * BM), row = ONE ? block : block * groups + k;
-    if ((ONE ? row : block * groups) >= rows || p.chunks > PARTS + 1 || (size_t)first + p.chunks > (size_t)a.items) return;   // (the latter two: starts out of order)
-    const size_t at = ((size_t)first * a.c.heads + head) * BM + min(row, rows - 1), step = (size_t)a.c.heads * BM;
+    const int tile = p.s.tiles - 1 - p.tile;
+    const int rows = min(PM, p.s.n * a.G - tile * PM), row = block * groups + k;
+    if (block * groups >= rows || p.chunks > PARTS + 1 || (size_t)first + p.chunks > (size_t)a.items) return;   // (the latter two: starts out of order)
+    const size_t at = ((size_t)first * a.c.heads + head) * PM + min(row, rows - 1), step = (size_t)a.c.heads * PM;
 
-    __shared__ float wt[ONE ? 1 : 16][PARTS + 1];
-    __shared__ float sm[4], sl[4];
-    __shared__ f4 sx[256];
-    float *f = wt[ONE ? 0 : k];
-    const int lanes = ONE ? 256 : w, t = ONE ? threadIdx.x : d;
+    __shared__ float wt[16][PARTS + 1];
+    float *f = wt[k];
     float m = LOWEST;
-    for (int c = t; c < p.chunks; c += lanes) {
+    for (int c = d; c < p.chunks; c += w) {
         const float2 ml = a.pml[at + c * step];
         if (ml.y != 0.0f) m = fmaxf(m, ml.x);
     }
-    for (int o = (ONE ? 64 : w) / 2; o; o >>= 1) m = fmaxf(m, __shfl_xor(m, o));
-    if constexpr (ONE) {
-        if ((threadIdx.x & 63) == 0) sm[threadIdx.x >> 6] = m;
-        __syncthreads();
-        m = fmaxf(fmaxf(sm[0], sm[1]), fmaxf(sm[2], sm[3]));
-    }
+    for (int o = w / 2; o; o >>= 1) m = fmaxf(m, __shfl_xor(m, o));
     float l = 0.0f;
-    for (int c = t; c < p.chunks; c += lanes) {
+    for (int c = d; c < p.chunks; c += w) {
         const float2 ml = a.pml[at + c * step];
         const float x = ml.y != 0.0f ? __builtin_amdgcn_exp2f(ml.x - reference(m)) : 0.0f;
         f[c] = x;
         l += x * ml.y;
     }
-    for (int o = (ONE ? 64 : w) / 2; o; o >>= 1) l += __shfl_xor(l, o);
-    if constexpr (ONE) {
-        if ((threadIdx.x & 63) == 0) sl[threadIdx.x >> 6] = l;
-    }
+    for (int o = w / 2; o; o >>= 1) l += __shfl_xor(l, o);
     __syncthreads();
-    if constexpr (ONE) l = (sl[0] + sl[1]) + (sl[2] + sl[3]);
-    f4 x = {0, 0, 0, 0};
-    if (d < quads) {
-        const float *y = a.po + at * a.c.dim + d * 4;
-        const size_t pitch = step * a.c.dim;
-#pragma unroll 8
-        for (int c = ONE ? k : 0; c < p.chunks; c += ONE ? groups : 1) {
-            const f4 v = *reinterpret_cast<const f4 *>(y + c * pitch);
-#pragma unroll
-            for (int i = 0; i < 4; i++) x[i] = __builtin_fmaf(f[c], v[i], x[i]);
-        }
-    }
-    if constexpr (ONE) {
-        sx[threadIdx.x] = x;
-        __syncthreads();
-        if (k) return;
-        for (int g = 1; g < groups; g++)
-#pragma unroll
-            for (int i = 0; i < 4; i++) x[i] += sx[g * w + d][i];
-    }
     if (d >= quads || row >= rows) return;
-    const int r = tile * BM + row, query = r / a.G;
+    f4 x = {0, 0, 0, 0};
+    const float *y = a.po + at * a.c.dim + d * 4;
+    const size_t pitch = step * a.c.dim;
+#pragma unroll 8
+    for (int c = 0; c < p.chunks; c++) {
+        const f4 v = *reinterpret_cast<const f4 *>(y + c * pitch);
+#pragma unroll
+        for (int i = 0; i < 4; i++) x[i] = __builtin_fmaf(f[c], v[i], x[i]);
+    }
+    const int r = tile * PM + row, query = r / a.G;
     float o[4];
     const float inv = l == 0.0f ? 0.0f : 1.0f / l;
 #pragma unroll
@@ -833,23 +943,34 @@ template <bool F32, bool BF, int BM, bool ONE> __global__ __launch_bounds__(256)
 }
 
 // ---- host ------------------------------------------------------------------------------------------------------------------------
-constexpr int DECODE_M = 16;
-
 struct Shape {
-    size_t tiles;   // the most tiles per K/V head that the call's lengths can give
-    int target;     // AttnArgs::target
+    size_t items;      // prompt: the most parts per K/V head that the call's lengths can give; else workgroups per K/V head
+    size_t tiles;      // prompt: the most tiles
+    int target;        // AttnArgs::target
+    int block;         // AttnArgs::block
+    size_t slots;      // parts per K/V head that the workspace holds
     int bm;
-    size_t items() const { return tiles + (size_t)target; }   // sum of tiles * ceil(span / chunk) <= target + tiles
-    size_t workspace(const es_hip_kv *kv) const { return target ? items() * kv->heads * bm * (kv->dim + 2) * sizeof(float) : 0; }
+    size_t sums(const es_hip_kv *kv) const { return slots * kv->heads * bm * (size_t)kv->dim * sizeof(float); }
+    size_t workspace(const es_hip_kv *kv) const { return sums(kv) + slots * kv->heads * bm * sizeof(float2); }
 };
 Shape shape_of(const es_hip_kv *kv, int nseq, int ntok, int heads, bool prompt) {
     const int G = heads / kv->heads;
-    Shape s;
-    s.bm = prompt ? PM : DECODE_M;
-    s.tiles = prompt ? (size_t)ntok * G / PM + nseq : (size_t)nseq * ((G + DECODE_M - 1) / DECODE_M);
-    const int parts = std::max(PARTS / kv->heads, 1);
-    const bool many = prompt && s.tiles >= (size_t)parts;
-    s.target = many || (long long)kv->max_pages * kv->page <= CHUNK_MIN ? 0 : parts;
+    const long long most = (long long)kv->max_pages * kv->page;
+    Shape s{};
+    if (prompt) {
+        s.bm = PM;
+        s.tiles = (size_t)ntok * G / PM + nseq;
+        const int parts = std::max(PARTS / kv->heads, 1);
+        s.target = s.tiles >= (size_t)parts || most <= CHUNK_MIN ? 0 : parts;
+        s.items = s.tiles + s.target;   // sum of tiles * ceil(span / chunk) <= tiles + target
+        s.slots = s.target ? s.items : 0;
+    } else {
+        s.bm = DECODE_M;
+        s.target = std::max(decode_groups(kv->dim) / kv->heads, 1);
+        s.items = s.target;
+        s.block = most <= 1 << BLOCK_WHOLE ? BLOCK_WHOLE : BLOCK;
+        s.slots = most > 1 << s.block ? 2 * s.items : 0;   // (0: every tile is one block)
+    }
     return s;
 }
 
@@ -860,23 +981,31 @@ int check_heads(const es_hip_kv *kv, int nseq, int ntok, int heads, KvView &v) {
     // (a launch holds 2^24 workgroups of 256)
     if ((long long)ntok * heads > 1 << 29 || (long long)nseq * heads > 1 << 23)
         return host_fail(ES_HIP_EINVAL, "more than 2^29 query rows, or 2^23 sequences times heads");
+    if (nseq && ((long long)kv->max_pages * kv->page / (1 << BLOCK) + 2) * nseq * (heads / kv->heads / DECODE_M + 1) > 1LL << 31)
+        return host_fail(ES_HIP_EINVAL, "more than 2^31 blocks of 128 keys");
     return ES_HIP_OK;
 }
 
 template <bool BF, int NQ> hipError_t launch(const AttnArgs &a, const Shape &s, bool prompt, hipStream_t st) {
-    const size_t grid = s.items() * a.c.heads;
-    if (prompt) {
-        auto f = a.c.dim <= 64 ? attn_prompt_kernel<BF, NQ, 64> : a.c.dim <= 128 ? attn_prompt_kernel<BF, NQ, 128> : attn_prompt_kernel<BF, NQ, 256>;
-        f<<<(unsigned)grid, 256, 0, st>>>(a);
-    } else {
+    const unsigned grid = (unsigned)(s.items * a.c.heads);
+    if (!prompt) {
         auto f = a.c.dim <= 64 ? attn_decode_kernel<BF, NQ, 64> : a.c.dim <= 128 ? attn_decode_kernel<BF, NQ, 128> : attn_decode_kernel<BF, NQ, 256>;
-        f<<<(unsigned)grid, 256, 0, st>>>(a);
+        f<<<grid, 256, 0, st>>>(a);
+        if (hipError_t e = hipGetLastError()) return e;
+        if (!s.slots) return hipSuccess;
+        // one row a workgroup where that leaves few of them, as many as it has groups of threads where there are many
+        const int groups = a.c.dim <= 64 ? 16 : a.c.dim <= 128 ? 8 : 4;
+        int together = 1;
+        while (together < groups && together < a.G && (long long)a.nseq * a.c.heads * ((a.G + together - 1) / together) > 256) together *= 2;
+        attn_decode_join_kernel<(NQ > 1), BF><<<(unsigned)((size_t)a.nseq * a.c.heads * ((a.G + together - 1) / together)), 256, 0, st>>>(a, together);
+        return hipGetLastError();
     }
+    auto f = a.c.dim <= 64 ? attn_prompt_kernel<BF, NQ, 64> : a.c.dim <= 128 ? attn_prompt_kernel<BF, NQ, 128> : attn_prompt_kernel<BF, NQ, 256>;
+    f<<<grid, 256, 0, st>>>(a);
     hipError_t e = hipGetLastError();
     if (e != hipSuccess || !s.target) return e;
     const int groups = a.c.dim <= 64 ? 16 : a.c.dim <= 128 ? 8 : 4;   // rows that a workgroup joins
-    auto f = prompt ? attn_join_kernel<(NQ > 1), BF, PM, false> : attn_join_kernel<(NQ > 1), BF, DECODE_M, true>;
-    f<<<(unsigned)(s.tiles * a.c.heads * (prompt ? PM / groups : std::min(DECODE_M, a.G))), 256, 0, st>>>(a);
+    attn_join_kernel<(NQ > 1), BF><<<(unsigned)(s.tiles * a.c.heads * (PM / groups)), 256, 0, st>>>(a);
     return hipGetLastError();
 }
 
@@ -904,7 +1033,7 @@ int attention(const es_hip_kv *kv, int nseq, const int *start, int ntok, int hea
     a.q = static_cast<const uint8_t *>(q);
     a.out = static_cast<uint8_t *>(out);
     a.po = static_cast<float *>(ws);
-    a.pml = reinterpret_cast<float2 *>(a.po + (need ? s.items() * kv->heads * s.bm * (size_t)kv->dim : 0));
+    a.pml = reinterpret_cast<float2 *>(static_cast<uint8_t *>(ws) + s.sums(kv));
     a.qstride = qstride * es;
     a.ostride = ostride * es;
     a.nseq = nseq;
@@ -913,7 +1042,8 @@ int attention(const es_hip_kv *kv, int nseq, const int *start, int ntok, int hea
     a.window = window;
     a.c2 = std::max(scale * 1.44269504088896340736f, 1.17549435e-38f);
     a.target = s.target;
-    a.items = (int)s.items();
+    a.block = s.block;
+    a.items = (int)s.items;
     const hipStream_t st = static_cast<hipStream_t>(stream);
     hipError_t e;
     if (kv->type == ES_HIP_BF16) e = type == ES_HIP_F32 ? launch<true, 3>(a, s, prompt, st) : launch<true, 1>(a, s, prompt, st);

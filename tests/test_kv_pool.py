@@ -256,7 +256,7 @@ out.update({
 })
 launched = counts[0]
 fine = {"append": ap(k), "same type": ap(k, t=E.F16), "decode": de(k), "prompt": pr(k), "copy": cp(k), "none": ap(k, ntok=0, start=P), "empty": de(k, nseq=0),
-        "no copy": cp(k, s=[], d=[]), "no layers": cp(k, nl=0), "short": code(L.attn_decode_dev, kv(max_pages=8), 3, 32, E.F32, P, 0, 0.1, 0, P, 0, None, 0)}
+        "no copy": cp(k, s=[], d=[]), "no layers": cp(k, nl=0), "short": code(L.attn_decode_dev, kv(max_pages=32), 3, 32, E.F32, P, 0, 0.1, 0, P, 0, None, 0)}
 print(json.dumps({"bad": out, "launched": launched, "fine": fine, "after": [counts[i] for i in range(5)]}))
 """
 
@@ -278,7 +278,7 @@ def one(f, *a):
     f(*a)
     return [[shapes[(n + i) % 64][j] for j in range(4)] for i in range(counts[0] - n)]
 for nseq, heads, kvh, maxp, ntok in [(1, 32, 4, 8, 1), (1, 32, 4, 8192, 1), (48, 14, 2, 400, 48), (600, 32, 8, 64, 600), (2, 71, 1, 64, 2),
-                                     (3, 32, 32, 9, 3)]:
+                                     (3, 32, 32, 33, 3)]:
     k = kv(heads=kvh, rows=nseq, max_pages=maxp)
     ws = L.attn_decode_workspace(k, nseq, heads)
     rows.append(["decode", nseq, heads, kvh, maxp * 16, ws, one(L.attn_decode_dev, k, nseq, heads, E.F32, P, 0, 0.1, 0, P, 0, P, ws)])
@@ -291,26 +291,39 @@ print(json.dumps(rows))
 
 
 def test_every_part_has_room(child):
-    """for any lengths: the parts that chunks of equal length give never outnumber the grid, nor their sums the workspace"""
+    """for any lengths: a prompt's parts never outnumber the grid, nor their sums the workspace; a decode call's blocks are dealt
+    out whole, each group begins at most one tile that others go on with, and the workspace holds two parts a group"""
     for kind, nseq, heads, kvh, tokens, ws, launches in child(GRIDS):
         G = heads // kvh
         grid = launches[0][0]
         assert grid % kvh == 0
-        assert (len(launches) == 2) == (ws > 0)
         rng = np.random.default_rng(1)
         for _ in range(200):
             if kind == "decode":
-                n, span, bm = np.ones(nseq, int), rng.integers(0, tokens + 1, nseq), 16
-            else:
-                cut = np.sort(rng.integers(0, tokens + 1, nseq - 1))
-                n, span, bm = np.diff(np.concatenate([[0], cut, [tokens]])), rng.integers(0, 1 << 20, nseq), 128
-            tiles = -(-n * G // bm)
+                assert len(launches) == (2 if ws else 1)
+                groups, tiles = grid // kvh, -(-G // 16)
+                assert (ws > 0) == (tokens > 512)
+                blocks = np.repeat(np.maximum(1, -(-rng.integers(0, tokens + 1, nseq) // (128 if ws else 512))), tiles)
+                at = np.concatenate([[0], np.cumsum(blocks)])
+                each = -(-at[-1] // groups)
+                a, b = at[:-1] // each, (at[1:] - 1) // each
+                assert b.max() < groups
+                begun = a[b > a]
+                assert len(set(begun)) == len(begun)
+                if ws:
+                    assert ws >= 2 * groups * kvh * 16 * (128 + 2) * 4
+                else:
+                    assert not len(begun)
+                continue
+            cut = np.sort(rng.integers(0, tokens + 1, nseq - 1))
+            n, span = np.diff(np.concatenate([[0], cut, [tokens]])), rng.integers(0, 1 << 20, nseq)
+            tiles = -(-n * G // 128)
+            assert len(launches) == (2 if ws else 1)
             if ws:   # the chunk that the device takes: total work over the parts aimed for
-                base = nseq * -(-G // 16) if kind == "decode" else tokens * G // 128 + nseq
-                target = grid // kvh - base
+                target = grid // kvh - (tokens * G // 128 + nseq)
                 chunk = max(128, -(-(-(-int((tiles * span).sum()) // target)) // 128) * 128)
                 parts = (tiles * np.maximum(1, -(-span // chunk))).sum()
-                assert ws >= parts * kvh * bm * (128 + 2) * 4
+                assert ws >= parts * kvh * 128 * (128 + 2) * 4
             else:
                 parts = tiles.sum()
             assert parts * kvh <= grid
