@@ -333,8 +333,7 @@ template <bool BF, int NQ, int DP> __global__ __launch_bounds__(256, DP == 64 &&
     constexpr bool F32 = NQ > 1;
     __shared__ float lm[4][BM], ll[4][BM];
     __shared__ __attribute__((aligned(16))) float lo_acc[4][BM][DP + 4];
-    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const int col = lane & 15, g = lane >> 4;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int head = blockIdx.x % a.c.heads, group = blockIdx.x / a.c.heads;
     const int rows = a.G, tiles = (a.G + BM - 1) / BM, dim = a.c.dim;
     const int shift16 = a.c.shift - 4;
@@ -342,6 +341,9 @@ template <bool BF, int NQ, int DP> __global__ __launch_bounds__(256, DP == 64 &&
     Deal deal(a, tiles);
     const uint32_t each = deal.each, end = min(deal.total, (group + 1) * each);
     for (uint32_t pos = group * each; pos < end;) {
+        int tid = threadIdx.x;
+        asm volatile("" : "+v"(tid));   // (or every address that depends on it is computed ahead of the loop, and kept in registers that the loop lacks)
+        const int lane = tid & 63, col = lane & 15, g = lane >> 4;
         unsigned long long past;
         while (!(past = __ballot(pos < deal.before + deal.bl.upto))) {
             deal.next(a, tiles);
@@ -516,7 +518,7 @@ template <bool BF, int NQ, int DP> __global__ __launch_bounds__(256, DP == 64 &&
         // a group's part of a tile that it begins is its second in the workspace, of one that it goes on with its first
         const size_t part = (size_t)head * BM * 2 * a.target + (size_t)group * 2 + (group == (int)(tile_at / each) ? 1 : 0);
         uint8_t *out = a.out + (size_t)seq * a.ostride + (size_t)(head * a.G + tile * BM) * dim * (F32 ? 4 : 2);
-        for (int e = threadIdx.x; e < BM * (DP / 4); e += 256) {
+        for (int e = tid; e < BM * (DP / 4); e += 256) {
             const int row = e / (DP / 4), d = e % (DP / 4) * 4;
             if (tile * BM + row >= rows || d >= dim) continue;
             float mm = LOWEST;
