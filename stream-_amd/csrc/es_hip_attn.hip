@@ -252,14 +252,26 @@ template <bool F32, bool BF> __device__ void store4(uint8_t *row, int d, const f
     }
 }
 
-// A run of 16 keys of one page, or as many of them as there are, for loads whose offsets count from its first row: what lies past its end reads as
-// zeros, and all of a run that is in no page (the bounds are the loads' own; no address needs a lane's registers but its offset). ONCE: nobody else
-// reads them soon (a non-temporal load).
+// Where runs of 16 keys of a sequence and head begin, one run per lane: bytes from a pool's start, negative in the upper half where the run is in
+// no page (or past `last`).
+struct Runs {
+    int lo, hi;
+    __device__ Runs(const KvView &c, const int *table, int head, int run, int last) {
+        const int page = run * 16 < last ? table[run >> (c.shift - 4)] : -1;
+        const size_t at = c.at(page, head, (run & ((1 << (c.shift - 4)) - 1)) << 4);
+        lo = (int)(uint32_t)at;
+        hi = page < 0 || page >= c.npages ? -1 : (int)(at >> 32);
+    }
+    __device__ bool none(int lane) const { return __builtin_amdgcn_readlane(hi, lane) < 0; }
+};
+// One of them, for loads whose offsets count from its first row: what lies past its `bytes` reads as zeros, and so does all of a run that is in no
+// page (the bounds are the loads' own; an address needs no lane's registers but its offset). ONCE: nobody else reads it soon (non-temporal).
 template <bool ONCE> struct Run {
     __amdgpu_buffer_rsrc_t r;
-    __device__ Run(const KvView &c, const uint8_t *pool, int page, int head, int token, int keys) {
-        const uint8_t *at = pool + c.at(max(page, 0), head, token);
-        r = __builtin_amdgcn_make_buffer_rsrc(const_cast<uint8_t *>(at), (short)0, page < 0 ? 0 : min(keys, 16) * c.dim * 2, 0x00020000);
+    __device__ Run(const uint8_t *pool, const Runs &all, int lane, int bytes) {
+        const int hi = __builtin_amdgcn_readlane(all.hi, lane);
+        const uint64_t at = (uint64_t)(uint32_t)max(hi, 0) << 32 | (uint32_t)__builtin_amdgcn_readlane(all.lo, lane);
+        r = __builtin_amdgcn_make_buffer_rsrc(const_cast<uint8_t *>(pool + at), (short)0, hi < 0 ? 0 : bytes, 0x00020000);
     }
     __device__ u4 load16(int lane_offset, int offset) const {
         return __builtin_bit_cast(u4, __builtin_amdgcn_raw_buffer_load_b128(r, lane_offset, offset, ONCE ? 2 : 0));
@@ -336,7 +348,6 @@ template <bool BF, int NQ, int DP> __global__ __launch_bounds__(256, DP == 64 &&
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int head = blockIdx.x % a.c.heads, group = blockIdx.x / a.c.heads;
     const int rows = a.G, tiles = (a.G + BM - 1) / BM, dim = a.c.dim;
-    const int shift16 = a.c.shift - 4;
 
     Deal deal(a, tiles);
     const uint32_t each = deal.each, end = min(deal.total, (group + 1) * each);
@@ -370,21 +381,15 @@ template <bool BF, int NQ, int DP> __global__ __launch_bounds__(256, DP == 64 &&
         for (int j = 0; j < DL; j++) acc[j] = f4{0, 0, 0, 0};
         float m = LOWEST, l = 0.0f;
 
-        // This wave's keys of step n: 32 from first + (4 n + wave) * 32 on, two runs of 16. Lane 2 i + h holds the page of run h of step
-        // 32 s + i (-1: none), of the 32 steps at hand and of the 32 after them.
-        auto fetch = [&](int n) {
-            const int u = (first >> 4) + ((n + (lane >> 1)) * 4 + wave) * 2 + (lane & 1);
-            const int page = u * 16 < last ? table[u >> shift16] : -1;
-            return page < a.c.npages ? page : -1;
-        };
-        int pg = fetch(0), pgn = fetch(32);
+        // This wave's keys of step n: 32 from first + (4 n + wave) * 32 on, two runs of 16. Lane 2 i + h holds where run h of step
+        // 32 s + i begins, of the 32 steps at hand and of the 32 after them.
+        auto fetch = [&](int n) { return Runs(a.c, table, head, (first >> 4) + ((n + (lane >> 1)) * 4 + wave) * 2 + (lane & 1), last); };
+        Runs pg = fetch(0), pgn = fetch(32);
         const int kd = (col * dim + g * 8) * 2, vd = (g * 4 * dim + col * DL) * 2;
         u4 kr[2][KS];             // run h, elements s * 32 + g * 8 of key col
         uint32_t vr[8][DL / 2];   // DL elements of the keys g * 4 + i (first four) and 16 + g * 4 + i
-        auto page_of = [&](int n, int h) { return __builtin_amdgcn_readlane(pg, (n & 31) * 2 + h); };
         auto run = [&](const uint8_t *pool, int n, int h) {
-            const int u = (first >> 4) + (n * 4 + wave) * 2 + h;
-            return Run<true>(a.c, pool, page_of(n, h), head, (u & ((1 << shift16) - 1)) << 4, last - u * 16);
+            return Run<true>(pool, pg, (n & 31) * 2 + h, min(last - (first + (n * 4 + wave) * 32 + h * 16), 16) * dim * 2);
         };
         auto load_k = [&](int n) {
 #pragma unroll
@@ -419,8 +424,8 @@ template <bool BF, int NQ, int DP> __global__ __launch_bounds__(256, DP == 64 &&
         const int mine = first + wave * 32, steps = mine < last ? (last - mine + 127) / 128 : 0;
         bool ok[2] = {false, false};
         if (steps > 0) {
-            ok[0] = page_of(0, 0) >= 0;
-            ok[1] = page_of(0, 1) >= 0;
+            ok[0] = !pg.none(0);
+            ok[1] = !pg.none(1);
             load_k(0);
             load_v(0);
         }
@@ -446,8 +451,8 @@ template <bool BF, int NQ, int DP> __global__ __launch_bounds__(256, DP == 64 &&
                     pg = pgn;
                     pgn = fetch(n + 33);
                 }
-                ok[0] = page_of(n + 1, 0) >= 0;
-                ok[1] = page_of(n + 1, 1) >= 0;
+                ok[0] = !pg.none((n + 1 & 31) * 2);
+                ok[1] = !pg.none((n + 1 & 31) * 2 + 1);
                 load_k(n + 1);
             }
             if (t0 < lo || t0 + 32 > last || !ok0 || !ok1) {   // what is not to be seen: no score, and zeros for whatever V holds
@@ -647,7 +652,6 @@ template <bool BF, int NQ, int DP> __global__ __launch_bounds__(256, DP == 256 |
     int first = p.s.base + (whole ? 0 : p.chunk * chunk);
     const int last = whole ? see_hi : min(see_hi, first + chunk);
     first = max(first, see_lo & ~(PN - 1));
-    const int shift16 = a.c.shift - 4;
     const int *table = a.c.table + (size_t)max(a.c.row(p.b), 0) * a.c.max_pages;
     const int dim = a.c.dim;
     const bool padded = dim < DP;
@@ -668,12 +672,10 @@ template <bool BF, int NQ, int DP> __global__ __launch_bounds__(256, DP == 256 |
         for (int i = 0; i < 16; i++) acc[j][i] = 0.0f;
     float m = LOWEST, l = 0.0f;
 
-    // the pages of 64 runs of 16 keys from run `pb` on, one per lane (-1: none), and of the 64 after them
-    auto fetch = [&](int u) {
-        const int g = u * 16 < last ? table[u >> shift16] : -1;
-        return g < a.c.npages ? g : -1;
-    };
-    int pb = first >> 4, pg = fetch(pb + lane), pgn = fetch(pb + 64 + lane);
+    // where 64 runs of 16 keys from run `pb` on begin, one per lane, and the 64 after them
+    auto fetch = [&](int u) { return Runs(a.c, table, head, u, last); };
+    int pb = first >> 4;
+    Runs pg = fetch(pb + lane), pgn = fetch(pb + 64 + lane);
 
     u4 kr[NK];
     uint32_t vr[4][VE / 2];
@@ -691,11 +693,10 @@ template <bool BF, int NQ, int DP> __global__ __launch_bounds__(256, DP == 256 |
         }
         int holes = 0;
         auto run = [&](const uint8_t *pool, int sub) {
-            const int u = (t0 >> 4) + sub;
-            return Run<false>(a.c, pool, __builtin_amdgcn_readlane(pg, u0 + sub), head, (u & ((1 << shift16) - 1)) << 4, last - u * 16);
+            return Run<false>(pool, pg, u0 + sub, min(last - t0 - sub * 16, 16) * dim * 2);
         };
 #pragma unroll
-        for (int u = 0; u < 4; u++) holes |= __builtin_amdgcn_readlane(pg, u0 + u) < 0 ? 1 << u : 0;
+        for (int u = 0; u < 4; u++) holes |= pg.none(u0 + u) ? 1 << u : 0;
 #pragma unroll
         for (int i = 0; i < NK; i++)   // pieces i: tokens kt + i * (256 / KC)
             kr[i] = run(a.c.k, KC == 8 ? (wave >> 1) + 2 * i : KC == 16 ? i : i >> 1).load16(k_off, KC == 32 ? (i & 1) * 16 * dim : 0);
