@@ -265,8 +265,14 @@ struct Runs {
     __device__ bool none(int lane) const { return __builtin_amdgcn_readlane(hi, lane) < 0; }
 };
 // One of them, for loads whose offsets count from its first row: what lies past its `bytes` reads as zeros, and so does all of a run that is in no
-// page (the bounds are the loads' own; an address needs no lane's registers but its offset). ONCE: nobody else reads it soon (non-temporal).
-template <bool ONCE> struct Run {
+// page (the bounds are the loads' own; an address needs no lane's registers but its offset). Run's loads are non-temporal: nobody else reads
+// these keys soon.
+__device__ u4 run_of(const uint8_t *pool, const Runs &all, int lane, int bytes) {   // (as four words)
+    const int hi = __builtin_amdgcn_readlane(all.hi, lane);
+    const uint64_t at = reinterpret_cast<uint64_t>(pool) + ((uint64_t)(uint32_t)max(hi, 0) << 32 | (uint32_t)__builtin_amdgcn_readlane(all.lo, lane));
+    return u4{(uint32_t)at, (uint32_t)(at >> 32) & 0xffff, hi < 0 ? 0 : (uint32_t)bytes, 0x00020000};
+}
+struct Run {
     __amdgpu_buffer_rsrc_t r;
     __device__ Run(const uint8_t *pool, const Runs &all, int lane, int bytes) {
         const int hi = __builtin_amdgcn_readlane(all.hi, lane);
@@ -274,10 +280,10 @@ template <bool ONCE> struct Run {
         r = __builtin_amdgcn_make_buffer_rsrc(const_cast<uint8_t *>(pool + at), (short)0, hi < 0 ? 0 : bytes, 0x00020000);
     }
     __device__ u4 load16(int lane_offset, int offset) const {
-        return __builtin_bit_cast(u4, __builtin_amdgcn_raw_buffer_load_b128(r, lane_offset, offset, ONCE ? 2 : 0));
+        return __builtin_bit_cast(u4, __builtin_amdgcn_raw_buffer_load_b128(r, lane_offset, offset, 2));
     }
     __device__ u2 load8(int lane_offset, int offset) const {
-        return __builtin_bit_cast(u2, __builtin_amdgcn_raw_buffer_load_b64(r, lane_offset, offset, ONCE ? 2 : 0));
+        return __builtin_bit_cast(u2, __builtin_amdgcn_raw_buffer_load_b64(r, lane_offset, offset, 2));
     }
 };
 
@@ -389,12 +395,12 @@ template <bool BF, int NQ, int DP> __global__ __launch_bounds__(256, DP == 64 &&
         u4 kr[2][KS];             // run h, elements s * 32 + g * 8 of key col
         uint32_t vr[8][DL / 2];   // DL elements of the keys g * 4 + i (first four) and 16 + g * 4 + i
         auto run = [&](const uint8_t *pool, int n, int h) {
-            return Run<true>(pool, pg, (n & 31) * 2 + h, min(last - (first + (n * 4 + wave) * 32 + h * 16), 16) * dim * 2);
+            return Run(pool, pg, (n & 31) * 2 + h, min(last - (first + (n * 4 + wave) * 32 + h * 16), 16) * dim * 2);
         };
         auto load_k = [&](int n) {
 #pragma unroll
             for (int h = 0; h < 2; h++) {
-                const Run<true> r = run(a.c.k, n, h);
+                const Run r = run(a.c.k, n, h);
 #pragma unroll
                 for (int s = 0; s < KS; s++) kr[h][s] = r.load16(kd + s * 64, 0);
             }
@@ -402,7 +408,7 @@ template <bool BF, int NQ, int DP> __global__ __launch_bounds__(256, DP == 64 &&
         auto load_v = [&](int n) {
 #pragma unroll
             for (int h = 0; h < 2; h++) {
-                const Run<true> r = run(a.c.v, n, h);
+                const Run r = run(a.c.v, n, h);
 #pragma unroll
                 for (int i = 0; i < 4; i++) {   // (elements past dim: others' in their place, in sums that are not written)
                     if constexpr (DL == 4) {
@@ -621,22 +627,33 @@ template <bool F32, bool BF> __global__ __launch_bounds__(256) void attn_decode_
 }
 
 // ---- a tile of prompt rows -------------------------------------------------------------------------------------------------------
-// A workgroup of four waves takes 128 rows, 32 a wave, against its keys, 64 at a time through LDS: K as it is, V turned to [element][key]
-// on its way from registers, its keys in the order in which the lanes hold the weights. The keys after next are on their way into registers
-// and the next are in the other half of LDS while these are multiplied.
-// V's element d is row (d % VE) * 16 + d / VE of its LDS tile and of O^T, VE = DP / 16: the 16 threads that hold a key's elements then write
-// consecutive rows, whose pitch of 36 words spreads them over the banks (and the eight lanes of a read), and a lane ends with runs of VE elements.
-// Keys that a row does not see have weight 0, and 0 times an infinity or NaN is not 0: V rows that no row sees are staged as zeros, and
-// so are such elements of keys that only some rows see; where there were any, they are added to those rows at the end.
-template <bool BF, int NQ, int DP> __global__ __launch_bounds__(256, DP == 256 || NQ == 3 ? 1 : 2) void attn_prompt_kernel(AttnArgs a) {
-    constexpr int KS = DP / 16, DT = DP / 32, KC = DP / 8;
-    constexpr int KP = DP + 8;            // LDS pitch of K, elements
-    constexpr int NK = PN * KC / 256;     // 16-byte pieces of K per thread
-    constexpr int VE = DP / 16;           // elements of V per thread, of 4 keys
+// A workgroup of four waves takes 128 rows, 32 a wave, against its keys, 64 at a time in LDS, where the next 64 go while these are multiplied:
+// straight from memory (a wave's instruction brings 64 pieces of 16 bytes to consecutive places; which piece, each lane says). K and V lie as
+// in the pools, key after key, but the pieces of a key are exchanged among themselves, so that the lanes of a read (16 keys' pieces of K; of V, the
+// 4 keys of a transposing read, 32 elements of each) fall on different banks: piece c of key t is at c ^ k_turn(t), c ^ v_turn(t).
+// Keys that a row does not see have weight 0, and 0 times an infinity or NaN is not 0: V rows that no row sees are zeros in LDS, and so are such
+// elements of keys that only some rows see; where there were any, they are added to those rows at the end.
+template <int DP> __device__ constexpr int k_turn(int t) { return DP == 64 ? t >> 1 & 7 : t & 15; }
+template <int DP> __device__ constexpr int v_turn(int t) { return DP == 64 ? (t >> 1 & 1) * 4 : (t & 3) * 4; }
+
+// 64 pieces of 16 bytes from a run into LDS: lane i's, at `lane_offset` + `offset` from the run's first row, to lds + 16 i; zeros past the run's end
+__device__ void run_to_lds(u4 r, int lane_offset, int offset, uint32_t lds) {
+    asm volatile("s_mov_b32 m0, %3\n\ts_nop 0\n\tbuffer_load_dwordx4 %0, %1, %2 offen lds" ::"v"(lane_offset), "s"(r), "s"(offset), "s"(lds) : "memory");
+}
+using s4 = short __attribute__((ext_vector_type(4)));
+// of 4 keys, one element each: lane i of 16 gives where 4 elements of key i / 4 are and takes element i of the 16
+__device__ u2 transposed(uint32_t lds) {
+    return __builtin_bit_cast(u2, __builtin_amdgcn_ds_read_tr16_b64_v4i16(reinterpret_cast<__attribute__((address_space(3))) s4 *>(lds)));
+}
+
+template <bool BF, int NQ, int DP> __global__ __launch_bounds__(256, DP == 256 || (NQ == 3 && DP == 128) ? 1 : 2) void attn_prompt_kernel(AttnArgs a) {
+    constexpr int KS = DP / 16, DT = DP / 32, CH = DP / 8;   // CH: pieces of a key
+    constexpr int NI = PN * CH / 256;                        // a wave's instructions for its 16 keys
+    constexpr int ROWS = 64 / CH;                            // keys of one
+    constexpr uint32_t TILE = PN * DP * 2;                   // bytes of K, or V, of a step
     constexpr bool F32 = NQ > 1;
-    constexpr int VP = PN + 8;            // and of V
-    __shared__ __attribute__((aligned(16))) uint16_t lk[2][PN * KP], lv[2][DP * VP];
-    __shared__ int odd;                   // elements of V were left out
+    __shared__ __attribute__((aligned(1024))) uint8_t lds[4 * TILE];   // K of even and odd steps, V of them
+    __shared__ int odd;                                      // elements of V were left out
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int col = lane & 31, half = lane >> 5;
     const int head = blockIdx.x % a.c.heads, item = blockIdx.x / a.c.heads;
@@ -654,7 +671,6 @@ template <bool BF, int NQ, int DP> __global__ __launch_bounds__(256, DP == 256 |
     first = max(first, see_lo & ~(PN - 1));
     const int *table = a.c.table + (size_t)max(a.c.row(p.b), 0) * a.c.max_pages;
     const int dim = a.c.dim;
-    const bool padded = dim < DP;
 
     const int r = min(tile * PM + wave * 32 + col, tile * PM + rows - 1);   // lanes past the last row repeat it
     const int query = r / a.G, pos = back + query, from = a.window ? pos - a.window + 1 : 0;
@@ -677,13 +693,22 @@ template <bool BF, int NQ, int DP> __global__ __launch_bounds__(256, DP == 256 |
     int pb = first >> 4;
     Runs pg = fetch(pb + lane), pgn = fetch(pb + 64 + lane);
 
-    u4 kr[NK];
-    uint32_t vr[4][VE / 2];
-    const int kt = tid / KC, kd = tid % KC * 8;        // this thread's first piece of K: token (of 64) and element
-    const int vt = tid / 16 * 4, vd = tid % 16 * VE;   // its 4 keys of V and their elements
-    const int k_off = ((kt & 15) * dim + kd) * 2, v_off = ((vt & 15) * dim + vd) * 2;
-    // loads the keys from t0 on into registers; which of their four runs are in no page
-    auto load = [&](int t0) {
+    // This wave brings run `wave` of each step: key n * ROWS + lane / CH of it and place lane % CH of that key by instruction n
+    const uint32_t lds0 = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) uint8_t *)lds;
+    constexpr int VN = DP == 256 ? 2 : 1;   // instructions after which V's pieces are exchanged the same way again
+    int k_from[NI], v_from[VN];
+#pragma unroll
+    for (int n = 0; n < NI; n++) {
+        const int t = n * ROWS + lane / CH, c = lane % CH ^ k_turn<DP>(t);
+        k_from[n] = c * 8 < dim ? (t * dim + c * 8) * 2 : 0x40000000;   // (elements past dim: past the run's end)
+    }
+#pragma unroll
+    for (int n = 0; n < VN; n++) {
+        const int t = n * ROWS + lane / CH, c = lane % CH ^ v_turn<DP>(t);
+        v_from[n] = c * 8 < dim ? (t * dim + c * 8) * 2 : 0x40000000;
+    }
+    // brings the keys from t0 on; which of their four runs are in no page
+    auto load = [&](int t0, int buf) {
         int u0 = (t0 >> 4) - pb;
         if (u0 >= 64) {
             pb += 64;
@@ -691,84 +716,61 @@ template <bool BF, int NQ, int DP> __global__ __launch_bounds__(256, DP == 256 |
             pg = pgn;
             pgn = fetch(pb + 64 + lane);
         }
-        int holes = 0;
-        auto run = [&](const uint8_t *pool, int sub) {
-            return Run<false>(pool, pg, u0 + sub, min(last - t0 - sub * 16, 16) * dim * 2);
-        };
+        const int bytes = min(last - t0 - wave * 16, 16) * dim * 2;
+        const u4 k = run_of(a.c.k, pg, u0 + wave, bytes), v = run_of(a.c.v, pg, u0 + wave, bytes);
+        const uint32_t to = lds0 + buf * TILE + wave * NI * 1024;
 #pragma unroll
-        for (int u = 0; u < 4; u++) holes |= pg.none(u0 + u) ? 1 << u : 0;
+        for (int n = 0; n < NI; n++) run_to_lds(k, k_from[n], 0, to + n * 1024);
 #pragma unroll
-        for (int i = 0; i < NK; i++)   // pieces i: tokens kt + i * (256 / KC)
-            kr[i] = run(a.c.k, KC == 8 ? (wave >> 1) + 2 * i : KC == 16 ? i : i >> 1).load16(k_off, KC == 32 ? (i & 1) * 16 * dim : 0);
-        const Run<false> v = run(a.c.v, wave);
+        for (int n = 0; n < NI; n++) run_to_lds(v, v_from[n % VN], n / VN * VN * ROWS * dim * 2, to + 2 * TILE + n * 1024);
+        return (int)(__ballot(pg.hi < 0) >> u0 & 15);
+    };
+    // V of the step from t0 on, where some row does not see all of its keys: zeros for what none sees or must not be multiplied by 0
+    auto clean = [&](int t0, int buf) {
+        constexpr uint32_t E = BF ? 0x7f80u : 0x7c00u;   // an exponent of ones
+        bool left = false;
+#pragma unroll 1
+        for (int i = tid; i < PN * CH; i += 256) {
+            u4 *at = reinterpret_cast<u4 *>(lds + (2 + buf) * TILE) + i;
+            u4 x = *at;
+            const bool none = t0 + i / CH < see_lo;
+            bool write = none;
 #pragma unroll
-        for (int k = 0; k < 4; k++) {   // (elements past dim: others' in their place, in rows of O^T that are not written)
-            if constexpr (VE == 4) {
-                const u2 x = v.load8(v_off, k * dim * 2);
-                vr[k][0] = x[0];
-                vr[k][1] = x[1];
-            } else {
-#pragma unroll
-                for (int w = 0; w < VE / 2; w += 4) {
-                    const u4 x = v.load16(v_off + w * 4, k * dim * 2);
-#pragma unroll
-                    for (int n = 0; n < 4; n++) vr[k][w + n] = x[n];
-                }
+            for (int w = 0; w < 4; w++) {
+                const uint32_t bad = ((x[w] & E) == E ? 0xffffu : 0) | ((x[w] >> 16 & E) == E ? 0xffff0000u : 0);
+                left |= bad && !none;
+                write |= bad != 0;
+                x[w] = none ? 0 : x[w] & ~bad;
             }
+            if (write) *at = x;
         }
-        return holes;
+        if (left) odd = 1;
     };
-    // registers to LDS: the keys from t0 on, loaded last
-    auto stage = [&](int t0, int buf) {
-        if (padded && kd >= dim) {   // elements past dim: zeros, which the query's zeros keep
-#pragma unroll
-            for (int i = 0; i < NK; i++) kr[i] = u4{0, 0, 0, 0};
-        }
-#pragma unroll
-        for (int i = 0; i < NK; i++)
-            *reinterpret_cast<u4 *>(&lk[buf][(kt + i * (256 / KC)) * KP + kd]) = kr[i];
-        if (t0 < see_lo) {
-#pragma unroll
-            for (int k = 0; k < 4; k++)
-                if (t0 + vt + k < see_lo) {
-#pragma unroll
-                    for (int w = 0; w < VE / 2; w++) vr[k][w] = 0;
-                }
-        }
-        if (t0 + PN > pos_lo + 1 || t0 < from_hi) {   // some row does not see all of them
-            constexpr uint32_t E = BF ? 0x7f80u : 0x7c00u;   // an exponent of ones
-            bool left = false;
-#pragma unroll
-            for (int k = 0; k < 4; k++)
-#pragma unroll
-                for (int w = 0; w < VE / 2; w++) {
-                    const uint32_t x = vr[k][w], bad = ((x & E) == E ? 0xffffu : 0) | ((x >> 16 & E) == E ? 0xffff0000u : 0);
-                    vr[k][w] = x & ~bad;
-                    left |= bad != 0;
-                }
-            if (left) odd = 1;
-        }
-        const int at = wave * 16 + (vt >> 2 & 1) * 8 + (vt >> 3 & 1) * 4;   // keys vt..vt+3 as the weights lie
-#pragma unroll
-        for (int e = 0; e < VE; e += 2) {
-            const int w = e / 2;
-            const u2 x = {pair<0>(vr[0][w], vr[1][w]), pair<0>(vr[2][w], vr[3][w])};
-            const u2 y = {pair<1>(vr[0][w], vr[1][w]), pair<1>(vr[2][w], vr[3][w])};
-            *reinterpret_cast<u2 *>(&lv[buf][(e * 16 + tid % 16) * VP + at]) = x;
-            *reinterpret_cast<u2 *>(&lv[buf][(e * 16 + 16 + tid % 16) * VP + at]) = y;
-        }
+    auto arrived = [] {   // everything that this wave brought is in LDS, then everything that all brought
+        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+        __syncthreads();
     };
+    // reads: K piece (k * 2 + half) of key h * 32 + col; of V, as transposed() takes them, 4 elements of key u * 16 + r * 8 + half * 4 + lane % 16 / 4
+    constexpr int KA = KS < 8 ? KS : 8, VA = DT < 4 ? DT : 4;   // (addresses that are not another's at a constant distance)
+    uint32_t k_at[KA], v_at[VA];
+#pragma unroll
+    for (int k = 0; k < KA; k++) k_at[k] = lds0 + col * DP * 2 + ((k * 2 + half) ^ k_turn<DP>(col)) * 16;
+#pragma unroll
+    for (int j = 0; j < VA; j++) {
+        const int t = half * 4 + (lane & 15) / 4, e = j * 32 + (lane >> 4 & 1) * 16 + (lane & 3) * 4;
+        v_at[j] = lds0 + 2 * TILE + t * DP * 2 + ((e / 8) ^ v_turn<DP>(t)) * 16 + e % 8 * 2;
+    }
     if (tid == 0) odd = 0;
     __syncthreads();
-    int holes = 0, next = 0;
-    if (first < last) {
-        holes = load(first);
-        stage(first, 0);
-        if (first + PN < last) next = load(first + PN);
-    }
-    __syncthreads();
-    int buf = 0;
-    for (int t0 = first; t0 < last; t0 += PN) {
+    int holes = 0, buf = 0;
+    if (first < last) holes = load(first, 0);
+    arrived();
+    for (int t0 = first; t0 < last; t0 += PN, buf ^= 1) {
+        const int next = t0 + PN < last ? load(t0 + PN, buf ^ 1) : 0;
+        if (t0 + PN > pos_lo + 1 || t0 < from_hi) {
+            clean(t0, buf);
+            __syncthreads();
+        }
         if (!(idle || t0 > wpos_hi || (a.window && t0 + PN <= wpos_lo - a.window + 1))) {
             f16v s[2];
 #pragma unroll
@@ -779,7 +781,7 @@ template <bool BF, int NQ, int DP> __global__ __launch_bounds__(256, DP == 256 |
             for (int k = 0; k < KS; k++)
 #pragma unroll
                 for (int h = 0; h < 2; h++) {
-                    const u4 kf = *reinterpret_cast<const u4 *>(&lk[buf][(h * 32 + col) * KP + k * 16 + half * 8]);
+                    const u4 kf = *reinterpret_cast<__attribute__((address_space(3))) const u4 *>(k_at[k % KA] + buf * TILE + h * 32 * DP * 2 + k / KA * 256);
 #pragma unroll
                     for (int t = 0; t < NQ; t++) s[h] = mfma32<BF>(kf, q[k][t], s[h]);
                 }
@@ -831,23 +833,20 @@ template <bool BF, int NQ, int DP> __global__ __launch_bounds__(256, DP == 256 |
             for (int u = 0; u < 4; u++)
 #pragma unroll
                 for (int j = 0; j < DT; j++) {
-                    const u4 vf = *reinterpret_cast<const u4 *>(&lv[buf][(j * 32 + col) * VP + u * 16 + half * 8]);
+                    const uint32_t at = v_at[j % VA] + buf * TILE + u * 16 * DP * 2 + j / VA * 256;
+                    const u2 v0 = transposed(at), v1 = transposed(at + 8 * DP * 2);
+                    const u4 vf = {v0[0], v0[1], v1[0], v1[1]};
 #pragma unroll
                     for (int t = 0; t < NQ; t++) acc[j] = mfma32<BF>(vf, pt[u][t], acc[j]);
                 }
         }
         holes = next;
-        if (t0 + PN < last) {
-            stage(t0 + PN, buf ^ 1);
-            if (t0 + 2 * PN < last) next = load(t0 + 2 * PN);
-        }
-        buf ^= 1;
-        __syncthreads();
+        arrived();
     }
     l += __shfl_xor(l, 32);
 
     if (wave * 32 + col >= rows) return;
-    // acc[j][i] is row j * 32 + i / 4 * 8 + half * 4 + i % 4 of O^T: element c * VE + j * 2 + i / 8, c = i / 4 % 2 * 8 + half * 4 + i % 4
+    // acc[j][i] is element j * 32 + i / 4 * 8 + half * 4 + i % 4
     if (odd) {   // what was left out, for the keys of the steps that were looked through (an infinity or NaN, whatever its weight)
         for (int t = max(first, see_lo); t < last; t++) {
             const int t0 = t & ~(PN - 1);
@@ -856,16 +855,14 @@ template <bool BF, int NQ, int DP> __global__ __launch_bounds__(256, DP == 256 |
             if (page < 0 || page >= a.c.npages) continue;
             const uint8_t *row = a.c.v + a.c.at(page, head, t & ((1 << a.c.shift) - 1));
 #pragma unroll
-            for (int i = 0; i < 8; i++) {
-                const int c = i / 4 * 8 + half * 4 + (i & 3);
-                if (c * VE >= dim) continue;
+            for (int j = 0; j < DT; j++)
 #pragma unroll
-                for (int e = 0; e < VE; e++) {
+                for (int i = 0; i < 16; i++) {
                     using T = std::conditional_t<BF, __bf16, _Float16>;
-                    const float v = c * VE + e < dim ? static_cast<float>(*reinterpret_cast<const T *>(row + (c * VE + e) * 2)) : 0.0f;
-                    if (!(fabsf(v) < INFINITY)) acc[e / 2][e % 2 * 8 + i] += v;
+                    const int d = j * 32 + i / 4 * 8 + half * 4 + (i & 3);
+                    const float v = d < dim ? static_cast<float>(*reinterpret_cast<const T *>(row + d * 2)) : 0.0f;
+                    if (!(fabsf(v) < INFINITY)) acc[j][i] += v;
                 }
-            }
         }
     }
     const bool done = p.chunks == 1;
@@ -874,22 +871,20 @@ template <bool BF, int NQ, int DP> __global__ __launch_bounds__(256, DP == 256 |
     if (!done && half == 0) a.pml[at] = float2{m, l};
     uint8_t *row = a.out + (size_t)(p.s.t0 + query) * a.ostride + qoff;
 #pragma unroll
-    for (int i = 0; i < 8; i++) {
-        const int c = i / 4 * 8 + half * 4 + (i & 3);
+    for (int j = 0; j < DT; j++)
 #pragma unroll
-        for (int e = 0; e < VE; e += 4) {
-            const int d = c * VE + e;
+        for (int i = 0; i < 16; i += 4) {
+            const int d = j * 32 + i * 2 + half * 4;
+            if (d >= dim) continue;
             float x[4];
 #pragma unroll
             for (int k = 0; k < 4; k++) {
-                x[k] = acc[(e + k) / 2][(e + k) % 2 * 8 + i] * inv;
+                x[k] = acc[j][i + k] * inv;
                 if (done && l == 0.0f) x[k] = 0.0f;
             }
-            if (d >= dim) continue;
             if (done) store4<F32, BF>(row, d, x);
             else *reinterpret_cast<f4 *>(a.po + at * dim + d) = f4{x[0], x[1], x[2], x[3]};
         }
-    }
 }
 
 // ---- parts joined ------------------------------------------------------------------------------------------------------------
