@@ -44,33 +44,33 @@ struct AttnArgs {
 // A tile is PM rows of one sequence and K/V head; a part is a tile's chunk of keys. Chunks have one length for the whole call, from the
 // lengths on the device: the least that leaves about `target` parts, so that few rows over many keys fill the device and a captured call
 // adapts to later lengths. Every wave finds its part by a scan over the sequences, 64 at a time.
-constexpr int PM = 128, PN = 64;   // rows of a tile, keys of a step
+constexpr int PM = 128, PN = 64;   // rows of a tile (of four waves; of eight twice as many), keys of a step
 
 struct Seq {
     int t0, n, len;      // first query row, queries, tokens
     int base, tiles;     // first key of the first chunk (a multiple of 64), tiles of PM rows
 };
-__device__ Seq seq_of(const AttnArgs &a, int b) {
+template <int BM> __device__ Seq seq_of(const AttnArgs &a, int b) {
     Seq s;
     s.t0 = min(max(a.start[b], 0), a.ntok);
     s.n = min(max(a.start[b + 1], s.t0), a.ntok) - s.t0;
     s.len = a.c.tokens(b);
     s.base = a.window ? max(0, s.len - s.n - a.window + 1) & ~63 : 0;
-    s.tiles = (int)(((long long)s.n * a.G + PM - 1) / PM);
+    s.tiles = (int)(((long long)s.n * a.G + BM - 1) / BM);
     return s;
 }
 
 constexpr int CHUNK_MIN = 128;   // keys
 
-__device__ int chunk_of(const AttnArgs &a) {
+template <int BM> __device__ int chunk_of(const AttnArgs &a) {
     if (!a.target) return 1 << 30;
     unsigned long long all = 0;
     if (a.nseq == 1) {
-        const Seq s = seq_of(a, 0);
+        const Seq s = seq_of<BM>(a, 0);
         all = (unsigned long long)s.tiles * (unsigned)(s.len - s.base);
     } else {
         for (int b = threadIdx.x & 63; b < a.nseq; b += 64) {
-            const Seq s = seq_of(a, b);
+            const Seq s = seq_of<BM>(a, b);
             all += (unsigned long long)s.tiles * (unsigned)(s.len - s.base);
         }
 #pragma unroll
@@ -98,12 +98,12 @@ __device__ uint32_t sum_up_to(uint32_t x) {   // over the lanes up to this one
 }
 // The part with number `item` (within one K/V head), or, TILES, the tile with that number and `chunk` 0; false if there is none. Starts that
 // are out of order may give any number of parts: they are counted modulo 2^32.
-template <bool TILES = false> __device__ bool part_of(const AttnArgs &a, int item, int chunk, Part &p) {
+template <int BM, bool TILES> __device__ bool part_of(const AttnArgs &a, int item, int chunk, Part &p) {
     const int lane = threadIdx.x & 63;
     uint32_t tiles_before = 0, parts_before = 0;
     if (a.nseq == 1) {
         p.b = 0;
-        p.s = seq_of(a, 0);
+        p.s = seq_of<BM>(a, 0);
         p.chunks = chunks_of(p.s, chunk);
         p.first = 0;
     } else {
@@ -113,7 +113,7 @@ template <bool TILES = false> __device__ bool part_of(const AttnArgs &a, int ite
             int chunks = 1;
             uint32_t parts = 0;
             if (g + lane < a.nseq) {
-                s = seq_of(a, g + lane);
+                s = seq_of<BM>(a, g + lane);
                 chunks = chunks_of(s, chunk);
                 parts = (uint32_t)s.tiles * (uint32_t)chunks;
             }
@@ -646,25 +646,26 @@ __device__ u2 transposed(uint32_t lds) {
     return __builtin_bit_cast(u2, __builtin_amdgcn_ds_read_tr16_b64_v4i16(reinterpret_cast<__attribute__((address_space(3))) s4 *>(lds)));
 }
 
-template <bool BF, int NQ, int DP> __global__ __launch_bounds__(256, DP == 256 || (NQ == 3 && DP == 128) ? 1 : 2) void attn_prompt_kernel(AttnArgs a) {
+template <bool BF, int NQ, int DP, int W, int NB> __global__ __launch_bounds__(64 * W, W == 8 || !(DP == 256 || (NQ == 3 && DP == 128)) ? 2 : 1) void attn_prompt_kernel(AttnArgs a) {
+    constexpr int BM = 32 * W;
     constexpr int KS = DP / 16, DT = DP / 32, CH = DP / 8;   // CH: pieces of a key
-    constexpr int NI = PN * CH / 256;                        // a wave's instructions for its 16 keys
+    constexpr int NI = PN * CH / (64 * W);                   // a wave's instructions for its PN / W keys
     constexpr int ROWS = 64 / CH;                            // keys of one
     constexpr uint32_t TILE = PN * DP * 2;                   // bytes of K, or V, of a step
     constexpr bool F32 = NQ > 1;
-    __shared__ __attribute__((aligned(1024))) uint8_t lds[4 * TILE];   // K of even and odd steps, V of them
+    __shared__ __attribute__((aligned(1024))) uint8_t lds[2 * NB * TILE];   // K of NB steps, V of them
     __shared__ int odd;                                      // elements of V were left out
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int col = lane & 31, half = lane >> 5;
     const int head = blockIdx.x % a.c.heads, item = blockIdx.x / a.c.heads;
-    const int chunk = chunk_of(a);
+    const int chunk = chunk_of<BM>(a);
     Part p;
-    if (!part_of(a, item, chunk, p)) return;
+    if (!part_of<BM, false>(a, item, chunk, p)) return;
     const bool whole = chunk == 1 << 30;
     const int tile = p.s.tiles - 1 - p.tile;   // the tiles that see most keys first
-    const int rows = min(PM, p.s.n * a.G - tile * PM);
+    const int rows = min(BM, p.s.n * a.G - tile * BM);
     const int back = p.s.len - p.s.n;          // query i stands at back + i
-    const int pos_lo = back + tile * PM / a.G, pos_hi = back + (tile * PM + rows - 1) / a.G;
+    const int pos_lo = back + tile * BM / a.G, pos_hi = back + (tile * BM + rows - 1) / a.G;
     const int see_lo = a.window ? max(0, pos_lo - a.window + 1) : 0, see_hi = pos_hi + 1;   // keys that some row sees
     int first = p.s.base + (whole ? 0 : p.chunk * chunk);
     const int last = whole ? see_hi : min(see_hi, first + chunk);
@@ -672,7 +673,7 @@ template <bool BF, int NQ, int DP> __global__ __launch_bounds__(256, DP == 256 |
     const int *table = a.c.table + (size_t)max(a.c.row(p.b), 0) * a.c.max_pages;
     const int dim = a.c.dim;
 
-    const int r = min(tile * PM + wave * 32 + col, tile * PM + rows - 1);   // lanes past the last row repeat it
+    const int r = min(tile * BM + wave * 32 + col, tile * BM + rows - 1);   // lanes past the last row repeat it
     const int query = r / a.G, pos = back + query, from = a.window ? pos - a.window + 1 : 0;
     const size_t qoff = (size_t)(head * a.G + r - query * a.G) * dim * (F32 ? 4 : 2);
     u4 q[KS][NQ];
@@ -693,18 +694,19 @@ template <bool BF, int NQ, int DP> __global__ __launch_bounds__(256, DP == 256 |
     int pb = first >> 4;
     Runs pg = fetch(pb + lane), pgn = fetch(pb + 64 + lane);
 
-    // This wave brings run `wave` of each step: key n * ROWS + lane / CH of it and place lane % CH of that key by instruction n
+    // This wave brings PN / W keys of each step, of run `mine`: key t0w + n * ROWS + lane / CH of it and place lane % CH of that key by instruction n
+    const int mine = wave * (PN / W) / 16, t0w = wave * (PN / W) % 16;
     const uint32_t lds0 = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) uint8_t *)lds;
     constexpr int VN = DP == 256 ? 2 : 1;   // instructions after which V's pieces are exchanged the same way again
     int k_from[NI], v_from[VN];
 #pragma unroll
     for (int n = 0; n < NI; n++) {
-        const int t = n * ROWS + lane / CH, c = lane % CH ^ k_turn<DP>(t);
+        const int t = t0w + n * ROWS + lane / CH, c = lane % CH ^ k_turn<DP>(t);
         k_from[n] = c * 8 < dim ? (t * dim + c * 8) * 2 : 0x40000000;   // (elements past dim: past the run's end)
     }
 #pragma unroll
     for (int n = 0; n < VN; n++) {
-        const int t = n * ROWS + lane / CH, c = lane % CH ^ v_turn<DP>(t);
+        const int t = t0w + n * ROWS + lane / CH, c = lane % CH ^ v_turn<DP>(t);
         v_from[n] = c * 8 < dim ? (t * dim + c * 8) * 2 : 0x40000000;
     }
     // brings the keys from t0 on; which of their four runs are in no page
@@ -716,13 +718,13 @@ template <bool BF, int NQ, int DP> __global__ __launch_bounds__(256, DP == 256 |
             pg = pgn;
             pgn = fetch(pb + 64 + lane);
         }
-        const int bytes = min(last - t0 - wave * 16, 16) * dim * 2;
-        const u4 k = run_of(a.c.k, pg, u0 + wave, bytes), v = run_of(a.c.v, pg, u0 + wave, bytes);
+        const int bytes = min(last - t0 - mine * 16, 16) * dim * 2;
+        const u4 k = run_of(a.c.k, pg, u0 + mine, bytes), v = run_of(a.c.v, pg, u0 + mine, bytes);
         const uint32_t to = lds0 + buf * TILE + wave * NI * 1024;
 #pragma unroll
         for (int n = 0; n < NI; n++) run_to_lds(k, k_from[n], 0, to + n * 1024);
 #pragma unroll
-        for (int n = 0; n < NI; n++) run_to_lds(v, v_from[n % VN], n / VN * VN * ROWS * dim * 2, to + 2 * TILE + n * 1024);
+        for (int n = 0; n < NI; n++) run_to_lds(v, v_from[n % VN], n / VN * VN * ROWS * dim * 2, to + NB * TILE + n * 1024);
         return (int)(__ballot(pg.hi < 0) >> u0 & 15);
     };
     // V of the step from t0 on, where some row does not see all of its keys: zeros for what none sees or must not be multiplied by 0
@@ -730,8 +732,8 @@ template <bool BF, int NQ, int DP> __global__ __launch_bounds__(256, DP == 256 |
         constexpr uint32_t E = BF ? 0x7f80u : 0x7c00u;   // an exponent of ones
         bool left = false;
 #pragma unroll 1
-        for (int i = tid; i < PN * CH; i += 256) {
-            u4 *at = reinterpret_cast<u4 *>(lds + (2 + buf) * TILE) + i;
+        for (int i = tid; i < PN * CH; i += 64 * W) {
+            u4 *at = reinterpret_cast<u4 *>(lds + (NB + buf) * TILE) + i;
             u4 x = *at;
             const bool none = t0 + i / CH < see_lo;
             bool write = none;
@@ -746,8 +748,9 @@ template <bool BF, int NQ, int DP> __global__ __launch_bounds__(256, DP == 256 |
         }
         if (left) odd = 1;
     };
-    auto arrived = [] {   // everything that this wave brought is in LDS, then everything that all brought
-        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    auto arrived = [&](bool all) {   // the next step's keys are in LDS (all: of every step asked for), then those that the other waves brought
+        if (all) asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+        else asm volatile("s_waitcnt vmcnt(%0)" ::"n"((NB - 2) * 2 * NI) : "memory");   // (what was asked for last comes last)
         __syncthreads();
     };
     // reads: K piece (k * 2 + half) of key h * 32 + col; of V, as transposed() takes them, 4 elements of key u * 16 + r * 8 + half * 4 + lane % 16 / 4
@@ -758,20 +761,34 @@ template <bool BF, int NQ, int DP> __global__ __launch_bounds__(256, DP == 256 |
 #pragma unroll
     for (int j = 0; j < VA; j++) {
         const int t = half * 4 + (lane & 15) / 4, e = j * 32 + (lane >> 4 & 1) * 16 + (lane & 3) * 4;
-        v_at[j] = lds0 + 2 * TILE + t * DP * 2 + ((e / 8) ^ v_turn<DP>(t)) * 16 + e % 8 * 2;
+        v_at[j] = lds0 + NB * TILE + t * DP * 2 + ((e / 8) ^ v_turn<DP>(t)) * 16 + e % 8 * 2;
     }
     if (tid == 0) odd = 0;
     __syncthreads();
-    int holes = 0, buf = 0;
-    if (first < last) holes = load(first, 0);
-    arrived();
-    for (int t0 = first; t0 < last; t0 += PN, buf ^= 1) {
-        const int next = t0 + PN < last ? load(t0 + PN, buf ^ 1) : 0;
+    int holes = 0, buf = 0;   // holes: four bits a step, this one's lowest
+#pragma unroll
+    for (int n = 0; n < NB - 1; n++)
+        if (first + n * PN < last) holes |= load(first + n * PN, n) << 4 * n;
+    arrived(true);
+    for (int t0 = first; t0 < last; t0 += PN) {
+        const bool more = t0 + (NB - 1) * PN < last;
+        if (more) holes |= load(t0 + (NB - 1) * PN, buf == 0 ? NB - 1 : buf - 1) << 4 * (NB - 1);
         if (t0 + PN > pos_lo + 1 || t0 < from_hi) {
             clean(t0, buf);
             __syncthreads();
         }
         if (!(idle || t0 > wpos_hi || (a.window && t0 + PN <= wpos_lo - a.window + 1))) {
+            uint32_t k_now[KA], v_now[VA];   // (kept as they are, so that what is added to them goes into the instructions)
+#pragma unroll
+            for (int k = 0; k < KA; k++) {
+                k_now[k] = k_at[k] + buf * TILE;
+                asm volatile("" : "+v"(k_now[k]));
+            }
+#pragma unroll
+            for (int j = 0; j < VA; j++) {
+                v_now[j] = v_at[j] + buf * TILE;
+                asm volatile("" : "+v"(v_now[j]));
+            }
             f16v s[2];
 #pragma unroll
             for (int h = 0; h < 2; h++)
@@ -781,7 +798,7 @@ template <bool BF, int NQ, int DP> __global__ __launch_bounds__(256, DP == 256 |
             for (int k = 0; k < KS; k++)
 #pragma unroll
                 for (int h = 0; h < 2; h++) {
-                    const u4 kf = *reinterpret_cast<__attribute__((address_space(3))) const u4 *>(k_at[k % KA] + buf * TILE + h * 32 * DP * 2 + k / KA * 256);
+                    const u4 kf = *reinterpret_cast<__attribute__((address_space(3))) const u4 *>(k_now[k % KA] + h * 32 * DP * 2 + k / KA * 256);
 #pragma unroll
                     for (int t = 0; t < NQ; t++) s[h] = mfma32<BF>(kf, q[k][t], s[h]);
                 }
@@ -795,7 +812,7 @@ template <bool BF, int NQ, int DP> __global__ __launch_bounds__(256, DP == 256 |
                         if (t > to || t < since) s[h][i] = LOWEST;
                     }
             }
-            if (holes) {
+            if (holes & 15) {
 #pragma unroll
                 for (int h = 0; h < 2; h++)
 #pragma unroll
@@ -833,15 +850,16 @@ template <bool BF, int NQ, int DP> __global__ __launch_bounds__(256, DP == 256 |
             for (int u = 0; u < 4; u++)
 #pragma unroll
                 for (int j = 0; j < DT; j++) {
-                    const uint32_t at = v_at[j % VA] + buf * TILE + u * 16 * DP * 2 + j / VA * 256;
+                    const uint32_t at = v_now[j % VA] + u * 16 * DP * 2 + j / VA * 256;
                     const u2 v0 = transposed(at), v1 = transposed(at + 8 * DP * 2);
                     const u4 vf = {v0[0], v0[1], v1[0], v1[1]};
 #pragma unroll
                     for (int t = 0; t < NQ; t++) acc[j] = mfma32<BF>(vf, pt[u][t], acc[j]);
                 }
         }
-        holes = next;
-        arrived();
+        holes >>= 4;
+        buf = buf == NB - 1 ? 0 : buf + 1;
+        arrived(!more);
     }
     l += __shfl_xor(l, 32);
 
@@ -891,14 +909,15 @@ template <bool BF, int NQ, int DP> __global__ __launch_bounds__(256, DP == 256 |
 // out of a prompt's row = sum over its parts of 2^(m of the part - the largest m) * (the part's sum), over the same of l: the weights first,
 // in LDS, then the sums in the order of the parts, dim / 4 threads (rounded up to 16, 32 or 64) a row, as many rows as that gives a workgroup.
 constexpr int PARTS = 512;   // workgroups that a call is split into, about: two per CU
+constexpr int TALL = 1;      // tiles of eight waves from so many times that many on
 template <bool F32, bool BF> __global__ __launch_bounds__(256) void attn_join_kernel(AttnArgs a) {
     const int quads = a.c.dim / 4, w = quads <= 16 ? 16 : quads <= 32 ? 32 : 64;   // threads per row
     const int d = threadIdx.x % w, k = threadIdx.x / w, groups = 256 / w;
     const int blocks = PM / groups;   // workgroups per tile
     const int head = blockIdx.x % a.c.heads, block = blockIdx.x / a.c.heads % blocks;
-    const int chunk = chunk_of(a);
+    const int chunk = chunk_of<PM>(a);
     Part p;
-    if (!part_of<true>(a, blockIdx.x / a.c.heads / blocks, chunk, p) || p.chunks == 1) return;   // (one part: written already)
+    if (!part_of<PM, true>(a, blockIdx.x / a.c.heads / blocks, chunk, p) || p.chunks == 1) return;   // (one part: written already)
     const uint32_t first = p.first + (uint32_t)p.tile * (uint32_t)p.chunks;
     const int tile = p.s.tiles - 1 - p.tile;
     const int rows = min(PM, p.s.n * a.G - tile * PM), row = block * groups + k;
@@ -942,6 +961,7 @@ template <bool F32, bool BF> __global__ __launch_bounds__(256) void attn_join_ke
 
 // ---- host ------------------------------------------------------------------------------------------------------------------------
 struct Shape {
+    bool tall;         // prompt: tiles of eight waves
     size_t items;      // prompt: the most parts per K/V head that the call's lengths can give; else workgroups per K/V head
     size_t tiles;      // prompt: the most tiles
     int target;        // AttnArgs::target
@@ -956,10 +976,11 @@ Shape shape_of(const es_hip_kv *kv, int nseq, int ntok, int heads, bool prompt) 
     const long long most = (long long)kv->max_pages * kv->page;
     Shape s{};
     if (prompt) {
-        s.bm = PM;
-        s.tiles = (size_t)ntok * G / PM + nseq;
         const int parts = std::max(PARTS / kv->heads, 1);
-        s.target = s.tiles >= (size_t)parts || most <= CHUNK_MIN ? 0 : parts;
+        s.tall = kv->dim <= 128 && (size_t)ntok * G / (2 * PM) >= (size_t)TALL * parts;
+        s.bm = s.tall ? 2 * PM : PM;
+        s.tiles = (size_t)ntok * G / s.bm + nseq;
+        s.target = s.tall || s.tiles >= (size_t)parts || most <= CHUNK_MIN ? 0 : parts;
         s.items = s.tiles + s.target;   // sum of tiles * ceil(span / chunk) <= tiles + target
         s.slots = s.target ? s.items : 0;
     } else {
@@ -998,7 +1019,12 @@ template <bool BF, int NQ> hipError_t launch(const AttnArgs &a, const Shape &s, 
         attn_decode_join_kernel<(NQ > 1), BF><<<(unsigned)((size_t)a.nseq * a.c.heads * ((a.G + together - 1) / together)), 256, 0, st>>>(a, together);
         return hipGetLastError();
     }
-    auto f = a.c.dim <= 64 ? attn_prompt_kernel<BF, NQ, 64> : a.c.dim <= 128 ? attn_prompt_kernel<BF, NQ, 128> : attn_prompt_kernel<BF, NQ, 256>;
+    if (s.tall) {
+        auto f = a.c.dim <= 64 ? attn_prompt_kernel<BF, NQ, 64, 8, 4> : attn_prompt_kernel<BF, NQ, 128, 8, 4>;
+        f<<<grid, 512, 0, st>>>(a);
+        return hipGetLastError();
+    }
+    auto f = a.c.dim <= 64 ? attn_prompt_kernel<BF, NQ, 64, 4, 3> : a.c.dim <= 128 ? attn_prompt_kernel<BF, NQ, 128, 4, 2> : attn_prompt_kernel<BF, NQ, 256, 4, 2>;
     f<<<grid, 256, 0, st>>>(a);
     hipError_t e = hipGetLastError();
     if (e != hipSuccess || !s.target) return e;
