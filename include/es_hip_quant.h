@@ -467,9 +467,10 @@ typedef struct {
 /* The rows of ntok new tokens into their pages, rounded to the cache's type (nearest even; fp16 overflows to infinity). The
  * call's sequence b brings rows start[b] to start[b + 1] - 1 of k and v, which are its last tokens: those at len - n to len - 1
  * (start: device, nseq + 1 entries, not decreasing; NULL: one token per sequence, ntok = nseq). Rows from start[nseq] on are
- * not read, as are rows whose token would lie before the first or in no page. src_type: ES_HIP_F32 or the cache's own type; token t's heads *
- * dim elements at k + t * kstride elements (0: packed), the same for v; aligned to their type. A page that several rows of
- * the table share is written through whichever asks: see es_hip_kv_seq_extend for private copies. */
+ * not read; nothing is written for rows whose token would lie before the first or in no page. src_type: ES_HIP_F32 or the
+ * cache's own type; token t's heads * dim elements at k + t * kstride elements (0: packed), the same for v; aligned to their
+ * type. A page that several rows of the table share is written through whichever asks: see es_hip_kv_seq_extend for
+ * private copies. */
 int es_hip_kv_append_dev(const es_hip_kv *kv, int nseq, const int *start, int ntok, uint32_t src_type, const void *k,
                          size_t kstride, const void *v, size_t vstride, void *stream);
 /* Attention of one new token per sequence, the last in its cache (append it first):

@@ -54,8 +54,9 @@ namespace {
 using namespace esq;
 
 // ---- new rows ------------------------------------------------------------------------------------------------------------
-// One thread per 8 elements: 16 bytes of the cache. Bound by its reads and writes where it is long, by its launch where it is
-// short; a token's place is three dependent loads (start, len, table), the same ones for all threads of its row.
+// One thread per 8 elements of K and the same of V: 16 bytes of each pool. Where its token goes are three dependent loads (start, len, table),
+// the same ones for all threads of the row, under which the elements' own loads are on their way. Bound by its reads and writes where it is
+// long (71 MB, fp32 to bf16, in 12.7 us), by its launch where it is short (one token 4.1 us, of which its kernel 2).
 struct AppendArgs {
     KvView c;
     const int *start;
@@ -63,7 +64,7 @@ struct AppendArgs {
     size_t kstride, vstride;   // bytes
     int nseq, token0, ntok;    // tokens of this launch and the first of them
     int all;                   // tokens of the call
-    int per;                   // threads per token: K then V, heads * dim / 8 each
+    int per;                   // threads per token: heads * dim / 8
 };
 
 template <bool BF> __device__ uint32_t round2(float a, float b) {
@@ -76,9 +77,24 @@ template <bool BF> __device__ uint32_t round2(float a, float b) {
     }
 }
 
+// 8 elements in the cache's type
+template <bool F32, bool BF> struct Eight {
+    struct __attribute__((packed, aligned(F32 ? 4 : 2))) Raw { uint32_t x[F32 ? 8 : 4]; } raw;
+    __device__ explicit Eight(const uint8_t *p) : raw(*reinterpret_cast<const Raw *>(p)) {}
+    __device__ u4 value() const {
+        u4 w;
+#pragma unroll
+        for (int j = 0; j < 4; j++) {
+            if constexpr (F32) w[j] = round2<BF>(__uint_as_float(raw.x[2 * j]), __uint_as_float(raw.x[2 * j + 1]));
+            else w[j] = raw.x[j];
+        }
+        return w;
+    }
+};
+
 template <bool F32, bool BF> __global__ __launch_bounds__(256) void kv_append_kernel(AppendArgs a) {
     const uint32_t i = blockIdx.x * 256u + threadIdx.x;
-    const int t = a.token0 + (int)(i / a.per), e = (int)(i % a.per);
+    const int t = a.token0 + (int)(i / a.per), c = (int)(i % a.per);
     if (t >= a.token0 + a.ntok) return;
     int b = t, back = 1;   // the token is the back-th last of sequence b
     if (a.start) {         // b: the last sequence that starts at or before t
@@ -89,36 +105,26 @@ template <bool F32, bool BF> __global__ __launch_bounds__(256) void kv_append_ke
         }
         b = lo;
         const int end = min(a.start[b + 1], a.all);
-        if (a.start[b] > t || end <= t) return;
+        if (a.start[b] > t || end <= t) return;   // (rows that are no sequence's are not read)
         back = end - t;
     }
+    const Eight<F32, BF> k(a.k + (size_t)t * a.kstride + (size_t)c * (F32 ? 32 : 16)), v(a.v + (size_t)t * a.vstride + (size_t)c * (F32 ? 32 : 16));
     const int r = a.c.row(b), pos = a.c.tokens(b) - back;
-    if (r < 0 || pos < 0) return;
-    const int page = a.c.table[(size_t)r * a.c.max_pages + (pos >> a.c.shift)];
+    const int page = r < 0 || pos < 0 ? -1 : a.c.table[(size_t)r * a.c.max_pages + (pos >> a.c.shift)];
+    const u4 kw = k.value(), vw = v.value();
     if (page < 0 || page >= a.c.npages) return;
-    const int half = a.per >> 1, dc = a.c.dim >> 3;
-    const bool isv = e >= half;
-    const int c = isv ? e - half : e, head = c / dc, d = (c - head * dc) * 8;
-    const uint8_t *src = (isv ? a.v + (size_t)t * a.vstride : a.k + (size_t)t * a.kstride);
-    u4 w;
-    if constexpr (F32) {
-        struct __attribute__((packed, aligned(4))) F8 { float x[8]; };
-        const F8 f = *reinterpret_cast<const F8 *>(src + (size_t)c * 32);
-#pragma unroll
-        for (int j = 0; j < 4; j++) w[j] = round2<BF>(f.x[2 * j], f.x[2 * j + 1]);
-    } else {
-        struct __attribute__((packed, aligned(2))) H8 { uint32_t x[4]; };
-        const H8 f = *reinterpret_cast<const H8 *>(src + (size_t)c * 16);
-#pragma unroll
-        for (int j = 0; j < 4; j++) w[j] = f.x[j];
-    }
-    *reinterpret_cast<u4 *>((isv ? a.c.v : a.c.k) + a.c.at(page, head, pos & ((1 << a.c.shift) - 1)) + d * 2) = w;
+    const int dc = a.c.dim >> 3, head = c / dc, d = (c - head * dc) * 8;
+    const size_t at = a.c.at(page, head, pos & ((1 << a.c.shift) - 1)) + d * 2;
+    *reinterpret_cast<u4 *>(a.c.k + at) = kw;
+    *reinterpret_cast<u4 *>(a.c.v + at) = vw;
 }
 
 // ---- pages copied ----------------------------------------------------------------------------------------------------------
-// The pairs travel with the launch (a kernel's arguments hold 4 KB): no list in memory, nothing to wait for. 16 KB per workgroup, four loads in
-// flight per thread. Bound by HBM where it is long.
+// The pairs travel with the launch (a kernel's arguments hold 4 KB): no list in memory, nothing to wait for. 16 KB per workgroup, four loads
+// in flight per thread. Bound by HBM where it is long: copies of COPY_ONCE bytes and more go past the caches (ONCE). us past them and through
+// them, bytes read and written: 63 MB 12.4 and 10.8, 126 MB 24.5 and 29.3, 786 MB 159 (4.9 TB/s) and 175.
 constexpr int COPY_PAIRS = 448, COPY_BYTES = 16384;
+constexpr size_t COPY_ONCE = 96u << 20;   // bytes read and written
 struct CopyArgs {
     uint8_t *k, *v;
     size_t layer_bytes;
@@ -126,7 +132,7 @@ struct CopyArgs {
     int src[COPY_PAIRS], dst[COPY_PAIRS];
 };
 
-__global__ __launch_bounds__(256) void kv_copy_kernel(CopyArgs a) {
+template <bool ONCE> __global__ __launch_bounds__(256) void kv_copy_kernel(CopyArgs a) {
     const int layer = blockIdx.z >> 1;
     uint8_t *pool = (blockIdx.z & 1 ? a.v : a.k) + (size_t)layer * a.layer_bytes;
     const uint8_t *s = pool + (size_t)a.src[blockIdx.y] * a.page_bytes;
@@ -135,10 +141,17 @@ __global__ __launch_bounds__(256) void kv_copy_kernel(CopyArgs a) {
     u4 x[4];
 #pragma unroll
     for (int i = 0; i < 4; i++)
-        if (at + i * 4096 < a.page_bytes) x[i] = *reinterpret_cast<const u4 *>(s + at + i * 4096);
+        if (at + i * 4096 < a.page_bytes) {
+            const u4 *p = reinterpret_cast<const u4 *>(s + at + i * 4096);
+            x[i] = ONCE ? __builtin_nontemporal_load(p) : *p;
+        }
 #pragma unroll
     for (int i = 0; i < 4; i++)
-        if (at + i * 4096 < a.page_bytes) *reinterpret_cast<u4 *>(d + at + i * 4096) = x[i];
+        if (at + i * 4096 < a.page_bytes) {
+            u4 *p = reinterpret_cast<u4 *>(d + at + i * 4096);
+            if constexpr (ONCE) __builtin_nontemporal_store(x[i], p);
+            else *p = x[i];
+        }
 }
 
 hipError_t copy_pages(uint8_t *k, uint8_t *v, size_t layer_bytes, size_t page_bytes, int nlayers, const int *src, const int *dst,
@@ -148,6 +161,7 @@ hipError_t copy_pages(uint8_t *k, uint8_t *v, size_t layer_bytes, size_t page_by
     a.v = v;
     a.layer_bytes = layer_bytes;
     a.page_bytes = (uint32_t)page_bytes;
+    const auto f = (double)page_bytes * nlayers * n * 4 >= COPY_ONCE ? kv_copy_kernel<true> : kv_copy_kernel<false>;
     for (int l = 0; l < nlayers; l += 16384)   // (a grid's z ends at 65535)
         for (int i = 0; i < n; i += COPY_PAIRS) {
             const int m = std::min(COPY_PAIRS, n - i);
@@ -155,7 +169,7 @@ hipError_t copy_pages(uint8_t *k, uint8_t *v, size_t layer_bytes, size_t page_by
             std::copy(dst + i, dst + i + m, a.dst);
             a.k = k + (size_t)l * layer_bytes;
             a.v = v + (size_t)l * layer_bytes;
-            kv_copy_kernel<<<dim3((unsigned)((page_bytes + COPY_BYTES - 1) / COPY_BYTES), m, 2 * std::min(16384, nlayers - l)), 256, 0, s>>>(a);
+            f<<<dim3((unsigned)((page_bytes + COPY_BYTES - 1) / COPY_BYTES), m, 2 * std::min(16384, nlayers - l)), 256, 0, s>>>(a);
             if (hipError_t e = hipGetLastError()) return e;
         }
     return hipSuccess;
@@ -422,7 +436,7 @@ int es_hip_kv_append_dev(const es_hip_kv *kv, int nseq, const int *start, int nt
     a.vstride = vstride * es;
     a.nseq = nseq;
     a.all = ntok;
-    a.per = (int)(row / 4);
+    a.per = (int)(row / 8);
     const int most = (1 << 30) / a.per;   // tokens per launch: thread numbers stay within 32 bits
     for (a.token0 = 0; a.token0 < ntok; a.token0 += a.ntok) {
         a.ntok = std::min(most, ntok - a.token0);
