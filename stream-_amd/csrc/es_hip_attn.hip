@@ -60,25 +60,34 @@ template <int BM> __device__ Seq seq_of(const AttnArgs &a, int b) {
     return s;
 }
 
-constexpr int CHUNK_MIN = 128;   // keys
+constexpr int CHUNK_MIN = 128, CHUNK_SAVES = 512;   // keys
 
+// The chunk's keys; 2^30: tiles are whole, which they stay unless chunks shorten the longest by more than CHUNK_SAVES: the parts' sums go through
+// memory and the join takes some 6 us, as much as 512 keys. us, whole and in chunks, 32 heads of 128 over 8, fp16: a prompt of 512 tokens 19 and
+// 28, of 1024 31 and 46; 64 tokens behind 2000 of 64 elements 18.5 (chunks of 512) and 14.
 template <int BM> __device__ int chunk_of(const AttnArgs &a) {
     if (!a.target) return 1 << 30;
     unsigned long long all = 0;
+    int longest = 0;
     if (a.nseq == 1) {
         const Seq s = seq_of<BM>(a, 0);
-        all = (unsigned long long)s.tiles * (unsigned)(s.len - s.base);
+        longest = s.len - s.base;
+        all = (unsigned long long)s.tiles * (unsigned)longest;
     } else {
         for (int b = threadIdx.x & 63; b < a.nseq; b += 64) {
             const Seq s = seq_of<BM>(a, b);
             all += (unsigned long long)s.tiles * (unsigned)(s.len - s.base);
+            if (s.tiles) longest = max(longest, s.len - s.base);
         }
 #pragma unroll
-        for (int d = 32; d; d >>= 1) all += __shfl_xor(all, d);
+        for (int d = 32; d; d >>= 1) {
+            all += __shfl_xor(all, d);
+            longest = max(longest, __shfl_xor(longest, d));
+        }
     }
     const unsigned long long per = (all + a.target - 1) / a.target;
-    const unsigned long long chunk = (per + CHUNK_MIN - 1) / CHUNK_MIN * CHUNK_MIN;
-    return __builtin_amdgcn_readfirstlane((int)min(max(chunk, (unsigned long long)CHUNK_MIN), 1ull << 30));
+    const unsigned long long chunk = max((per + CHUNK_MIN - 1) / CHUNK_MIN * CHUNK_MIN, (unsigned long long)CHUNK_MIN);
+    return __builtin_amdgcn_readfirstlane((unsigned long long)longest <= chunk + CHUNK_SAVES ? 1 << 30 : (int)chunk);
 }
 __device__ int chunks_of(const Seq &s, int chunk) { return max(1, (s.len - s.base + chunk - 1) / chunk); }
 
@@ -907,56 +916,60 @@ template <bool BF, int NQ, int DP, int W, int NB> __global__ __launch_bounds__(6
 
 // ---- parts joined ------------------------------------------------------------------------------------------------------------
 // out of a prompt's row = sum over its parts of 2^(m of the part - the largest m) * (the part's sum), over the same of l: the weights first,
-// in LDS, then the sums in the order of the parts, dim / 4 threads (rounded up to 16, 32 or 64) a row, as many rows as that gives a workgroup.
+// in LDS, then the sums in the order of the parts, dim / 4 threads (rounded up to 16, 32 or 64) a row, as many rows as that gives a workgroup
+// at a time, of `blocks` workgroups to a tile in turn.
 constexpr int PARTS = 512;   // workgroups that a call is split into, about: two per CU
 constexpr int TALL = 1;      // tiles of eight waves from so many times that many on
-template <bool F32, bool BF> __global__ __launch_bounds__(256) void attn_join_kernel(AttnArgs a) {
+template <bool F32, bool BF> __global__ __launch_bounds__(256) void attn_join_kernel(AttnArgs a, int blocks) {
     const int quads = a.c.dim / 4, w = quads <= 16 ? 16 : quads <= 32 ? 32 : 64;   // threads per row
     const int d = threadIdx.x % w, k = threadIdx.x / w, groups = 256 / w;
-    const int blocks = PM / groups;   // workgroups per tile
     const int head = blockIdx.x % a.c.heads, block = blockIdx.x / a.c.heads % blocks;
     const int chunk = chunk_of<PM>(a);
     Part p;
     if (!part_of<PM, true>(a, blockIdx.x / a.c.heads / blocks, chunk, p) || p.chunks == 1) return;   // (one part: written already)
     const uint32_t first = p.first + (uint32_t)p.tile * (uint32_t)p.chunks;
     const int tile = p.s.tiles - 1 - p.tile;
-    const int rows = min(PM, p.s.n * a.G - tile * PM), row = block * groups + k;
-    if (block * groups >= rows || p.chunks > PARTS + 1 || (size_t)first + p.chunks > (size_t)a.items) return;   // (the latter two: starts out of order)
-    const size_t at = ((size_t)first * a.c.heads + head) * PM + min(row, rows - 1), step = (size_t)a.c.heads * PM;
-
+    const int rows = min(PM, p.s.n * a.G - tile * PM);
+    if (p.chunks > PARTS + 1 || (size_t)first + p.chunks > (size_t)a.items) return;   // (starts out of order)
     __shared__ float wt[16][PARTS + 1];
     float *f = wt[k];
-    float m = LOWEST;
-    for (int c = d; c < p.chunks; c += w) {
-        const float2 ml = a.pml[at + c * step];
-        if (ml.y != 0.0f) m = fmaxf(m, ml.x);
-    }
-    for (int o = w / 2; o; o >>= 1) m = fmaxf(m, __shfl_xor(m, o));
-    float l = 0.0f;
-    for (int c = d; c < p.chunks; c += w) {
-        const float2 ml = a.pml[at + c * step];
-        const float x = ml.y != 0.0f ? __builtin_amdgcn_exp2f(ml.x - reference(m)) : 0.0f;
-        f[c] = x;
-        l += x * ml.y;
-    }
-    for (int o = w / 2; o; o >>= 1) l += __shfl_xor(l, o);
-    __syncthreads();
-    if (d >= quads || row >= rows) return;
-    f4 x = {0, 0, 0, 0};
-    const float *y = a.po + at * a.c.dim + d * 4;
-    const size_t pitch = step * a.c.dim;
+    for (int row0 = block * groups; row0 < rows; row0 += blocks * groups) {
+        const int row = row0 + k;
+        const size_t at = ((size_t)first * a.c.heads + head) * PM + min(row, rows - 1), step = (size_t)a.c.heads * PM;
+        float m = LOWEST;
+        for (int c = d; c < p.chunks; c += w) {
+            const float2 ml = a.pml[at + c * step];
+            if (ml.y != 0.0f) m = fmaxf(m, ml.x);
+        }
+        for (int o = w / 2; o; o >>= 1) m = fmaxf(m, __shfl_xor(m, o));
+        float l = 0.0f;
+        for (int c = d; c < p.chunks; c += w) {
+            const float2 ml = a.pml[at + c * step];
+            const float x = ml.y != 0.0f ? __builtin_amdgcn_exp2f(ml.x - reference(m)) : 0.0f;
+            f[c] = x;
+            l += x * ml.y;
+        }
+        for (int o = w / 2; o; o >>= 1) l += __shfl_xor(l, o);
+        __syncthreads();
+        if (d < quads && row < rows) {
+            f4 x = {0, 0, 0, 0};
+            const float *y = a.po + at * a.c.dim + d * 4;
+            const size_t pitch = step * a.c.dim;
 #pragma unroll 8
-    for (int c = 0; c < p.chunks; c++) {
-        const f4 v = *reinterpret_cast<const f4 *>(y + c * pitch);
+            for (int c = 0; c < p.chunks; c++) {
+                const f4 v = *reinterpret_cast<const f4 *>(y + c * pitch);
 #pragma unroll
-        for (int i = 0; i < 4; i++) x[i] = __builtin_fmaf(f[c], v[i], x[i]);
+                for (int i = 0; i < 4; i++) x[i] = __builtin_fmaf(f[c], v[i], x[i]);
+            }
+            const int r = tile * PM + row, query = r / a.G;
+            float o[4];
+            const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+#pragma unroll
+            for (int i = 0; i < 4; i++) o[i] = l == 0.0f ? 0.0f : x[i] * inv;
+            store4<F32, BF>(a.out + (size_t)(p.s.t0 + query) * a.ostride + (size_t)(head * a.G + r - query * a.G) * a.c.dim * (F32 ? 4 : 2), d * 4, o);
+        }
+        __syncthreads();   // the next rows' weights go where these were
     }
-    const int r = tile * PM + row, query = r / a.G;
-    float o[4];
-    const float inv = l == 0.0f ? 0.0f : 1.0f / l;
-#pragma unroll
-    for (int i = 0; i < 4; i++) o[i] = l == 0.0f ? 0.0f : x[i] * inv;
-    store4<F32, BF>(a.out + (size_t)(p.s.t0 + query) * a.ostride + (size_t)(head * a.G + r - query * a.G) * a.c.dim * (F32 ? 4 : 2), d * 4, o);
 }
 
 // ---- host ------------------------------------------------------------------------------------------------------------------------
@@ -980,7 +993,7 @@ Shape shape_of(const es_hip_kv *kv, int nseq, int ntok, int heads, bool prompt) 
         s.tall = kv->dim <= 128 && (size_t)ntok * G / (2 * PM) >= (size_t)TALL * parts;
         s.bm = s.tall ? 2 * PM : PM;
         s.tiles = (size_t)ntok * G / s.bm + nseq;
-        s.target = s.tall || s.tiles >= (size_t)parts || most <= CHUNK_MIN ? 0 : parts;
+        s.target = s.tall || s.tiles >= (size_t)parts || most <= CHUNK_MIN + CHUNK_SAVES ? 0 : parts;
         s.items = s.tiles + s.target;   // sum of tiles * ceil(span / chunk) <= tiles + target
         s.slots = s.target ? s.items : 0;
     } else {
@@ -1029,7 +1042,8 @@ template <bool BF, int NQ> hipError_t launch(const AttnArgs &a, const Shape &s, 
     hipError_t e = hipGetLastError();
     if (e != hipSuccess || !s.target) return e;
     const int groups = a.c.dim <= 64 ? 16 : a.c.dim <= 128 ? 8 : 4;   // rows that a workgroup joins
-    attn_join_kernel<(NQ > 1), BF><<<(unsigned)(s.tiles * a.c.heads * (PM / groups)), 256, 0, st>>>(a);
+    const int blocks = (int)std::min<size_t>(PM / groups, std::max<size_t>(1, 1024 / (s.tiles * a.c.heads)));   // workgroups per tile: many tiles have one part each
+    attn_join_kernel<(NQ > 1), BF><<<(unsigned)(s.tiles * a.c.heads * blocks), 256, 0, st>>>(a, blocks);
     return hipGetLastError();
 }
 
