@@ -44,19 +44,19 @@ struct AttnArgs {
 // A tile is PM rows of one sequence and K/V head; a part is a tile's chunk of keys. Chunks have one length for the whole call, from the
 // lengths on the device: the least that leaves about `target` parts, so that few rows over many keys fill the device and a captured call
 // adapts to later lengths. Every wave finds its part by a scan over the sequences, 64 at a time.
-constexpr int PM = 128, PN = 64;   // rows of a tile (of four waves; of eight twice as many), keys of a step
+constexpr int PM = 128, PN = 64;   // rows of a tile, keys of a step
 
 struct Seq {
     int t0, n, len;      // first query row, queries, tokens
     int base, tiles;     // first key of the first chunk (a multiple of 64), tiles of PM rows
 };
-template <int BM> __device__ Seq seq_of(const AttnArgs &a, int b) {
+__device__ Seq seq_of(const AttnArgs &a, int b) {
     Seq s;
     s.t0 = min(max(a.start[b], 0), a.ntok);
     s.n = min(max(a.start[b + 1], s.t0), a.ntok) - s.t0;
     s.len = a.c.tokens(b);
     s.base = a.window ? max(0, s.len - s.n - a.window + 1) & ~63 : 0;
-    s.tiles = (int)(((long long)s.n * a.G + BM - 1) / BM);
+    s.tiles = (int)(((long long)s.n * a.G + PM - 1) / PM);
     return s;
 }
 
@@ -65,17 +65,17 @@ constexpr int CHUNK_MIN = 128, CHUNK_SAVES = 512;   // keys
 // The chunk's keys; 2^30: tiles are whole, which they stay unless chunks shorten the longest by more than CHUNK_SAVES: the parts' sums go through
 // memory and the join takes some 6 us, as much as 512 keys. us, whole and in chunks, 32 heads of 128 over 8, fp16: a prompt of 512 tokens 19 and
 // 28, of 1024 31 and 46; 64 tokens behind 2000 of 64 elements 18.5 (chunks of 512) and 14.
-template <int BM> __device__ int chunk_of(const AttnArgs &a) {
+__device__ int chunk_of(const AttnArgs &a) {
     if (!a.target) return 1 << 30;
     unsigned long long all = 0;
     int longest = 0;
     if (a.nseq == 1) {
-        const Seq s = seq_of<BM>(a, 0);
+        const Seq s = seq_of(a, 0);
         longest = s.len - s.base;
         all = (unsigned long long)s.tiles * (unsigned)longest;
     } else {
         for (int b = threadIdx.x & 63; b < a.nseq; b += 64) {
-            const Seq s = seq_of<BM>(a, b);
+            const Seq s = seq_of(a, b);
             all += (unsigned long long)s.tiles * (unsigned)(s.len - s.base);
             if (s.tiles) longest = max(longest, s.len - s.base);
         }
@@ -107,12 +107,12 @@ __device__ uint32_t sum_up_to(uint32_t x) {   // over the lanes up to this one
 }
 // The part with number `item` (within one K/V head), or, TILES, the tile with that number and `chunk` 0; false if there is none. Starts that
 // are out of order may give any number of parts: they are counted modulo 2^32.
-template <int BM, bool TILES> __device__ bool part_of(const AttnArgs &a, int item, int chunk, Part &p) {
+template <bool TILES> __device__ bool part_of(const AttnArgs &a, int item, int chunk, Part &p) {
     const int lane = threadIdx.x & 63;
     uint32_t tiles_before = 0, parts_before = 0;
     if (a.nseq == 1) {
         p.b = 0;
-        p.s = seq_of<BM>(a, 0);
+        p.s = seq_of(a, 0);
         p.chunks = chunks_of(p.s, chunk);
         p.first = 0;
     } else {
@@ -122,7 +122,7 @@ template <int BM, bool TILES> __device__ bool part_of(const AttnArgs &a, int ite
             int chunks = 1;
             uint32_t parts = 0;
             if (g + lane < a.nseq) {
-                s = seq_of<BM>(a, g + lane);
+                s = seq_of(a, g + lane);
                 chunks = chunks_of(s, chunk);
                 parts = (uint32_t)s.tiles * (uint32_t)chunks;
             }
@@ -655,10 +655,10 @@ __device__ u2 transposed(uint32_t lds) {
     return __builtin_bit_cast(u2, __builtin_amdgcn_ds_read_tr16_b64_v4i16(reinterpret_cast<__attribute__((address_space(3))) s4 *>(lds)));
 }
 
-template <bool BF, int NQ, int DP, int W, int NB> __global__ __launch_bounds__(64 * W, W == 8 || !(DP == 256 || (NQ == 3 && DP == 128)) ? 2 : 1) void attn_prompt_kernel(AttnArgs a) {
-    constexpr int BM = 32 * W;
+template <bool BF, int NQ, int DP> __global__ __launch_bounds__(256, DP == 256 || (NQ == 3 && DP == 128) ? 1 : 2) void attn_prompt_kernel(AttnArgs a) {
+    constexpr int NB = DP == 64 ? 3 : 2;                     // steps of keys in LDS
     constexpr int KS = DP / 16, DT = DP / 32, CH = DP / 8;   // CH: pieces of a key
-    constexpr int NI = PN * CH / (64 * W);                   // a wave's instructions for its PN / W keys
+    constexpr int NI = CH / 4;                               // a wave's instructions for its 16 keys
     constexpr int ROWS = 64 / CH;                            // keys of one
     constexpr uint32_t TILE = PN * DP * 2;                   // bytes of K, or V, of a step
     constexpr bool F32 = NQ > 1;
@@ -667,14 +667,14 @@ template <bool BF, int NQ, int DP, int W, int NB> __global__ __launch_bounds__(6
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int col = lane & 31, half = lane >> 5;
     const int head = blockIdx.x % a.c.heads, item = blockIdx.x / a.c.heads;
-    const int chunk = chunk_of<BM>(a);
+    const int chunk = chunk_of(a);
     Part p;
-    if (!part_of<BM, false>(a, item, chunk, p)) return;
+    if (!part_of<false>(a, item, chunk, p)) return;
     const bool whole = chunk == 1 << 30;
     const int tile = p.s.tiles - 1 - p.tile;   // the tiles that see most keys first
-    const int rows = min(BM, p.s.n * a.G - tile * BM);
+    const int rows = min(PM, p.s.n * a.G - tile * PM);
     const int back = p.s.len - p.s.n;          // query i stands at back + i
-    const int pos_lo = back + tile * BM / a.G, pos_hi = back + (tile * BM + rows - 1) / a.G;
+    const int pos_lo = back + tile * PM / a.G, pos_hi = back + (tile * PM + rows - 1) / a.G;
     const int see_lo = a.window ? max(0, pos_lo - a.window + 1) : 0, see_hi = pos_hi + 1;   // keys that some row sees
     int first = p.s.base + (whole ? 0 : p.chunk * chunk);
     const int last = whole ? see_hi : min(see_hi, first + chunk);
@@ -682,7 +682,7 @@ template <bool BF, int NQ, int DP, int W, int NB> __global__ __launch_bounds__(6
     const int *table = a.c.table + (size_t)max(a.c.row(p.b), 0) * a.c.max_pages;
     const int dim = a.c.dim;
 
-    const int r = min(tile * BM + wave * 32 + col, tile * BM + rows - 1);   // lanes past the last row repeat it
+    const int r = min(tile * PM + wave * 32 + col, tile * PM + rows - 1);   // lanes past the last row repeat it
     const int query = r / a.G, pos = back + query, from = a.window ? pos - a.window + 1 : 0;
     const size_t qoff = (size_t)(head * a.G + r - query * a.G) * dim * (F32 ? 4 : 2);
     u4 q[KS][NQ];
@@ -703,19 +703,18 @@ template <bool BF, int NQ, int DP, int W, int NB> __global__ __launch_bounds__(6
     int pb = first >> 4;
     Runs pg = fetch(pb + lane), pgn = fetch(pb + 64 + lane);
 
-    // This wave brings PN / W keys of each step, of run `mine`: key t0w + n * ROWS + lane / CH of it and place lane % CH of that key by instruction n
-    const int mine = wave * (PN / W) / 16, t0w = wave * (PN / W) % 16;
+    // This wave brings run `wave` of each step: key n * ROWS + lane / CH of it and place lane % CH of that key by instruction n
     const uint32_t lds0 = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) uint8_t *)lds;
     constexpr int VN = DP == 256 ? 2 : 1;   // instructions after which V's pieces are exchanged the same way again
     int k_from[NI], v_from[VN];
 #pragma unroll
     for (int n = 0; n < NI; n++) {
-        const int t = t0w + n * ROWS + lane / CH, c = lane % CH ^ k_turn<DP>(t);
+        const int t = n * ROWS + lane / CH, c = lane % CH ^ k_turn<DP>(t);
         k_from[n] = c * 8 < dim ? (t * dim + c * 8) * 2 : 0x40000000;   // (elements past dim: past the run's end)
     }
 #pragma unroll
     for (int n = 0; n < VN; n++) {
-        const int t = t0w + n * ROWS + lane / CH, c = lane % CH ^ v_turn<DP>(t);
+        const int t = n * ROWS + lane / CH, c = lane % CH ^ v_turn<DP>(t);
         v_from[n] = c * 8 < dim ? (t * dim + c * 8) * 2 : 0x40000000;
     }
     // brings the keys from t0 on; which of their four runs are in no page
@@ -727,8 +726,8 @@ template <bool BF, int NQ, int DP, int W, int NB> __global__ __launch_bounds__(6
             pg = pgn;
             pgn = fetch(pb + 64 + lane);
         }
-        const int bytes = min(last - t0 - mine * 16, 16) * dim * 2;
-        const u4 k = run_of(a.c.k, pg, u0 + mine, bytes), v = run_of(a.c.v, pg, u0 + mine, bytes);
+        const int bytes = min(last - t0 - wave * 16, 16) * dim * 2;
+        const u4 k = run_of(a.c.k, pg, u0 + wave, bytes), v = run_of(a.c.v, pg, u0 + wave, bytes);
         const uint32_t to = lds0 + buf * TILE + wave * NI * 1024;
 #pragma unroll
         for (int n = 0; n < NI; n++) run_to_lds(k, k_from[n], 0, to + n * 1024);
@@ -741,7 +740,7 @@ template <bool BF, int NQ, int DP, int W, int NB> __global__ __launch_bounds__(6
         constexpr uint32_t E = BF ? 0x7f80u : 0x7c00u;   // an exponent of ones
         bool left = false;
 #pragma unroll 1
-        for (int i = tid; i < PN * CH; i += 64 * W) {
+        for (int i = tid; i < PN * CH; i += 256) {
             u4 *at = reinterpret_cast<u4 *>(lds + (NB + buf) * TILE) + i;
             u4 x = *at;
             const bool none = t0 + i / CH < see_lo;
@@ -811,6 +810,17 @@ template <bool BF, int NQ, int DP, int W, int NB> __global__ __launch_bounds__(6
 #pragma unroll
                     for (int t = 0; t < NQ; t++) s[h] = mfma32<BF>(kf, q[k][t], s[h]);
                 }
+            // Six reads of K under way, or (below) four fragments of V: as the compiler left it, each product waited for its own. With three terms the
+            // products are long enough. 8192 tokens, us, with and without: heads of 256, fp16 1495 and 1704, fp32 2236 and 2530; of 128 611 and 624.
+            if constexpr (NQ < 3) {
+                __builtin_amdgcn_sched_group_barrier(0x100, 6, 0);
+#pragma unroll
+                for (int i = 0; i < 2 * KS - 6; i++) {
+                    __builtin_amdgcn_sched_group_barrier(0x8, NQ, 0);
+                    __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
+                }
+                __builtin_amdgcn_sched_group_barrier(0x8, 6 * NQ, 0);
+            }
             if (t0 + PN > wpos_lo + 1 || t0 < wfrom_hi) {
                 const int to = pos - t0 - half * 4, since = from - t0 - half * 4;
 #pragma unroll
@@ -865,6 +875,15 @@ template <bool BF, int NQ, int DP, int W, int NB> __global__ __launch_bounds__(6
 #pragma unroll
                     for (int t = 0; t < NQ; t++) acc[j] = mfma32<BF>(vf, pt[u][t], acc[j]);
                 }
+            if constexpr (NQ < 3) {
+                __builtin_amdgcn_sched_group_barrier(0x100, 8, 1);
+#pragma unroll
+                for (int i = 0; i < 4 * DT - 4; i++) {
+                    __builtin_amdgcn_sched_group_barrier(0x8, NQ, 1);
+                    __builtin_amdgcn_sched_group_barrier(0x100, 2, 1);
+                }
+                __builtin_amdgcn_sched_group_barrier(0x8, 4 * NQ, 1);
+            }
         }
         holes >>= 4;
         buf = buf == NB - 1 ? 0 : buf + 1;
@@ -881,15 +900,19 @@ template <bool BF, int NQ, int DP, int W, int NB> __global__ __launch_bounds__(6
             const int page = table[t >> a.c.shift];
             if (page < 0 || page >= a.c.npages) continue;
             const uint8_t *row = a.c.v + a.c.at(page, head, t & ((1 << a.c.shift) - 1));
+            int lane_d = half * 4;
+            asm volatile("" : "+v"(lane_d));   // (or what depends on it is computed ahead of the loop, for all elements)
 #pragma unroll
-            for (int j = 0; j < DT; j++)
+            for (int j = 0; j < DT; j++) {
 #pragma unroll
                 for (int i = 0; i < 16; i++) {
                     using T = std::conditional_t<BF, __bf16, _Float16>;
-                    const int d = j * 32 + i / 4 * 8 + half * 4 + (i & 3);
+                    const int d = j * 32 + i / 4 * 8 + lane_d + (i & 3);
                     const float v = d < dim ? static_cast<float>(*reinterpret_cast<const T *>(row + d * 2)) : 0.0f;
                     if (!(fabsf(v) < INFINITY)) acc[j][i] += v;
                 }
+                __builtin_amdgcn_sched_barrier(0);   // (not all of the row's loads at once, for which there are no registers)
+            }
         }
     }
     const bool done = p.chunks == 1;
@@ -919,14 +942,13 @@ template <bool BF, int NQ, int DP, int W, int NB> __global__ __launch_bounds__(6
 // in LDS, then the sums in the order of the parts, dim / 4 threads (rounded up to 16, 32 or 64) a row, as many rows as that gives a workgroup
 // at a time, of `blocks` workgroups to a tile in turn.
 constexpr int PARTS = 512;   // workgroups that a call is split into, about: two per CU
-constexpr int TALL = 1;      // tiles of eight waves from so many times that many on
 template <bool F32, bool BF> __global__ __launch_bounds__(256) void attn_join_kernel(AttnArgs a, int blocks) {
     const int quads = a.c.dim / 4, w = quads <= 16 ? 16 : quads <= 32 ? 32 : 64;   // threads per row
     const int d = threadIdx.x % w, k = threadIdx.x / w, groups = 256 / w;
     const int head = blockIdx.x % a.c.heads, block = blockIdx.x / a.c.heads % blocks;
-    const int chunk = chunk_of<PM>(a);
+    const int chunk = chunk_of(a);
     Part p;
-    if (!part_of<PM, true>(a, blockIdx.x / a.c.heads / blocks, chunk, p) || p.chunks == 1) return;   // (one part: written already)
+    if (!part_of<true>(a, blockIdx.x / a.c.heads / blocks, chunk, p) || p.chunks == 1) return;   // (one part: written already)
     const uint32_t first = p.first + (uint32_t)p.tile * (uint32_t)p.chunks;
     const int tile = p.s.tiles - 1 - p.tile;
     const int rows = min(PM, p.s.n * a.G - tile * PM);
@@ -974,7 +996,6 @@ template <bool F32, bool BF> __global__ __launch_bounds__(256) void attn_join_ke
 
 // ---- host ------------------------------------------------------------------------------------------------------------------------
 struct Shape {
-    bool tall;         // prompt: tiles of eight waves
     size_t items;      // prompt: the most parts per K/V head that the call's lengths can give; else workgroups per K/V head
     size_t tiles;      // prompt: the most tiles
     int target;        // AttnArgs::target
@@ -990,10 +1011,9 @@ Shape shape_of(const es_hip_kv *kv, int nseq, int ntok, int heads, bool prompt) 
     Shape s{};
     if (prompt) {
         const int parts = std::max(PARTS / kv->heads, 1);
-        s.tall = kv->dim <= 128 && (size_t)ntok * G / (2 * PM) >= (size_t)TALL * parts;
-        s.bm = s.tall ? 2 * PM : PM;
-        s.tiles = (size_t)ntok * G / s.bm + nseq;
-        s.target = s.tall || s.tiles >= (size_t)parts || most <= CHUNK_MIN + CHUNK_SAVES ? 0 : parts;
+        s.bm = PM;
+        s.tiles = (size_t)ntok * G / PM + nseq;
+        s.target = s.tiles >= (size_t)parts || most <= CHUNK_MIN + CHUNK_SAVES ? 0 : parts;
         s.items = s.tiles + s.target;   // sum of tiles * ceil(span / chunk) <= tiles + target
         s.slots = s.target ? s.items : 0;
     } else {
@@ -1032,12 +1052,7 @@ template <bool BF, int NQ> hipError_t launch(const AttnArgs &a, const Shape &s, 
         attn_decode_join_kernel<(NQ > 1), BF><<<(unsigned)((size_t)a.nseq * a.c.heads * ((a.G + together - 1) / together)), 256, 0, st>>>(a, together);
         return hipGetLastError();
     }
-    if (s.tall) {
-        auto f = a.c.dim <= 64 ? attn_prompt_kernel<BF, NQ, 64, 8, 4> : attn_prompt_kernel<BF, NQ, 128, 8, 4>;
-        f<<<grid, 512, 0, st>>>(a);
-        return hipGetLastError();
-    }
-    auto f = a.c.dim <= 64 ? attn_prompt_kernel<BF, NQ, 64, 4, 3> : a.c.dim <= 128 ? attn_prompt_kernel<BF, NQ, 128, 4, 2> : attn_prompt_kernel<BF, NQ, 256, 4, 2>;
+    auto f = a.c.dim <= 64 ? attn_prompt_kernel<BF, NQ, 64> : a.c.dim <= 128 ? attn_prompt_kernel<BF, NQ, 128> : attn_prompt_kernel<BF, NQ, 256>;
     f<<<grid, 256, 0, st>>>(a);
     hipError_t e = hipGetLastError();
     if (e != hipSuccess || !s.target) return e;

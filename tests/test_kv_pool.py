@@ -317,10 +317,9 @@ def test_every_part_has_room(child):
                 continue
             cut = np.sort(rng.integers(0, tokens + 1, nseq - 1))
             n, span = np.diff(np.concatenate([[0], cut, [tokens]])), rng.integers(0, 1 << 20, nseq)
-            tiles = -(-n * G // (launches[0][2] // 2))   # 32 rows a wave
+            tiles = -(-n * G // 128)
             assert len(launches) == (2 if ws else 1)
             if ws:   # the chunk that the device takes: total work over the parts aimed for
-                assert launches[0][2] == 256
                 target = grid // kvh - (tokens * G // 128 + nseq)
                 chunk = max(128, -(-(-(-int((tiles * span).sum()) // target)) // 128) * 128)
                 if (span * (tiles > 0)).max() <= chunk + 512:
