@@ -33,7 +33,8 @@ struct AttnArgs {
     float *po;                 // parts' sums: the same of [dim]
     float2 *pml;               // parts' m and l: [part][row of the tile] (one query per sequence: [head][row][part], two parts a workgroup)
     size_t qstride, ostride;   // bytes
-    int nseq, ntok, G, window;
+    int nseq, ntok, G;
+    int window;                // below the tokens that a table row holds; 0: none
     float c2;                  // scale * log2(e)
     int target;                // parts aimed for per K/V head; 0: every tile is one part. One query per sequence: workgroups
     int block;                 // one query per sequence: log2 of the keys of a block
@@ -1092,7 +1093,7 @@ int attention(const es_hip_kv *kv, int nseq, const int *start, int ntok, int hea
     a.nseq = nseq;
     a.ntok = ntok;
     a.G = heads / kv->heads;
-    a.window = window;
+    a.window = window >= kv->max_pages * kv->page ? 0 : window;   // (len - n - window then fits an int, whatever n)
     a.c2 = std::max(scale * 1.44269504088896340736f, 1.17549435e-38f);
     a.target = s.target;
     a.block = s.block;

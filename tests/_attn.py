@@ -87,18 +87,18 @@ def attention(cache, starts, q, scale, window=0, seq=None):
             continue
         K, V, ok = cache.rows(r)
         n, f = len(K), starts[b + 1] - starts[b]
-        j = np.arange(n)
-        for i in range(f):
-            pos = n - f + i
-            seen = ok & (j <= pos) & ((j > pos - window) if window else True)
-            if not seen.any():
-                continue
-            for h in range(q.shape[1]):
-                s = scale * (K[seen, h // G] @ q[starts[b] + i, h])
-                p = np.exp(s - s.max())
-                p /= p.sum()
-                out[starts[b] + i, h] = p @ V[seen, h // G]
-                mag[starts[b] + i, h] = p @ np.abs(V[seen, h // G])
+        pos, j = np.arange(n - f, n)[:, None], np.arange(n)
+        seen = ok & (j <= pos) & ((j > pos - window) if window else True)
+        some = seen.any(1)
+        if not some.any():
+            continue
+        K, V = np.where(ok[:, None, None], K, 0.0), np.where(ok[:, None, None], V, 0.0)
+        for h in range(q.shape[1]):
+            s = np.where(seen, scale * (q[starts[b]:starts[b + 1], h] @ K[:, h // G].T), -np.inf)
+            p = np.exp(s - np.where(some, s.max(1), 0.0)[:, None])
+            p /= np.where(some, p.sum(1), 1.0)[:, None]
+            out[starts[b]:starts[b + 1], h] = p @ V[:, h // G]
+            mag[starts[b]:starts[b + 1], h] = p @ np.abs(V[:, h // G])
     return out, mag
 
 

@@ -121,6 +121,63 @@ def test_decode_long(hip, types, lens, page):
     assert np.array_equal(got, run(hip, c, starts, q, t, 0.125, decode=True))   # the same from call to call
 
 
+@pytest.mark.parametrize("dim,heads,kvh,page", [(128, 40, 2, 32), (200, 17, 1, 16), (256, 6, 3, 64), (72, 8, 8, 16)])
+@pytest.mark.parametrize("types", TYPES, ids=ids)
+def test_decode_long_heads(hip, types, dim, heads, kvh, page):
+    """split tiles of every width, more than one tile to a K/V head among them"""
+    t, ct = types
+    rng = np.random.default_rng(dim)
+    c = Cache(ct, kvh, dim, page, [1900, 130, 4000], rng)
+    c.fill(rng)
+    q = queries(rng, 3, heads, dim, t)
+    check(c, [0, 1, 2, 3], q, t, dim ** -0.5, run(hip, c, [0, 1, 2, 3], q, t, dim ** -0.5, decode=True))
+
+
+@pytest.mark.parametrize("types", TYPES, ids=ids)
+def test_decode_many_sequences(hip, types):
+    """more sequences than a wave has lanes, of 0 to 1500 tokens, by number"""
+    t, ct = types
+    rng = np.random.default_rng(31)
+    lens = [int(x) for x in np.exp(rng.uniform(0, np.log(1500), 150))]
+    lens[3] = lens[70] = 0
+    c = Cache(ct, 2, 64, 16, lens, rng)
+    c.fill(rng)
+    seq = [int(x) for x in rng.permutation(150)] + [-1, 70, 7]
+    starts = list(range(len(seq) + 1))
+    q = queries(rng, len(seq), 8, 64, t)
+    check(c, starts, q, t, 0.125, run(hip, c, starts, q, t, 0.125, seq=seq, decode=True), seq=seq)
+
+
+def test_decode_many_kv_heads(hip):
+    """so many K/V heads that each has one workgroup, which goes through more than 64 blocks of a sequence"""
+    rng = np.random.default_rng(32)
+    c = Cache(E.F16, 512, 8, 16, [9000, 333], rng)
+    x = rng.standard_normal((2,) + c.k.shape).astype(np.float32)
+    c.k, c.v = to_bits(x[0], E.F16), to_bits(x[1], E.F16)
+    q = queries(rng, 2, 512, 8, E.F32)
+    check(c, [0, 1, 2], q, E.F32, 0.4, run(hip, c, [0, 1, 2], q, E.F32, 0.4, decode=True))
+
+
+@pytest.mark.parametrize("prompt", [False, True])
+@pytest.mark.parametrize("types", TYPES, ids=ids)
+def test_out_in_place_of_q(hip, types, prompt):
+    t, ct = types
+    rng = np.random.default_rng(33)
+    c = Cache(ct, 2, 64, 16, [2000, 90], rng)
+    c.fill(rng)
+    starts = [0, 60, 150] if prompt else [0, 1, 2]
+    q = queries(rng, starts[-1], 8, 64, t)
+    kv, keep = c.upload(hip)
+    dq, ds = hip.upload(q), hip.upload(np.array(starts, np.int32))
+    ws = hip.attn_prompt_workspace(kv, 2, starts[-1], 8, t) if prompt else hip.attn_decode_workspace(kv, 2, 8)
+    dw = hip.alloc(ws)
+    if prompt:
+        hip.attn_prompt_dev(kv, 2, ds, starts[-1], 8, t, dq, 0, 0.125, 0, dq, 0, dw, ws)
+    else:
+        hip.attn_decode_dev(kv, 2, 8, t, dq, 0, 0.125, 0, dq, 0, dw, ws)
+    check(c, starts, q, t, 0.125, hip.download(dq, np.zeros_like(q)))
+
+
 @pytest.mark.parametrize("window", [1, 2, 16, 17, 100, 128, 1000, 5000])
 @pytest.mark.parametrize("types", TYPES, ids=ids)
 def test_decode_window(hip, types, window):
@@ -210,6 +267,12 @@ def test_decode_far_offsets(hip):
     dw = hip.alloc(ws)
     hip.attn_decode_dev(kv, 1, heads, E.F32, dq, 0, 1 / 16, 0, do, 0, dw, ws)
     check(c, [0, 1], q, E.F32, 1 / 16, hip.download(do, np.zeros_like(q)))
+    q = queries(rng, 30, heads, dim, E.F32)
+    dq, do, ds = hip.upload(q), hip.alloc(q.nbytes), hip.upload(np.array([0, 30], np.int32))
+    ws = hip.attn_prompt_workspace(kv, 1, 30, heads, E.F32)
+    dw = hip.alloc(ws)
+    hip.attn_prompt_dev(kv, 1, ds, 30, heads, E.F32, dq, 0, 1 / 16, 0, do, 0, dw, ws)
+    check(c, [0, 30], q, E.F32, 1 / 16, hip.download(do, np.zeros_like(q)))
 
 
 # ---- prompts -----------------------------------------------------------------------------------------------------------------
@@ -253,6 +316,18 @@ def test_prompt_window(hip, types, window):
     check(c, starts, q, t, 0.125, run(hip, c, starts, q, t, 0.125, window), window)
 
 
+@pytest.mark.parametrize("window", [3000, 1 << 30, (1 << 31) - 1])
+@pytest.mark.parametrize("decode", [False, True])
+def test_window_wider_than_the_cache(hip, window, decode):
+    """split tiles beside padding that brings more queries than it has tokens"""
+    rng = np.random.default_rng(36)
+    c = Cache(E.F16, 1, 64, 16, [2500, 0, 3, 700], rng)
+    c.fill(rng)
+    starts = [0, 1, 2, 3, 4] if decode else [0, 9, 49, 60, 63]
+    q = queries(rng, starts[-1], 4, 64, E.F32)
+    check(c, starts, q, E.F32, 0.125, run(hip, c, starts, q, E.F32, 0.125, window, decode=decode), window)
+
+
 @pytest.mark.parametrize("lens,new", [([3000], [5]), ([2500, 30, 700], [17, 30, 1]), ([1500], [200])])
 @pytest.mark.parametrize("types", TYPES, ids=ids)
 def test_prompt_behind_long_prefix(hip, types, lens, new):
@@ -266,6 +341,44 @@ def test_prompt_behind_long_prefix(hip, types, lens, new):
     got = run(hip, c, starts, q, t, 0.125)
     check(c, starts, q, t, 0.125, got)
     assert np.array_equal(got, run(hip, c, starts, q, t, 0.125))
+
+
+@pytest.mark.parametrize("dim,heads,kvh,page", [(128, 32, 4, 32), (200, 5, 1, 16), (256, 6, 3, 64), (72, 8, 8, 1024)])
+@pytest.mark.parametrize("types", TYPES, ids=ids)
+def test_prompt_prefix_heads(hip, types, dim, heads, kvh, page):
+    t, ct = types
+    rng = np.random.default_rng(dim)
+    lens, new = [2200, 1300], [33, 64]
+    c = Cache(ct, kvh, dim, page, lens, rng)
+    c.fill(rng)
+    starts = [0] + np.cumsum(new).tolist()
+    q = queries(rng, starts[-1], heads, dim, t)
+    check(c, starts, q, t, dim ** -0.5, run(hip, c, starts, q, t, dim ** -0.5))
+
+
+@pytest.mark.parametrize("types", TYPES, ids=ids)
+def test_prompt_many_sequences(hip, types):
+    """more sequences than a wave has lanes, split and whole tiles among them, by number"""
+    t, ct = types
+    rng = np.random.default_rng(34)
+    lens = [int(x) for x in np.exp(rng.uniform(0, np.log(1500), 140))]
+    new = [min(n, int(x)) for n, x in zip(lens, rng.integers(0, 12, 140))]
+    c = Cache(ct, 1, 64, 16, lens, rng)
+    c.fill(rng)
+    seq = [int(x) for x in rng.permutation(140)]
+    starts = [0] + np.cumsum([new[s] for s in seq]).tolist()
+    q = queries(rng, starts[-1], 4, 64, t)
+    check(c, starts, q, t, 0.125, run(hip, c, starts, q, t, 0.125, seq=seq), seq=seq)
+
+
+def test_prompt_whole_tiles_over_long_prefix(hip):
+    """enough rows that no tile is split, over more keys than a wave looks up the pages of at a time"""
+    rng = np.random.default_rng(35)
+    c = Cache(E.BF16, 64, 8, 16, [3000], rng)
+    x = rng.standard_normal((2,) + c.k.shape).astype(np.float32)
+    c.k, c.v = to_bits(x[0], E.BF16), to_bits(x[1], E.BF16)
+    q = queries(rng, 300, 256, 8, E.F32)
+    check(c, [0, 300], q, E.F32, 0.4, run(hip, c, [0, 300], q, E.F32, 0.4))
 
 
 @pytest.mark.parametrize("types", TYPES, ids=ids)
