@@ -452,7 +452,8 @@ int  es_hip_cache_get_stats(const es_hip_cache *c, es_hip_cache_stats *out);
  * The arrays on the device are read when the work runs, so a captured call follows their later contents; the struct itself is
  * read at the call. Whatever they hold, no access leaves the pools: len is taken as at least 0 and at most max_pages * page,
  * a sequence whose row is outside [0, rows) has no tokens, and the tokens of a page outside [0, npages) take no part (nothing
- * is written for them, no query sees them), so that padded batches and tables with holes are in order. */
+ * is written for them, no query sees them), so that padded batches and tables with holes are in order. The calling thread's
+ * current device is the one of the buffers and the stream, here as in every other call. */
 typedef struct {
     uint32_t type;      /* ES_HIP_F16 or ES_HIP_BF16 */
     int heads, dim;     /* K/V heads; elements per head, a multiple of 8 up to 256 */
@@ -469,8 +470,8 @@ typedef struct {
  * (start: device, nseq + 1 entries, not decreasing; NULL: one token per sequence, ntok = nseq). Rows from start[nseq] on are
  * not read; nothing is written for rows whose token would lie before the first or in no page. src_type: ES_HIP_F32 or the
  * cache's own type; token t's heads * dim elements at k + t * kstride elements (0: packed), the same for v; aligned to their
- * type. A page that several rows of the table share is written through whichever asks: see es_hip_kv_seq_extend for
- * private copies. */
+ * type. A page that several rows of the table share is written through whichever asks (of two tokens of one call that have the
+ * same place, either may stay): see es_hip_kv_seq_extend for private copies. */
 int es_hip_kv_append_dev(const es_hip_kv *kv, int nseq, const int *start, int ntok, uint32_t src_type, const void *k,
                          size_t kstride, const void *v, size_t vstride, void *stream);
 /* Attention of one new token per sequence, the last in its cache (append it first):
@@ -478,10 +479,13 @@ int es_hip_kv_append_dev(const es_hip_kv *kv, int nseq, const int *start, int nt
  * (window 0: all), with head h reading K/V head h / (heads / kv->heads). heads: a multiple of kv->heads. type: q's and out's,
  * ES_HIP_F32 (with either cache) or the cache's own; head h of sequence b at q + b * qstride + h * dim elements (0: packed), the
  * same for out; aligned to their type. scale is positive and finite. A sequence without tokens gets zeros. Tokens that
- * a query does not see have no influence, whatever their rows hold. fp32 q is carried to 22 bits or more through the matrix
- * products, as are the weights p; with a 16-bit q, p is rounded to the cache's type.
+ * a query does not see have no influence, whatever their rows hold; an infinity or NaN that it sees in V comes out as an infinity
+ * or NaN in that element. fp32 q is carried to 22 bits or more through the matrix products, as are the weights p; with a 16-bit q,
+ * p is rounded to the cache's type. out may be q itself, with one stride, and overlaps nothing else that the call reads. Limits:
+ * 2^29 query rows (tokens times heads), 2^23 sequences times heads, 2^31 blocks of 128 keys that the table rows could hold.
  * ws: the caller's device workspace of at least es_hip_attn_decode_workspace bytes (16-byte aligned; 0 bytes: may be NULL); its
- * contents need no setup and nothing is kept in it between calls, but calls that may overlap need one each. Nothing is
+ * contents need no setup and nothing is kept in it between calls, but calls that may overlap, captured graphs among them, need
+ * one each. (The workspace functions return 0 for what the calls refuse, es_hip_last_error() the reason.) Nothing is
  * allocated, copied or waited for: the call can be captured. */
 size_t es_hip_attn_decode_workspace(const es_hip_kv *kv, int nseq, int heads);
 int es_hip_attn_decode_dev(const es_hip_kv *kv, int nseq, int heads, uint32_t type, const void *q, size_t qstride, float scale,

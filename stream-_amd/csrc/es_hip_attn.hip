@@ -2,17 +2,19 @@
 // this replaces): out = softmax(scale q k^T) v with one pass over the keys, keeping per query the running maximum m, the sum
 // l of 2^(s - m) and the weighted sum of v rows, all in fp32; a growing maximum scales l and the sum by 2^(m_old - m_new).
 //
-// Rows. The G = heads / kv heads query heads that share a K/V head are rows of one product, for every token of a tile: row r
-// of a sequence is query r / G, head r % G. A prompt's tile is then 128 rows of few tokens (little lost to causality) and a decode
+// Rows. The G = heads / kv heads query heads that share a K/V head are rows of one product, for every token of a tile: row r of
+// a sequence is query r / G, head r % G. A prompt's tile is then 128 rows of few tokens (little lost to causality) and a decode
 // tile the G heads of the one token, and each K or V element that is read serves all of them.
 //
-// Orientation. Both products run transposed, S^T = K q^T and O^T = V^T P^T: a query is a column, so that its m, l and scale live in
-// the lanes of that column, and the layout in which the matrix cores leave S^T is the one in which they take P^T as the second
-// operand, up to an order of the keys that V^T is given too: the weights never leave their registers.
+// Orientation. Both products run transposed, S^T = K q^T and O^T = V^T P^T: a query is a column, so that its m, l and scale
+// live in the lanes of that column, and the layout in which the matrix cores leave S^T is the one in which they take P^T as the
+// second operand, up to an order of the keys that V^T is given too: the weights never leave their registers.
 //
 // fp32 queries. q is split into as many terms of the cache's type as carry fp32's 24 bits (two of fp16 after scaling the row to
 // 2^14, 22 bits; three of bf16), one product each into the same sums, and so are the weights. K and V are exact as they are.
-// fp16 weights are 2^15 p, so that keys down to 2^-29 of the largest keep all their bits.
+// fp16 weights are 2^15 p, so that keys down to 2^-29 of the largest keep all their bits. Queries of the cache's own type go in
+// as they are, and their weights are rounded once to that type, as out will be: half a step of it relative to each, no more
+// than storing the weights would cost; l adds up the unrounded ones.
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
@@ -30,8 +32,8 @@ struct AttnArgs {
     const int *start;          // null: one query per sequence
     const uint8_t *q;
     uint8_t *out;
-    float *po;                 // parts' sums: the same of [dim]
-    float2 *pml;               // parts' m and l: [part][row of the tile] (one query per sequence: [head][row][part], two parts a workgroup)
+    float2 *pml;               // parts' m and l: [part][head][row of the tile] (one query per sequence: [head][row][part])
+    float *po;                 // parts' sums: [dim] for each of those
     size_t qstride, ostride;   // bytes
     int nseq, ntok, G;
     int window;                // below the tokens that a table row holds; 0: none
@@ -42,9 +44,9 @@ struct AttnArgs {
 };
 
 // ---- which work a prompt's workgroup takes ---------------------------------------------------------------------------------------
-// A tile is PM rows of one sequence and K/V head; a part is a tile's chunk of keys. Chunks have one length for the whole call, from the
-// lengths on the device: the least that leaves about `target` parts, so that few rows over many keys fill the device and a captured call
-// adapts to later lengths. Every wave finds its part by a scan over the sequences, 64 at a time.
+// A tile is PM rows of one sequence and K/V head; a part is a tile's chunk of keys. Chunks have one length for the whole call,
+// from the lengths on the device: the least that leaves about `target` parts, so that few rows over many keys fill the device
+// and a captured call adapts to later lengths. Every wave finds its part by a scan over the sequences, 64 at a time.
 constexpr int PM = 128, PN = 64;   // rows of a tile, keys of a step
 
 struct Seq {
@@ -63,9 +65,10 @@ __device__ Seq seq_of(const AttnArgs &a, int b) {
 
 constexpr int CHUNK_MIN = 128, CHUNK_SAVES = 512;   // keys
 
-// The chunk's keys; 2^30: tiles are whole, which they stay unless chunks shorten the longest by more than CHUNK_SAVES: the parts' sums go through
-// memory and the join takes some 6 us, as much as 512 keys. us, whole and in chunks, 32 heads of 128 over 8, fp16: a prompt of 512 tokens 19 and
-// 28, of 1024 31 and 46; 64 tokens behind 2000 of 64 elements 18.5 (chunks of 512) and 14.
+// The chunk's keys; 2^30: tiles are whole, which they stay unless chunks shorten the longest by more than CHUNK_SAVES: the
+// parts' sums go through memory and the join takes some 6 us, as much as 512 keys. us, whole and in chunks, 32 heads of 128
+// over 8, fp16: a prompt of 512 tokens 19 and 28, of 1024 31 and 46; 64 tokens behind 2000 of 64 elements 18.5 (chunks of 512)
+// and 14.
 __device__ int chunk_of(const AttnArgs &a) {
     if (!a.target) return 1 << 30;
     unsigned long long all = 0;
@@ -106,8 +109,8 @@ __device__ uint32_t sum_up_to(uint32_t x) {   // over the lanes up to this one
     }
     return x;
 }
-// The part with number `item` (within one K/V head), or, TILES, the tile with that number and `chunk` 0; false if there is none. Starts that
-// are out of order may give any number of parts: they are counted modulo 2^32.
+// The part with number `item` (within one K/V head), or, TILES, the tile with that number and `chunk` 0; false if there is
+// none. Starts that are out of order may give any number of parts: they are counted modulo 2^32.
 template <bool TILES> __device__ bool part_of(const AttnArgs &a, int item, int chunk, Part &p) {
     const int lane = threadIdx.x & 63;
     uint32_t tiles_before = 0, parts_before = 0;
@@ -210,7 +213,7 @@ __device__ u4 load8(const uint8_t *row, int d, int dim) {
 }
 
 // A query row's terms for the K steps of a product of KS * KL elements a step (lane group g of the row holds elements g * 8 of
-// each), and what the row's scores are multiplied by. xor_lanes: the lanes, apart by that and up, that share a row.
+// each), and what the row's scores are multiplied by. The lanes that share a row are XOR, 2 XOR, ... apart.
 template <bool BF, int NQ, int KS, int KL, int XOR>
 __device__ float load_query(const uint8_t *row, bool valid, int g, int dim, float c2, u4 (&q)[KS][NQ]) {
     if constexpr (NQ == 1) {
@@ -262,8 +265,8 @@ template <bool F32, bool BF> __device__ void store4(uint8_t *row, int d, const f
     }
 }
 
-// Where runs of 16 keys of a sequence and head begin, one run per lane: bytes from a pool's start, negative in the upper half where the run is in
-// no page (or past `last`).
+// Where runs of 16 keys of a sequence and head begin, one run per lane, in bytes from a pool's start; the upper half is negative
+// where the run is in no page, or past `last`.
 struct Runs {
     int lo, hi;
     __device__ Runs(const KvView &c, const int *table, int head, int run, int last) {
@@ -274,10 +277,12 @@ struct Runs {
     }
     __device__ bool none(int lane) const { return __builtin_amdgcn_readlane(hi, lane) < 0; }
 };
-// One of them, for loads whose offsets count from its first row: what lies past its `bytes` reads as zeros, and so does all of a run that is in no
-// page (the bounds are the loads' own; an address needs no lane's registers but its offset). Run's loads are non-temporal: nobody else reads
-// these keys soon.
-__device__ u4 run_of(const uint8_t *pool, const Runs &all, int lane, int bytes) {   // (as four words)
+// A buffer descriptor of one of them, for loads whose offsets count from its first row: the loads check their own bounds, so that
+// what lies past its `bytes` reads as zeros, and so does all of a run that is in no page, and no lane holds an address, only
+// its offset. run_of gives it as four words, for asm; Run loads by it, past the caches, as nobody else reads a decode call's keys
+// soon. us so and through the caches: 131072 tokens, 4 heads of 128, 51 and 58; 32 sequences of 77 to 8192 tokens 38 and 42; only
+// what the last-level cache holds whole loses (48 windows of 4096 tokens, 2 heads of 64, 79 MB: 24 and 22).
+__device__ u4 run_of(const uint8_t *pool, const Runs &all, int lane, int bytes) {
     const int hi = __builtin_amdgcn_readlane(all.hi, lane);
     const uint64_t at = reinterpret_cast<uint64_t>(pool) + ((uint64_t)(uint32_t)max(hi, 0) << 32 | (uint32_t)__builtin_amdgcn_readlane(all.lo, lane));
     return u4{(uint32_t)at, (uint32_t)(at >> 32) & 0xffff, hi < 0 ? 0 : (uint32_t)bytes, 0x00020000};
@@ -303,15 +308,19 @@ template <int J> __device__ uint32_t pair(uint32_t first, uint32_t second) {
 }
 
 // ---- one query per sequence ----------------------------------------------------------------------------------------------------
-// A tile is the G query heads of a sequence's K/V head (16 of them, where there are more), its keys blocks of 128. The tiles' blocks, one
-// after another, are dealt out evenly: workgroup w of a K/V head takes blocks [w * each, (w + 1) * each) of them, whatever sequences they are of,
-// so that a ragged batch keeps every workgroup busy to the end. What a workgroup has of a tile that others have parts of goes to the workspace,
-// and a second launch joins them. (The last workgroup of a tile to arrive could do that in the same launch, but 128 of them counting in one word and
-// one CU reading all their sums took 78 us for one sequence of 131072 tokens, where the two launches take TWO.)
+// A tile is the G query heads of a sequence's K/V head (16 of them, where there are more), its keys blocks of 128. The tiles'
+// blocks, one after another, are dealt out evenly: workgroup w of a K/V head takes blocks [w * each, (w + 1) * each) of them,
+// whatever sequences they are of, so that a ragged batch keeps every workgroup busy to the end. What a workgroup has of a tile
+// that others have parts of goes to the workspace, and a second launch joins them. (The last workgroup of a tile to arrive
+// could do that in the same launch, but 128 of them counting in one word and one CU reading all their sums took 78 us for one
+// sequence of 131072 tokens, where the two launches take 51.) Where no table row holds more than 512 tokens, a tile is one block and one launch does:
+// one sequence of 500 tokens, 32 heads of 64 over 8, 7.1 us, in blocks of 128 with the second launch 10.1.
 //
-// Inside: four waves, each 32 keys at a time in turn, joined in LDS at the end. Nothing is staged: a lane loads its K fragments as the matrix
-// cores take them (key lane % 16, 8 elements) and, of V, the DP / 16 elements from (lane % 16) * DP / 16 on of the 8 keys whose weights it
-// holds, which it turns into 8 keys of one element each with byte permutes. Bound by HBM where the caches are long.
+// Inside: four waves, each 32 keys at a time in turn, joined in LDS at the end. Nothing is staged: a lane loads its K fragments
+// as the matrix cores take them (key lane % 16, 8 elements) and, of V, the DP / 16 elements from (lane % 16) * DP / 16 on of
+// the 8 keys whose weights it holds, which it turns into 8 keys of one element each with byte permutes. A fragment read this
+// way is used once, so that LDS would only add a copy. Bound by HBM where the caches are long: 131072 tokens of 4 heads of 128,
+// fp16, 268 MB in 51 us (5.3 TB/s, joined), where a plain read reaches 6.2.
 constexpr int BLOCK = 7, BLOCK_WHOLE = 9, DECODE_M = 16;   // (log2)
 // workgroups, all heads together: as many as fit the device at once, and no more than bring it to the memory's rate
 constexpr int decode_groups(int dim) { return dim <= 128 ? 512 : 256; }
@@ -397,8 +406,8 @@ template <bool BF, int NQ, int DP> __global__ __launch_bounds__(256, DP == 64 &&
         for (int j = 0; j < DL; j++) acc[j] = f4{0, 0, 0, 0};
         float m = LOWEST, l = 0.0f;
 
-        // This wave's keys of step n: 32 from first + (4 n + wave) * 32 on, two runs of 16. Lane 2 i + h holds where run h of step
-        // 32 s + i begins, of the 32 steps at hand and of the 32 after them.
+        // This wave's keys of step n: 32 from first + (4 n + wave) * 32 on, two runs of 16. Lane 2 i + h holds where run h of
+        // step 32 s + i begins, of the 32 steps at hand and of the 32 after them.
         auto fetch = [&](int n) { return Runs(a.c, table, head, (first >> 4) + ((n + (lane >> 1)) * 4 + wave) * 2 + (lane & 1), last); };
         Runs pg = fetch(0), pgn = fetch(32);
         const int kd = (col * dim + g * 8) * 2, vd = (g * 4 * dim + col * DL) * 2;
@@ -436,7 +445,8 @@ template <bool BF, int NQ, int DP> __global__ __launch_bounds__(256, DP == 64 &&
                 }
             }
         };
-        // The next step's K is loaded once this one's scores are there and its V once this one's is summed, into the same registers.
+        // The next step's K is loaded once this one's scores are there and its V once this one's is summed, into the same
+        // registers.
         const int mine = first + wave * 32, steps = mine < last ? (last - mine + 127) / 128 : 0;
         bool ok[2] = {false, false};
         if (steps > 0) {
@@ -568,9 +578,10 @@ template <bool BF, int NQ, int DP> __global__ __launch_bounds__(256, DP == 64 &&
     }
 }
 
-// The parts of `together` rows of a tile a workgroup (a power of two), dim / 4 threads (rounded up to 16, 32 or 64) to a row and the 256 / that /
-// together such groups of a row sharing its parts: each group finds the weights 2^(m - the largest m) for itself, in LDS. The sums' first loads, which
-// need no weights, go out before them; what order they are added in, the lengths alone give.
+// The parts of `together` rows of a tile a workgroup (a power of two), dim / 4 threads (rounded up to 16, 32 or 64) to a row
+// and the 256 / that / together such groups of a row sharing its parts: each group finds the weights 2^(m - the largest m) for
+// itself, in LDS. The sums' first loads, which need no weights, go out before them; what order they are added in, the lengths
+// alone give.
 template <bool F32, bool BF> __global__ __launch_bounds__(256) void attn_decode_join_kernel(AttnArgs a, int together) {
     constexpr int BM = DECODE_M, AHEAD = 16, MOST = 512;
     const int tiles = (a.G + BM - 1) / BM, dim = a.c.dim, quads = dim / 4;
@@ -637,16 +648,25 @@ template <bool F32, bool BF> __global__ __launch_bounds__(256) void attn_decode_
 }
 
 // ---- a tile of prompt rows -------------------------------------------------------------------------------------------------------
-// A workgroup of four waves takes 128 rows, 32 a wave, against its keys, 64 at a time in LDS, where the next 64 go while these are multiplied:
-// straight from memory (a wave's instruction brings 64 pieces of 16 bytes to consecutive places; which piece, each lane says). K and V lie as
-// in the pools, key after key, but the pieces of a key are exchanged among themselves, so that the lanes of a read (16 keys' pieces of K; of V, the
-// 4 keys of a transposing read, 32 elements of each) fall on different banks: piece c of key t is at c ^ k_turn(t), c ^ v_turn(t).
-// Keys that a row does not see have weight 0, and 0 times an infinity or NaN is not 0: V rows that no row sees are zeros in LDS, and so are such
-// elements of keys that only some rows see; where there were any, they are added to those rows at the end.
+// A workgroup of four waves takes 128 rows, 32 a wave, against its keys, 64 at a time in LDS, where the next 64 go while these
+// are multiplied: straight from memory (a wave's instruction brings 64 pieces of 16 bytes to consecutive places; which piece,
+// each lane says). K and V lie as in the pools, key after key, but the pieces of a key are exchanged among themselves, so that
+// the lanes of a read (16 keys' pieces of K; of V, the 4 keys of a transposing read, 32 elements of each) fall on different
+// banks: piece c of key t is at c ^ k_turn(t), c ^ v_turn(t).
+//
+// Keys that a row does not see have weight 0, and 0 times an infinity or NaN is not 0: V rows that no row sees are zeros in LDS,
+// and so are such elements of keys that only some rows see; where there were any, they are added to those rows at the end.
+//
+// Bound by the matrix cores and their power: 16384 tokens, 32 heads of 128 over 4, fp16, 2.25 ms, 980 TFLOP/s counted causally.
+// Both waves of a SIMD together keep the matrix cores busy for 45% of the cycles, at 2.0 GHz; a large library product, busy for
+// 70%, is clocked at 1.4 and gives 1320. Two workgroups a CU: with 64 rows a wave, which halves the reads of LDS, only one
+// fits, and the exponentials of one wave no longer pass under the products of another: 2.94 ms. Tiles of 256 rows in eight
+// waves: within 2%.
 template <int DP> __device__ constexpr int k_turn(int t) { return DP == 64 ? t >> 1 & 7 : t & 15; }
 template <int DP> __device__ constexpr int v_turn(int t) { return DP == 64 ? (t >> 1 & 1) * 4 : (t & 3) * 4; }
 
-// 64 pieces of 16 bytes from a run into LDS: lane i's, at `lane_offset` + `offset` from the run's first row, to lds + 16 i; zeros past the run's end
+// 64 pieces of 16 bytes from a run into LDS: lane i's, at `lane_offset` + `offset` from the run's first row, to lds + 16 i;
+// zeros past the run's end
 __device__ void run_to_lds(u4 r, int lane_offset, int offset, uint32_t lds) {
     asm volatile("s_mov_b32 m0, %3\n\ts_nop 0\n\tbuffer_load_dwordx4 %0, %1, %2 offen lds" ::"v"(lane_offset), "s"(r), "s"(offset), "s"(lds) : "memory");
 }
@@ -736,7 +756,8 @@ template <bool BF, int NQ, int DP> __global__ __launch_bounds__(256, DP == 256 |
         for (int n = 0; n < NI; n++) run_to_lds(v, v_from[n % VN], n / VN * VN * ROWS * dim * 2, to + NB * TILE + n * 1024);
         return (int)(__ballot(pg.hi < 0) >> u0 & 15);
     };
-    // V of the step from t0 on, where some row does not see all of its keys: zeros for what none sees or must not be multiplied by 0
+    // V of the step from t0 on, where some row does not see all of its keys: zeros for what none sees or must not be multiplied
+    // by 0
     auto clean = [&](int t0, int buf) {
         constexpr uint32_t E = BF ? 0x7f80u : 0x7c00u;   // an exponent of ones
         bool left = false;
@@ -762,7 +783,8 @@ template <bool BF, int NQ, int DP> __global__ __launch_bounds__(256, DP == 256 |
         else asm volatile("s_waitcnt vmcnt(%0)" ::"n"((NB - 2) * 2 * NI) : "memory");   // (what was asked for last comes last)
         __syncthreads();
     };
-    // reads: K piece (k * 2 + half) of key h * 32 + col; of V, as transposed() takes them, 4 elements of key u * 16 + r * 8 + half * 4 + lane % 16 / 4
+    // reads: K piece (k * 2 + half) of key h * 32 + col; of V, as transposed() takes them, 4 elements of key u * 16 + r * 8 +
+    // half * 4 + lane % 16 / 4
     constexpr int KA = KS < 8 ? KS : 8, VA = DT < 4 ? DT : 4;   // (addresses that are not another's at a constant distance)
     uint32_t k_at[KA], v_at[VA];
 #pragma unroll
@@ -811,8 +833,9 @@ template <bool BF, int NQ, int DP> __global__ __launch_bounds__(256, DP == 256 |
 #pragma unroll
                     for (int t = 0; t < NQ; t++) s[h] = mfma32<BF>(kf, q[k][t], s[h]);
                 }
-            // Six reads of K under way, or (below) four fragments of V: as the compiler left it, each product waited for its own. With three terms the
-            // products are long enough. 8192 tokens, us, with and without: heads of 256, fp16 1495 and 1704, fp32 2236 and 2530; of 128 611 and 624.
+            // Six reads of K under way, or (below) four fragments of V: as the compiler left it, each product waited for its
+            // own. With three terms the products are long enough. 8192 tokens, us, with and without: heads of 256, fp16 1495
+            // and 1704, fp32 2236 and 2530; of 128 611 and 624.
             if constexpr (NQ < 3) {
                 __builtin_amdgcn_sched_group_barrier(0x100, 6, 0);
 #pragma unroll
@@ -939,9 +962,9 @@ template <bool BF, int NQ, int DP> __global__ __launch_bounds__(256, DP == 256 |
 }
 
 // ---- parts joined ------------------------------------------------------------------------------------------------------------
-// out of a prompt's row = sum over its parts of 2^(m of the part - the largest m) * (the part's sum), over the same of l: the weights first,
-// in LDS, then the sums in the order of the parts, dim / 4 threads (rounded up to 16, 32 or 64) a row, as many rows as that gives a workgroup
-// at a time, of `blocks` workgroups to a tile in turn.
+// out of a prompt's row = sum over its parts of 2^(m of the part - the largest m) * (the part's sum), over the same of l: the
+// weights first, in LDS, then the sums in the order of the parts, dim / 4 threads (rounded up to 16, 32 or 64) a row, as many
+// rows as that gives a workgroup at a time, of `blocks` workgroups to a tile in turn.
 constexpr int PARTS = 512;   // workgroups that a call is split into, about: two per CU
 template <bool F32, bool BF> __global__ __launch_bounds__(256) void attn_join_kernel(AttnArgs a, int blocks) {
     const int quads = a.c.dim / 4, w = quads <= 16 ? 16 : quads <= 32 ? 32 : 64;   // threads per row

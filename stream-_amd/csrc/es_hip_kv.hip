@@ -54,9 +54,10 @@ namespace {
 using namespace esq;
 
 // ---- new rows ------------------------------------------------------------------------------------------------------------
-// One thread per 8 elements of K and the same of V: 16 bytes of each pool. Where its token goes are three dependent loads (start, len, table),
-// the same ones for all threads of the row, under which the elements' own loads are on their way. Bound by its reads and writes where it is
-// long (71 MB, fp32 to bf16, in 12.7 us), by its launch where it is short (one token 4.1 us, of which its kernel 2).
+// One thread per 8 elements of K and the same of V: 16 bytes of each pool. Where its token goes are three dependent loads
+// (start, len, table), the same ones for all threads of the row, under which the elements' own loads are on their way. Bound by
+// its reads and writes where it is long (71 MB, fp32 to bf16, in 12.7 us), by its launch where it is short (one token 4.1 us,
+// of which its kernel 2).
 struct AppendArgs {
     KvView c;
     const int *start;
@@ -120,9 +121,10 @@ template <bool F32, bool BF> __global__ __launch_bounds__(256) void kv_append_ke
 }
 
 // ---- pages copied ----------------------------------------------------------------------------------------------------------
-// The pairs travel with the launch (a kernel's arguments hold 4 KB): no list in memory, nothing to wait for. 16 KB per workgroup, four loads
-// in flight per thread. Bound by HBM where it is long: copies of COPY_ONCE bytes and more go past the caches (ONCE). us past them and through
-// them, bytes read and written: 63 MB 12.4 and 10.8, 126 MB 24.5 and 29.3, 786 MB 159 (4.9 TB/s) and 175.
+// The pairs travel with the launch (a kernel's arguments hold 4 KB): no list in memory, nothing to wait for. 16 KB per
+// workgroup, four loads in flight per thread. Bound by HBM where it is long: copies of COPY_ONCE bytes and more go past the
+// caches (ONCE). us past them and through them, bytes read and written: 63 MB 12.4 and 10.8, 126 MB 24.5 and 29.3, 786 MB 159
+// (4.9 TB/s) and 175.
 constexpr int COPY_PAIRS = 448, COPY_BYTES = 16384;
 constexpr size_t COPY_ONCE = 96u << 20;   // bytes read and written
 struct CopyArgs {
