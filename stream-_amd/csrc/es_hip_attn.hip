@@ -39,6 +39,7 @@ struct AttnArgs {
     int window;                // below the tokens that a table row holds; 0: none
     float c2;                  // scale * log2(e)
     int target;                // parts aimed for per K/V head; 0: every tile is one part. One query per sequence: workgroups
+    bool pairs;                // target is two workgroups a CU
     int block;                 // one query per sequence: log2 of the keys of a block
     int items;                 // parts per K/V head that there is room for
 };
@@ -48,6 +49,9 @@ struct AttnArgs {
 // from the lengths on the device: the least that leaves about `target` parts, so that few rows over many keys fill the device
 // and a captured call adapts to later lengths. Every wave finds its part by a scan over the sequences, 64 at a time.
 constexpr int PM = 128, PN = 64;   // rows of a tile, keys of a step
+// workgroups that a CU holds at once (registers and LDS), with queries of nq terms and heads of dim elements
+constexpr int prompt_per_cu(int nq, int dim) { return dim > 128 || (nq == 3 && dim > 64) ? 1 : 2; }
+constexpr int PARTS = 256, MOST_PARTS = 512;   // parts that a call is split into, per workgroup that a CU holds; and at most
 
 struct Seq {
     int t0, n, len;      // first query row, queries, tokens
@@ -63,35 +67,58 @@ __device__ Seq seq_of(const AttnArgs &a, int b) {
     return s;
 }
 
-constexpr int CHUNK_MIN = 128, CHUNK_SAVES = 512;   // keys
+constexpr int CHUNK_MIN = 128, CHUNK_SAVES = 512, CHUNK_PAIRS = 384;   // keys
 
 // The chunk's keys; 2^30: tiles are whole, which they stay unless chunks shorten the longest by more than CHUNK_SAVES: the
 // parts' sums go through memory and the join takes some 6 us, as much as 512 keys. us, whole and in chunks, 32 heads of 128
 // over 8, fp16: a prompt of 512 tokens 19 and 28, of 1024 31 and 46; 64 tokens behind 2000 of 64 elements 18.5 (chunks of 512)
 // and 14.
+// One sequence: its tiles' chunks are as many as there is room for (target), and half as many where that is two to a CU and they
+// are of CHUNK_PAIRS keys or less, since twice the parts cost more than the second workgroup of a CU gains: 64 tokens behind
+// 7937, 32 heads of 128 over 4, us, so and in twice the chunks: fp16 27 and 31, fp32 33 and 37; 64 behind 29936, whose chunks
+// are longer, would take 60 instead of 57.
+// Several: the mean share of a place, and, where a CU holds but one workgroup, longer until the sequences' last chunks find room too.
+// Two to a CU even out by themselves, with chunks of whole 128s. us, in bf16 of 256 elements, where one fits, longer and not:
+// 3 sequences of 1250 to 2500 tokens, the last 300 new, 128 and 169; in fp16 of 128, where two fit: 16 of 1500 to 3000, the last 16 new,
+// longer 51 and not 46, with chunks of whole 64s 61.
 __device__ int chunk_of(const AttnArgs &a) {
     if (!a.target) return 1 << 30;
-    unsigned long long all = 0;
-    int longest = 0;
+    int chunk, longest = 0;
     if (a.nseq == 1) {
         const Seq s = seq_of(a, 0);
         longest = s.len - s.base;
-        all = (unsigned long long)s.tiles * (unsigned)longest;
+        const float chunks = fmaxf(1.0f, floorf((float)a.target / (float)max(s.tiles, 1)));
+        chunk = (int)((float)longest / chunks + PN) & -PN;
+        chunk = max(a.pairs && chunk <= CHUNK_PAIRS ? chunk * 2 : chunk, CHUNK_MIN);
     } else {
+        const unsigned step = a.pairs ? CHUNK_MIN : PN;
+        auto rounded = [&](unsigned long long keys) {
+            return (int)min(max((keys + step - 1) / step * step, (unsigned long long)CHUNK_MIN), 1ull << 30);
+        };
+        int tiles = 0, span = 0;   // this lane's sequence, where there are no more than 64
+        unsigned long long all = 0;
         for (int b = threadIdx.x & 63; b < a.nseq; b += 64) {
             const Seq s = seq_of(a, b);
-            all += (unsigned long long)s.tiles * (unsigned)(s.len - s.base);
-            if (s.tiles) longest = max(longest, s.len - s.base);
+            tiles = s.tiles;
+            span = s.len - s.base;
+            all += (unsigned long long)tiles * (unsigned)span;
+            if (tiles) longest = max(longest, span);
         }
 #pragma unroll
         for (int d = 32; d; d >>= 1) {
             all += __shfl_xor(all, d);
             longest = max(longest, __shfl_xor(longest, d));
         }
+        chunk = rounded((all + a.target - 1) / a.target);
+        for (int i = 0; i < 8 && !a.pairs && a.nseq <= 64 && chunk < 1 << 30; i++) {
+            uint32_t parts = (uint32_t)tiles * (uint32_t)max(1, (span + chunk - 1) / chunk);
+#pragma unroll
+            for (int d = 32; d; d >>= 1) parts += __shfl_xor(parts, d);
+            if (parts <= (uint32_t)a.target) break;
+            chunk = max(chunk + PN, rounded((unsigned long long)chunk * parts / a.target));
+        }
     }
-    const unsigned long long per = (all + a.target - 1) / a.target;
-    const unsigned long long chunk = max((per + CHUNK_MIN - 1) / CHUNK_MIN * CHUNK_MIN, (unsigned long long)CHUNK_MIN);
-    return __builtin_amdgcn_readfirstlane((unsigned long long)longest <= chunk + CHUNK_SAVES ? 1 << 30 : (int)chunk);
+    return __builtin_amdgcn_readfirstlane((long long)longest <= (long long)chunk + CHUNK_SAVES ? 1 << 30 : chunk);
 }
 __device__ int chunks_of(const Seq &s, int chunk) { return max(1, (s.len - s.base + chunk - 1) / chunk); }
 
@@ -130,7 +157,8 @@ template <bool TILES> __device__ bool part_of(const AttnArgs &a, int item, int c
                 chunks = chunks_of(s, chunk);
                 parts = (uint32_t)s.tiles * (uint32_t)chunks;
             }
-            const uint32_t mine = TILES ? (uint32_t)s.tiles : parts, upto = sum_up_to(mine), parts_upto = TILES ? sum_up_to(parts) : upto;
+            const uint32_t mine = TILES ? (uint32_t)s.tiles : parts, upto = sum_up_to(mine);
+            const uint32_t parts_upto = TILES ? sum_up_to(parts) : upto;
             uint32_t &before = TILES ? tiles_before : parts_before;
             const unsigned long long past = __ballot((uint32_t)item < before + upto);
             if (past) {
@@ -676,7 +704,7 @@ __device__ u2 transposed(uint32_t lds) {
     return __builtin_bit_cast(u2, __builtin_amdgcn_ds_read_tr16_b64_v4i16(reinterpret_cast<__attribute__((address_space(3))) s4 *>(lds)));
 }
 
-template <bool BF, int NQ, int DP> __global__ __launch_bounds__(256, DP == 256 || (NQ == 3 && DP == 128) ? 1 : 2) void attn_prompt_kernel(AttnArgs a) {
+template <bool BF, int NQ, int DP> __global__ __launch_bounds__(256, prompt_per_cu(NQ, DP)) void attn_prompt_kernel(AttnArgs a) {
     constexpr int NB = DP == 64 ? 3 : 2;                     // steps of keys in LDS
     constexpr int KS = DP / 16, DT = DP / 32, CH = DP / 8;   // CH: pieces of a key
     constexpr int NI = CH / 4;                               // a wave's instructions for its 16 keys
@@ -965,7 +993,6 @@ template <bool BF, int NQ, int DP> __global__ __launch_bounds__(256, DP == 256 |
 // out of a prompt's row = sum over its parts of 2^(m of the part - the largest m) * (the part's sum), over the same of l: the
 // weights first, in LDS, then the sums in the order of the parts, dim / 4 threads (rounded up to 16, 32 or 64) a row, as many
 // rows as that gives a workgroup at a time, of `blocks` workgroups to a tile in turn.
-constexpr int PARTS = 512;   // workgroups that a call is split into, about: two per CU
 template <bool F32, bool BF> __global__ __launch_bounds__(256) void attn_join_kernel(AttnArgs a, int blocks) {
     const int quads = a.c.dim / 4, w = quads <= 16 ? 16 : quads <= 32 ? 32 : 64;   // threads per row
     const int d = threadIdx.x % w, k = threadIdx.x / w, groups = 256 / w;
@@ -976,8 +1003,8 @@ template <bool F32, bool BF> __global__ __launch_bounds__(256) void attn_join_ke
     const uint32_t first = p.first + (uint32_t)p.tile * (uint32_t)p.chunks;
     const int tile = p.s.tiles - 1 - p.tile;
     const int rows = min(PM, p.s.n * a.G - tile * PM);
-    if (p.chunks > PARTS + 1 || (size_t)first + p.chunks > (size_t)a.items) return;   // (starts out of order)
-    __shared__ float wt[16][PARTS + 1];
+    if (p.chunks > MOST_PARTS + 1 || (size_t)first + p.chunks > (size_t)a.items) return;   // (starts out of order)
+    __shared__ float wt[16][MOST_PARTS + 1];
     float *f = wt[k];
     for (int row0 = block * groups; row0 < rows; row0 += blocks * groups) {
         const int row = row0 + k;
@@ -1023,18 +1050,21 @@ struct Shape {
     size_t items;      // prompt: the most parts per K/V head that the call's lengths can give; else workgroups per K/V head
     size_t tiles;      // prompt: the most tiles
     int target;        // AttnArgs::target
+    bool pairs;        // AttnArgs::pairs
     int block;         // AttnArgs::block
     size_t slots;      // parts per K/V head that the workspace holds
     int bm;
     size_t sums(const es_hip_kv *kv) const { return slots * kv->heads * bm * (size_t)kv->dim * sizeof(float); }
     size_t workspace(const es_hip_kv *kv) const { return sums(kv) + slots * kv->heads * bm * sizeof(float2); }
 };
-Shape shape_of(const es_hip_kv *kv, int nseq, int ntok, int heads, bool prompt) {
+Shape shape_of(const es_hip_kv *kv, int nseq, int ntok, int heads, uint32_t type, bool prompt) {
     const int G = heads / kv->heads;
     const long long most = (long long)kv->max_pages * kv->page;
     Shape s{};
     if (prompt) {
-        const int parts = std::max(PARTS / kv->heads, 1);
+        const int per_cu = prompt_per_cu(kv->type == ES_HIP_BF16 && type == ES_HIP_F32 ? 3 : type == ES_HIP_F32 ? 2 : 1, kv->dim);
+        const int parts = std::max(PARTS * per_cu / kv->heads, 1);
+        s.pairs = per_cu == 2;
         s.bm = PM;
         s.tiles = (size_t)ntok * G / PM + nseq;
         s.target = s.tiles >= (size_t)parts || most <= CHUNK_MIN + CHUNK_SAVES ? 0 : parts;
@@ -1102,7 +1132,7 @@ int attention(const es_hip_kv *kv, int nseq, const int *start, int ntok, int hea
     if (!qstride) qstride = row;
     if (!ostride) ostride = row;
     if (ntok > 1 && (qstride < row || ostride < row)) return host_fail(ES_HIP_EINVAL, "rows overlap (stride below heads * dim)");
-    const Shape s = shape_of(kv, nseq, ntok, heads, prompt);
+    const Shape s = shape_of(kv, nseq, ntok, heads, type, prompt);
     const size_t need = s.workspace(kv);
     if (need && (!ws || ws_bytes < need || (reinterpret_cast<uintptr_t>(ws) & 15)))
         return host_fail(ES_HIP_EINVAL, "workspace missing, too small or misaligned (16 bytes)");
@@ -1119,6 +1149,7 @@ int attention(const es_hip_kv *kv, int nseq, const int *start, int ntok, int hea
     a.window = window >= kv->max_pages * kv->page ? 0 : window;   // (len - n - window then fits an int, whatever n)
     a.c2 = std::max(scale * 1.44269504088896340736f, 1.17549435e-38f);
     a.target = s.target;
+    a.pairs = s.pairs;
     a.block = s.block;
     a.items = (int)s.items;
     const hipStream_t st = static_cast<hipStream_t>(stream);
@@ -1135,14 +1166,13 @@ extern "C" {
 size_t es_hip_attn_decode_workspace(const es_hip_kv *kv, int nseq, int heads) {
     KvView v;
     if (check_heads(kv, nseq, nseq, heads, v) || !nseq) return 0;
-    return shape_of(kv, nseq, nseq, heads, false).workspace(kv);
+    return shape_of(kv, nseq, nseq, heads, ES_HIP_F32, false).workspace(kv);
 }
 
 size_t es_hip_attn_prompt_workspace(const es_hip_kv *kv, int nseq, int ntok, int heads, uint32_t type) {
     KvView v;
-    (void)type;
     if (check_heads(kv, nseq, ntok, heads, v) || !nseq || !ntok) return 0;
-    return shape_of(kv, nseq, ntok, heads, true).workspace(kv);
+    return shape_of(kv, nseq, ntok, heads, type, true).workspace(kv);
 }
 
 int es_hip_attn_decode_dev(const es_hip_kv *kv, int nseq, int heads, uint32_t type, const void *q, size_t qstride, float scale,

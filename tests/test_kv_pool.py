@@ -282,10 +282,12 @@ for nseq, heads, kvh, maxp, ntok in [(1, 32, 4, 8, 1), (1, 32, 4, 8192, 1), (48,
     k = kv(heads=kvh, rows=nseq, max_pages=maxp)
     ws = L.attn_decode_workspace(k, nseq, heads)
     rows.append(["decode", nseq, heads, kvh, maxp * 16, ws, one(L.attn_decode_dev, k, nseq, heads, E.F32, P, 0, 0.1, 0, P, 0, P, ws)])
-for nseq, heads, kvh, maxp, ntok in [(1, 32, 4, 500, 64), (1, 32, 4, 1024, 16384), (8, 32, 8, 210, 9000), (5, 14, 2, 100, 5)]:
-    k = kv(heads=kvh, rows=nseq, max_pages=maxp)
+for nseq, heads, kvh, maxp, ntok, t in [(1, 32, 4, 500, 64, E.F16), (1, 32, 4, 1024, 16384, E.F16), (8, 32, 8, 210, 9000, E.F16), (5, 14, 2, 100, 5, E.F16),
+                                        (1, 32, 4, 500, 64, E.BF16), (5, 14, 2, 100, 5, E.BF16), (40, 14, 2, 100, 70, E.BF16)]:
+    k = kv(heads=kvh, rows=nseq, max_pages=maxp, type=t)   # (a CU holds one workgroup with a bf16 cache, else two)
     ws = L.attn_prompt_workspace(k, nseq, ntok, heads, E.F32)
-    rows.append(["prompt", nseq, heads, kvh, ntok, ws, one(L.attn_prompt_dev, k, nseq, P, ntok, heads, E.F32, P, 0, 0.1, 0, P, 0, P, ws)])
+    pairs = [t == E.F16]
+    rows.append(["prompt", nseq, heads, kvh, ntok, ws, one(L.attn_prompt_dev, k, nseq, P, ntok, heads, E.F32, P, 0, 0.1, 0, P, 0, P, ws)] + pairs)
 print(json.dumps(rows))
 """
 
@@ -293,7 +295,8 @@ print(json.dumps(rows))
 def test_every_part_has_room(child):
     """for any lengths: a prompt's parts never outnumber the grid, nor their sums the workspace; a decode call's blocks are dealt
     out whole, each group begins at most one tile that others go on with, and the workspace holds two parts a group"""
-    for kind, nseq, heads, kvh, tokens, ws, launches in child(GRIDS):
+    for kind, nseq, heads, kvh, tokens, ws, launches, *pairs in child(GRIDS):
+        pairs = pairs == [True]
         G = heads // kvh
         grid = launches[0][0]
         assert grid % kvh == 0
@@ -319,9 +322,20 @@ def test_every_part_has_room(child):
             n, span = np.diff(np.concatenate([[0], cut, [tokens]])), rng.integers(0, 1 << 20, nseq)
             tiles = -(-n * G // 128)
             assert len(launches) == (2 if ws else 1)
-            if ws:   # the chunk that the device takes: total work over the parts aimed for
+            if ws:   # the chunk that the device takes: total work over the parts aimed for, longer until the last chunks have room
                 target = grid // kvh - (tokens * G // 128 + nseq)
-                chunk = max(128, -(-(-(-int((tiles * span).sum()) // target)) // 128) * 128)
+                step = 128 if pairs else 64
+                rounded = lambda keys: max(128, -(-keys // step) * step)
+                if nseq == 1:
+                    chunk = int(span[0] / max(1, target // max(1, int(tiles[0]))) + 64) // 64 * 64
+                    chunk = max(128, chunk * 2 if pairs and chunk <= 384 else chunk)
+                else:
+                    chunk = rounded(-(-int((tiles * span).sum()) // target))
+                    for _ in range(0 if pairs else 8):
+                        n = int((tiles * np.maximum(1, -(-span // chunk))).sum())
+                        if n <= target:
+                            break
+                        chunk = max(chunk + 64, rounded(chunk * n // target))
                 if (span * (tiles > 0)).max() <= chunk + 512:
                     chunk = 1 << 30
                 parts = (tiles * np.maximum(1, -(-span // chunk))).sum()
