@@ -350,8 +350,13 @@ template <int J> __device__ uint32_t pair(uint32_t first, uint32_t second) {
 // way is used once, so that LDS would only add a copy. Bound by HBM where the caches are long: 131072 tokens of 4 heads of 128,
 // fp16, 268 MB in 51 us (5.3 TB/s, joined), where a plain read reaches 6.2.
 constexpr int BLOCK = 7, BLOCK_WHOLE = 9, DECODE_M = 16;   // (log2)
-// workgroups, all heads together: as many as fit the device at once, and no more than bring it to the memory's rate
-constexpr int decode_groups(int dim) { return dim <= 128 ? 512 : 256; }
+// Workgroups that a CU holds at once. The three terms of a query of 128 elements do not fit half a SIMD's registers: at two to a CU
+// they are spilled, and 32 sequences of 1024 to 8192 tokens, 4 heads, take 68 us, not 54.
+constexpr int decode_per_cu(int nq, int dim) { return dim > 128 || (nq == 3 && dim > 64) ? 1 : 2; }
+// Workgroups, all heads together: as many as fit the device at once and bring it to the memory's rate; half of that for one
+// sequence, whose tiles have the more parts to join: 20000 and 131072 tokens of 8 heads of 128, us, 21.8 and 87.5 with 256,
+// 24.0 and 89.2 with 512.
+constexpr int decode_groups(int nq, int dim, int nseq) { return nseq > 1 ? 256 * decode_per_cu(nq, dim) : 256; }
 
 // the sequences' blocks: lane i has those of sequence g + i
 struct Blocks {
@@ -393,7 +398,7 @@ struct Deal {
     __device__ uint32_t first_of(int in) const { return before + (uint32_t)__builtin_amdgcn_readlane((int)(bl.upto - bl.mine), in); }
 };
 
-template <bool BF, int NQ, int DP> __global__ __launch_bounds__(256, DP == 64 && NQ < 3 ? 3 : DP <= 128 ? 2 : 1) void attn_decode_kernel(AttnArgs a) {
+template <bool BF, int NQ, int DP> __global__ __launch_bounds__(256, DP == 64 && NQ < 3 ? 3 : decode_per_cu(NQ, DP)) void attn_decode_kernel(AttnArgs a) {
     constexpr int KS = DP / 32, DL = DP / 16, BM = DECODE_M;
     constexpr bool F32 = NQ > 1;
     __shared__ float lm[4][BM], ll[4][BM];
@@ -1060,9 +1065,10 @@ struct Shape {
 Shape shape_of(const es_hip_kv *kv, int nseq, int ntok, int heads, uint32_t type, bool prompt) {
     const int G = heads / kv->heads;
     const long long most = (long long)kv->max_pages * kv->page;
+    const int nq = type != ES_HIP_F32 ? 1 : kv->type == ES_HIP_BF16 ? 3 : 2;
     Shape s{};
     if (prompt) {
-        const int per_cu = prompt_per_cu(kv->type == ES_HIP_BF16 && type == ES_HIP_F32 ? 3 : type == ES_HIP_F32 ? 2 : 1, kv->dim);
+        const int per_cu = prompt_per_cu(nq, kv->dim);
         const int parts = std::max(PARTS * per_cu / kv->heads, 1);
         s.pairs = per_cu == 2;
         s.bm = PM;
@@ -1072,7 +1078,7 @@ Shape shape_of(const es_hip_kv *kv, int nseq, int ntok, int heads, uint32_t type
         s.slots = s.target ? s.items : 0;
     } else {
         s.bm = DECODE_M;
-        s.target = std::max(decode_groups(kv->dim) / kv->heads, 1);
+        s.target = std::max(decode_groups(nq, kv->dim, nseq) / kv->heads, 1);
         s.items = s.target;
         s.block = most <= 1 << BLOCK_WHOLE ? BLOCK_WHOLE : BLOCK;
         s.slots = most > 1 << s.block ? 2 * s.items : 0;   // (0: every tile is one block)
@@ -1166,7 +1172,7 @@ extern "C" {
 size_t es_hip_attn_decode_workspace(const es_hip_kv *kv, int nseq, int heads) {
     KvView v;
     if (check_heads(kv, nseq, nseq, heads, v) || !nseq) return 0;
-    return shape_of(kv, nseq, nseq, heads, ES_HIP_F32, false).workspace(kv);
+    return shape_of(kv, nseq, nseq, heads, kv->type, false).workspace(kv);   // (fp32 queries need as much, or less)
 }
 
 size_t es_hip_attn_prompt_workspace(const es_hip_kv *kv, int nseq, int ntok, int heads, uint32_t type) {
