@@ -1,6 +1,6 @@
 // Attention over the paged key-value cache (attention_n of the reference, src/es_engine.c:975, whose loops over a host cache
 // this replaces): out = softmax(scale q k^T) v with one pass over the keys, keeping per query the running maximum m, the sum
-// l of 2^(s - m) and the weighted sum of v rows, all in fp32; a growing maximum scales l and the sum by 2^(m_old - m_new).
+// l of 2^(s - m) and the weighted sum of v rows, all in fp32; an m that moves scales l and the sum by 2^(m_old - m_new).
 //
 // Rows. The G = heads / kv heads query heads that share a K/V head are rows of one product, for every token of a tile: row r of
 // a sequence is query r / G, head r % G. A prompt's tile is then 128 rows of few tokens (little lost to causality) and a decode
@@ -12,9 +12,8 @@
 //
 // fp32 queries. q is split into as many terms of the cache's type as carry fp32's 24 bits (two of fp16 after scaling the row to
 // 2^14, 22 bits; three of bf16), one product each into the same sums, and so are the weights. K and V are exact as they are.
-// fp16 weights are 2^15 p, so that keys down to 2^-29 of the largest keep all their bits. Queries of the cache's own type go in
-// as they are, and their weights are rounded once to that type, as out will be: half a step of it relative to each, no more
-// than storing the weights would cost; l adds up the unrounded ones.
+// Queries of the cache's own type go in as they are, and their weights are rounded once to that type, as out will be: half a
+// step of it relative to each, no more than storing the weights would cost; l adds up the unrounded ones.
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
@@ -213,7 +212,12 @@ template <bool BF, int N> __device__ void split(const float (&x)[8], u4 (&y)[N])
 }
 
 constexpr float LOWEST = -INFINITY;
-template <bool BF> constexpr float SHIFT = BF ? 0.0f : 15.0f;   // weights are 2^SHIFT p
+// Weights are 2^SHIFT p, p relative to m, which in fp16 keeps all bits of keys down to 2^-29 of the largest (bf16 has fp32's range).
+template <bool BF> constexpr float SHIFT = BF ? 0.0f : 15.0f;
+// A prompt's m may lie below the largest score by up to LAG (in powers of two), and moves, with the sums so far, only past that; its
+// weights are 2^(SHIFT - LAG) p. us, so and where m follows every maximum: 16384 tokens, 32 heads of 128 over 4, fp16, 2241
+// and 2311; 8 prompts of 99 to 3333 tokens, bf16, 268 and 281. (Decode waits for memory: no difference.)
+template <bool BF> constexpr float LAG = BF ? 8.0f : 3.0f;
 // the exponent that weights are taken relative to: a row that has seen no key (or only minus infinity) keeps zeros, not NaN
 __device__ float reference(float m) { return m == LOWEST ? 0.0f : m; }
 
@@ -901,7 +905,7 @@ template <bool BF, int NQ, int DP> __global__ __launch_bounds__(256, prompt_per_
 #pragma unroll
                 for (int i = 0; i < 16; i++) big = fmaxf(big, s[h][i]);
             big = fmaxf(big, __shfl_xor(big, 32)) * cs;
-            if (__any(big > m)) {
+            if (__any(big > m + LAG<BF>)) {
                 const float now = fmaxf(m, big), f = __builtin_amdgcn_exp2f(m - reference(now));
                 m = now;
                 l *= f;
@@ -910,7 +914,7 @@ template <bool BF, int NQ, int DP> __global__ __launch_bounds__(256, prompt_per_
 #pragma unroll
                     for (int i = 0; i < 16; i++) acc[j][i] *= f;
             }
-            const float ref = SHIFT<BF> - reference(m);
+            const float ref = SHIFT<BF> - LAG<BF> - reference(m);
             u4 pt[4][NQ];
 #pragma unroll
             for (int u = 0; u < 4; u++) {

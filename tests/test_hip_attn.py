@@ -158,6 +158,29 @@ def test_decode_many_kv_heads(hip):
     check(c, [0, 1, 2], q, E.F32, 0.4, run(hip, c, [0, 1, 2], q, E.F32, 0.4, decode=True))
 
 
+@pytest.mark.parametrize("rise", [0.01, 0.045, 0.2, -0.2])
+@pytest.mark.parametrize("prompt", [False, True])
+@pytest.mark.parametrize("types", TYPES, ids=ids)
+def test_scores_that_rise_slowly(hip, types, prompt, rise):
+    """by less than what moves the reference of the weights, from one step of keys to the next, and by more"""
+    t, ct = types
+    rng = np.random.default_rng(37)
+    n, dim = 700, 64
+    c = Cache(ct, 1, dim, 16, [n], rng)
+    c.fill(rng)
+    k = from_bits(c.k, ct)
+    for j in range(n):
+        page, i = c.table[0, j // 16], j % 16
+        k[page, 0, i] *= 0.05
+        k[page, 0, i, 0] = rise * np.log(2) * j
+    c.k = to_bits(k, ct)
+    new = 130 if prompt else 1
+    q = from_bits(queries(rng, new, 4, dim, t), t)
+    q[..., 0] = 1.0
+    q = to_bits(q, t)
+    check(c, [0, new], q, t, 1.0, run(hip, c, [0, new], q, t, 1.0, decode=not prompt))
+
+
 @pytest.mark.parametrize("prompt", [False, True])
 @pytest.mark.parametrize("types", TYPES, ids=ids)
 def test_out_in_place_of_q(hip, types, prompt):
