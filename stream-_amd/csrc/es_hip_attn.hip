@@ -126,14 +126,17 @@ struct Part {
     uint32_t first;               // number of the sequence's first part
     Seq s;
 };
-__device__ uint32_t sum_up_to(uint32_t x) {   // over the lanes up to this one
-    const int lane = threadIdx.x & 63;
-#pragma unroll
-    for (int d = 1; d < 64; d <<= 1) {
-        const uint32_t o = __shfl_up(x, d);
-        if (lane >= d) x += o;
-    }
-    return x;
+// over the lanes up to this one, by lane moves: from 1, 2, 4 and 8 below within a row of 16, a row's last lane to the next row,
+// of rows 1 and 3, and the second row's to the upper two
+__device__ uint32_t sum_up_to(uint32_t n) {
+    int x = (int)n;
+    x += __builtin_amdgcn_update_dpp(0, x, 0x111, 0xf, 0xf, true);
+    x += __builtin_amdgcn_update_dpp(0, x, 0x112, 0xf, 0xf, true);
+    x += __builtin_amdgcn_update_dpp(0, x, 0x114, 0xf, 0xf, true);
+    x += __builtin_amdgcn_update_dpp(0, x, 0x118, 0xf, 0xf, true);
+    x += __builtin_amdgcn_update_dpp(0, x, 0x142, 0xa, 0xf, false);
+    x += __builtin_amdgcn_update_dpp(0, x, 0x143, 0xc, 0xf, false);
+    return (uint32_t)x;
 }
 // The part with number `item` (within one K/V head), or, TILES, the tile with that number and `chunk` 0; false if there is
 // none. Starts that are out of order may give any number of parts: they are counted modulo 2^32.
@@ -180,6 +183,32 @@ template <bool TILES> __device__ bool part_of(const AttnArgs &a, int item, int c
     p.tile = TILES ? item : item / p.chunks;
     p.chunk = TILES ? 0 : item - p.tile * p.chunks;
     return item >= 0 && p.tile < p.s.tiles;
+}
+
+// f of a lane's value and that of the lane D (16 or 32) away, the same on both sides
+template <int D, class F> __device__ float with_lane(float x, F f) {
+    static_assert(D == 16 || D == 32);
+    const uint32_t b = __float_as_uint(x);
+    if constexpr (D == 32) {
+        const auto r = __builtin_amdgcn_permlane32_swap(b, b, false, false);
+        return f(__uint_as_float(r[0]), __uint_as_float(r[1]));
+    } else {
+        const auto r = __builtin_amdgcn_permlane16_swap(b, b, false, false);
+        return f(__uint_as_float(r[0]), __uint_as_float(r[1]));
+    }
+}
+struct Max { __device__ float operator()(float a, float b) const { return fmaxf(a, b); } };
+struct Sum { __device__ float operator()(float a, float b) const { return a + b; } };
+// f over w = 16, 32 or 64 lanes in a row, to all of them
+template <class F> __device__ float over_lanes(float x, int w, F f) {
+    auto moved = [&](auto ctrl) { return __uint_as_float(__builtin_amdgcn_update_dpp(0, __float_as_uint(x), decltype(ctrl)::value, 0xf, 0xf, false)); };
+    x = f(x, moved(std::integral_constant<int, 0xb1>()));    // the neighbour, the other pair of four, and, once fours and eights agree,
+    x = f(x, moved(std::integral_constant<int, 0x4e>()));    // the mirror image in eight and in sixteen
+    x = f(x, moved(std::integral_constant<int, 0x141>()));
+    x = f(x, moved(std::integral_constant<int, 0x140>()));
+    if (w >= 32) x = with_lane<16>(x, f);
+    if (w == 64) x = with_lane<32>(x, f);
+    return x;
 }
 
 // ---- arithmetic --------------------------------------------------------------------------------------------------------------
@@ -245,7 +274,7 @@ __device__ u4 load8(const uint8_t *row, int d, int dim) {
 }
 
 // A query row's terms for the K steps of a product of KS * KL elements a step (lane group g of the row holds elements g * 8 of
-// each), and what the row's scores are multiplied by. The lanes that share a row are XOR, 2 XOR, ... apart.
+// each), and what the row's scores are multiplied by. The lanes that share a row are XOR, 2 XOR, ... apart (XOR: 16 or 32).
 template <bool BF, int NQ, int KS, int KL, int XOR>
 __device__ float load_query(const uint8_t *row, bool valid, int g, int dim, float c2, u4 (&q)[KS][NQ]) {
     if constexpr (NQ == 1) {
@@ -263,8 +292,8 @@ __device__ float load_query(const uint8_t *row, bool valid, int g, int dim, floa
         }
         int e = 0;
         if constexpr (!BF) {   // to 2^14 <= the largest < 2^15: both terms far from fp16's limits
-#pragma unroll
-            for (int d = XOR; d < 64; d <<= 1) big = fmaxf(big, __shfl_xor(big, d));
+            if constexpr (XOR == 16) big = with_lane<16>(big, Max());
+            big = with_lane<32>(big, Max());
             if (big > 0.0f && big < INFINITY) e = 14 - (static_cast<int>(__float_as_uint(big) >> 23) - 127);
             e = min(e, 126);
         }
@@ -435,9 +464,6 @@ template <bool BF, int NQ, int DP> __global__ __launch_bounds__(256, DP == 64 &&
         const int r = tile * BM + col;
         const int *table = a.c.table + (size_t)max(a.c.row(seq), 0) * a.c.max_pages;
 
-        u4 q[KS][NQ];
-        const float cs = load_query<BF, NQ, KS, 32, 16>(a.q + (size_t)seq * a.qstride + (size_t)(head * a.G + r) * dim * (F32 ? 4 : 2),
-                                                        r < rows, g, dim, a.c2, q);
         f4 acc[DL];
 #pragma unroll
         for (int j = 0; j < DL; j++) acc[j] = f4{0, 0, 0, 0};
@@ -447,6 +473,9 @@ template <bool BF, int NQ, int DP> __global__ __launch_bounds__(256, DP == 64 &&
         // step 32 s + i begins, of the 32 steps at hand and of the 32 after them.
         auto fetch = [&](int n) { return Runs(a.c, table, head, (first >> 4) + ((n + (lane >> 1)) * 4 + wave) * 2 + (lane & 1), last); };
         Runs pg = fetch(0), pgn = fetch(32);
+        u4 q[KS][NQ];
+        const float cs = load_query<BF, NQ, KS, 32, 16>(a.q + (size_t)seq * a.qstride + (size_t)(head * a.G + r) * dim * (F32 ? 4 : 2),
+                                                        r < rows, g, dim, a.c2, q);
         const int kd = (col * dim + g * 8) * 2, vd = (g * 4 * dim + col * DL) * 2;
         u4 kr[2][KS];             // run h, elements s * 32 + g * 8 of key col
         uint32_t vr[8][DL / 2];   // DL elements of the keys g * 4 + i (first four) and 16 + g * 4 + i
@@ -532,8 +561,7 @@ template <bool BF, int NQ, int DP> __global__ __launch_bounds__(256, DP == 64 &&
             float big = LOWEST;
 #pragma unroll
             for (int i = 0; i < 8; i++) big = fmaxf(big, s[i >> 2][i & 3]);
-            big = fmaxf(big, __shfl_xor(big, 16));
-            big = fmaxf(big, __shfl_xor(big, 32)) * cs;
+            big = with_lane<32>(with_lane<16>(big, Max()), Max()) * cs;
             if (__any(big > m)) {
                 const float now = fmaxf(m, big), f = __builtin_amdgcn_exp2f(m - reference(now));
                 m = now;
@@ -568,8 +596,7 @@ template <bool BF, int NQ, int DP> __global__ __launch_bounds__(256, DP == 64 &&
             }
             if (more) load_v(n + 1);
         }
-        l += __shfl_xor(l, 16);
-        l += __shfl_xor(l, 32);
+        l = with_lane<32>(with_lane<16>(l, Sum()), Sum());
 
         // the four waves' m, l and sums; lane (g, col) holds elements (g * 4 + i) * DL + j of head col
         if (g == 0) {
@@ -649,14 +676,14 @@ template <bool F32, bool BF> __global__ __launch_bounds__(256) void attn_decode_
         const float2 ml = a.pml[part(n)];
         if (ml.y != 0.0f) m = fmaxf(m, ml.x);
     }
-    for (int o = w / 2; o; o >>= 1) m = fmaxf(m, __shfl_xor(m, o));
+    m = over_lanes(m, w, Max());
     for (uint32_t n = d; n < parts; n += w) {
         const float2 ml = a.pml[part(n)];
         const float f = ml.y != 0.0f ? __builtin_amdgcn_exp2f(ml.x - reference(m)) : 0.0f;
         wt[k][n] = f;
         l += f * ml.y;
     }
-    for (int o = w / 2; o; o >>= 1) l += __shfl_xor(l, o);
+    l = over_lanes(l, w, Sum());
     __syncthreads();
     f4 x = {0, 0, 0, 0};
 #pragma unroll
@@ -904,7 +931,7 @@ template <bool BF, int NQ, int DP> __global__ __launch_bounds__(256, prompt_per_
             for (int h = 0; h < 2; h++)
 #pragma unroll
                 for (int i = 0; i < 16; i++) big = fmaxf(big, s[h][i]);
-            big = fmaxf(big, __shfl_xor(big, 32)) * cs;
+            big = with_lane<32>(big, Max()) * cs;
             if (__any(big > m + LAG<BF>)) {
                 const float now = fmaxf(m, big), f = __builtin_amdgcn_exp2f(m - reference(now));
                 m = now;
@@ -950,7 +977,7 @@ template <bool BF, int NQ, int DP> __global__ __launch_bounds__(256, prompt_per_
         buf = buf == NB - 1 ? 0 : buf + 1;
         arrived(!more);
     }
-    l += __shfl_xor(l, 32);
+    l = with_lane<32>(l, Sum());
 
     if (wave * 32 + col >= rows) return;
     // acc[j][i] is element j * 32 + i / 4 * 8 + half * 4 + i % 4
@@ -1023,7 +1050,7 @@ template <bool F32, bool BF> __global__ __launch_bounds__(256) void attn_join_ke
             const float2 ml = a.pml[at + c * step];
             if (ml.y != 0.0f) m = fmaxf(m, ml.x);
         }
-        for (int o = w / 2; o; o >>= 1) m = fmaxf(m, __shfl_xor(m, o));
+        m = over_lanes(m, w, Max());
         float l = 0.0f;
         for (int c = d; c < p.chunks; c += w) {
             const float2 ml = a.pml[at + c * step];
@@ -1031,7 +1058,7 @@ template <bool F32, bool BF> __global__ __launch_bounds__(256) void attn_join_ke
             f[c] = x;
             l += x * ml.y;
         }
-        for (int o = w / 2; o; o >>= 1) l += __shfl_xor(l, o);
+        l = over_lanes(l, w, Sum());
         __syncthreads();
         if (d < quads && row < rows) {
             f4 x = {0, 0, 0, 0};
