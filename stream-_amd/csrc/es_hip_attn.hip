@@ -39,6 +39,7 @@ struct AttnArgs {
     float c2;                  // scale * log2(e)
     int target;                // parts aimed for per K/V head; 0: every tile is one part. One query per sequence: workgroups
     bool pairs;                // target is two workgroups a CU
+    uint32_t inverse;          // 2^32 / target, rounded down (2^32 - 1 for 1)
     int block;                 // one query per sequence: log2 of the keys of a block
     int items;                 // parts per K/V head that there is room for
 };
@@ -420,7 +421,9 @@ struct Deal {
     __device__ Deal(const AttnArgs &a, int tiles) : bl(blocks_from(a, 0, tiles)) {
         total = (uint32_t)__builtin_amdgcn_readlane((int)bl.upto, 63);
         for (int g = 64; g < a.nseq; g += 64) total += (uint32_t)__builtin_amdgcn_readlane((int)blocks_from(a, g, tiles).upto, 63);
-        each = (total + a.target - 1) / a.target;
+        const uint32_t n = total + a.target - 1;
+        each = __umulhi(n, a.inverse);   // n / target, or one less
+        each += n - each * a.target >= (uint32_t)a.target;
     }
     // on to the sequences from g on (a multiple of 64)
     __device__ void next(const AttnArgs &a, int tiles) {
@@ -456,7 +459,7 @@ template <bool BF, int NQ, int DP> __global__ __launch_bounds__(256, DP == 64 &&
         const uint32_t s0 = deal.first_of(in);
         int base;
         const int blocks = blocks_of(a, hi, base);
-        const int tile = (int)((pos - s0) / blocks), block = (int)((pos - s0) - (uint32_t)tile * blocks);
+        const int tile = tiles == 1 ? 0 : (int)((pos - s0) / blocks), block = (int)((pos - s0) - (uint32_t)tile * blocks);
         const int here = (int)min((uint32_t)(blocks - block), end - pos);
         const uint32_t tile_at = pos - block;   // the tile's first block among all
         pos += here;
@@ -1187,6 +1190,7 @@ int attention(const es_hip_kv *kv, int nseq, const int *start, int ntok, int hea
     a.c2 = std::max(scale * 1.44269504088896340736f, 1.17549435e-38f);
     a.target = s.target;
     a.pairs = s.pairs;
+    a.inverse = s.target > 1 ? (uint32_t)((1ull << 32) / s.target) : ~0u;
     a.block = s.block;
     a.items = (int)s.items;
     const hipStream_t st = static_cast<hipStream_t>(stream);
