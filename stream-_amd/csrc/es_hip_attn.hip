@@ -71,16 +71,15 @@ constexpr int CHUNK_MIN = 128, CHUNK_SAVES = 512, CHUNK_PAIRS = 384;   // keys
 
 // The chunk's keys; 2^30: tiles are whole, which they stay unless chunks shorten the longest by more than CHUNK_SAVES: the
 // parts' sums go through memory and the join takes some 6 us, as much as 512 keys. us, whole and in chunks, 32 heads of 128
-// over 8, fp16: a prompt of 512 tokens 19 and 28, of 1024 31 and 46; 64 tokens behind 2000 of 64 elements 18.5 (chunks of 512)
-// and 14.
+// over 8, fp16: a prompt of 512 tokens 17 and 28, of 1024 31 and 44; 64 tokens behind 1936 of 64 elements 34 and 14.
 // One sequence: its tiles' chunks are as many as there is room for (target), and half as many where that is two to a CU and they
 // are of CHUNK_PAIRS keys or less, since twice the parts cost more than the second workgroup of a CU gains: 64 tokens behind
-// 7937, 32 heads of 128 over 4, us, so and in twice the chunks: fp16 27 and 31, fp32 33 and 37; 64 behind 29936, whose chunks
-// are longer, would take 60 instead of 57.
-// Several: the mean share of a place, and, where a CU holds but one workgroup, longer until the sequences' last chunks find room too.
-// Two to a CU even out by themselves, with chunks of whole 128s. us, in bf16 of 256 elements, where one fits, longer and not:
-// 3 sequences of 1250 to 2500 tokens, the last 300 new, 128 and 169; in fp16 of 128, where two fit: 16 of 1500 to 3000, the last 16 new,
-// longer 51 and not 46, with chunks of whole 64s 61.
+// 7937, 32 heads of 128 over 4, us, so and in twice the chunks: fp16 26 and 31, fp32 33 and 38; 64 behind 29936, whose chunks
+// are longer, would take 61 instead of 52.
+// Several: the mean share of a place, and, where a CU holds but one workgroup, longer until the sequences' last chunks find room
+// too. Two to a CU even out by themselves, with chunks of whole 128s. us, in bf16 of 256 elements, where one fits, longer and
+// not: 3 sequences of 1250 to 2500 tokens, the last 300 new, 107 and 188; in fp16 of 128, where two fit: 16 of 1500 to 3000, the
+// last 16 new, longer 48 and not 43, with chunks of whole 64s 59.
 __device__ int chunk_of(const AttnArgs &a) {
     if (!a.target) return 1 << 30;
     int chunk, longest = 0;
@@ -245,8 +244,8 @@ constexpr float LOWEST = -INFINITY;
 // Weights are 2^SHIFT p, p relative to m, which in fp16 keeps all bits of keys down to 2^-29 of the largest (bf16 has fp32's range).
 template <bool BF> constexpr float SHIFT = BF ? 0.0f : 15.0f;
 // A prompt's m may lie below the largest score by up to LAG (in powers of two), and moves, with the sums so far, only past that; its
-// weights are 2^(SHIFT - LAG) p. us, so and where m follows every maximum: 16384 tokens, 32 heads of 128 over 4, fp16, 2241
-// and 2311; 8 prompts of 99 to 3333 tokens, bf16, 268 and 281. (Decode waits for memory: no difference.)
+// weights are 2^(SHIFT - LAG) p. us, so and where m follows every maximum: 16384 tokens, 32 heads of 128 over 4, fp16, 2135
+// and 2211; 8 prompts of 99 to 3333 tokens, bf16, 268 and 281. (Decode waits for memory: no difference.)
 template <bool BF> constexpr float LAG = BF ? 8.0f : 3.0f;
 // the exponent that weights are taken relative to: a row that has seen no key (or only minus infinity) keeps zeros, not NaN
 __device__ float reference(float m) { return m == LOWEST ? 0.0f : m; }
@@ -342,8 +341,8 @@ struct Runs {
 // A buffer descriptor of one of them, for loads whose offsets count from its first row: the loads check their own bounds, so that
 // what lies past its `bytes` reads as zeros, and so does all of a run that is in no page, and no lane holds an address, only
 // its offset. run_of gives it as four words, for asm; Run loads by it, past the caches, as nobody else reads a decode call's keys
-// soon. us so and through the caches: 131072 tokens, 4 heads of 128, 51 and 58; 32 sequences of 77 to 8192 tokens 38 and 42; only
-// what the last-level cache holds whole loses (48 windows of 4096 tokens, 2 heads of 64, 79 MB: 24 and 22).
+// soon. us so and through the caches: 131072 tokens, 4 heads of 128, 49 and 55; 32 sequences of 77 to 8192 tokens 35.9 and 36.4; what
+// the last-level cache holds whole gains nothing (48 windows of 4096 tokens, 2 heads of 64, 79 MB: 21.6 and 21.4).
 __device__ u4 run_of(const uint8_t *pool, const Runs &all, int lane, int bytes) {
     const int hi = __builtin_amdgcn_readlane(all.hi, lane);
     const uint64_t at = reinterpret_cast<uint64_t>(pool) + ((uint64_t)(uint32_t)max(hi, 0) << 32 | (uint32_t)__builtin_amdgcn_readlane(all.lo, lane));
@@ -375,22 +374,20 @@ template <int J> __device__ uint32_t pair(uint32_t first, uint32_t second) {
 // whatever sequences they are of, so that a ragged batch keeps every workgroup busy to the end. What a workgroup has of a tile
 // that others have parts of goes to the workspace, and a second launch joins them. (The last workgroup of a tile to arrive
 // could do that in the same launch, but 128 of them counting in one word and one CU reading all their sums took 78 us for one
-// sequence of 131072 tokens, where the two launches take 51.) Where no table row holds more than 512 tokens, a tile is one block and one launch does:
-// one sequence of 500 tokens, 32 heads of 64 over 8, 7.1 us, in blocks of 128 with the second launch 10.1.
+// sequence of 131072 tokens, where the two launches take 48.) Where no table row holds more than 512 tokens, a tile is one block and one launch does:
+// one sequence of 500 tokens, 32 heads of 64 over 8, 6.6 us, in blocks of 128 with the second launch 9.7.
 //
 // Inside: four waves, each 32 keys at a time in turn, joined in LDS at the end. Nothing is staged: a lane loads its K fragments
 // as the matrix cores take them (key lane % 16, 8 elements) and, of V, the DP / 16 elements from (lane % 16) * DP / 16 on of
 // the 8 keys whose weights it holds, which it turns into 8 keys of one element each with byte permutes. A fragment read this
 // way is used once, so that LDS would only add a copy. Bound by HBM where the caches are long: 131072 tokens of 4 heads of 128,
-// fp16, 268 MB in 51 us (5.3 TB/s, joined), where a plain read reaches 6.2.
+// fp16, 268 MB in 48 us (5.6 TB/s, joined; 42, 6.4 TB/s, before that), where a plain read reaches 6.2.
 constexpr int BLOCK = 7, BLOCK_WHOLE = 9, DECODE_M = 16;   // (log2)
-// Workgroups that a CU holds at once. The three terms of a query of 128 elements do not fit half a SIMD's registers: at two to a CU
-// they are spilled, and 32 sequences of 1024 to 8192 tokens, 4 heads, take 68 us, not 54.
-constexpr int decode_per_cu(int nq, int dim) { return dim > 128 || (nq == 3 && dim > 64) ? 1 : 2; }
+constexpr int decode_per_cu(int dim) { return dim <= 128 ? 2 : 1; }   // workgroups that a CU holds at once
 // Workgroups, all heads together: as many as fit the device at once and bring it to the memory's rate; half of that for one
-// sequence, whose tiles have the more parts to join: 20000 and 131072 tokens of 8 heads of 128, us, 21.8 and 87.5 with 256,
-// 24.0 and 89.2 with 512.
-constexpr int decode_groups(int nq, int dim, int nseq) { return nseq > 1 ? 256 * decode_per_cu(nq, dim) : 256; }
+// sequence, whose tiles have the more parts to join: 20000 and 131072 tokens of 8 heads of 128, us, 21 and 87 with 256,
+// 23 and 90 with 512.
+constexpr int decode_groups(int dim, int nseq) { return nseq > 1 ? 256 * decode_per_cu(dim) : 256; }
 
 // the sequences' blocks: lane i has those of sequence g + i
 struct Blocks {
@@ -434,7 +431,7 @@ struct Deal {
     __device__ uint32_t first_of(int in) const { return before + (uint32_t)__builtin_amdgcn_readlane((int)(bl.upto - bl.mine), in); }
 };
 
-template <bool BF, int NQ, int DP> __global__ __launch_bounds__(256, DP == 64 && NQ < 3 ? 3 : decode_per_cu(NQ, DP)) void attn_decode_kernel(AttnArgs a) {
+template <bool BF, int NQ, int DP> __global__ __launch_bounds__(256, DP == 64 && NQ < 3 ? 3 : decode_per_cu(DP)) void attn_decode_kernel(AttnArgs a) {
     constexpr int KS = DP / 32, DL = DP / 16, BM = DECODE_M;
     constexpr bool F32 = NQ > 1;
     __shared__ float lm[4][BM], ll[4][BM];
@@ -724,11 +721,11 @@ template <bool F32, bool BF> __global__ __launch_bounds__(256) void attn_decode_
 // Keys that a row does not see have weight 0, and 0 times an infinity or NaN is not 0: V rows that no row sees are zeros in LDS,
 // and so are such elements of keys that only some rows see; where there were any, they are added to those rows at the end.
 //
-// Bound by the matrix cores and their power: 16384 tokens, 32 heads of 128 over 4, fp16, 2.25 ms, 980 TFLOP/s counted causally.
-// Both waves of a SIMD together keep the matrix cores busy for 45% of the cycles, at 2.0 GHz; a large library product, busy for
+// Bound by the matrix cores and their power: 16384 tokens, 32 heads of 128 over 4, fp16, 2.19 ms, 1005 TFLOP/s counted causally. The
+// waves of a SIMD together keep the matrix cores busy for 57% of the cycles, at 1.9 to 2 GHz; a large library product, busy for
 // 70%, is clocked at 1.4 and gives 1320. Two workgroups a CU: with 64 rows a wave, which halves the reads of LDS, only one
-// fits, and the exponentials of one wave no longer pass under the products of another: 2.94 ms. Tiles of 256 rows in eight
-// waves: within 2%.
+// fits, and the exponentials of one wave no longer pass under the products of another: 2.94 ms where this had 2.25. Tiles of
+// 256 rows in eight waves: within 2%.
 template <int DP> __device__ constexpr int k_turn(int t) { return DP == 64 ? t >> 1 & 7 : t & 15; }
 template <int DP> __device__ constexpr int v_turn(int t) { return DP == 64 ? (t >> 1 & 1) * 4 : (t & 3) * 4; }
 
@@ -901,8 +898,8 @@ template <bool BF, int NQ, int DP> __global__ __launch_bounds__(256, prompt_per_
                     for (int t = 0; t < NQ; t++) s[h] = mfma32<BF>(kf, q[k][t], s[h]);
                 }
             // Six reads of K under way, or (below) four fragments of V: as the compiler left it, each product waited for its
-            // own. With three terms the products are long enough. 8192 tokens, us, with and without: heads of 256, fp16 1495
-            // and 1704, fp32 2236 and 2530; of 128 611 and 624.
+            // own. With three terms the products are long enough. 8192 tokens, us, with and without: heads of 256, fp16 1330
+            // and 1534, fp32 2017 and 2363; of 128 555 and 563.
             if constexpr (NQ < 3) {
                 __builtin_amdgcn_sched_group_barrier(0x100, 6, 0);
 #pragma unroll
@@ -1112,7 +1109,7 @@ Shape shape_of(const es_hip_kv *kv, int nseq, int ntok, int heads, uint32_t type
         s.slots = s.target ? s.items : 0;
     } else {
         s.bm = DECODE_M;
-        s.target = std::max(decode_groups(nq, kv->dim, nseq) / kv->heads, 1);
+        s.target = std::max(decode_groups(kv->dim, nseq) / kv->heads, 1);
         s.items = s.target;
         s.block = most <= 1 << BLOCK_WHOLE ? BLOCK_WHOLE : BLOCK;
         s.slots = most > 1 << s.block ? 2 * s.items : 0;   // (0: every tile is one block)
