@@ -1,0 +1,108 @@
+"""How many bits fp32 queries and the softmax weights keep on their way through attention's matrix products: 22 or more, as
+es_hip_quant.h promises. Queries, keys and values are chosen so that an output element is one key's weight and that weight hangs on the
+low bits; the GPU's outputs are checked, and, on the CPU, that the checks tell a model of the arithmetic from one that keeps fewer.
+
+Every case has 32 keys (one wave's in decode: no joining between) and compares out_j / out_0, where key 0's weight is 1: what all
+weights have in common, the sum above all, cancels. u = 2^-24 is half a step of fp32 relative to the value."""
+import numpy as np
+import pytest
+
+import es_hip_quant as E
+from _attn import Cache, from_bits, to_bits
+
+N = 32
+U = 2.0 ** -24
+LN2 = np.float32(0.693147182464599609375)   # times the fp32 log2(e) it is 1 in fp32: scores are exponents of 2
+TERMS = {E.F16: 2, E.BF16: 3}
+TYPES = [E.F16, E.BF16]
+NAMES = {E.F16: "f16", E.BF16: "bf16"}
+
+
+def spread(ct):
+    """Exponents -j / 32, exact: weights of every mantissa. 2^x (a step: 2 u), the weights' terms (fp16: 2^-11 of 2^-11; bf16:
+    2^-24, both within 2^-22 = 4 u), the scale's roundings (u), the outputs' (2 u)."""
+    return [1.0], -np.arange(N)[:, None] / 32, LN2, 9 * U
+
+
+def low_terms(ct):
+    """q0 = q1 plus what only q0's last term carries, K = (j, -j): scores are that last term times j, from 0 to 4 in powers of two.
+    The products and their sums are exact. The exponent's roundings (scale, its product with log2(e), the fused one: u each of at
+    most 4), 2^x and the terms of the weights as above, the outputs': 12 ln 2 u + 2 u + 4 u + 2 u, for either key."""
+    last, rest = (5 * 2.0 ** -14, 1.0) if ct == E.F16 else (5 * 2.0 ** -22, 1 + 3 * 2.0 ** -10)
+    j = np.arange(N)
+    return [rest + last, rest], np.stack([j, -j], 1).astype(float), np.float32(LN2 / (8 * last)), 2 * 17 * U
+
+
+CASES = [spread, low_terms]
+
+
+def off(case, ct, out):
+    """out[..., j] = weight of key j over the sum: the largest relative error of out_j / out_0, over the tolerance"""
+    q, k, scale, tol = case(ct)
+    want = np.exp(float(scale) * (k @ np.array(q)))
+    out = np.asarray(out, float)
+    return (np.abs(out / out[..., :1] / want * want[0] - 1) / tol).max()
+
+
+# ---- the checks on models of the arithmetic ------------------------------------------------------------------------------------
+def split(x, ct, n):
+    r, y = np.asarray(x, np.float32), []
+    for _ in range(n):
+        y.append(from_bits(to_bits(r, ct), ct).astype(np.float32))
+        r = r - y[-1]
+    return sum(t.astype(float) for t in y)
+
+
+def model(case, ct, q_terms, w_terms):
+    """weights 2^(s - m), in fp32 where the kernels are"""
+    q, k, scale, _ = case(ct)
+    c2 = np.float32(scale * np.float32(1.44269504088896340736))
+    s = k @ split(q, ct, q_terms)
+    m = np.float32((s * c2).max())
+    w = np.exp2((s * float(c2) - float(m)).astype(np.float32).astype(float)).astype(np.float32)
+    return (split(w, ct, w_terms) * float(np.float32(1) / w.sum(dtype=np.float32))).astype(np.float32)
+
+
+@pytest.mark.parametrize("ct", TYPES, ids=NAMES.get)
+@pytest.mark.parametrize("case", CASES)
+def test_checks_accept_what_keeps_the_bits(case, ct):
+    assert off(case, ct, model(case, ct, TERMS[ct], TERMS[ct])) <= 1
+
+
+@pytest.mark.parametrize("ct", TYPES, ids=NAMES.get)
+def test_checks_refuse_what_does_not(ct):
+    n = TERMS[ct]
+    assert off(spread, ct, model(spread, ct, n, n - 1)) > 4
+    assert off(low_terms, ct, model(low_terms, ct, n - 1, n)) > 100
+
+
+# ---- on the GPU ----------------------------------------------------------------------------------------------------------------
+@pytest.mark.gpu
+@pytest.mark.parametrize("dim", [64, 128, 256])
+@pytest.mark.parametrize("prompt", [False, True])
+@pytest.mark.parametrize("ct", TYPES, ids=NAMES.get)
+@pytest.mark.parametrize("case", CASES)
+def test_bits_of_queries_and_weights(hip, case, ct, prompt, dim):
+    qs, ks, scale, _ = case(ct)
+    c = Cache(ct, 1, dim, 16, [N], np.random.default_rng(1))
+    k = np.zeros((N, 1, dim))
+    k[:, 0, :len(qs)] = ks
+    v = np.zeros((N, 1, dim))
+    v[np.arange(N), 0, np.arange(N)] = 1
+    c.put(0, 0, to_bits(k, ct), to_bits(v, ct))
+    kv, keep = c.upload(hip)
+    heads, new = 2, 1
+    q = np.zeros((new, heads, dim), np.float32)
+    q[..., :len(qs)] = qs
+    dq, do, ds = hip.upload(q), hip.alloc(q.nbytes), hip.upload(np.array([0, new], np.int32))
+    ws = hip.attn_prompt_workspace(kv, 1, new, heads, E.F32) if prompt else hip.attn_decode_workspace(kv, 1, heads)
+    dw = hip.alloc(max(ws, 16))
+    if prompt:
+        hip.attn_prompt_dev(kv, 1, ds, new, heads, E.F32, dq, 0, float(scale), 0, do, 0, dw, ws)
+    else:
+        hip.attn_decode_dev(kv, 1, heads, E.F32, dq, 0, float(scale), 0, do, 0, dw, ws)
+    got = hip.download(do, np.zeros_like(q))
+    assert not got[..., N:].any()
+    r = off(case, ct, got[..., :N])
+    print(f"{case.__name__} {NAMES[ct]} {'prompt' if prompt else 'decode'} {dim}: {r:.3f} of the tolerance", flush=True)
+    assert r <= 1
