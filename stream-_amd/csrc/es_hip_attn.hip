@@ -242,13 +242,40 @@ template <bool BF, int N> __device__ void split(const float (&x)[8], u4 (&y)[N])
 
 constexpr float LOWEST = -INFINITY;
 // Weights are 2^SHIFT p, p relative to m, which in fp16 keeps all bits of keys down to 2^-29 of the largest (bf16 has fp32's range).
-template <bool BF> constexpr float SHIFT = BF ? 0.0f : 15.0f;
+template <bool BF> constexpr int SHIFT = BF ? 0 : 15;
 // A prompt's m may lie below the largest score by up to LAG (in powers of two), and moves, with the sums so far, only past that; its
 // weights are 2^(SHIFT - LAG) p. us, so and where m follows every maximum: 16384 tokens, 32 heads of 128 over 4, fp16, 2135
 // and 2211; 8 prompts of 99 to 3333 tokens, bf16, 268 and 281. (Decode waits for memory: no difference.)
-template <bool BF> constexpr float LAG = BF ? 8.0f : 3.0f;
+template <bool BF, int NQ> constexpr int LAG = BF && NQ == 1 ? 8 : 3;
 // the exponent that weights are taken relative to: a row that has seen no key (or only minus infinity) keeps zeros, not NaN
 __device__ float reference(float m) { return m == LOWEST ? 0.0f : m; }
+
+// A constant in the exponent rounds it: between 8 and 16 half a step of fp32 is 2^-21, 3.3e-7 of the weight, more than the weights'
+// terms lose (2^-22); between 2 and 4 it is 8e-8. So the two terms of fp16, which need a 2^BY of 12 or 15, take it as a factor, when
+// they are rounded, and their l at the end: exact, and no instruction more than without (decode of 500 tokens 6.66 us and, in the exponent,
+// 6.62; 64 prompt tokens behind 7937 31.0 and 30.8). Three terms of bf16 keep the constant small. One term is rounded to 2^-9 or 2^-12 at once, and
+// takes any in the exponent.
+template <int NQ> constexpr bool FACTOR = NQ == 2;
+template <int NQ, int BY> __device__ float weights_sum(float l) { return FACTOR<NQ> ? l * (1 << (BY & 31)) : l; }
+template <int NQ, int BY> __device__ float weight(float s, float cs, float ref) {
+    return __builtin_amdgcn_exp2f(__builtin_fmaf(s, cs, FACTOR<NQ> ? -ref : BY - ref));
+}
+template <bool BF, int NQ, int BY> __device__ void split_weights(const float (&x)[8], u4 (&y)[NQ]) {
+    if constexpr (!FACTOR<NQ>) {
+        split<BF, NQ>(x, y);
+    } else {
+        static_assert(!BF && NQ == 2);
+        constexpr float f = 1 << BY;
+        h8 v, w;
+#pragma unroll
+        for (int i = 0; i < 8; i++) {
+            v[i] = static_cast<_Float16>(__builtin_fmaf(x[i], f, 0.0f));
+            w[i] = static_cast<_Float16>(__builtin_fmaf(x[i], f, -static_cast<float>(v[i])));
+        }
+        y[0] = __builtin_bit_cast(u4, v);
+        y[1] = __builtin_bit_cast(u4, w);
+    }
+}
 
 // Eight elements of a query row, from d on (zeros past dim): fp32 or 16 bits.
 __device__ void load8(const uint8_t *row, int d, int dim, float (&x)[8]) {
@@ -571,15 +598,15 @@ template <bool BF, int NQ, int DP> __global__ __launch_bounds__(256, DP == 64 &&
 #pragma unroll
                     for (int i = 0; i < 4; i++) acc[j][i] *= f;
             }
-            const float ref = SHIFT<BF> - reference(m);
+            const float ref = reference(m);
             float w8[8];
 #pragma unroll
             for (int i = 0; i < 8; i++) {
-                w8[i] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[i >> 2][i & 3], cs, ref));
+                w8[i] = weight<NQ, SHIFT<BF>>(s[i >> 2][i & 3], cs, ref);
                 l += w8[i];
             }
             u4 pt[NQ];
-            split<BF, NQ>(w8, pt);
+            split_weights<BF, NQ, SHIFT<BF>>(w8, pt);
 #pragma unroll
             for (int j = 0; j < DL; j += 2) {
                 u4 v0, v1;
@@ -596,7 +623,7 @@ template <bool BF, int NQ, int DP> __global__ __launch_bounds__(256, DP == 64 &&
             }
             if (more) load_v(n + 1);
         }
-        l = with_lane<32>(with_lane<16>(l, Sum()), Sum());
+        l = weights_sum<NQ, SHIFT<BF>>(with_lane<32>(with_lane<16>(l, Sum()), Sum()));
 
         // the four waves' m, l and sums; lane (g, col) holds elements (g * 4 + i) * DL + j of head col
         if (g == 0) {
@@ -747,6 +774,7 @@ template <bool BF, int NQ, int DP> __global__ __launch_bounds__(256, prompt_per_
     constexpr int ROWS = 64 / CH;                            // keys of one
     constexpr uint32_t TILE = PN * DP * 2;                   // bytes of K, or V, of a step
     constexpr bool F32 = NQ > 1;
+    constexpr int BY = SHIFT<BF> - LAG<BF, NQ>;              // weights are 2^BY p
     __shared__ __attribute__((aligned(1024))) uint8_t lds[2 * NB * TILE];   // K of NB steps, V of them
     __shared__ int odd;                                      // elements of V were left out
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -932,7 +960,7 @@ template <bool BF, int NQ, int DP> __global__ __launch_bounds__(256, prompt_per_
 #pragma unroll
                 for (int i = 0; i < 16; i++) big = fmaxf(big, s[h][i]);
             big = with_lane<32>(big, Max()) * cs;
-            if (__any(big > m + LAG<BF>)) {
+            if (__any(big > m + LAG<BF, NQ>)) {
                 const float now = fmaxf(m, big), f = __builtin_amdgcn_exp2f(m - reference(now));
                 m = now;
                 l *= f;
@@ -941,17 +969,17 @@ template <bool BF, int NQ, int DP> __global__ __launch_bounds__(256, prompt_per_
 #pragma unroll
                     for (int i = 0; i < 16; i++) acc[j][i] *= f;
             }
-            const float ref = SHIFT<BF> - LAG<BF> - reference(m);
+            const float ref = reference(m);
             u4 pt[4][NQ];
 #pragma unroll
             for (int u = 0; u < 4; u++) {
                 float w8[8];
 #pragma unroll
                 for (int i = 0; i < 8; i++) {
-                    w8[i] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[u >> 1][(u & 1) * 8 + i], cs, ref));
+                    w8[i] = weight<NQ, BY>(s[u >> 1][(u & 1) * 8 + i], cs, ref);
                     l += w8[i];
                 }
-                split<BF, NQ>(w8, pt[u]);
+                split_weights<BF, NQ, BY>(w8, pt[u]);
             }
 #pragma unroll
             for (int u = 0; u < 4; u++)
@@ -977,7 +1005,7 @@ template <bool BF, int NQ, int DP> __global__ __launch_bounds__(256, prompt_per_
         buf = buf == NB - 1 ? 0 : buf + 1;
         arrived(!more);
     }
-    l = with_lane<32>(l, Sum());
+    l = weights_sum<NQ, BY>(with_lane<32>(l, Sum()));
 
     if (wave * 32 + col >= rows) return;
     // acc[j][i] is element j * 32 + i / 4 * 8 + half * 4 + i % 4

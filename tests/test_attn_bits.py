@@ -18,6 +18,12 @@ TYPES = [E.F16, E.BF16]
 NAMES = {E.F16: "f16", E.BF16: "bf16"}
 
 
+def near(ct):
+    """Exponents -j 2^-21: weights 1 - j 2^-21 ln 2. The exponents are exact, the weights' first terms are 1 and the rest has few
+    bits, so that what is left is 2^x (a step, u here, for each of the two) and the outputs' last rounding (u each)."""
+    return [2.0 ** -10], -np.arange(N)[:, None] * 2.0 ** -11, LN2, 4 * U
+
+
 def spread(ct):
     """Exponents -j / 32, exact: weights of every mantissa. 2^x (a step: 2 u), the weights' terms (fp16: 2^-11 of 2^-11; bf16:
     2^-24, both within 2^-22 = 4 u), the scale's roundings (u), the outputs' (2 u)."""
@@ -33,7 +39,7 @@ def low_terms(ct):
     return [rest + last, rest], np.stack([j, -j], 1).astype(float), np.float32(LN2 / (8 * last)), 2 * 17 * U
 
 
-CASES = [spread, low_terms]
+CASES = [near, spread, low_terms]
 
 
 def off(case, ct, out):
@@ -53,27 +59,30 @@ def split(x, ct, n):
     return sum(t.astype(float) for t in y)
 
 
-def model(case, ct, q_terms, w_terms):
-    """weights 2^(s - m), in fp32 where the kernels are"""
+def model(case, ct, q_terms, w_terms, before, after):
+    """weights 2^(s - m + before) 2^after, in fp32 where the kernels are"""
     q, k, scale, _ = case(ct)
     c2 = np.float32(scale * np.float32(1.44269504088896340736))
     s = k @ split(q, ct, q_terms)
     m = np.float32((s * c2).max())
-    w = np.exp2((s * float(c2) - float(m)).astype(np.float32).astype(float)).astype(np.float32)
+    w = np.exp2((s * float(c2) + float(np.float32(before) - m)).astype(np.float32).astype(float)).astype(np.float32) * np.float32(2.0 ** after)
     return (split(w, ct, w_terms) * float(np.float32(1) / w.sum(dtype=np.float32))).astype(np.float32)
 
 
 @pytest.mark.parametrize("ct", TYPES, ids=NAMES.get)
 @pytest.mark.parametrize("case", CASES)
 def test_checks_accept_what_keeps_the_bits(case, ct):
-    assert off(case, ct, model(case, ct, TERMS[ct], TERMS[ct])) <= 1
+    for after in (0, 15, 12, -8):
+        assert off(case, ct, model(case, ct, TERMS[ct], TERMS[ct], 0, after if (after > 0) == (ct == E.F16) else 0)) <= 1
 
 
 @pytest.mark.parametrize("ct", TYPES, ids=NAMES.get)
 def test_checks_refuse_what_does_not(ct):
     n = TERMS[ct]
-    assert off(spread, ct, model(spread, ct, n, n - 1)) > 4
-    assert off(low_terms, ct, model(low_terms, ct, n - 1, n)) > 100
+    for before in ((15, 12) if ct == E.F16 else (-8,)):   # added to the exponent, a constant rounds it
+        assert off(near, ct, model(near, ct, n, n, before, 0)) > 1.2
+    assert off(spread, ct, model(spread, ct, n, n - 1, 0, 0)) > 4
+    assert off(low_terms, ct, model(low_terms, ct, n - 1, n, 0, 0)) > 100
 
 
 # ---- on the GPU ----------------------------------------------------------------------------------------------------------------
