@@ -485,7 +485,7 @@ int es_hip_kv_append_dev(const es_hip_kv *kv, int nseq, const int *start, int nt
  * 2^29 query rows (tokens times heads), 2^23 sequences times heads, 2^31 blocks of 128 keys that the table rows could hold.
  * ws: the caller's device workspace of at least es_hip_attn_decode_workspace bytes (16-byte aligned; 0 bytes: may be NULL); its
  * contents need no setup and nothing is kept in it between calls, but calls that may overlap, captured graphs among them, need
- * one each. (The workspace functions return 0 for what the calls refuse, es_hip_last_error() the reason.) Nothing is
+ * one each; es_hip_attn_workspace_upto sizes one for calls of every size. (The workspace functions return 0 for what the calls refuse, es_hip_last_error() the reason.) Nothing is
  * allocated, copied or waited for: the call can be captured. */
 size_t es_hip_attn_decode_workspace(const es_hip_kv *kv, int nseq, int heads);
 int es_hip_attn_decode_dev(const es_hip_kv *kv, int nseq, int heads, uint32_t type, const void *q, size_t qstride, float scale,
@@ -499,6 +499,10 @@ size_t es_hip_attn_prompt_workspace(const es_hip_kv *kv, int nseq, int ntok, int
 int es_hip_attn_prompt_dev(const es_hip_kv *kv, int nseq, const int *start, int ntok, int heads, uint32_t type, const void *q,
                            size_t qstride, float scale, int window, void *out, size_t ostride, void *ws, size_t ws_bytes,
                            void *stream);
+/* Bytes that are enough for every attention call on this cache, whatever q's type: decode of up to nseq sequences, prompts of up to
+ * nseq sequences and ntok tokens together. (The two functions above answer for one call, and a prompt call of many rows may need
+ * less than one of few, or nothing: what is enough for the largest call need not be for a smaller one.) */
+size_t es_hip_attn_workspace_upto(const es_hip_kv *kv, int nseq, int ntok, int heads);
 /* Page src[i] copied over page dst[i], for i < n, in the K and V pools of nlayers layers, layer l's pools at kv->k and kv->v +
  * l * layer_bytes (0: packed). src and dst are host arrays, read at the call; no page is a destination twice, or a
  * source and a destination. table, len and seq are not used. */

@@ -1241,6 +1241,21 @@ size_t es_hip_attn_prompt_workspace(const es_hip_kv *kv, int nseq, int ntok, int
     return shape_of(kv, nseq, ntok, heads, type, true).workspace(kv);
 }
 
+size_t es_hip_attn_workspace_upto(const es_hip_kv *kv, int nseq, int ntok, int heads) {
+    KvView v;
+    if (check_heads(kv, nseq, ntok, heads, v) || !nseq) return 0;
+    size_t most = shape_of(kv, nseq, nseq, heads, kv->type, false).workspace(kv);   // (decode: never less for more sequences)
+    for (uint32_t type : {(uint32_t)ES_HIP_F32, kv->type}) {
+        // a prompt's slots are its tiles plus the parts aimed for, as long as the tiles are fewer than those
+        Shape s = shape_of(kv, 1, 1, heads, type, true);
+        const size_t tiles = shape_of(kv, nseq, ntok, heads, type, true).tiles;
+        if (!ntok || !s.target) continue;   // (no call has parts if one of a token has none)
+        s.slots = std::min(tiles, (size_t)s.target - 1) + s.target;
+        most = std::max(most, s.workspace(kv));
+    }
+    return most;
+}
+
 int es_hip_attn_decode_dev(const es_hip_kv *kv, int nseq, int heads, uint32_t type, const void *q, size_t qstride, float scale,
                            int window, void *out, size_t ostride, void *ws, size_t ws_bytes, void *stream) {
     return attention(kv, nseq, nullptr, nseq, heads, type, q, qstride, scale, window, out, ostride, ws, ws_bytes, stream);

@@ -330,6 +330,7 @@ class Lib:
             ("es_hip_cache_wait", i, [vp, i]), ("es_hip_cache_step", i, [vp]),
             ("es_hip_kv_append_dev", i, [vp, i, vp, i, u32, vp, sz, vp, sz, vp]),
             ("es_hip_attn_decode_workspace", sz, [vp, i, i]), ("es_hip_attn_prompt_workspace", sz, [vp, i, i, i, u32]),
+            ("es_hip_attn_workspace_upto", sz, [vp, i, i, i]),
             ("es_hip_attn_decode_dev", i, [vp, i, i, u32, vp, sz, C.c_float, i, vp, sz, vp, sz, vp]),
             ("es_hip_attn_prompt_dev", i, [vp, i, vp, i, i, u32, vp, sz, C.c_float, i, vp, sz, vp, sz, vp]),
             ("es_hip_kv_copy_pages_dev", i, [vp, i, sz, vp, vp, i, vp]),
@@ -561,6 +562,10 @@ class Lib:
 
     def attn_prompt_workspace(self, kv, nseq, ntok, heads, t) -> int:
         return self._L.es_hip_attn_prompt_workspace(C.byref(kv), nseq, ntok, heads, t)
+
+    def attn_workspace_upto(self, kv, nseq, ntok, heads) -> int:
+        """for every decode and prompt call of up to nseq sequences and ntok tokens"""
+        return self._L.es_hip_attn_workspace_upto(C.byref(kv), nseq, ntok, heads)
 
     def attn_decode_dev(self, kv, nseq, heads, t, q, qstride, scale, window, out, ostride, ws, ws_bytes, stream=None):
         self._check(self._L.es_hip_attn_decode_dev(C.byref(kv), nseq, heads, t, self._ptr(q), qstride, scale, window,
