@@ -1157,6 +1157,10 @@ int check_heads(const es_hip_kv *kv, int nseq, int ntok, int heads, KvView &v) {
     return ES_HIP_OK;
 }
 
+int check_type(const es_hip_kv *kv, uint32_t type) {
+    return type == ES_HIP_F32 || type == kv->type ? ES_HIP_OK : host_fail(ES_HIP_EINVAL, "q and out are F32 or of the cache's type");
+}
+
 template <bool BF, int NQ> hipError_t launch(const AttnArgs &a, const Shape &s, bool prompt, hipStream_t st) {
     const unsigned grid = (unsigned)(s.items * a.c.heads);
     if (!prompt) {
@@ -1187,7 +1191,7 @@ int attention(const es_hip_kv *kv, int nseq, const int *start, int ntok, int hea
     AttnArgs a;
     const bool prompt = start != nullptr;
     if (int rc = check_heads(kv, nseq, ntok, heads, a.c)) return rc;
-    if (type != ES_HIP_F32 && type != kv->type) return host_fail(ES_HIP_EINVAL, "q and out are F32 or of the cache's type");
+    if (int rc = check_type(kv, type)) return rc;
     if (!(scale > 0.0f) || !std::isfinite(scale * 1.5f)) return host_fail(ES_HIP_EINVAL, "scale is positive and finite");
     if (window < 0) return host_fail(ES_HIP_EINVAL, "negative window");
     if (nseq == 0 || ntok == 0) return ES_HIP_OK;
@@ -1237,7 +1241,7 @@ size_t es_hip_attn_decode_workspace(const es_hip_kv *kv, int nseq, int heads) {
 
 size_t es_hip_attn_prompt_workspace(const es_hip_kv *kv, int nseq, int ntok, int heads, uint32_t type) {
     KvView v;
-    if (check_heads(kv, nseq, ntok, heads, v) || !nseq || !ntok) return 0;
+    if (check_heads(kv, nseq, ntok, heads, v) || check_type(kv, type) || !nseq || !ntok) return 0;
     return shape_of(kv, nseq, ntok, heads, type, true).workspace(kv);
 }
 

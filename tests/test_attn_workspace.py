@@ -52,3 +52,17 @@ print(json.dumps([L.attn_workspace_upto(k, s, n, h) for k, s, n, h in
                  + [L.attn_workspace_upto(good, 3, 0, 32) - L.attn_decode_workspace(good, 3, 32)]))
 """)
     assert got == [0] * 7
+
+
+def test_no_bytes_for_a_type_that_the_call_refuses(child):   # noqa: F811
+    got = child(r"""
+P, out = 1 << 20, []
+for cache in (E.F16, E.BF16):
+    k = kv(type=cache)
+    for t in (E.F32, E.F16, E.BF16, 2, 99):
+        fine = code(L.attn_prompt_dev, k, 3, P, 9, 32, t, P, 0, 0.1, 0, P, 0, P, 1 << 30) == 0
+        out.append([fine, L.attn_prompt_workspace(k, 3, 9, 32, t) > 0, "type" in L.last_error() or "F32" in L.last_error()])
+print(json.dumps(out))
+""")
+    assert all(fine == some for fine, some, _ in got) and sum(fine for fine, _, _ in got) == 4
+    assert all(named for fine, _, named in got if not fine)
