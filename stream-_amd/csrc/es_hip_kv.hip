@@ -4,9 +4,8 @@
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
-#include <climits>
 #include <new>
-#include <queue>
+#include <functional>
 #include <vector>
 
 #include "es_hip_attn.h"
