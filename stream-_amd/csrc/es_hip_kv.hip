@@ -4,8 +4,8 @@
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
-#include <new>
 #include <functional>
+#include <new>
 #include <vector>
 
 #include "es_hip_attn.h"
