@@ -70,12 +70,16 @@ __device__ Seq seq_of(const AttnArgs &a, int b) {
 constexpr int CHUNK_MIN = 128, CHUNK_SAVES = 512, CHUNK_PAIRS = 384;   // keys
 
 // The chunk's keys; 2^30: tiles are whole, which they stay unless chunks shorten the longest by more than CHUNK_SAVES: the
-// parts' sums go through memory and the join takes some 6 us, as much as 512 keys. us, whole and in chunks, 32 heads of 128
-// over 8, fp16: a prompt of 512 tokens 17 and 28, of 1024 31 and 44; 64 tokens behind 1936 of 64 elements 34 and 14.
+// parts' sums go through memory and a second launch joins them. us, whole and in chunks, 32 heads over 8, fp16: a prompt of 700
+// tokens, heads of 64 16 and 19, of 128 22 and 25, of 256 40 and 42; of 1000 21 and 26, 29 and 41, 51 and 51 (fp32 over bf16 34 and 38,
+// 54 and 53, 131 and 131); the last 16 of 1500 tokens 27 and 11, 34 and 13, 62 and 19 (44 and 13, 68 and 17, 167 and 31). One
+// number for all errs where rows are few, their parts soon joined: the last 16 of 700 stay whole, 15 and 10 for heads of
+// 64 in fp16, 26 and 14 for 128 in fp32 over fp16.
 // One sequence: its tiles' chunks are as many as there is room for (target), and half as many where that is two to a CU and they
-// are of CHUNK_PAIRS keys or less, since twice the parts cost more than the second workgroup of a CU gains: 64 tokens behind
-// 7937, 32 heads of 128 over 4, us, so and in twice the chunks: fp16 26 and 31, fp32 33 and 38; 64 behind 29936, whose chunks
-// are longer, would take 61 instead of 52.
+// are of CHUNK_PAIRS keys or less, since twice the parts cost more than the second workgroup of a CU gains. The last 64 of so many
+// tokens, 32 heads of 128 over 4, us, in half the chunks and in all: 3000 fp16 20 and 22, fp32 23 and 27; 8001 26 and 29, 32 and 36; 12000 (the
+// last that has half) 30 and 32, 39 and 43; 16000 35 and 37, 47 and 50; 30000 53 and 51, 75 and 76. The last 256 of 8001 over 8 57 and
+// 53, 80 and 79; heads of 64 the same within 2 us.
 // Several: the mean share of a place, and, where a CU holds but one workgroup, longer until the sequences' last chunks find room
 // too. Two to a CU even out by themselves, with chunks of whole 128s. us, in bf16 of 256 elements, where one fits, longer and
 // not: 3 sequences of 1250 to 2500 tokens, the last 300 new, 107 and 188; in fp16 of 128, where two fit: 16 of 1500 to 3000, the
@@ -396,7 +400,8 @@ template <int J> __device__ uint32_t pair(uint32_t first, uint32_t second) {
 }
 
 // ---- one query per sequence ----------------------------------------------------------------------------------------------------
-// A tile is the G query heads of a sequence's K/V head (16 of them, where there are more), its keys blocks of 128. The tiles'
+// A tile is the G query heads of a sequence's K/V head (16 of them, where there are more, and every 16 read K and V for themselves: 32
+// sequences of 4096 tokens, 2 K/V heads of 128, 8 to 64 heads each, fp16: 8 28 us, 16 30, 17 41, 32 42, 64 78), its keys blocks of 128. The tiles'
 // blocks, one after another, are dealt out evenly: workgroup w of a K/V head takes blocks [w * each, (w + 1) * each) of them,
 // whatever sequences they are of, so that a ragged batch keeps every workgroup busy to the end. What a workgroup has of a tile
 // that others have parts of goes to the workspace, and a second launch joins them. (The last workgroup of a tile to arrive
