@@ -481,7 +481,8 @@ int es_hip_kv_append_dev(const es_hip_kv *kv, int nseq, const int *start, int nt
  * same for out; aligned to their type. scale is positive and finite. A sequence without tokens gets zeros. Tokens that
  * a query does not see have no influence, whatever their rows hold; an infinity or NaN that it sees in V comes out as an infinity
  * or NaN in that element. fp32 q is carried to 22 bits or more through the matrix products, as are the weights p; with a 16-bit q,
- * p is rounded to the cache's type. out may be q itself, with one stride, and overlaps nothing else that the call reads. Limits:
+ * decode carries p to 14 bits (BF16; F16 20) or more, out's rounding being 9 (12), and a prompt rounds p to the cache's type: bring q as
+ * fp32 for more. Sums are fp32's: values of BF16 whose sum over the keys passes its range come out as infinities or NaN. out may be q itself, with one stride, and overlaps nothing else that the call reads. Limits:
  * 2^29 query rows (tokens times heads), 2^23 sequences times heads, 2^31 blocks of 128 keys that the table rows could hold.
  * ws: the caller's device workspace of at least es_hip_attn_decode_workspace bytes (16-byte aligned; 0 bytes: may be NULL); its
  * contents need no setup and nothing is kept in it between calls, but calls that may overlap, captured graphs among them, need

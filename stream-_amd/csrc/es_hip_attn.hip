@@ -12,8 +12,11 @@
 //
 // fp32 queries. q is split into as many terms of the cache's type as carry fp32's 24 bits (two of fp16 after scaling the row to
 // 2^14, 22 bits; three of bf16), one product each, and so are the weights. K and V are exact as they are.
-// Queries of the cache's own type go in as they are, and their weights are rounded once to that type, as out will be: half a
-// step of it relative to each, no more than storing the weights would cost; l adds up the unrounded ones.
+// Queries of the cache's own type go in as they are. Their weights are two terms in decode, which waits for memory: errors against 64 bits
+// are those of out's own rounding (131072 tokens, fp16, 2.1e-4; 47.85 us, and with one term 2.6e-4 and 47.7). A prompt rounds them once to
+// the type, as out will be: half a step of it relative to each, no more than storing the weights would cost. Its matrix cores are
+// what it waits for: two terms would take 2.91 ms, not 2.13, for 16384 tokens of fp16 (error 1.9e-4, not 2.5e-4), 340 us, not
+// 264, for 8 prompts of 99 to 3333 in bf16. Who needs more brings q as fp32. l adds up the unrounded weights.
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
@@ -257,18 +260,35 @@ __device__ float reference(float m) { return m == LOWEST ? 0.0f : m; }
 // A constant in the exponent rounds it: between 8 and 16 half a step of fp32 is 2^-21, 3.3e-7 of the weight, more than the weights'
 // terms lose (2^-22); between 2 and 4 it is 8e-8. So the two terms of fp16, which need a 2^BY of 12 or 15, take it as a factor, when
 // they are rounded, and their l at the end: exact, and no instruction more than without (decode of 500 tokens 6.66 us and, in the exponent,
-// 6.62; 64 prompt tokens behind 7937 31.0 and 30.8). Three terms of bf16 keep the constant small. One term is rounded to 2^-9 or 2^-12 at once, and
-// takes any in the exponent.
+// 6.62; 64 prompt tokens behind 7937 31.0 and 30.8). Three terms of bf16 keep the constant small. With 16-bit queries, whose out is rounded to 2^-9 or
+// 2^-12, any goes into the exponent.
 template <int NQ> constexpr bool FACTOR = NQ == 2;
 template <int NQ, int BY> __device__ float weights_sum(float l) { return FACTOR<NQ> ? l * (1 << (BY & 31)) : l; }
 template <int NQ, int BY> __device__ float weight(float s, float cs, float ref) {
     return __builtin_amdgcn_exp2f(__builtin_fmaf(s, cs, FACTOR<NQ> ? -ref : BY - ref));
 }
-template <bool BF, int NQ, int BY> __device__ void split_weights(const float (&x)[8], u4 (&y)[NQ]) {
-    if constexpr (!FACTOR<NQ>) {
-        split<BF, NQ>(x, y);
+template <bool BF, int NQ, int BY, int NP> __device__ void split_weights(const float (&x)[8], u4 (&y)[NP]) {   // NP terms
+    if constexpr (NQ == 1 && NP == 2) {
+        // Both terms cut off, the second's last bit set: it is off by less than its last place (2^-14 of the weight in bf16, 2^-20 in fp16),
+        // to either side, and greater than 0, so that an infinity in V comes out as one.
+#pragma unroll
+        for (int i = 0; i < 8; i += 2) {
+            if constexpr (BF) {
+                const uint32_t a = __float_as_uint(x[i]), b = __float_as_uint(x[i + 1]);
+                const float ra = x[i] - __uint_as_float(a & 0xffff0000u), rb = x[i + 1] - __uint_as_float(b & 0xffff0000u);
+                y[0][i / 2] = __builtin_amdgcn_perm(b, a, 0x07060302u);
+                y[1][i / 2] = __builtin_amdgcn_perm(__float_as_uint(rb), __float_as_uint(ra), 0x07060302u) | 0x00010001u;
+            } else {
+                const auto v = __builtin_amdgcn_cvt_pkrtz(x[i], x[i + 1]);
+                const auto w = __builtin_amdgcn_cvt_pkrtz(x[i] - static_cast<float>(v[0]), x[i + 1] - static_cast<float>(v[1]));
+                y[0][i / 2] = __builtin_bit_cast(uint32_t, v);
+                y[1][i / 2] = __builtin_bit_cast(uint32_t, w) | 0x00010001u;
+            }
+        }
+    } else if constexpr (!FACTOR<NQ>) {
+        split<BF, NP>(x, y);
     } else {
-        static_assert(!BF && NQ == 2);
+        static_assert(!BF && NP == 2);
         constexpr float f = 1 << BY;
         h8 v, w;
 #pragma unroll
@@ -465,6 +485,7 @@ struct Deal {
 
 template <bool BF, int NQ, int DP> __global__ __launch_bounds__(256, DP == 64 && NQ < 3 ? 3 : decode_per_cu(DP)) void attn_decode_kernel(AttnArgs a) {
     constexpr int KS = DP / 32, DL = DP / 16, BM = DECODE_M;
+    constexpr int NP = NQ == 1 ? 2 : NQ;   // terms of the weights
     constexpr bool F32 = NQ > 1;
     __shared__ float lm[4][BM], ll[4][BM];
     __shared__ __attribute__((aligned(16))) float lo_acc[4][BM][DP + 4];
@@ -619,7 +640,7 @@ template <bool BF, int NQ, int DP> __global__ __launch_bounds__(256, DP == 64 &&
                 w8[i] = weight<NQ, SHIFT<BF>>(s[i >> 2][i & 3], cs, ref);
                 l += w8[i];
             }
-            u4 pt[NQ];
+            u4 pt[NP];
             split_weights<BF, NQ, SHIFT<BF>>(w8, pt);
 #pragma unroll
             for (int j = 0; j < DL; j += 2) {
@@ -630,7 +651,7 @@ template <bool BF, int NQ, int DP> __global__ __launch_bounds__(256, DP == 64 &&
                     v1[k] = pair<1>(vr[2 * k][j / 2], vr[2 * k + 1][j / 2]);
                 }
 #pragma unroll
-                for (int t = 0; t < NQ; t++) {
+                for (int t = 0; t < NP; t++) {
                     acc[j] = mfma16<BF>(v0, pt[t], acc[j]);
                     acc[j + 1] = mfma16<BF>(v1, pt[t], acc[j + 1]);
                 }

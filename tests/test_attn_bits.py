@@ -110,6 +110,43 @@ def test_checks_refuse_what_does_not(ct):
     assert off(many_low_terms, ct, model(many_low_terms, ct, n, n, 0, 0, apart=False)) > 100
 
 
+def cut(x, ct):
+    """fp32 -> the type's bits, towards zero"""
+    if ct == E.BF16:
+        return (x.view(np.uint32) >> 16).astype(np.uint16)
+    y = to_bits(x, ct)
+    return y - (from_bits(y, ct) > x).astype(np.uint16)
+
+
+# Decode with 16-bit queries: out_j = (w_j v_j - w_0) / l, where v_j is 2^(j / 32) in the cache's type, so that what is left has few of
+# the weights' leading bits and the output's rounding is small next to theirs.
+def against(ct, terms=None):
+    """v, exact outputs, tolerance (and a model's outputs, of terms cut off): two terms of a weight, the last bit of the second set, are within
+    2^-14 of it in bf16, 2^-20 in fp16, the exponent with its constant within 3.3e-7 and 2^x within 2 u, for w_j and for w_0; then the
+    output's own rounding"""
+    a = np.arange(N) / 32
+    v = from_bits(to_bits(np.exp2(a), ct), ct)
+    w = np.exp2(-a)
+    exact = (w * v - 1) / w.sum()
+    tol = 2 * ((2.0 ** -14 if ct == E.BF16 else 2.0 ** -20) + 3.3e-7 + 2 * U) / w.sum() + {E.F16: 2.0 ** -11, E.BF16: 2.0 ** -8}[ct] * np.abs(exact)
+    if terms is None:
+        return v, exact, tol
+    w32 = w.astype(np.float32) * np.float32(2 ** 15)
+    first = cut(w32, ct) if terms == 2 else to_bits(w32, ct)
+    x = from_bits(first, ct)
+    if terms == 2:
+        x = x + from_bits(cut(w32 - x.astype(np.float32), ct) | 1, ct)
+    out = (x * v - x[0]) / float(w32.sum())
+    return v, exact, tol, from_bits(to_bits(out.astype(np.float32), ct), ct)
+
+
+@pytest.mark.parametrize("ct", TYPES, ids=NAMES.get)
+def test_checks_of_16_bit_decode(ct):
+    for terms in (1, 2):
+        _, exact, tol, out = against(ct, terms)
+        assert (np.abs(out - exact) <= tol)[1:].all() == (terms == 2)
+
+
 # ---- on the GPU ----------------------------------------------------------------------------------------------------------------
 @pytest.mark.gpu
 @pytest.mark.parametrize("dim", [64, 128, 256])
@@ -138,4 +175,29 @@ def test_bits_of_queries_and_weights(hip, case, ct, prompt, dim):
     assert not got[..., N:].any()
     r = off(case, ct, got[..., :N])
     print(f"{case.__name__} {NAMES[ct]} {'prompt' if prompt else 'decode'} {dim}: {r:.3f} of the tolerance", flush=True)
+    assert r <= 1
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dim", [64, 128, 256])
+@pytest.mark.parametrize("ct", TYPES, ids=NAMES.get)
+def test_decode_of_16_bit_queries_keeps_two_terms_of_the_weights(hip, ct, dim):
+    v, exact, tol = against(ct)
+    c = Cache(ct, 1, dim, 16, [N], np.random.default_rng(1))
+    k, vs = np.zeros((N, 1, dim)), np.zeros((N, 1, dim))
+    k[:, 0, 0] = -np.arange(N) / 32
+    vs[np.arange(N), 0, np.arange(N)] = v
+    vs[0, 0, :N] = -1
+    c.put(0, 0, to_bits(k, ct), to_bits(vs, ct))
+    kv, keep = c.upload(hip)
+    q = np.zeros((1, 2, dim))
+    q[..., 0] = 1
+    q = to_bits(q, ct)
+    dq, do = hip.upload(q), hip.alloc(q.nbytes)
+    ws = hip.attn_decode_workspace(kv, 1, 2)
+    dw = hip.alloc(max(ws, 16))
+    hip.attn_decode_dev(kv, 1, 2, ct, dq, 0, float(LN2), 0, do, 0, dw, ws)
+    got = from_bits(hip.download(do, np.zeros_like(q)), ct)
+    r = (np.abs(got[..., 1:N] - exact[1:]) / tol[1:]).max()
+    print(f"16-bit decode {NAMES[ct]} {dim}: {r:.3f} of the tolerance", flush=True)
     assert r <= 1
