@@ -470,8 +470,8 @@ typedef struct {
  * (start: device, nseq + 1 entries, not decreasing; NULL: one token per sequence, ntok = nseq). Rows from start[nseq] on are
  * not read; nothing is written for rows whose token would lie before the first or in no page. src_type: ES_HIP_F32 or the
  * cache's own type; token t's heads * dim elements at k + t * kstride elements (0: packed), the same for v; aligned to their
- * type. A page that several rows of the table share is written through whichever asks (of two tokens of one call that have the
- * same place, either may stay): see es_hip_kv_seq_extend for private copies. */
+ * type. A page that several rows of the table share is written through whichever asks (where two tokens of one call have the same
+ * place, it holds elements of either): see es_hip_kv_seq_extend for private copies. */
 int es_hip_kv_append_dev(const es_hip_kv *kv, int nseq, const int *start, int ntok, uint32_t src_type, const void *k,
                          size_t kstride, const void *v, size_t vstride, void *stream);
 /* Attention of one new token per sequence, the last in its cache (append it first):
@@ -481,9 +481,10 @@ int es_hip_kv_append_dev(const es_hip_kv *kv, int nseq, const int *start, int nt
  * same for out; aligned to their type. scale is positive and finite. A sequence without tokens gets zeros. Tokens that
  * a query does not see have no influence, whatever their rows hold; an infinity or NaN that it sees in V comes out as an infinity
  * or NaN in that element. fp32 q is carried to 22 bits or more through the matrix products, as are the weights p; with a 16-bit q,
- * decode carries p to 14 bits (BF16; F16 20) or more, out's rounding being 9 (12), and a prompt rounds p to the cache's type: bring q as
- * fp32 for more. Sums are fp32's: values of BF16 whose sum over the keys passes its range come out as infinities or NaN. out may be q itself, with one stride, and overlaps nothing else that the call reads. Limits:
- * 2^29 query rows (tokens times heads), 2^23 sequences times heads, 2^31 blocks of 128 keys that the table rows could hold.
+ * decode carries p to 14 bits or more (F16: 20), which does not show beside out's rounding, and a prompt rounds p to the cache's
+ * type: bring q as fp32 for more. Sums are fp32's: where a sum of |v| over the keys passes its range, which takes BF16, infinities
+ * or NaN come out. out may be q itself, with one stride, and overlaps nothing else that the call reads. Limits: 2^29 query rows
+ * (tokens times heads), 2^23 sequences times heads, 2^31 blocks of 128 keys that the table rows could hold.
  * ws: the caller's device workspace of at least es_hip_attn_decode_workspace bytes (16-byte aligned; 0 bytes: may be NULL); its
  * contents need no setup and nothing is kept in it between calls, but calls that may overlap, captured graphs among them, need
  * one each; es_hip_attn_workspace_upto sizes one for calls of every size. (The workspace functions return 0 for what the calls refuse, es_hip_last_error() the reason.) Nothing is
