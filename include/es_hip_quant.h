@@ -487,8 +487,8 @@ int es_hip_kv_append_dev(const es_hip_kv *kv, int nseq, const int *start, int nt
  * (tokens times heads), 2^23 sequences times heads, 2^31 blocks of 128 keys that the table rows could hold.
  * ws: the caller's device workspace of at least es_hip_attn_decode_workspace bytes (16-byte aligned; 0 bytes: may be NULL); its
  * contents need no setup and nothing is kept in it between calls, but calls that may overlap, captured graphs among them, need
- * one each; es_hip_attn_workspace_upto sizes one for calls of every size. (The workspace functions return 0 for what the calls refuse, es_hip_last_error() the reason.) Nothing is
- * allocated, copied or waited for: the call can be captured. */
+ * one each; es_hip_attn_workspace_upto sizes one for calls of every size. (The workspace functions return 0 for what the calls
+ * refuse, es_hip_last_error() the reason.) Nothing is allocated, copied or waited for: the call can be captured. */
 size_t es_hip_attn_decode_workspace(const es_hip_kv *kv, int nseq, int heads);
 int es_hip_attn_decode_dev(const es_hip_kv *kv, int nseq, int heads, uint32_t type, const void *q, size_t qstride, float scale,
                            int window, void *out, size_t ostride, void *ws, size_t ws_bytes, void *stream);
