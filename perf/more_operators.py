@@ -261,9 +261,9 @@ def _kv(s):
     if "kv" not in s:
         E, _ = _lib()
         c = s["case"]
-        s["kv"] = E.Kv(TYPES[c.get("cache", "f8")][1], c["kv"], c["dim"], c["page"], s["k"].shape[0], s["k"].data_ptr(), s["v"].data_ptr(),
-                       s["table"].data_ptr(), s["len"].data_ptr(), None, c["seqs"], s["most"],
-                       None if s["ks"] is None else s["ks"].data_ptr(), None if s["vs"] is None else s["vs"].data_ptr())
+        fields = (TYPES[c.get("cache", "f8")][1], c["kv"], c["dim"], c["page"], s["k"].shape[0], s["k"].data_ptr(), s["v"].data_ptr(),
+                  s["table"].data_ptr(), s["len"].data_ptr(), None, c["seqs"], s["most"])
+        s["kv"] = E.Kv(*fields) if s["ks"] is None else E.Kv8(*fields, s["ks"].data_ptr(), s["vs"].data_ptr())
     return s["kv"]
 
 
