@@ -45,6 +45,9 @@ enum {
 };
 /* GGML type ids of the unquantized types that the key-value cache and its attention take (not weight formats) */
 enum { ES_HIP_F32 = 0, ES_HIP_F16 = 1, ES_HIP_BF16 = 30 };
+/* a cache in 8 bits (no GGML type: numbers from 256 on are this library's): 1 sign, 4 exponent and 3 mantissa bits, bias 7, largest 448,
+ * 0x7f and 0xff NaN, no infinities, with a scale for every 16 tokens of a K/V head */
+enum { ES_HIP_F8 = 256 };
 
 /* fp32 epilogue order, see the header comment */
 enum { ES_HIP_ORDER_X86_CONTRACT = 0, ES_HIP_ORDER_X86_STRICT = 1, ES_HIP_ORDER_SCALAR = 2 };
@@ -455,8 +458,8 @@ int  es_hip_cache_get_stats(const es_hip_cache *c, es_hip_cache_stats *out);
  * is written for them, no query sees them), so that padded batches and tables with holes are in order. The calling thread's
  * current device is the one of the buffers and the stream, here as in every other call. */
 typedef struct {
-    uint32_t type;      /* ES_HIP_F16 or ES_HIP_BF16 */
-    int heads, dim;     /* K/V heads; elements per head, a multiple of 8 up to 256 */
+    uint32_t type;      /* ES_HIP_F16, ES_HIP_BF16 or ES_HIP_F8 */
+    int heads, dim;     /* K/V heads; elements per head, a multiple of 8 up to 256 (F8: of 16) */
     int page, npages;   /* tokens per page, a power of two from 16 to 1024; pages in the pools */
     void *k, *v;        /* device, 16-byte aligned */
     const int *table;   /* device */
@@ -464,12 +467,21 @@ typedef struct {
     const int *seq;     /* device: the call's sequence b is row seq[b]; NULL: row b */
     int rows;           /* rows of table and entries of len */
     int max_pages;      /* entries of a table row */
+    float *k_scale, *v_scale;   /* device, F8 alone (not looked at for other types): a power of two for every 16 tokens of a page and
+                           head, tokens 16 u to 16 u + 15 of head h in page p at (p * heads + h) * (page / 16) + u */
 } es_hip_kv;
+/* An F8 cache. Its elements stand for the number times its 16 tokens' scale 2^e, -100 <= e <= 120, exactly; half the memory and
+ * reads of a 16-bit cache, with elements off by at most 2^-4 of themselves, or 2^(e - 10) where they are small. Attention takes what they
+ * stand for, as bf16. es_hip_kv_append_dev gives 16 tokens the least scale whose 448-fold is not less than any of their elements (infinities and
+ * NaN, which become NaN, aside; from 2^-100 to 2^120, beyond which an element may stand for an infinity). Where some of the 16 were written by an
+ * earlier call, those before the call's own stay, with no smaller a scale; should it grow, they are rounded to it once more: that loses
+ * only bits below 2^(e - 9). No two sequences of a call may write to the same 16 tokens (a sequence named
+ * twice, pages shared without es_hip_kv_seq_extend's copies): what they then hold is undefined. */
 /* The rows of ntok new tokens into their pages, rounded to the cache's type (nearest even; fp16 overflows to infinity). The
  * call's sequence b brings rows start[b] to start[b + 1] - 1 of k and v, which are its last tokens: those at len - n to len - 1
  * (start: device, nseq + 1 entries, not decreasing; NULL: one token per sequence, ntok = nseq). Rows from start[nseq] on are
  * not read; nothing is written for rows whose token would lie before the first or in no page. src_type: ES_HIP_F32 or the
- * cache's own type; token t's heads * dim elements at k + t * kstride elements (0: packed), the same for v; aligned to their
+ * cache's own type (an F8 cache: F32, F16 or BF16; at most 2^26 runs of 16 tokens times heads); token t's heads * dim elements at k + t * kstride elements (0: packed), the same for v; aligned to their
  * type. A page that several rows of the table share is written through whichever asks (where two tokens of one call have the same
  * place, it holds elements of either): see es_hip_kv_seq_extend for private copies. */
 int es_hip_kv_append_dev(const es_hip_kv *kv, int nseq, const int *start, int ntok, uint32_t src_type, const void *k,
@@ -477,7 +489,7 @@ int es_hip_kv_append_dev(const es_hip_kv *kv, int nseq, const int *start, int nt
 /* Attention of one new token per sequence, the last in its cache (append it first):
  *   out[b][h] = sum over j of p[j] * v[j],  p = softmax over j of scale * (q[b][h] . k[j]),  len - window <= j < len
  * (window 0: all), with head h reading K/V head h / (heads / kv->heads). heads: a multiple of kv->heads. type: q's and out's,
- * ES_HIP_F32 (with either cache) or the cache's own; head h of sequence b at q + b * qstride + h * dim elements (0: packed), the
+ * ES_HIP_F32 (with any cache) or the cache's own (an F8 cache's: ES_HIP_BF16); head h of sequence b at q + b * qstride + h * dim elements (0: packed), the
  * same for out; aligned to their type. scale is positive and finite. A sequence without tokens gets zeros. Tokens that
  * a query does not see have no influence, whatever their rows hold; an infinity or NaN that it sees in V comes out as an infinity
  * or NaN in that element. fp32 q is carried to 22 bits or more through the matrix products, as are the weights p; with a 16-bit q,
@@ -501,12 +513,19 @@ size_t es_hip_attn_prompt_workspace(const es_hip_kv *kv, int nseq, int ntok, int
 int es_hip_attn_prompt_dev(const es_hip_kv *kv, int nseq, const int *start, int ntok, int heads, uint32_t type, const void *q,
                            size_t qstride, float scale, int window, void *out, size_t ostride, void *ws, size_t ws_bytes,
                            void *stream);
+/* The same through a window that leaves the first `sinks` tokens of the sequence in sight: position pos sees tokens j <= pos with
+ * j < sinks or j > pos - window (window 0: all). 0 sinks: the calls above. The same workspace. What lies between is not read. */
+int es_hip_attn_decode_sinks_dev(const es_hip_kv *kv, int nseq, int heads, uint32_t type, const void *q, size_t qstride, float scale,
+                                 int window, int sinks, void *out, size_t ostride, void *ws, size_t ws_bytes, void *stream);
+int es_hip_attn_prompt_sinks_dev(const es_hip_kv *kv, int nseq, const int *start, int ntok, int heads, uint32_t type, const void *q,
+                                 size_t qstride, float scale, int window, int sinks, void *out, size_t ostride, void *ws,
+                                 size_t ws_bytes, void *stream);
 /* Bytes that are enough for every attention call on this cache, whatever q's type: decode of up to nseq sequences, prompts of up to
  * nseq sequences and ntok tokens together. (The two functions above answer for one call, and a prompt call of many rows may need
  * less than one of few, or nothing: what is enough for the largest call need not be for a smaller one.) */
 size_t es_hip_attn_workspace_upto(const es_hip_kv *kv, int nseq, int ntok, int heads);
 /* Page src[i] copied over page dst[i], for i < n, in the K and V pools of nlayers layers, layer l's pools at kv->k and kv->v +
- * l * layer_bytes (0: packed). src and dst are host arrays, read at the call; no page is a destination twice, or a
+ * l * layer_bytes (0: packed); an F8 cache's scales with them, layer l's l * layer_bytes / (16 * dim) floats on. src and dst are host arrays, read at the call; no page is a destination twice, or a
  * source and a destination. table, len and seq are not used. */
 int es_hip_kv_copy_pages_dev(const es_hip_kv *kv, int nlayers, size_t layer_bytes, const int *src, const int *dst, int n,
                              void *stream);

@@ -4,6 +4,8 @@
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
+#include <cstddef>
+#include <cstring>
 #include <functional>
 #include <new>
 #include <vector>
@@ -15,16 +17,23 @@ namespace esq {
 
 int kv_check(const es_hip_kv *kv, int nseq, KvView &v, bool paged) {
     if (!kv) return host_fail(ES_HIP_EINVAL, "null cache");
-    if (kv->type != ES_HIP_F16 && kv->type != ES_HIP_BF16) return host_fail(ES_HIP_EINVAL, "the cache's type is F16 or BF16");
+    const bool eight = kv->type == ES_HIP_F8;
+    if (kv->type != ES_HIP_F16 && kv->type != ES_HIP_BF16 && !eight) return host_fail(ES_HIP_EINVAL, "the cache's type is F16, BF16 or F8");
     if (kv->heads < 1 || kv->heads > 4096 || kv->dim < 8 || kv->dim > 256 || kv->dim % 8)
         return host_fail(ES_HIP_EINVAL, "1 to 4096 K/V heads of a multiple of 8 up to 256 elements");
+    if (eight && kv->dim % 16) return host_fail(ES_HIP_EINVAL, "an F8 cache's heads have a multiple of 16 elements");
     if (kv->page < 16 || kv->page > 1024 || (kv->page & (kv->page - 1)))
         return host_fail(ES_HIP_EINVAL, "a page is a power of two from 16 to 1024 tokens");
     if (kv->npages < 1) return host_fail(ES_HIP_EINVAL, "no pages");
     if (!kv->k || !kv->v || ((reinterpret_cast<uintptr_t>(kv->k) | reinterpret_cast<uintptr_t>(kv->v)) & 15))
         return host_fail(ES_HIP_EINVAL, "null or misaligned pools (16 bytes)");
+    // (the scales' fields are read for F8 alone: a program built when the struct ended before them has none)
+    if (eight && (!kv->k_scale || !kv->v_scale || ((reinterpret_cast<uintptr_t>(kv->k_scale) | reinterpret_cast<uintptr_t>(kv->v_scale)) & 3)))
+        return host_fail(ES_HIP_EINVAL, "null or misaligned scales of an F8 cache");
     v.k = static_cast<uint8_t *>(kv->k);
     v.v = static_cast<uint8_t *>(kv->v);
+    v.ks = eight ? kv->k_scale : nullptr;
+    v.vs = eight ? kv->v_scale : nullptr;
     v.heads = kv->heads;
     v.dim = kv->dim;
     v.shift = __builtin_ctz((unsigned)kv->page);
@@ -114,9 +123,142 @@ template <bool F32, bool BF> __global__ __launch_bounds__(256) void kv_append_ke
     const u4 kw = k.value(), vw = v.value();
     if (page < 0 || page >= a.c.npages) return;
     const int dc = a.c.dim >> 3, head = c / dc, d = (c - head * dc) * 8;
-    const size_t at = a.c.at(page, head, pos & ((1 << a.c.shift) - 1)) + d * 2;
+    const size_t at = (a.c.row_at(page, head, pos & ((1 << a.c.shift) - 1)) * a.c.dim + d) * 2;
     *reinterpret_cast<u4 *>(a.c.k + at) = kw;
     *reinterpret_cast<u4 *>(a.c.v + at) = vw;
+}
+
+// ---- new rows in 8 bits --------------------------------------------------------------------------------------------------------
+// A wave per run of 16 tokens and K/V head that gets tokens, of K or of V: its elements in registers, 8 a lane at a time, their
+// largest over the lanes, the scale, and the numbers. A run that had tokens before the call keeps them: its scale never
+// shrinks, and where it grows they are rounded once more to the new one, which is exact but for what falls below 2^-6 of it (so that
+// adding tokens one by one and all at once differ there alone). Powers of two make all of this exact arithmetic: no result hangs
+// on how a division was rounded.
+//
+// Runs are found by slots: sequence b has those from start[b] / 16 + 2 b on, at least as many as the runs that its tokens can touch
+// ((n + 14) / 16 + 1 of n), and a wave finds its sequence by 64 probes at a time.
+constexpr int E_LEAST = -100, E_MOST = 120;   // the scales' exponents
+__device__ int exponent(float scale) { return min(max((int)(__float_as_uint(scale) >> 23 & 255) - 127, E_LEAST), E_MOST); }
+__device__ float power(int e) { return __uint_as_float((uint32_t)(e + 127) << 23); }
+// the least e with largest <= 448 * 2^e = 1.75 * 2^(e + 8)
+__device__ int exponent_for(float largest) {
+    const uint32_t u = __float_as_uint(largest);
+    return min(max((int)(u >> 23) - 127 - 8 + ((u & 0x7fffff) > 0x600000), E_LEAST), E_MOST);
+}
+__device__ bool finite(float x) { return fabsf(x) < INFINITY; }
+
+enum { ROW_F32, ROW_F16, ROW_BF16 };
+// 8 elements as they come
+template <int ROW> struct Row8 {
+    struct __attribute__((packed, aligned(ROW == ROW_F32 ? 4 : 2))) Raw { uint32_t x[ROW == ROW_F32 ? 8 : 4]; } raw;
+    __device__ void load(const uint8_t *p) { raw = *reinterpret_cast<const Raw *>(p); }
+    __device__ float get(int i) const {
+        if constexpr (ROW == ROW_F32) return __uint_as_float(raw.x[i]);
+        else if constexpr (ROW == ROW_BF16) return __uint_as_float(i & 1 ? raw.x[i / 2] & 0xffff0000u : raw.x[i / 2] << 16);
+        else return static_cast<float>(__builtin_bit_cast(_Float16, (uint16_t)(raw.x[i / 2] >> (i & 1) * 16)));
+    }
+};
+__device__ u2 eight_numbers(const float (&x)[8]) {
+    u2 y;
+#pragma unroll
+    for (int i = 0; i < 2; i++)
+        y[i] = __builtin_amdgcn_cvt_pk_fp8_f32(x[4 * i + 2], x[4 * i + 3], __builtin_amdgcn_cvt_pk_fp8_f32(x[4 * i], x[4 * i + 1], 0, false), true);
+    return y;
+}
+
+struct AppendArgs8 {
+    KvView c;
+    float *ks, *vs;
+    const int *start;
+    const uint8_t *k, *v;
+    size_t kstride, vstride;   // bytes
+    int nseq, ntok, slots;
+};
+
+template <int ROW, int DP> __global__ __launch_bounds__(256) void kv_append8_kernel(AppendArgs8 a) {
+    constexpr int NI = DP / 32, ES = ROW == ROW_F32 ? 4 : 2;
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const long long item = (long long)blockIdx.x * 4 + wave;
+    const int slot = (int)(item / a.c.heads), head = (int)(item - (long long)slot * a.c.heads);
+    if (slot >= a.slots) return;
+    int b = slot, t0 = slot, n = 1, j = 0;   // the sequence, its rows, the number of the run among those it may touch
+    if (a.start) {
+        int at = 0, end = a.nseq;
+        for (;;) {
+            const int step = (end - at + 63) >> 6, i = min(at + lane * step, a.nseq - 1);
+            const int from = a.start[i], to = a.start[i + 1];
+            const int before = __builtin_popcountll(__ballot(at + lane * step < end && (from >> 4) + 2 * i <= slot));
+            if (!before) return;
+            at += (before - 1) * step;
+            if (step == 1) {
+                b = at;
+                t0 = __builtin_amdgcn_readlane(from, before - 1);
+                j = slot - (t0 >> 4) - 2 * b;
+                n = __builtin_amdgcn_readlane(to, before - 1);
+                break;
+            }
+            end = min(end, at + step);
+        }
+        t0 = min(max(t0, 0), a.ntok);
+        n = min(max(n, t0), a.ntok) - t0;
+    }
+    const int r = a.c.row(b), len = a.c.tokens(b), first = len - n;
+    const int begin = (max(first, 0) & -16) + j * 16, lo = max(max(first, 0), begin), hi = min(len, begin + 16);
+    if (r < 0 || j < 0 || lo >= hi) return;
+    const int page = a.c.table[(size_t)r * a.c.max_pages + (begin >> a.c.shift)];
+    if (page < 0 || page >= a.c.npages) return;
+    const bool is_v = blockIdx.y;
+    const size_t row = a.c.row_at(page, head, begin & ((1 << a.c.shift) - 1));
+    uint8_t *pool = (is_v ? a.c.v : a.c.k) + row * a.c.dim;
+    float *scale = (is_v ? a.vs : a.ks) + (row >> 4);
+    const uint8_t *src = (is_v ? a.v : a.k) + (size_t)(t0 + lo - first) * (is_v ? a.vstride : a.kstride) + (size_t)head * a.c.dim * ES;
+    const size_t stride = is_v ? a.vstride : a.kstride;
+    const int per = a.c.dim >> 3, mine = (hi - lo) * per;   // eights of elements
+    const bool more = lo > begin;
+    const int e_old = more ? exponent(*scale) : E_LEAST;
+
+    Row8<ROW> x[NI];
+    float largest = 0.0f;
+#pragma unroll
+    for (int i = 0; i < NI; i++) {
+        const int id = lane + i * 64, t = id / per, d = (id - t * per) * 8;
+        if (id < mine) {
+            x[i].load(src + t * stride + d * ES);
+#pragma unroll
+            for (int k = 0; k < 8; k++) largest = fmaxf(largest, finite(x[i].get(k)) ? fabsf(x[i].get(k)) : 0.0f);
+        }
+    }
+    largest = over_lanes(largest, 64, Max());
+    const int e = max(exponent_for(largest), e_old);
+    if (more && e > e_old) {
+        const float by = power(max(e_old - e, -32));   // (2^-32: every number to 0)
+        for (int id = lane; id < (lo - begin) * per; id += 64) {
+            u2 *p = reinterpret_cast<u2 *>(pool) + id;
+            const u2 w = *p;
+            float y[8];
+#pragma unroll
+            for (int i = 0; i < 2; i++) {
+                const auto y0 = __builtin_amdgcn_cvt_pk_f32_fp8(w[i], false), y1 = __builtin_amdgcn_cvt_pk_f32_fp8(w[i], true);
+                y[i * 4] = y0[0] * by;
+                y[i * 4 + 1] = y0[1] * by;
+                y[i * 4 + 2] = y1[0] * by;
+                y[i * 4 + 3] = y1[1] * by;
+            }
+            *p = eight_numbers(y);
+        }
+    }
+    const float by = power(-e);
+    u2 *to = reinterpret_cast<u2 *>(pool + (size_t)(lo - begin) * a.c.dim);
+#pragma unroll
+    for (int i = 0; i < NI; i++) {
+        if (lane + i * 64 < mine) {
+            float y[8];
+#pragma unroll
+            for (int k = 0; k < 8; k++) y[k] = finite(x[i].get(k)) ? x[i].get(k) * by : __uint_as_float(0x7fc00000u);
+            to[lane + i * 64] = eight_numbers(y);
+        }
+    }
+    if (lane == 0) *scale = power(e);
 }
 
 // ---- pages copied ----------------------------------------------------------------------------------------------------------
@@ -128,12 +270,14 @@ constexpr int COPY_PAIRS = 448, COPY_BYTES = 16384;
 constexpr size_t COPY_ONCE = 96u << 20;   // bytes read and written
 struct CopyArgs {
     uint8_t *k, *v;
-    size_t layer_bytes;
+    float *ks, *vs;        // an 8-bit cache's scales
+    size_t layer_bytes, layer_scales;
+    int page_scales;
     uint32_t page_bytes;   // a multiple of 256
     int src[COPY_PAIRS], dst[COPY_PAIRS];
 };
 
-template <bool ONCE> __global__ __launch_bounds__(256) void kv_copy_kernel(CopyArgs a) {
+template <bool ONCE, bool E8> __global__ __launch_bounds__(256) void kv_copy_kernel(CopyArgs a) {
     const int layer = blockIdx.z >> 1;
     uint8_t *pool = (blockIdx.z & 1 ? a.v : a.k) + (size_t)layer * a.layer_bytes;
     const uint8_t *s = pool + (size_t)a.src[blockIdx.y] * a.page_bytes;
@@ -153,24 +297,41 @@ template <bool ONCE> __global__ __launch_bounds__(256) void kv_copy_kernel(CopyA
             if constexpr (ONCE) __builtin_nontemporal_store(x[i], p);
             else *p = x[i];
         }
+    if constexpr (E8) {   // this workgroup's share of the page's scales
+        float *scales = (blockIdx.z & 1 ? a.vs : a.ks) + (size_t)layer * a.layer_scales;
+        const int share = (a.page_scales + gridDim.x - 1) / gridDim.x, first = blockIdx.x * share;
+        for (int i = first + threadIdx.x; i < min(first + share, a.page_scales); i += 256)
+            scales[(size_t)a.dst[blockIdx.y] * a.page_scales + i] = scales[(size_t)a.src[blockIdx.y] * a.page_scales + i];
+    }
 }
 
-hipError_t copy_pages(uint8_t *k, uint8_t *v, size_t layer_bytes, size_t page_bytes, int nlayers, const int *src, const int *dst,
-                      int n, hipStream_t s) {
+// the pools of nlayers layers: where the first one's are, and how far apart the layers are
+struct Layers {
+    uint8_t *k, *v;
+    float *ks, *vs;   // null: a 16-bit cache
+    size_t layer_bytes, page_bytes, page_scales;   // page_scales: scales of a page
+    int nlayers;
+    size_t layer_scales() const { return page_scales ? layer_bytes / (page_bytes / page_scales) : 0; }
+};
+
+hipError_t copy_pages(const Layers &c, const int *src, const int *dst, int n, hipStream_t s) {
     CopyArgs a;
-    a.k = k;
-    a.v = v;
-    a.layer_bytes = layer_bytes;
-    a.page_bytes = (uint32_t)page_bytes;
-    const auto f = (double)page_bytes * nlayers * n * 4 >= COPY_ONCE ? kv_copy_kernel<true> : kv_copy_kernel<false>;
-    for (int l = 0; l < nlayers; l += 16384)   // (a grid's z ends at 65535)
+    a.layer_bytes = c.layer_bytes;
+    a.layer_scales = c.layer_scales();
+    a.page_bytes = (uint32_t)c.page_bytes;
+    a.page_scales = (int)c.page_scales;
+    const bool once = (double)c.page_bytes * c.nlayers * n * 4 >= COPY_ONCE;
+    const auto f = c.ks ? (once ? kv_copy_kernel<true, true> : kv_copy_kernel<false, true>) : (once ? kv_copy_kernel<true, false> : kv_copy_kernel<false, false>);
+    for (int l = 0; l < c.nlayers; l += 16384)   // (a grid's z ends at 65535)
         for (int i = 0; i < n; i += COPY_PAIRS) {
             const int m = std::min(COPY_PAIRS, n - i);
             std::copy(src + i, src + i + m, a.src);
             std::copy(dst + i, dst + i + m, a.dst);
-            a.k = k + (size_t)l * layer_bytes;
-            a.v = v + (size_t)l * layer_bytes;
-            f<<<dim3((unsigned)((page_bytes + COPY_BYTES - 1) / COPY_BYTES), m, 2 * std::min(16384, nlayers - l)), 256, 0, s>>>(a);
+            a.k = c.k + (size_t)l * c.layer_bytes;
+            a.v = c.v + (size_t)l * c.layer_bytes;
+            a.ks = c.ks ? c.ks + (size_t)l * a.layer_scales : nullptr;
+            a.vs = c.vs ? c.vs + (size_t)l * a.layer_scales : nullptr;
+            f<<<dim3((unsigned)((c.page_bytes + COPY_BYTES - 1) / COPY_BYTES), m, 2 * std::min(16384, c.nlayers - l)), 256, 0, s>>>(a);
             if (hipError_t e = hipGetLastError()) return e;
         }
     return hipSuccess;
@@ -208,7 +369,8 @@ struct es_hip_kv_pool {
     uint32_t type = 0;
     int nlayers = 0, heads = 0, dim = 0, page = 0, npages = 0, max_seqs = 0, max_pages = 0;
     size_t page_bytes = 0, layer_bytes = 0;
-    uint8_t *mem = nullptr;   // K of every layer, then V
+    size_t page_scales = 0;   // an 8-bit cache's scales of a page
+    uint8_t *mem = nullptr;   // K of every layer, then V; an 8-bit cache: then the scales of K, and of V
     int *table = nullptr, *len = nullptr;
     std::vector<int> refs;    // sequences that hold the page
     std::vector<int> spare;   // a heap, the lowest number first
@@ -226,7 +388,17 @@ struct es_hip_kv_pool {
     }
     bool has(int s) const { return s >= 0 && s < max_seqs && seqs[s].live; }
     size_t pool_bytes() const { return layer_bytes * nlayers; }
+    size_t layer_scales() const { return page_scales * npages; }
+    float *scales(int layer, bool v) const {
+        if (!page_scales) return nullptr;
+        return reinterpret_cast<float *>(mem + 2 * pool_bytes()) + ((size_t)(v ? nlayers : 0) + layer) * layer_scales();
+    }
+    Layers layers() const;
 };
+
+Layers es_hip_kv_pool::layers() const {
+    return {mem, mem + pool_bytes(), scales(0, false), scales(0, true), layer_bytes, page_bytes, page_scales, nlayers};
+}
 
 namespace {
 
@@ -348,8 +520,7 @@ int extend(es_hip_kv_pool *p, const int *seqs, const int *n, int count, hipStrea
         sets.length(seqs[i], q.len);
     }
     if (!p->mem) return ES_HIP_OK;
-    hipError_t e = copy_pages(p->mem, p->mem + p->pool_bytes(), p->layer_bytes, p->page_bytes, p->nlayers, src.data(), dst.data(),
-                              (int)src.size(), st);
+    hipError_t e = copy_pages(p->layers(), src.data(), dst.data(), (int)src.size(), st);
     if (e == hipSuccess) e = sets.send(p, st);
     return e == hipSuccess ? ES_HIP_OK : host_hip_fail(e, "page launch");
 }
@@ -405,8 +576,7 @@ int compact(es_hip_kv_pool *p, hipStream_t st) {
     p->spare.clear();
     for (int g = used; g < p->npages; g++) p->spare.push_back(g);   // ascending: a heap as it is
     if (!p->mem || src.empty()) return used;
-    hipError_t e = copy_pages(p->mem, p->mem + p->pool_bytes(), p->layer_bytes, p->page_bytes, p->nlayers, src.data(), dst.data(),
-                              (int)src.size(), st);
+    hipError_t e = copy_pages(p->layers(), src.data(), dst.data(), (int)src.size(), st);
     if (e == hipSuccess) e = sets.send(p, st);
     return e == hipSuccess ? used : host_hip_fail(e, "page launch");
 }
@@ -420,7 +590,9 @@ int es_hip_kv_append_dev(const es_hip_kv *kv, int nseq, const int *start, int nt
     if (int rc = host_need_device()) return rc;
     AppendArgs a;
     if (int rc = kv_check(kv, nseq, a.c, true)) return rc;
-    if (src_type != ES_HIP_F32 && src_type != kv->type) return host_fail(ES_HIP_EINVAL, "rows are F32 or of the cache's type");
+    const bool eight = kv->type == ES_HIP_F8;
+    if (src_type != ES_HIP_F32 && (eight ? src_type != ES_HIP_F16 && src_type != ES_HIP_BF16 : src_type != kv->type))
+        return host_fail(ES_HIP_EINVAL, "rows are F32 or of the cache's type (an F8 cache: F32, F16 or BF16)");
     if (ntok < 0 || (!start && ntok != nseq)) return host_fail(ES_HIP_EINVAL, "ntok is negative, or not nseq without start");
     if (ntok == 0 || nseq == 0) return ES_HIP_OK;
     const size_t es = src_type == ES_HIP_F32 ? 4 : 2, row = (size_t)kv->heads * kv->dim;
@@ -430,6 +602,31 @@ int es_hip_kv_append_dev(const es_hip_kv *kv, int nseq, const int *start, int nt
     if (!kstride) kstride = row;
     if (!vstride) vstride = row;
     if (ntok > 1 && (kstride < row || vstride < row)) return host_fail(ES_HIP_EINVAL, "rows overlap (stride below heads * dim)");
+    if (eight) {
+        AppendArgs8 e;
+        e.c = a.c;
+        e.ks = kv->k_scale;
+        e.vs = kv->v_scale;
+        e.start = start;
+        e.k = static_cast<const uint8_t *>(k);
+        e.v = static_cast<const uint8_t *>(v);
+        e.kstride = kstride * es;
+        e.vstride = vstride * es;
+        e.nseq = nseq;
+        e.ntok = ntok;
+        const long long slots = start ? (long long)ntok / 16 + 2LL * nseq + 1 : nseq, waves = slots * kv->heads;
+        if (waves >= 1LL << 26) return host_fail(ES_HIP_EINVAL, "more than 2^26 runs of 16 tokens times heads");   // (a launch holds 2^24 workgroups of 256)
+        e.slots = (int)slots;
+        const int dp = kv->dim <= 64 ? 0 : kv->dim <= 128 ? 1 : 2;
+        static constexpr void (*kernels[3][3])(AppendArgs8) = {
+            {kv_append8_kernel<ROW_F32, 64>, kv_append8_kernel<ROW_F32, 128>, kv_append8_kernel<ROW_F32, 256>},
+            {kv_append8_kernel<ROW_F16, 64>, kv_append8_kernel<ROW_F16, 128>, kv_append8_kernel<ROW_F16, 256>},
+            {kv_append8_kernel<ROW_BF16, 64>, kv_append8_kernel<ROW_BF16, 128>, kv_append8_kernel<ROW_BF16, 256>}};
+        const auto f = kernels[src_type == ES_HIP_F32 ? ROW_F32 : src_type == ES_HIP_F16 ? ROW_F16 : ROW_BF16][dp];
+        f<<<dim3((unsigned)((waves + 3) / 4), 2), 256, 0, static_cast<hipStream_t>(stream)>>>(e);
+        const hipError_t err = hipGetLastError();
+        return err == hipSuccess ? ES_HIP_OK : host_hip_fail(err, "append launch");
+    }
     a.start = start;
     a.k = static_cast<const uint8_t *>(k);
     a.v = static_cast<const uint8_t *>(v);
@@ -457,10 +654,11 @@ int es_hip_kv_copy_pages_dev(const es_hip_kv *kv, int nlayers, size_t layer_byte
     if (int rc = kv_check(kv, 0, c, false)) return rc;
     if (nlayers < 0 || n < 0 || (n && (!src || !dst))) return host_fail(ES_HIP_EINVAL, "bad page list or number of layers");
     if (nlayers == 0 || n == 0) return ES_HIP_OK;
-    const size_t page_bytes = (size_t)kv->heads * kv->page * kv->dim * 2;
+    const bool eight = kv->type == ES_HIP_F8;
+    const size_t page_bytes = (size_t)kv->heads * kv->page * kv->dim * (eight ? 1 : 2), page_scales = eight ? (size_t)kv->heads * kv->page / 16 : 0;
     if (!layer_bytes) layer_bytes = page_bytes * kv->npages;
-    if (nlayers > 1 && (layer_bytes < page_bytes * kv->npages || layer_bytes % 16))
-        return host_fail(ES_HIP_EINVAL, "layers overlap, or a layer is not a multiple of 16 bytes");
+    if (nlayers > 1 && (layer_bytes < page_bytes * kv->npages || layer_bytes % (eight ? 16 * kv->dim : 16)))
+        return host_fail(ES_HIP_EINVAL, "layers overlap, or a layer is not a multiple of 16 bytes (F8: of 16 tokens)");
     try {
         std::vector<uint64_t> is_src((kv->npages + 63) / 64, 0), is_dst((kv->npages + 63) / 64, 0);
         for (int i = 0; i < n; i++) {
@@ -476,7 +674,8 @@ int es_hip_kv_copy_pages_dev(const es_hip_kv *kv, int nlayers, size_t layer_byte
     } catch (const std::bad_alloc &) {
         return no_memory();
     }
-    const hipError_t e = copy_pages(c.k, c.v, layer_bytes, page_bytes, nlayers, src, dst, n, static_cast<hipStream_t>(stream));
+    const Layers layers = {c.k, c.v, eight ? kv->k_scale : nullptr, eight ? kv->v_scale : nullptr, layer_bytes, page_bytes, page_scales, nlayers};
+    const hipError_t e = copy_pages(layers, src, dst, n, static_cast<hipStream_t>(stream));
     return e == hipSuccess ? ES_HIP_OK : host_hip_fail(e, "page copy launch");
 }
 
@@ -487,7 +686,8 @@ int es_hip_kv_pool_create(es_hip_kv_pool **out, uint32_t type, int nlayers, int 
     if (nlayers < 0 || max_seqs < 1 || max_pages < 1) return host_fail(ES_HIP_EINVAL, "bad number of layers, sequences or pages");
     if ((long long)max_seqs * max_pages > 1LL << 40) return host_fail(ES_HIP_EINVAL, "max_seqs * max_pages exceeds 2^40");
     es_hip_kv kv = {type, heads, dim, page, npages, reinterpret_cast<void *>(16), reinterpret_cast<void *>(16),
-                    reinterpret_cast<const int *>(16), reinterpret_cast<const int *>(16), nullptr, max_seqs, max_pages};
+                    reinterpret_cast<const int *>(16), reinterpret_cast<const int *>(16), nullptr, max_seqs, max_pages,
+                    reinterpret_cast<float *>(16), reinterpret_cast<float *>(16)};
     KvView v;
     if (int rc = kv_check(&kv, 1, v, true)) return rc;
     if (nlayers)
@@ -503,7 +703,8 @@ int es_hip_kv_pool_create(es_hip_kv_pool **out, uint32_t type, int nlayers, int 
         p->npages = npages;
         p->max_seqs = max_seqs;
         p->max_pages = max_pages;
-        p->page_bytes = (size_t)heads * page * dim * 2;
+        p->page_bytes = (size_t)heads * page * dim * (type == ES_HIP_F8 ? 1 : 2);
+        p->page_scales = type == ES_HIP_F8 ? (size_t)heads * page / 16 : 0;
         p->layer_bytes = p->page_bytes * npages;
         p->refs.assign(npages, 0);
         p->spare.resize(npages);
@@ -516,7 +717,7 @@ int es_hip_kv_pool_create(es_hip_kv_pool **out, uint32_t type, int nlayers, int 
     if (nlayers) {
         size_t all;
         hipError_t e = hipErrorOutOfMemory;
-        if (!__builtin_mul_overflow(p->layer_bytes, (size_t)nlayers * 2, &all)) e = hipMalloc(reinterpret_cast<void **>(&p->mem), all);
+        if (!__builtin_mul_overflow(p->layer_bytes + p->layer_scales() * sizeof(float), (size_t)nlayers * 2, &all)) e = hipMalloc(reinterpret_cast<void **>(&p->mem), all);
         if (e == hipSuccess) e = hipMalloc(reinterpret_cast<void **>(&p->table), (size_t)max_seqs * max_pages * sizeof(int));
         if (e == hipSuccess) e = hipMalloc(reinterpret_cast<void **>(&p->len), (size_t)max_seqs * sizeof(int));
         if (e == hipSuccess) e = hipMemset(p->len, 0, (size_t)max_seqs * sizeof(int));
@@ -541,7 +742,10 @@ void es_hip_kv_pool_destroy(es_hip_kv_pool *p) {
 int es_hip_kv_pool_view(const es_hip_kv_pool *p, int layer, es_hip_kv *out) {
     if (!p || !out || layer < 0 || layer >= p->nlayers) return host_fail(ES_HIP_EINVAL, "null pool or output, or no such layer");
     uint8_t *k = p->mem + (size_t)layer * p->layer_bytes;
-    *out = {p->type, p->heads, p->dim, p->page, p->npages, k, k + p->pool_bytes(), p->table, p->len, nullptr, p->max_seqs, p->max_pages};
+    const es_hip_kv kv = {p->type, p->heads, p->dim, p->page, p->npages, k, k + p->pool_bytes(), p->table, p->len, nullptr, p->max_seqs, p->max_pages,
+                          p->scales(layer, false), p->scales(layer, true)};
+    // (the scales' fields are written for F8 alone, as they are read)
+    memcpy(out, &kv, p->page_scales ? sizeof(kv) : offsetof(es_hip_kv, k_scale));
     return ES_HIP_OK;
 }
 

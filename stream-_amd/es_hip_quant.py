@@ -21,7 +21,7 @@ Q4_0, Q5_0, Q8_0, Q2_K, Q3_K, Q4_K, Q5_K, Q6_K = 2, 6, 8, 10, 11, 12, 13, 14
 TYPES = {"Q4_0": Q4_0, "Q5_0": Q5_0, "Q8_0": Q8_0, "Q2_K": Q2_K, "Q3_K": Q3_K, "Q4_K": Q4_K, "Q5_K": Q5_K, "Q6_K": Q6_K}
 ORDER_X86_CONTRACT, ORDER_X86_STRICT, ORDER_SCALAR = 0, 1, 2
 NOALLOC_SCRATCH_BYTES = 32 << 20   # ES_HIP_NOALLOC_SCRATCH_BYTES
-F32, F16, BF16 = 0, 1, 30          # the key-value cache's and its attention's types
+F32, F16, BF16, F8 = 0, 1, 30, 256  # the key-value cache's and its attention's types
 BLOCK_ELEMS = {Q4_0: 32, Q5_0: 32, Q8_0: 32, Q2_K: 256, Q3_K: 256, Q4_K: 256, Q5_K: 256, Q6_K: 256}
 BLOCK_BYTES = {Q4_0: 18, Q5_0: 22, Q8_0: 34, Q2_K: 84, Q3_K: 110, Q4_K: 144, Q5_K: 176, Q6_K: 210}
 ACT_BYTES = {Q4_0: 36, Q5_0: 36, Q8_0: 36, Q2_K: 292, Q3_K: 292, Q4_K: 292, Q5_K: 292, Q6_K: 292}
@@ -42,6 +42,10 @@ class Kv(C.Structure):   # es_hip_kv
     _fields_ = [("type", C.c_uint32), ("heads", C.c_int), ("dim", C.c_int), ("page", C.c_int), ("npages", C.c_int),
                 ("k", C.c_void_p), ("v", C.c_void_p), ("table", C.c_void_p), ("len", C.c_void_p), ("seq", C.c_void_p),
                 ("rows", C.c_int), ("max_pages", C.c_int)]
+
+
+class Kv8(Kv):   # the same with the fields that an F8 cache has behind them (the library reads them for that type alone)
+    _fields_ = [("k_scale", C.c_void_p), ("v_scale", C.c_void_p)]
 
 
 class Moe(C.Structure):   # es_hip_moe
@@ -223,7 +227,7 @@ class KvPool:
     """es_hip_kv_pool: sequences and pages of a paged key-value cache (nlayers = 0: bookkeeping only)"""
 
     def __init__(self, lib, t, nlayers, heads, dim, page, npages, max_seqs, max_pages):
-        self.lib, self.h = lib, None
+        self.lib, self.h, self.Kv = lib, None, Kv8 if t == F8 else Kv
         h = C.c_void_p()
         lib._check(lib._L.es_hip_kv_pool_create(C.byref(h), t, nlayers, heads, dim, page, npages, max_seqs, max_pages))
         self.h = h.value
@@ -238,7 +242,7 @@ class KvPool:
 
     def view(self, layer, seq=None) -> Kv:
         """the layer's Kv; seq: a device list of a batch's sequence numbers"""
-        kv = Kv()
+        kv = self.Kv()
         self.lib._check(self.lib._L.es_hip_kv_pool_view(self.h, layer, C.byref(kv)))
         kv.seq = None if seq is None else int(seq)
         return kv
@@ -333,6 +337,8 @@ class Lib:
             ("es_hip_attn_workspace_upto", sz, [vp, i, i, i]),
             ("es_hip_attn_decode_dev", i, [vp, i, i, u32, vp, sz, C.c_float, i, vp, sz, vp, sz, vp]),
             ("es_hip_attn_prompt_dev", i, [vp, i, vp, i, i, u32, vp, sz, C.c_float, i, vp, sz, vp, sz, vp]),
+            ("es_hip_attn_decode_sinks_dev", i, [vp, i, i, u32, vp, sz, C.c_float, i, i, vp, sz, vp, sz, vp]),
+            ("es_hip_attn_prompt_sinks_dev", i, [vp, i, vp, i, i, u32, vp, sz, C.c_float, i, i, vp, sz, vp, sz, vp]),
             ("es_hip_kv_copy_pages_dev", i, [vp, i, sz, vp, vp, i, vp]),
             ("es_hip_kv_pool_create", i, [vp, u32, i, i, i, i, i, i, i]), ("es_hip_kv_pool_destroy", None, [vp]),
             ("es_hip_kv_pool_view", i, [vp, i, vp]), ("es_hip_kv_pool_free_pages", i, [vp]),
@@ -574,6 +580,15 @@ class Lib:
     def attn_prompt_dev(self, kv, nseq, start, ntok, heads, t, q, qstride, scale, window, out, ostride, ws, ws_bytes, stream=None):
         self._check(self._L.es_hip_attn_prompt_dev(C.byref(kv), nseq, self._ptr(start), ntok, heads, t, self._ptr(q), qstride,
                                                    scale, window, self._ptr(out), ostride, self._ptr(ws), ws_bytes, stream))
+
+    def attn_decode_sinks_dev(self, kv, nseq, heads, t, q, qstride, scale, window, sinks, out, ostride, ws, ws_bytes, stream=None):
+        self._check(self._L.es_hip_attn_decode_sinks_dev(C.byref(kv), nseq, heads, t, self._ptr(q), qstride, scale, window, sinks,
+                                                         self._ptr(out), ostride, self._ptr(ws), ws_bytes, stream))
+
+    def attn_prompt_sinks_dev(self, kv, nseq, start, ntok, heads, t, q, qstride, scale, window, sinks, out, ostride, ws, ws_bytes,
+                              stream=None):
+        self._check(self._L.es_hip_attn_prompt_sinks_dev(C.byref(kv), nseq, self._ptr(start), ntok, heads, t, self._ptr(q), qstride,
+                                                         scale, window, sinks, self._ptr(out), ostride, self._ptr(ws), ws_bytes, stream))
 
     def kv_copy_pages_dev(self, kv, nlayers, layer_bytes, src, dst, stream=None):
         """src, dst: page numbers on the host"""
