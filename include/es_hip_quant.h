@@ -489,7 +489,7 @@ int es_hip_kv_append_dev(const es_hip_kv *kv, int nseq, const int *start, int nt
 /* Attention of one new token per sequence, the last in its cache (append it first):
  *   out[b][h] = sum over j of p[j] * v[j],  p = softmax over j of scale * (q[b][h] . k[j]),  len - window <= j < len
  * (window 0: all), with head h reading K/V head h / (heads / kv->heads). heads: a multiple of kv->heads. type: q's and out's,
- * ES_HIP_F32 (with any cache) or the cache's own (an F8 cache's: ES_HIP_BF16); head h of sequence b at q + b * qstride + h * dim elements (0: packed), the
+ * ES_HIP_F32 (with any cache) or the cache's own (an F8 cache's: F16 or BF16); head h of sequence b at q + b * qstride + h * dim elements (0: packed), the
  * same for out; aligned to their type. scale is positive and finite. A sequence without tokens gets zeros. Tokens that
  * a query does not see have no influence, whatever their rows hold; an infinity or NaN that it sees in V comes out as an infinity
  * or NaN in that element. fp32 q is carried to 22 bits or more through the matrix products, as are the weights p; with a 16-bit q,

@@ -89,7 +89,7 @@ struct AttnArgs {
 
 // the kernels of caches in 8 bits, and of 16-bit caches with sinks (es_hip_attn_f8.hip, es_hip_attn_sinks.hip)
 using AttnKernel = void (*)(AttnArgs);
-AttnKernel attn_f8_kernel(bool prompt, bool fp32, int dim, bool sinks);
+AttnKernel attn_f8_kernel(bool prompt, uint32_t type, int dim, bool sinks);   // type: of the queries
 AttnKernel attn_sinks_kernel(bool prompt, bool bf16, bool fp32, int dim);
 
 }  // namespace esq

@@ -25,7 +25,7 @@ struct Shape {
 Shape shape_of(const es_hip_kv *kv, int nseq, int ntok, int heads, uint32_t type, bool prompt) {
     const int G = heads / kv->heads;
     const long long most = (long long)kv->max_pages * kv->page;
-    const int nq = type != ES_HIP_F32 ? 1 : kv->type == ES_HIP_F16 ? 2 : 3;
+    const int nq = type != ES_HIP_F32 ? 1 : kv->type == ES_HIP_BF16 ? 3 : 2;
     Shape s{};
     if (prompt) {
         const int per_cu = prompt_per_cu(nq, kv->dim);
@@ -58,11 +58,9 @@ int check_heads(const es_hip_kv *kv, int nseq, int ntok, int heads, KvView &v) {
     return ES_HIP_OK;
 }
 
-// the 16-bit type that queries and outputs may have
-uint32_t query_type(const es_hip_kv *kv) { return kv->type == ES_HIP_F8 ? (uint32_t)ES_HIP_BF16 : kv->type; }
 int check_type(const es_hip_kv *kv, uint32_t type) {
-    return type == ES_HIP_F32 || type == query_type(kv) ? ES_HIP_OK
-                                                         : host_fail(ES_HIP_EINVAL, "q and out are F32 or of the cache's type (an F8 cache: BF16)");
+    const bool fits = kv->type == ES_HIP_F8 ? type == ES_HIP_F16 || type == ES_HIP_BF16 : type == kv->type;
+    return type == ES_HIP_F32 || fits ? ES_HIP_OK : host_fail(ES_HIP_EINVAL, "q and out are F32 or of the cache's type (an F8 cache: F32, F16 or BF16)");
 }
 
 template <bool BF, int NQ> AttnKernel kernel_of(bool prompt, int dim) {
@@ -129,12 +127,12 @@ int attention(const es_hip_kv *kv, int nseq, const int *start, int ntok, int hea
     a.block = s.block;
     a.items = (int)s.items;
     const hipStream_t st = static_cast<hipStream_t>(stream);
-    const bool f32 = type == ES_HIP_F32, bf = kv->type != ES_HIP_F16;
-    const AttnKernel f = kv->type == ES_HIP_F8 ? attn_f8_kernel(prompt, f32, kv->dim, a.sinks > 0)
+    const bool f32 = type == ES_HIP_F32, bf = kv->type == ES_HIP_BF16;
+    const AttnKernel f = kv->type == ES_HIP_F8 ? attn_f8_kernel(prompt, type, kv->dim, a.sinks > 0)
                          : a.sinks             ? attn_sinks_kernel(prompt, bf, f32, kv->dim)
                          : bf                  ? (f32 ? kernel_of<true, 3>(prompt, kv->dim) : kernel_of<true, 1>(prompt, kv->dim))
                                                : (f32 ? kernel_of<false, 2>(prompt, kv->dim) : kernel_of<false, 1>(prompt, kv->dim));
-    const hipError_t e = f32 ? launch<true, true>(f, a, s, prompt, st) : bf ? launch<false, true>(f, a, s, prompt, st) : launch<false, false>(f, a, s, prompt, st);
+    const hipError_t e = f32 ? launch<true, true>(f, a, s, prompt, st) : type == ES_HIP_BF16 ? launch<false, true>(f, a, s, prompt, st) : launch<false, false>(f, a, s, prompt, st);
     return e == hipSuccess ? ES_HIP_OK : host_hip_fail(e, "attention launch");
 }
 
@@ -145,7 +143,7 @@ extern "C" {
 size_t es_hip_attn_decode_workspace(const es_hip_kv *kv, int nseq, int heads) {
     KvView v;
     if (check_heads(kv, nseq, nseq, heads, v) || !nseq) return 0;
-    return shape_of(kv, nseq, nseq, heads, query_type(kv), false).workspace(kv);   // (fp32 queries need as much, or less)
+    return shape_of(kv, nseq, nseq, heads, kv->type, false).workspace(kv);   // (fp32 queries need as much, or less)
 }
 
 size_t es_hip_attn_prompt_workspace(const es_hip_kv *kv, int nseq, int ntok, int heads, uint32_t type) {
@@ -157,8 +155,8 @@ size_t es_hip_attn_prompt_workspace(const es_hip_kv *kv, int nseq, int ntok, int
 size_t es_hip_attn_workspace_upto(const es_hip_kv *kv, int nseq, int ntok, int heads) {
     KvView v;
     if (check_heads(kv, nseq, ntok, heads, v) || !nseq) return 0;
-    size_t most = shape_of(kv, nseq, nseq, heads, query_type(kv), false).workspace(kv);   // (decode: never less for more sequences)
-    for (uint32_t type : {(uint32_t)ES_HIP_F32, query_type(kv)}) {
+    size_t most = shape_of(kv, nseq, nseq, heads, kv->type, false).workspace(kv);   // (decode: never less for more sequences)
+    for (uint32_t type : {(uint32_t)ES_HIP_F32, kv->type}) {
         // a prompt's slots are its tiles plus the parts aimed for, as long as the tiles are fewer than those
         Shape s = shape_of(kv, 1, 1, heads, type, true);
         const size_t tiles = shape_of(kv, nseq, ntok, heads, type, true).tiles;

@@ -257,6 +257,21 @@ template <bool BF, int NQ, int BY, int NP> __device__ void split_weights(const f
     }
 }
 
+// fp32 weights as three bf16 terms, exactly: 24 bits cut off 8 at a time
+__device__ void split_whole(const float (&x)[8], u4 (&y)[3]) {
+#pragma unroll
+    for (int i = 0; i < 8; i += 2) {
+        float r[2] = {x[i], x[i + 1]};
+#pragma unroll
+        for (int t = 0; t < 3; t++) {
+            const uint32_t a = __float_as_uint(r[0]), b = __float_as_uint(r[1]);
+            y[t][i / 2] = __builtin_amdgcn_perm(b, a, 0x07060302u);
+            r[0] -= __uint_as_float(a & 0xffff0000u);
+            r[1] -= __uint_as_float(b & 0xffff0000u);
+        }
+    }
+}
+
 // Eight elements of a query row, from d on (zeros past dim): fp32 or 16 bits.
 __device__ void load8(const uint8_t *row, int d, int dim, float (&x)[8]) {
     struct __attribute__((packed, aligned(4))) F8 { float x[8]; };
@@ -384,12 +399,13 @@ template <bool ONCE> struct Run {   // ONCE: past the caches
     }
 };
 
-// numbers of 8 bits, times a power of two, as bf16: exact
-template <bool UPPER> __device__ uint32_t two_of(uint32_t x, float scale) {
-    return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(x, scale, UPPER));
+// numbers of 8 bits, times a power of two, as bf16 (or, times 1, as fp16): exact
+template <bool BF, bool UPPER> __device__ uint32_t two_of(uint32_t x, float scale) {
+    if constexpr (BF) return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(x, scale, UPPER));
+    else return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(x, 1.0f, UPPER));
 }
-__device__ u4 eight_of(uint32_t x, uint32_t y, float scale) {
-    return u4{two_of<false>(x, scale), two_of<true>(x, scale), two_of<false>(y, scale), two_of<true>(y, scale)};
+template <bool BF> __device__ u4 eight_of(uint32_t x, uint32_t y, float scale) {
+    return u4{two_of<BF, false>(x, scale), two_of<BF, true>(x, scale), two_of<BF, false>(y, scale), two_of<BF, true>(y, scale)};
 }
 
 // two rows' elements j of 2 packed elements, as a pair
@@ -463,10 +479,12 @@ struct Deal {
 
 template <bool BF, int NQ, int DP, bool E8 = false, bool SINKS = false>
 __global__ __launch_bounds__(256, DP == 64 && NQ < 3 ? 3 : decode_per_cu(DP)) void attn_decode_kernel(AttnArgs a) {
-    static_assert(BF || !E8);
     constexpr int KS = DP / 32, DL = DP / 16, BM = DECODE_M;
+    constexpr bool UNSCALED = E8 && !BF;     // K goes into the product without its scales, which the scores take
+    constexpr bool WBF = BF || E8;           // weights and V are bf16
     constexpr int ES = E8 ? 1 : 2;           // bytes of an element
-    constexpr int NP = NQ == 1 ? 2 : NQ;   // terms of the weights
+    constexpr int AHEAD = E8 ? 2 : 1;        // steps of keys on their way
+    constexpr int NP = NQ == 1 ? 2 : E8 ? 3 : NQ;   // terms of the weights
     constexpr bool F32 = NQ > 1;
     __shared__ float lm[4][BM], ll[4][BM];
     __shared__ __attribute__((aligned(16))) float lo_acc[4][BM][DP + 4];
@@ -513,60 +531,58 @@ __global__ __launch_bounds__(256, DP == 64 && NQ < 3 ? 3 : decode_per_cu(DP)) vo
         };
         Runs<E8> pg = fetch(0), pgn = fetch(32);
         u4 q[KS][NQ];
-        const float cs = load_query<BF, NQ, KS, 32, 16, E8>(a.q + (size_t)seq * a.qstride + (size_t)(head * a.G + r) * dim * (F32 ? 4 : 2),
+        const float q_scale = load_query<BF, NQ, KS, 32, 16, E8>(a.q + (size_t)seq * a.qstride + (size_t)(head * a.G + r) * dim * (F32 ? 4 : 2),
                                                         r < rows, g, dim, a.c2, q);
         // A lane's 16 bytes of an 8-bit row are the elements that its group has of two steps.
         const int kd = (col * dim + g * (16 / ES)) * ES, vd = (g * 4 * dim + col * DL) * ES;
-        u4 kr[2][KS * ES / 2];         // run h, elements s * 32 + g * 8 of key col (8 bits: s * 64 + g * 16)
-        uint32_t vr[8][DL * ES / 4];   // DL elements of the keys g * 4 + i (first four) and 16 + g * 4 + i
-        float ks[2], vs[2];            // the runs' scales
+        u4 kr[AHEAD][2][KS * ES / 2];         // run h, elements s * 32 + g * 8 of key col (8 bits: s * 64 + g * 16)
+        uint32_t vr[AHEAD][8][DL * ES / 4];   // DL elements of the keys g * 4 + i (first four) and 16 + g * 4 + i
+        float ks[AHEAD][2], vs[AHEAD][2];     // the runs' scales
+        bool ok[AHEAD][2];                    // the runs are in pages
         auto run = [&](const uint8_t *pool, int n, int h) {
             return Run<true>(pool, pg, (n & 31) * 2 + h, min(last - (first + (n * 4 + wave) * 32 + h * 16), 16) * dim * ES);
         };
-        auto load_k = [&](int n) {
+        auto load_k = [&](auto at, int n) {
+            constexpr int A = decltype(at)::value;
 #pragma unroll
             for (int h = 0; h < 2; h++) {
                 const Run<true> r = run(a.c.k, n, h);
-                if constexpr (E8) ks[h] = pg.k_scale((n & 31) * 2 + h);
+                ok[A][h] = !pg.none((n & 31) * 2 + h);
+                if constexpr (E8) ks[A][h] = pg.k_scale((n & 31) * 2 + h);
 #pragma unroll
-                for (int s = 0; s < KS * ES / 2; s++) kr[h][s] = r.load16(kd + s * 64, 0);
+                for (int s = 0; s < KS * ES / 2; s++) kr[A][h][s] = r.load16(kd + s * 64, 0);
             }
         };
-        auto load_v = [&](int n) {
+        auto load_v = [&](auto at, int n) {
+            constexpr int A = decltype(at)::value;
 #pragma unroll
             for (int h = 0; h < 2; h++) {
                 const Run<true> r = run(a.c.v, n, h);
-                if constexpr (E8) vs[h] = pg.v_scale((n & 31) * 2 + h);
+                if constexpr (E8) vs[A][h] = pg.v_scale((n & 31) * 2 + h);
 #pragma unroll
                 for (int i = 0; i < 4; i++) {   // (elements past dim: others' in their place, in sums that are not written)
                     if constexpr (DL * ES == 4) {
-                        vr[h * 4 + i][0] = r.load4(vd, i * dim * ES);
+                        vr[A][h * 4 + i][0] = r.load4(vd, i * dim * ES);
                     } else if constexpr (DL * ES == 8) {
                         const u2 y = r.load8(vd, i * dim * ES);
-                        vr[h * 4 + i][0] = y[0];
-                        vr[h * 4 + i][1] = y[1];
+                        vr[A][h * 4 + i][0] = y[0];
+                        vr[A][h * 4 + i][1] = y[1];
                     } else {
 #pragma unroll
                         for (int w = 0; w < DL * ES / 4; w += 4) {
                             const u4 y = r.load16(vd + w * 4, i * dim * ES);
 #pragma unroll
-                            for (int k = 0; k < 4; k++) vr[h * 4 + i][w + k] = y[k];
+                            for (int k = 0; k < 4; k++) vr[A][h * 4 + i][w + k] = y[k];
                         }
                     }
                 }
             }
         };
-        // The next step's K is loaded once this one's scores are there and its V once this one's is summed, into the same
+        // The K of the step AHEAD is loaded once this one's scores are there and its V once this one's is summed, into the same
         // registers.
         const int mine = first + wave * 32, steps = mine < last ? (last - mine + 127) / 128 : 0;
-        bool ok[2] = {false, false};
-        if (steps > 0) {
-            ok[0] = !pg.none(0);
-            ok[1] = !pg.none(1);
-            load_k(0);
-            load_v(0);
-        }
-        for (int n = 0; n < steps; n++) {
+        auto step = [&](auto at, int n) {
+            constexpr int A = decltype(at)::value;
             const int t0 = mine + n * 128;
             f4 s[2];
             if (dim < DP) {   // elements past dim: zeros, which the query's zeros keep
@@ -574,15 +590,15 @@ __global__ __launch_bounds__(256, DP == 64 && NQ < 3 ? 3 : decode_per_cu(DP)) vo
                 for (int h = 0; h < 2; h++)
 #pragma unroll
                     for (int k = 0; k < KS * ES / 2; k++)
-                        if ((k * 64 + g * 16) / ES >= dim) kr[h][k] = u4{0, 0, 0, 0};
+                        if ((k * 64 + g * 16) / ES >= dim) kr[A][h][k] = u4{0, 0, 0, 0};
             }
             u4 kf[2][KS];
 #pragma unroll
             for (int h = 0; h < 2; h++)
 #pragma unroll
                 for (int k = 0; k < KS; k++) {
-                    if constexpr (E8) kf[h][k] = eight_of(kr[h][k / 2][k % 2 * 2], kr[h][k / 2][k % 2 * 2 + 1], ks[h]);
-                    else kf[h][k] = kr[h][k];
+                    if constexpr (E8) kf[h][k] = eight_of<BF>(kr[A][h][k / 2][k % 2 * 2], kr[A][h][k / 2][k % 2 * 2 + 1], ks[A][h]);
+                    else kf[h][k] = kr[A][h][k];
                 }
             // A sum for each term, the smallest added first: the matrix cores round a sum after every 8 products, which loses small terms'
             // next to a large one's one by one. fp32 over fp16, error against 64 bits, so and with all terms in one sum: 500 keys of 64
@@ -599,15 +615,18 @@ __global__ __launch_bounds__(256, DP == 64 && NQ < 3 ? 3 : decode_per_cu(DP)) vo
 #pragma unroll
                     for (int i = 0; i < 4; i++) s[h][i] = t == NQ - 1 ? part[h][i] : s[h][i] + part[h][i];
             }
-            const bool ok0 = ok[0], ok1 = ok[1], more = n + 1 < steps;
+            float cs[2] = {q_scale, q_scale};   // what the runs' scores are multiplied by
+            if constexpr (UNSCALED) {
+                cs[0] *= ks[A][0];
+                cs[1] *= ks[A][1];
+            }
+            const bool ok0 = ok[A][0], ok1 = ok[A][1], more = n + AHEAD < steps;
             if (more) {
-                if (((n + 1) & 31) == 0) {
+                if (((n + AHEAD) & 31) == 0) {
                     pg = pgn;
-                    pgn = fetch(n + 33);
+                    pgn = fetch(n + AHEAD + 32);
                 }
-                ok[0] = !pg.none((n + 1 & 31) * 2);
-                ok[1] = !pg.none((n + 1 & 31) * 2 + 1);
-                load_k(n + 1);
+                load_k(at, n + AHEAD);
             }
             const int sinks = SINKS ? a.sinks : 0;
             if ((t0 < lo && t0 + 32 > sinks) || t0 + 32 > last || !ok0 || !ok1) {   // what is not to be seen: no score, and zeros for whatever V holds
@@ -618,14 +637,19 @@ __global__ __launch_bounds__(256, DP == 64 && NQ < 3 ? 3 : decode_per_cu(DP)) vo
                     if (before || t >= last || !(i < 4 ? ok0 : ok1)) s[i >> 2][i & 3] = LOWEST;
                     if (before) {
 #pragma unroll
-                        for (int w = 0; w < DL * ES / 4; w++) vr[i][w] = 0;
+                        for (int w = 0; w < DL * ES / 4; w++) vr[A][i][w] = 0;
                     }
                 }
             }
             float big = LOWEST;
+            if constexpr (UNSCALED) {
+                big = fmaxf(fmaxf(fmaxf(s[0][0], s[0][1]), fmaxf(s[0][2], s[0][3])) * cs[0], fmaxf(fmaxf(s[1][0], s[1][1]), fmaxf(s[1][2], s[1][3])) * cs[1]);
+                big = with_lane<32>(with_lane<16>(big, Max()), Max());
+            } else {
 #pragma unroll
-            for (int i = 0; i < 8; i++) big = fmaxf(big, s[i >> 2][i & 3]);
-            big = with_lane<32>(with_lane<16>(big, Max()), Max()) * cs;
+                for (int i = 0; i < 8; i++) big = fmaxf(big, s[i >> 2][i & 3]);
+                big = with_lane<32>(with_lane<16>(big, Max()), Max()) * q_scale;
+            }
             if (__any(big > m)) {
                 const float now = fmaxf(m, big), f = __builtin_amdgcn_exp2f(m - reference(now));
                 m = now;
@@ -639,34 +663,49 @@ __global__ __launch_bounds__(256, DP == 64 && NQ < 3 ? 3 : decode_per_cu(DP)) vo
             float w8[8];
 #pragma unroll
             for (int i = 0; i < 8; i++) {
-                w8[i] = weight<NQ, SHIFT<BF>>(s[i >> 2][i & 3], cs, ref);
+                w8[i] = weight<NQ, SHIFT<WBF>>(s[i >> 2][i & 3], cs[i >> 2], ref);
                 l += w8[i];
             }
             u4 pt[NP];
-            split_weights<BF, NQ, SHIFT<BF>>(w8, pt);
+            if constexpr (NP == 3 && E8) split_whole(w8, pt);
+            else split_weights<WBF, NQ, SHIFT<WBF>>(w8, pt);
 #pragma unroll
             for (int j = 0; j < DL; j += 2) {
                 u4 v0, v1;
 #pragma unroll
                 for (int k = 0; k < 4; k++) {
                     if constexpr (E8) {   // two keys' elements j and j + 1 in a word, key by key
-                        const uint32_t x = __builtin_amdgcn_perm(vr[2 * k + 1][j / 4], vr[2 * k][j / 4], j & 2 ? 0x07030602u : 0x05010400u);
-                        v0[k] = two_of<false>(x, vs[k / 2]);
-                        v1[k] = two_of<true>(x, vs[k / 2]);
+                        const uint32_t x = __builtin_amdgcn_perm(vr[A][2 * k + 1][j / 4], vr[A][2 * k][j / 4], j & 2 ? 0x07030602u : 0x05010400u);
+                        v0[k] = two_of<true, false>(x, vs[A][k / 2]);
+                        v1[k] = two_of<true, true>(x, vs[A][k / 2]);
                     } else {
-                        v0[k] = pair<0>(vr[2 * k][j / 2], vr[2 * k + 1][j / 2]);
-                        v1[k] = pair<1>(vr[2 * k][j / 2], vr[2 * k + 1][j / 2]);
+                        v0[k] = pair<0>(vr[A][2 * k][j / 2], vr[A][2 * k + 1][j / 2]);
+                        v1[k] = pair<1>(vr[A][2 * k][j / 2], vr[A][2 * k + 1][j / 2]);
                     }
                 }
 #pragma unroll
                 for (int t = 0; t < NP; t++) {
-                    acc[j] = mfma16<BF>(v0, pt[t], acc[j]);
-                    acc[j + 1] = mfma16<BF>(v1, pt[t], acc[j + 1]);
+                    acc[j] = mfma16<WBF>(v0, pt[t], acc[j]);
+                    acc[j + 1] = mfma16<WBF>(v1, pt[t], acc[j + 1]);
                 }
             }
-            if (more) load_v(n + 1);
+            if (more) load_v(at, n + AHEAD);
+        };
+        using First = std::integral_constant<int, 0>;
+        using Second = std::integral_constant<int, AHEAD - 1>;
+        if (steps > 0) {
+            load_k(First(), 0);
+            load_v(First(), 0);
         }
-        l = weights_sum<NQ, SHIFT<BF>>(with_lane<32>(with_lane<16>(l, Sum()), Sum()));
+        if (AHEAD > 1 && steps > 1) {
+            load_k(Second(), 1);
+            load_v(Second(), 1);
+        }
+        for (int n = 0; n < steps; n += AHEAD) {
+            step(First(), n);
+            if (AHEAD > 1 && n + 1 < steps) step(Second(), n + 1);
+        }
+        l = weights_sum<NQ, SHIFT<WBF>>(with_lane<32>(with_lane<16>(l, Sum()), Sum()));
 
         // the four waves' m, l and sums; lane (g, col) holds elements (g * 4 + i) * DL + j of head col
         if (g == 0) {
@@ -812,7 +851,7 @@ __device__ u2 transposed(uint32_t lds) {
 
 template <bool BF, int NQ, int DP, bool E8 = false, bool SINKS = false>
 __global__ __launch_bounds__(256, prompt_per_cu(NQ, DP)) void attn_prompt_kernel(AttnArgs a) {
-    static_assert(BF || !E8);
+    constexpr bool UNSCALED = E8 && !BF;                     // (see below)
     constexpr int NB = DP == 64 && !E8 ? 3 : 2;              // steps of keys in LDS
     constexpr int ES = E8 ? 1 : 2;                           // bytes of an element in the pools
     constexpr int KS = DP / 16, DT = DP / 32, CH = DP / 8;   // CH: pieces of a key
@@ -823,6 +862,8 @@ __global__ __launch_bounds__(256, prompt_per_cu(NQ, DP)) void attn_prompt_kernel
     constexpr int BY = SHIFT<BF> - LAG<BF, NQ>;              // weights are 2^BY p
     __shared__ __attribute__((aligned(1024))) uint8_t lds[2 * NB * TILE];   // K of NB steps, V of them
     __shared__ int odd;                                      // elements of V were left out
+    // UNSCALED: of each step's four runs the scales of K and of V, and the exponents of the latter
+    __shared__ f4 run_ks[UNSCALED ? NB : 1], run_vs[UNSCALED ? NB : 1], run_ve[UNSCALED ? NB : 1];
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int col = lane & 31, half = lane >> 5;
     const int head = blockIdx.x % a.c.heads, item = blockIdx.x / a.c.heads;
@@ -872,6 +913,11 @@ __global__ __launch_bounds__(256, prompt_per_cu(NQ, DP)) void attn_prompt_kernel
 #pragma unroll
         for (int i = 0; i < 16; i++) acc[j][i] = 0.0f;
     float m = LOWEST, l = 0.0f;
+    // UNSCALED: K and V go into the products as the numbers are, in fp16, which takes fp32 queries in two terms, not bf16's three (16384
+    // scores' worth of them in 2/3 of the matrix cores' time). K's scales are factors of the scores. V's are factors of the weights, and as fp16
+    // has not the range for both, the sums have a reference of their own: m2, the maximum of score plus exponent of the run's scale, which
+    // keeps the bits of what weighs most in a row's sum, whatever the scales. by_scale is 2^(BY + m - m2).
+    float m2 = LOWEST, by_scale = 1 << (BY & 31);
 
     // where 64 runs of 16 keys from run `pb` on begin, one per lane, and the 64 after them
     auto fetch = [&](int u) { return Runs<E8>(a.c, table, head, at_key(u * 16) >> 4, u * 16 < last); };
@@ -931,11 +977,16 @@ __global__ __launch_bounds__(256, prompt_per_cu(NQ, DP)) void attn_prompt_kernel
         for (int n = 0; n < R8; n++) {
             const int t = n * ROWS8 + lane / CH8, c = lane % CH8 * 2;
             uint8_t *key = lds + buf * TILE + (wave * 16 + t) * DP * 2;
-            *reinterpret_cast<u4 *>(key + (c ^ k_turn<DP>(t)) * 16) = eight_of(k8[n][0], k8[n][1], ks);
-            *reinterpret_cast<u4 *>(key + (c + 1 ^ k_turn<DP>(t)) * 16) = eight_of(k8[n][2], k8[n][3], ks);
+            *reinterpret_cast<u4 *>(key + (c ^ k_turn<DP>(t)) * 16) = eight_of<BF>(k8[n][0], k8[n][1], ks);
+            *reinterpret_cast<u4 *>(key + (c + 1 ^ k_turn<DP>(t)) * 16) = eight_of<BF>(k8[n][2], k8[n][3], ks);
             key += NB * TILE;
-            *reinterpret_cast<u4 *>(key + (c ^ v_turn<DP>(t)) * 16) = eight_of(v8[n][0], v8[n][1], vs);
-            *reinterpret_cast<u4 *>(key + (c + 1 ^ v_turn<DP>(t)) * 16) = eight_of(v8[n][2], v8[n][3], vs);
+            *reinterpret_cast<u4 *>(key + (c ^ v_turn<DP>(t)) * 16) = eight_of<BF>(v8[n][0], v8[n][1], vs);
+            *reinterpret_cast<u4 *>(key + (c + 1 ^ v_turn<DP>(t)) * 16) = eight_of<BF>(v8[n][2], v8[n][3], vs);
+        }
+        if (UNSCALED && lane == 0) {
+            run_ks[buf][wave] = ks;
+            run_vs[buf][wave] = vs;
+            run_ve[buf][wave] = (float)((int)(__float_as_uint(vs) >> 23 & 255) - 127);
         }
     };
     // V of the step from t0 on, where some row does not see all of its keys: zeros for what none sees or must not be multiplied
@@ -1059,32 +1110,75 @@ __global__ __launch_bounds__(256, prompt_per_cu(NQ, DP)) void attn_prompt_kernel
                     for (int i = 0; i < 16; i++)
                         if (holes >> (h * 2 + i / 8) & 1) s[h][i] = LOWEST;
             }
-            float big = LOWEST;
-#pragma unroll
-            for (int h = 0; h < 2; h++)
-#pragma unroll
-                for (int i = 0; i < 16; i++) big = fmaxf(big, s[h][i]);
-            big = with_lane<32>(big, Max()) * cs;
-            if (__any(big > m + LAG<BF, NQ>)) {
-                const float now = fmaxf(m, big), f = __builtin_amdgcn_exp2f(m - reference(now));
-                m = now;
-                l *= f;
-#pragma unroll
-                for (int j = 0; j < DT; j++)
-#pragma unroll
-                    for (int i = 0; i < 16; i++) acc[j][i] *= f;
-            }
-            const float ref = reference(m);
             u4 pt[4][NQ];
+            if constexpr (UNSCALED) {
+                const f4 k4 = run_ks[buf], v4 = run_vs[buf], e4 = run_ve[buf];
+                float big = LOWEST, big2 = LOWEST, csr[4];
 #pragma unroll
-            for (int u = 0; u < 4; u++) {
-                float w8[8];
+                for (int u = 0; u < 4; u++) {
+                    float x = LOWEST;
 #pragma unroll
-                for (int i = 0; i < 8; i++) {
-                    w8[i] = weight<NQ, BY>(s[u >> 1][(u & 1) * 8 + i], cs, ref);
-                    l += w8[i];
+                    for (int i = 0; i < 8; i++) x = fmaxf(x, s[u >> 1][(u & 1) * 8 + i]);
+                    csr[u] = cs * k4[u];
+                    x *= csr[u];
+                    big = fmaxf(big, x);
+                    big2 = fmaxf(big2, x + e4[u]);
                 }
-                split_weights<BF, NQ, BY>(w8, pt[u]);
+                big = with_lane<32>(big, Max());
+                big2 = with_lane<32>(big2, Max());
+                if (__any(big > m + LAG<BF, NQ> || big2 > m2 + LAG<BF, NQ>)) {
+                    const float now = fmaxf(m, big), now2 = fmaxf(m2, big2), f = __builtin_amdgcn_exp2f(m2 - reference(now2));
+                    l *= __builtin_amdgcn_exp2f(m - reference(now));
+                    m = now;
+                    m2 = now2;
+                    by_scale = __builtin_amdgcn_exp2f(BY + (reference(m) - reference(m2)));
+#pragma unroll
+                    for (int j = 0; j < DT; j++)
+#pragma unroll
+                        for (int i = 0; i < 16; i++) acc[j][i] *= f;
+                }
+                const float ref = reference(m);
+#pragma unroll
+                for (int u = 0; u < 4; u++) {
+                    const float by = fminf(by_scale * v4[u], 0x1p126f);   // (a weight that this is too little for has underflowed)
+                    h8 v, w;
+#pragma unroll
+                    for (int i = 0; i < 8; i++) {
+                        const float x = __builtin_amdgcn_exp2f(__builtin_fmaf(s[u >> 1][(u & 1) * 8 + i], csr[u], -ref));
+                        l += x;
+                        v[i] = static_cast<_Float16>(__builtin_fmaf(x, by, 0.0f));
+                        if constexpr (NQ == 2) w[i] = static_cast<_Float16>(__builtin_fmaf(x, by, -static_cast<float>(v[i])));
+                    }
+                    pt[u][0] = __builtin_bit_cast(u4, v);
+                    if constexpr (NQ == 2) pt[u][1] = __builtin_bit_cast(u4, w);
+                }
+            } else {
+                float big = LOWEST;
+#pragma unroll
+                for (int h = 0; h < 2; h++)
+#pragma unroll
+                    for (int i = 0; i < 16; i++) big = fmaxf(big, s[h][i]);
+                big = with_lane<32>(big, Max()) * cs;
+                if (__any(big > m + LAG<BF, NQ>)) {
+                    const float now = fmaxf(m, big), f = __builtin_amdgcn_exp2f(m - reference(now));
+                    m = now;
+                    l *= f;
+#pragma unroll
+                    for (int j = 0; j < DT; j++)
+#pragma unroll
+                        for (int i = 0; i < 16; i++) acc[j][i] *= f;
+                }
+                const float ref = reference(m);
+#pragma unroll
+                for (int u = 0; u < 4; u++) {
+                    float w8[8];
+#pragma unroll
+                    for (int i = 0; i < 8; i++) {
+                        w8[i] = weight<NQ, BY>(s[u >> 1][(u & 1) * 8 + i], cs, ref);
+                        l += w8[i];
+                    }
+                    split_weights<BF, NQ, BY>(w8, pt[u]);
+                }
             }
 #pragma unroll
             for (int u = 0; u < 4; u++)
@@ -1111,7 +1205,8 @@ __global__ __launch_bounds__(256, prompt_per_cu(NQ, DP)) void attn_prompt_kernel
         if constexpr (E8) __syncthreads();
         else arrived(!more);
     }
-    l = weights_sum<NQ, BY>(with_lane<32>(l, Sum()));
+    l = with_lane<32>(l, Sum());
+    if constexpr (!UNSCALED) l = weights_sum<NQ, BY>(l);
 
     if (wave * 32 + col >= rows) return;
     // acc[j][i] is element j * 32 + i / 4 * 8 + half * 4 + i % 4
@@ -1123,7 +1218,7 @@ __global__ __launch_bounds__(256, prompt_per_cu(NQ, DP)) void attn_prompt_kernel
             if (page < 0 || page >= a.c.npages) continue;
             const size_t at = a.c.row_at(page, head, t & ((1 << a.c.shift) - 1));
             const uint8_t *row = a.c.v + at * dim * ES;
-            const float scale = E8 ? a.c.vs[at >> 4] : 1.0f;
+            const float scale = E8 && !UNSCALED ? a.c.vs[at >> 4] : 1.0f;
             int lane_d = half * 4;
             asm volatile("" : "+v"(lane_d));   // (or what depends on it is computed ahead of the loop, for all elements)
 #pragma unroll
@@ -1143,7 +1238,8 @@ __global__ __launch_bounds__(256, prompt_per_cu(NQ, DP)) void attn_prompt_kernel
     }
     const bool done = p.chunks == 1;
     const size_t at = ((size_t)item * a.c.heads + head) * PM + wave * 32 + col;
-    const float inv = !done ? 1.0f : l == 0.0f ? 0.0f : 1.0f / l;
+    float inv = !done ? 1.0f : l == 0.0f ? 0.0f : 1.0f / l;
+    if constexpr (UNSCALED) inv *= __builtin_amdgcn_exp2f(reference(m2) - reference(m) - BY);   // the sums relative to m
     if (!done && half == 0) a.pml[at] = float2{m, l};
     uint8_t *row = a.out + (size_t)(p.s.t0 + query) * a.ostride + qoff;
 #pragma unroll

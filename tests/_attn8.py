@@ -42,7 +42,7 @@ def exponent_for(x):
 class Cache8:
     """pools filled with what must not be read (NaN codes, infinite scales), a page table, lengths"""
 
-    t = E.BF16   # what queries of 16 bits are, and the matrix products (for _attn.tolerance)
+    t = E.BF16   # the type of a prompt's weights, that of its queries if that is of 16 bits (for _attn.tolerance)
 
     def __init__(self, heads, dim, page, lens, rng, spare=3, max_pages=None):
         self.heads, self.dim, self.page = heads, dim, page

@@ -25,11 +25,11 @@ for n, b in dict(ks=dict(k_scale=None), vs=dict(v_scale=None), align=dict(v_scal
     if L.attn_decode_workspace(k, 3, 32) or L.attn_prompt_workspace(k, 3, 9, 32, E.F32) or L.attn_workspace_upto(k, 3, 9, 32): out["workspace " + n] = 0
 k = kv8()
 out.update({"a type": ap(k, t=E.F8), "a type2": ap(k, t=2), "a many": ap(k, start=P, ntok=(1 << 31) - 1), "a manyseq": ap(kv8(seq=4096), nseq=1 << 26, ntok=1 << 26),
-            "d f16": de(k, t=E.F16), "d f8": de(k, t=E.F8), "p f16": pr(k, t=E.F16), "p f8": pr(k, t=E.F8), "c layer": cp(k, lb=100 * 4 * 16 * 128 + 16),
+            "d f8": de(k, t=E.F8), "d bf16": de(kv(), t=E.BF16), "p f8": pr(k, t=E.F8), "c layer": cp(k, lb=100 * 4 * 16 * 128 + 16),
             "d sinks": de(kv(), s=-1, w=5), "p sinks": pr(kv(), s=-1, w=5), "d window": de(k, s=1, w=-1), "p start": pr(k, start=None, s=1, w=5)})
 launched = counts[0]
 fine = {"append": ap(k), "starts": ap(k, start=P, ntok=9), "f16": ap(k, t=E.F16), "bf16": ap(k, t=E.BF16), "none": ap(k, ntok=0, start=P),
-        "decode": de(k), "prompt": pr(k), "bf16 q": de(k, t=E.BF16), "copy": cp(k), "sinks": de(kv(), w=9, s=2), "p sinks": pr(kv(), w=9, s=1 << 30),
+        "decode": de(k), "prompt": pr(k), "bf16 q": de(k, t=E.BF16), "f16 q": pr(k, t=E.F16), "copy": cp(k), "sinks": de(kv(), w=9, s=2), "p sinks": pr(kv(), w=9, s=1 << 30),
         "all": de(kv(), w=(1 << 31) - 1, s=(1 << 31) - 1)}
 print(json.dumps({"bad": out, "launched": launched, "fine": fine, "after": [counts[i] for i in range(5)]}))
 """
@@ -41,7 +41,7 @@ def test_refusals(child):  # noqa: F811
     assert got["launched"] == 0
     assert set(got["fine"].values()) == {0}
     # four appends and a copy of one launch, seven attention calls of two: nothing allocated, copied or waited for
-    assert got["after"] == [5 + 2 * 6, 0, 0, 0, 0]
+    assert got["after"] == [5 + 2 * 7, 0, 0, 0, 0]
 
 
 GRIDS = r"""
