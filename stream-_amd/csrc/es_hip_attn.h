@@ -85,11 +85,13 @@ struct AttnArgs {
     uint32_t inverse;          // 2^32 / target, rounded down (2^32 - 1 for 1)
     int block;                 // one query per sequence: log2 of the keys of a block
     int items;                 // parts per K/V head that there is room for
+    bool weigh;                // one query per sequence: beginning a tile is counted too
 };
 
-// the kernels of caches in 8 bits, and of 16-bit caches with sinks (es_hip_attn_f8.hip, es_hip_attn_sinks.hip)
+// the kernels of caches in 8 bits (type: of the queries), and of 16-bit caches with sinks, which are compiled in files of their own
 using AttnKernel = void (*)(AttnArgs);
-AttnKernel attn_f8_kernel(bool prompt, uint32_t type, int dim, bool sinks);   // type: of the queries
+AttnKernel attn_f8_decode_kernel(uint32_t type, int dim, bool sinks, int nseq);
+AttnKernel attn_f8_prompt_kernel(uint32_t type, int dim, bool sinks);
 AttnKernel attn_sinks_kernel(bool prompt, bool bf16, bool fp32, int dim);
 
 }  // namespace esq

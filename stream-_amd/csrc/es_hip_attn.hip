@@ -38,7 +38,7 @@ Shape shape_of(const es_hip_kv *kv, int nseq, int ntok, int heads, uint32_t type
         s.slots = s.target ? s.items : 0;
     } else {
         s.bm = DECODE_M;
-        s.target = std::max(decode_groups(kv->dim, nseq) / kv->heads, 1);
+        s.target = std::min(std::max(decode_groups(kv->dim, nseq, kv->type == ES_HIP_F8) / kv->heads, 1), DECODE_PARTS);
         s.items = s.target;
         s.block = most <= 1 << BLOCK_WHOLE ? BLOCK_WHOLE : BLOCK;
         s.slots = most > 1 << s.block ? 2 * s.items : 0;   // (0: every tile is one block)
@@ -126,9 +126,10 @@ int attention(const es_hip_kv *kv, int nseq, const int *start, int ntok, int hea
     a.inverse = s.target > 1 ? (uint32_t)((1ull << 32) / s.target) : ~0u;
     a.block = s.block;
     a.items = (int)s.items;
+    a.weigh = kv->type == ES_HIP_F8 && nseq > 1;
     const hipStream_t st = static_cast<hipStream_t>(stream);
     const bool f32 = type == ES_HIP_F32, bf = kv->type == ES_HIP_BF16;
-    const AttnKernel f = kv->type == ES_HIP_F8 ? attn_f8_kernel(prompt, type, kv->dim, a.sinks > 0)
+    const AttnKernel f = kv->type == ES_HIP_F8 ? (prompt ? attn_f8_prompt_kernel(type, kv->dim, a.sinks > 0) : attn_f8_decode_kernel(type, kv->dim, a.sinks > 0, nseq))
                          : a.sinks             ? attn_sinks_kernel(prompt, bf, f32, kv->dim)
                          : bf                  ? (f32 ? kernel_of<true, 3>(prompt, kv->dim) : kernel_of<true, 1>(prompt, kv->dim))
                                                : (f32 ? kernel_of<false, 2>(prompt, kv->dim) : kernel_of<false, 1>(prompt, kv->dim));

@@ -376,7 +376,7 @@ template <bool E8> struct Runs {
 // its offset. run_of gives it as four words, for asm; Run loads by it, past the caches, as nobody else reads a decode call's keys
 // soon. us so and through the caches: 131072 tokens, 4 heads of 128, 49 and 55; 32 sequences of 77 to 8192 tokens 35.9 and 36.4; what
 // the last-level cache holds whole gains nothing (48 windows of 4096 tokens, 2 heads of 64, 79 MB: 21.6 and 21.4).
-__device__ u4 run_of(const uint8_t *pool, const Runs<false> &all, int lane, int bytes) {
+template <bool E8> __device__ u4 run_of(const uint8_t *pool, const Runs<E8> &all, int lane, int bytes) {
     const int hi = __builtin_amdgcn_readlane(all.hi, lane);
     const uint64_t at = reinterpret_cast<uint64_t>(pool) + ((uint64_t)(uint32_t)max(hi, 0) << 32 | (uint32_t)__builtin_amdgcn_readlane(all.lo, lane));
     return u4{(uint32_t)at, (uint32_t)(at >> 32) & 0xffff, hi < 0 ? 0 : (uint32_t)bytes, 0x00020000};
@@ -429,13 +429,15 @@ template <int J> __device__ uint32_t pair(uint32_t first, uint32_t second) {
 // way is used once, so that LDS would only add a copy. Bound by HBM where the caches are long: 131072 tokens of 4 heads of 128,
 // fp16, 268 MB in 48 us (5.6 TB/s, joined; 42, 6.4 TB/s, before that), where a plain read reaches 6.2.
 constexpr int BLOCK = 7, BLOCK_WHOLE = 9, DECODE_M = 16;   // (log2)
-constexpr int decode_per_cu(int dim) { return dim <= 128 ? 2 : 1; }   // workgroups that a CU holds at once
+constexpr int DECODE_PARTS = 512;   // parts of a tile that can be joined, and so workgroups of a K/V head, at most
+// workgroups that a CU holds at once (8 bits, heads of 64: 64 sequences of 1000 to 9000 tokens, 8 heads, fp32, with two 60 us, three 57, four 58)
+constexpr int decode_per_cu(int dim, bool eight) { return eight && dim <= 64 ? 3 : dim <= 128 ? 2 : 1; }
 // Workgroups, all heads together: as many as fit the device at once and bring it to the memory's rate; half of that for one
 // sequence, whose tiles have the more parts to join: 20000 and 131072 tokens of 8 heads of 128, us, 21 and 87 with 256,
 // 23 and 90 with 512.
-constexpr int decode_groups(int dim, int nseq) { return nseq > 1 ? 256 * decode_per_cu(dim) : 256; }
+constexpr int decode_groups(int dim, int nseq, bool eight) { return nseq > 1 ? 256 * decode_per_cu(dim, eight) : 256; }
 
-// the sequences' blocks: lane i has those of sequence g + i
+// the sequences' blocks: lane i has those of sequence g + i, and `extra` more for each of its tiles
 struct Blocks {
     int len;
     uint32_t mine, upto;   // of the sequence; of the group's sequences up to it
@@ -444,46 +446,70 @@ __device__ int blocks_of(const AttnArgs &a, int len, int &base) {   // of one ti
     base = a.window ? max(0, (max(0, len - a.window) & ~63) - a.kept) : 0;
     return max(1, (len - base + (1 << a.block) - 1) >> a.block);
 }
-__device__ Blocks blocks_from(const AttnArgs &a, int g, int tiles) {
+__device__ Blocks blocks_from(const AttnArgs &a, int g, int tiles, int extra) {
     Blocks x{0, 0, 0};
     const int b = g + (threadIdx.x & 63);
     int base;
     if (b < a.nseq) {
         x.len = a.c.tokens(b);
-        x.mine = (uint32_t)tiles * (uint32_t)blocks_of(a, x.len, base);
+        x.mine = (uint32_t)tiles * (uint32_t)(blocks_of(a, x.len, base) + extra);
     }
     x.upto = a.nseq == 1 ? (uint32_t)__builtin_amdgcn_readfirstlane((int)x.mine) : sum_up_to(x.mine);
     return x;
 }
 
-// Every workgroup's way to its blocks: lane i holds those of the sequences `group` + i, of which there are `before` before.
-struct Deal {
+// Every workgroup's way to its blocks: lane i holds those of the sequences `group` + i, of which there are `before` before. Blocks are dealt out
+// evenly, `each` to a workgroup. 8 bits (a.weigh): beginning another tile costs a workgroup about what a block does (its pages, its query and its keys
+// are waited for, its sums joined), which shows where a workgroup's share would hold three of the shortest tiles: then every tile counts `extra` = 1
+// block more, ahead of its own. us, without and with: 32 sequences of 77 to 8192 tokens, 4 heads of 128, 27.1 and 23.6.
+template <bool WEIGH> struct Deal {
     Blocks bl;
     uint32_t total, each, before = 0;
-    int group = 0;
-    __device__ Deal(const AttnArgs &a, int tiles) : bl(blocks_from(a, 0, tiles)) {
-        total = (uint32_t)__builtin_amdgcn_readlane((int)bl.upto, 63);
-        for (int g = 64; g < a.nseq; g += 64) total += (uint32_t)__builtin_amdgcn_readlane((int)blocks_from(a, g, tiles).upto, 63);
+    int group = 0, extra = 0;
+    __device__ static uint32_t share(const AttnArgs &a, uint32_t total) {
         const uint32_t n = total + a.target - 1;
-        each = __umulhi(n, a.inverse);   // n / target, or one less
-        each += n - each * a.target >= (uint32_t)a.target;
+        const uint32_t each = __umulhi(n, a.inverse);   // n / target, or one less
+        return each + (n - each * a.target >= (uint32_t)a.target);
+    }
+    __device__ Deal(const AttnArgs &a, int tiles) : bl(blocks_from(a, 0, tiles, 0)) {
+        total = (uint32_t)__builtin_amdgcn_readlane((int)bl.upto, 63);
+        for (int g = 64; g < a.nseq; g += 64) total += (uint32_t)__builtin_amdgcn_readlane((int)blocks_from(a, g, tiles, 0).upto, 63);
+        each = share(a, total);
+        if (WEIGH && a.weigh) {
+            const int lane = threadIdx.x & 63;
+            uint32_t least = lane < a.nseq ? bl.mine : ~0u;
+            for (int g = 64 + lane; g < a.nseq; g += 64) {
+                int base;
+                least = min(least, (uint32_t)tiles * (uint32_t)blocks_of(a, a.c.tokens(g), base));
+            }
+            if (__any(3 * (uint64_t)least <= (uint64_t)each * tiles)) {
+                extra = 1;
+                total += (uint32_t)tiles * a.nseq;
+                each = share(a, total);
+                bl.upto += (uint32_t)tiles * min(lane + 1, a.nseq);
+                bl.mine += lane < a.nseq ? tiles : 0;
+            }
+        }
     }
     // on to the sequences from g on (a multiple of 64)
     __device__ void next(const AttnArgs &a, int tiles) {
         before += (uint32_t)__builtin_amdgcn_readlane((int)bl.upto, 63);
         group += 64;
-        bl = blocks_from(a, group, tiles);
+        bl = blocks_from(a, group, tiles, extra);
     }
     __device__ uint32_t first_of(int in) const { return before + (uint32_t)__builtin_amdgcn_readlane((int)(bl.upto - bl.mine), in); }
 };
 
-template <bool BF, int NQ, int DP, bool E8 = false, bool SINKS = false>
-__global__ __launch_bounds__(256, DP == 64 && NQ < 3 ? 3 : decode_per_cu(DP)) void attn_decode_kernel(AttnArgs a) {
+// AHEAD: steps of a wave's keys on their way. One is enough where other workgroups' are on theirs, and leaves more registers; with 8 bits, a
+// step of heads of 64, or one workgroup to a CU, two are better (decode_ahead). us with one and two, fp32: 131072 tokens of one sequence, 4 heads
+// of 128, 33.7 and 32.0; 32 sequences of 77 to 8192 27.1 and 28.6; 64 sequences of 1000 to 9000, 8 heads of 64, 64.6 and 60.3.
+constexpr int decode_ahead(int dim, int nseq) { return dim <= 64 || nseq == 1 ? 2 : 1; }
+template <bool BF, int NQ, int DP, bool E8 = false, bool SINKS = false, int AHEAD = 1>
+__global__ __launch_bounds__(256, DP == 64 && NQ < 3 ? 3 : decode_per_cu(DP, E8)) void attn_decode_kernel(AttnArgs a) {
     constexpr int KS = DP / 32, DL = DP / 16, BM = DECODE_M;
     constexpr bool UNSCALED = E8 && !BF;     // K goes into the product without its scales, which the scores take
     constexpr bool WBF = BF || E8;           // weights and V are bf16
     constexpr int ES = E8 ? 1 : 2;           // bytes of an element
-    constexpr int AHEAD = E8 ? 2 : 1;        // steps of keys on their way
     constexpr int NP = NQ == 1 ? 2 : E8 ? 3 : NQ;   // terms of the weights
     constexpr bool F32 = NQ > 1;
     __shared__ float lm[4][BM], ll[4][BM];
@@ -492,7 +518,7 @@ __global__ __launch_bounds__(256, DP == 64 && NQ < 3 ? 3 : decode_per_cu(DP)) vo
     const int head = blockIdx.x % a.c.heads, group = blockIdx.x / a.c.heads;
     const int rows = a.G, tiles = (a.G + BM - 1) / BM, dim = a.c.dim;
 
-    Deal deal(a, tiles);
+    Deal<E8> deal(a, tiles);
     const uint32_t each = deal.each, end = min(deal.total, (group + 1) * each);
     for (uint32_t pos = group * each; pos < end;) {
         int tid = threadIdx.x;
@@ -510,7 +536,12 @@ __global__ __launch_bounds__(256, DP == 64 && NQ < 3 ? 3 : decode_per_cu(DP)) vo
         const int blocks = blocks_of(a, len, base);
         // SINKS: keys are numbered without the `base` that lie behind the first a.kept and before the window
         const int hi = SINKS ? len - base : len;
-        const int tile = tiles == 1 ? 0 : (int)((pos - s0) / blocks), block = (int)((pos - s0) - (uint32_t)tile * blocks);
+        const int extra = E8 ? deal.extra : 0, tile = tiles == 1 ? 0 : (int)((pos - s0) / (blocks + extra));
+        int block = (int)((pos - s0) - (uint32_t)tile * (blocks + extra)) - extra;
+        if (E8 && block < 0) {
+            if (++pos >= end) break;
+            block = 0;
+        }
         const int here = (int)min((uint32_t)(blocks - block), end - pos);
         const uint32_t tile_at = pos - block;   // the tile's first block among all
         pos += here;
@@ -756,17 +787,17 @@ __global__ __launch_bounds__(256, DP == 64 && NQ < 3 ? 3 : decode_per_cu(DP)) vo
 // itself, in LDS. The sums' first loads, which need no weights, go out before them; what order they are added in, the lengths
 // alone give.
 template <bool F32, bool BF> __global__ __launch_bounds__(256) void attn_decode_join_kernel(AttnArgs a, int together) {
-    constexpr int BM = DECODE_M, AHEAD = 16, MOST = 512;
+    constexpr int BM = DECODE_M, AHEAD = 16, MOST = DECODE_PARTS;
     const int tiles = (a.G + BM - 1) / BM, dim = a.c.dim, quads = dim / 4;
     const int w = quads <= 16 ? 16 : quads <= 32 ? 32 : 64, d = threadIdx.x % w, k = threadIdx.x / w, shares = 256 / w / together;
     const int blocks_per_head = (a.G + together - 1) / together;
     const int seq = blockIdx.x / (a.c.heads * blocks_per_head), rest = blockIdx.x - seq * (a.c.heads * blocks_per_head);
     const int head = rest / blocks_per_head, r0 = (rest - head * blocks_per_head) * together;   // (together divides 16: rows of one tile)
-    Deal deal(a, tiles);
+    Deal<true> deal(a, tiles);
     while (seq >= deal.group + 64) deal.next(a, tiles);
     int base;
     const int blocks = blocks_of(a, __builtin_amdgcn_readlane(deal.bl.len, seq - deal.group), base);
-    const uint32_t at = deal.first_of(seq - deal.group) + (uint32_t)(r0 / BM) * blocks;
+    const uint32_t at = deal.first_of(seq - deal.group) + (uint32_t)(r0 / BM) * (blocks + deal.extra) + deal.extra;
     const uint32_t from = at / deal.each, parts = (at + blocks - 1) / deal.each - from + 1;
     if (parts == 1 || parts > MOST || from + parts > (uint32_t)a.target) return;   // (one: written already; the others cannot be while the lengths stay)
     const int r = r0 + k % together, share = k / together;
@@ -938,13 +969,8 @@ __global__ __launch_bounds__(256, prompt_per_cu(NQ, DP)) void attn_prompt_kernel
         const int t = n * ROWS + lane / CH, c = lane % CH ^ v_turn<DP>(t);
         v_from[n] = c * 8 < dim ? (t * dim + c * 8) * 2 : 0x40000000;
     }
-    // An 8-bit cache's keys wait a step in registers, 16 bytes of key n * ROWS8 + lane / CH8 in each, and are turned into bf16 on
-    // their way to LDS, where they lie as a 16-bit cache's do.
-    constexpr int CH8 = DP / 16, ROWS8 = 64 / CH8, R8 = E8 ? DP / 64 : 1;
-    u4 k8[R8], v8[R8];
-    float ks = 1.0f, vs = 1.0f;
-    // brings the keys from t0 on, to LDS (8 bits: to registers); which of their four runs are in no page
-    auto load = [&](int t0, int buf) {
+    // the window of runs moved on to the one from t0 on: its number there; `holes` gets which of the step's four are in no page
+    auto seek = [&](int t0, int &none) {
         int u0 = (t0 >> 4) - pb;
         if (u0 >= 64) {
             pb += 64;
@@ -952,42 +978,66 @@ __global__ __launch_bounds__(256, prompt_per_cu(NQ, DP)) void attn_prompt_kernel
             pg = pgn;
             pgn = fetch(pb + 64 + lane);
         }
-        const int bytes = min(last - t0 - wave * 16, 16) * dim * ES;
-        if constexpr (E8) {
-            const Run<false> k(a.c.k, pg, u0 + wave, bytes), v(a.c.v, pg, u0 + wave, bytes);
-            const int from = lane % CH8 * 16 < dim ? lane / CH8 * dim + lane % CH8 * 16 : 0x40000000;   // (elements past dim: past the run's end)
-            ks = pg.k_scale(u0 + wave);
-            vs = pg.v_scale(u0 + wave);
-#pragma unroll
-            for (int n = 0; n < R8; n++) k8[n] = k.load16(from, n * ROWS8 * dim);
-#pragma unroll
-            for (int n = 0; n < R8; n++) v8[n] = v.load16(from, n * ROWS8 * dim);
-        } else {
-            const u4 k = run_of(a.c.k, pg, u0 + wave, bytes), v = run_of(a.c.v, pg, u0 + wave, bytes);
-            const uint32_t to = lds0 + buf * TILE + wave * NI * 1024;
-#pragma unroll
-            for (int n = 0; n < NI; n++) run_to_lds(k, k_from[n], 0, to + n * 1024);
-#pragma unroll
-            for (int n = 0; n < NI; n++) run_to_lds(v, v_from[n % VN], n / VN * VN * ROWS * dim * 2, to + NB * TILE + n * 1024);
-        }
-        return (int)(__ballot(pg.hi < 0) >> u0 & 15);
+        none = (int)(__ballot(pg.hi < 0) >> u0 & 15);
+        return u0 + wave;
     };
-    auto settle = [&](int buf) {   // 8 bits: what load() brought, to LDS
+    auto bytes_of = [&](int t0) { return min(last - t0 - wave * 16, 16) * dim * ES; };
+    // brings the keys from t0 on to LDS; which of their four runs are in no page
+    auto load = [&](int t0, int buf) {
+        int none;
+        const int u = seek(t0, none);
+        const u4 k = run_of(a.c.k, pg, u, bytes_of(t0)), v = run_of(a.c.v, pg, u, bytes_of(t0));
+        const uint32_t to = lds0 + buf * TILE + wave * NI * 1024;
+#pragma unroll
+        for (int n = 0; n < NI; n++) run_to_lds(k, k_from[n], 0, to + n * 1024);
+#pragma unroll
+        for (int n = 0; n < NI; n++) run_to_lds(v, v_from[n % VN], n / VN * VN * ROWS * dim * 2, to + NB * TILE + n * 1024);
+        return none;
+    };
+    // 8 bits: the next step's keys wait in registers, 16 bytes of key n * ROWS8 + lane / CH8 in each, and are turned into 16 bits on their way
+    // to LDS, where they lie as a 16-bit cache's do: at the beginning of a step, with the step after it asked for then; or, SHARED, K there and
+    // V at the end, in the same registers, with V asked for at the beginning and K at the end. us, so and SHARED, 4096 tokens, 32 heads over 8: of 128,
+    // bf16 156 and 162 (fp32 the same within 3%, a prompt's last 64 tokens 38.2 and 39.1), of 64 fp32 182 and 172, of 256 (2048 tokens), where both
+    // do not fit the registers, fp32 250 and 232, bf16 105 and 105.
+    constexpr bool SHARED = NQ == 2 && DP != 128;
+    constexpr int CH8 = DP / 16, ROWS8 = 64 / CH8, R8 = E8 ? DP / 64 : 1;
+    u4 x8[SHARED ? 1 : 2][R8];
+    float scale8[SHARED ? 1 : 2];
+    auto load8 = [&](auto is_v, int t0, int u) {
+        const int from = lane % CH8 * 16 < dim ? lane / CH8 * dim + lane % CH8 * 16 : 0x40000000;   // (elements past dim: past the run's end)
+        const Run<false> r(is_v ? a.c.v : a.c.k, pg, u, bytes_of(t0));
+        constexpr int W = !SHARED && is_v;
+#pragma unroll
+        for (int n = 0; n < R8; n++) x8[W][n] = r.load16(from, n * ROWS8 * dim);
+        scale8[W] = is_v ? pg.v_scale(u) : pg.k_scale(u);
+    };
+    auto settle = [&](auto is_v, int buf) {
+        constexpr int W = !SHARED && is_v;
+        const float scale = scale8[W];
 #pragma unroll
         for (int n = 0; n < R8; n++) {
-            const int t = n * ROWS8 + lane / CH8, c = lane % CH8 * 2;
-            uint8_t *key = lds + buf * TILE + (wave * 16 + t) * DP * 2;
-            *reinterpret_cast<u4 *>(key + (c ^ k_turn<DP>(t)) * 16) = eight_of<BF>(k8[n][0], k8[n][1], ks);
-            *reinterpret_cast<u4 *>(key + (c + 1 ^ k_turn<DP>(t)) * 16) = eight_of<BF>(k8[n][2], k8[n][3], ks);
-            key += NB * TILE;
-            *reinterpret_cast<u4 *>(key + (c ^ v_turn<DP>(t)) * 16) = eight_of<BF>(v8[n][0], v8[n][1], vs);
-            *reinterpret_cast<u4 *>(key + (c + 1 ^ v_turn<DP>(t)) * 16) = eight_of<BF>(v8[n][2], v8[n][3], vs);
+            const int t = n * ROWS8 + lane / CH8, c = lane % CH8 * 2, turn = is_v ? v_turn<DP>(t) : k_turn<DP>(t);
+            uint8_t *key = lds + ((is_v ? NB : 0) + buf) * TILE + (wave * 16 + t) * DP * 2;
+            *reinterpret_cast<u4 *>(key + (c ^ turn) * 16) = eight_of<BF>(x8[W][n][0], x8[W][n][1], scale);
+            *reinterpret_cast<u4 *>(key + (c + 1 ^ turn) * 16) = eight_of<BF>(x8[W][n][2], x8[W][n][3], scale);
         }
         if (UNSCALED && lane == 0) {
-            run_ks[buf][wave] = ks;
-            run_vs[buf][wave] = vs;
-            run_ve[buf][wave] = (float)((int)(__float_as_uint(vs) >> 23 & 255) - 127);
+            if (is_v) {
+                run_vs[buf][wave] = scale;
+                run_ve[buf][wave] = (float)((int)(__float_as_uint(scale) >> 23 & 255) - 127);
+            } else {
+                run_ks[buf][wave] = scale;
+            }
         }
+    };
+    using K8 = std::false_type;
+    using V8 = std::true_type;
+    int u8 = 0;   // the number of the run whose K is in registers
+    auto load_k8 = [&](int t0) {
+        int none;
+        u8 = seek(t0, none);
+        load8(K8(), t0, u8);
+        return none;
     };
     // V of the step from t0 on, where some row does not see all of its keys: zeros for what none sees or must not be multiplied
     // by 0
@@ -1032,9 +1082,14 @@ __global__ __launch_bounds__(256, prompt_per_cu(NQ, DP)) void attn_prompt_kernel
     int holes = 0, buf = 0;   // holes: four bits a step, this one's lowest
     if constexpr (E8) {
         if (first < last) {
-            holes = load(first, 0);
-            settle(0);
-            if (first + PN < last) holes |= load(first + PN, 0) << 4;
+            holes = load_k8(first);
+            settle(K8(), 0);
+            load8(V8(), first, u8);
+            settle(V8(), 0);
+            if (first + PN < last) {
+                holes |= load_k8(first + PN) << 4;
+                if (!SHARED) load8(V8(), first + PN, u8);
+            }
         }
         __syncthreads();
     } else {
@@ -1047,8 +1102,18 @@ __global__ __launch_bounds__(256, prompt_per_cu(NQ, DP)) void attn_prompt_kernel
         const int t0 = at_key(n0);
         const bool more = n0 + (NB - 1) * PN < last;
         if constexpr (E8) {
-            if (more) settle(buf ^ 1);
-            if (n0 + 2 * PN < last) holes |= load(n0 + 2 * PN, 0) << 8;
+            if (more) {
+                settle(K8(), buf ^ 1);
+                if constexpr (SHARED) {
+                    load8(V8(), n0 + PN, u8);
+                } else {
+                    settle(V8(), buf ^ 1);
+                    if (n0 + 2 * PN < last) {
+                        holes |= load_k8(n0 + 2 * PN) << 8;
+                        load8(V8(), n0 + 2 * PN, u8);
+                    }
+                }
+            }
         } else {
             if (more) holes |= load(n0 + (NB - 1) * PN, buf == 0 ? NB - 1 : buf - 1) << 4 * (NB - 1);
         }
@@ -1202,8 +1267,15 @@ __global__ __launch_bounds__(256, prompt_per_cu(NQ, DP)) void attn_prompt_kernel
         }
         holes >>= 4;
         buf = buf == NB - 1 ? 0 : buf + 1;
-        if constexpr (E8) __syncthreads();
-        else arrived(!more);
+        if constexpr (E8) {
+            if constexpr (SHARED) {
+                if (more) settle(V8(), buf);
+                if (n0 + 2 * PN < last) holes |= load_k8(n0 + 2 * PN) << 4;
+            }
+            __syncthreads();
+        } else {
+            arrived(!more);
+        }
     }
     l = with_lane<32>(l, Sum());
     if constexpr (!UNSCALED) l = weights_sum<NQ, BY>(l);

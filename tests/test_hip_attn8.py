@@ -245,6 +245,16 @@ def test_decode_long(hip, types, dim, heads, kvh, page, lens):
     assert np.array_equal(got, run(hip, c, starts, q, t, dim ** -0.5, decode=True))   # the same from call to call
 
 
+@pytest.mark.parametrize("types", F8, ids=ids)
+def test_decode_most_parts(hip, types):
+    """one K/V head of 64 elements, whose one long sequence is split over more workgroups than any other call's"""
+    t, ct = types
+    rng = np.random.default_rng(70)
+    c = cache_of(ct, 1, 64, 1024, [70000, 3], rng)
+    c.fill(rng)
+    both(hip, c, [0, 1, 2], queries(rng, 2, 2, 64, t), t, 0.125, decode=True)
+
+
 @pytest.mark.parametrize("dim", [16, 64, 80, 128, 208, 256])
 @pytest.mark.parametrize("types", F8, ids=ids)
 def test_prompt_packed(hip, types, dim):
