@@ -926,6 +926,10 @@ __global__ __launch_bounds__(256, prompt_per_cu(NQ, DP)) void attn_prompt_kernel
         first = max(first, see_lo & ~(PN - 1));
     }
     auto at_key = [&](int n) { return SINKS && n >= a.kept ? n + left : n; };   // the token that key n is
+    // every row sees all sinks, and none of the keys behind them in their last step, which are then not brought: zeros
+    const bool sinks_alone = SINKS && see_lo >= a.kept;
+    const int sinks_end = SINKS ? __builtin_amdgcn_readfirstlane(sinks_alone ? min(a.sinks, last) : last) : 0;
+    auto in_sight = [&](int n) { return SINKS && n < a.kept ? sinks_end : last; };   // the end of the keys to bring from n on
     const int *table = a.c.table + (size_t)max(a.c.row(p.b), 0) * a.c.max_pages;
     const int dim = a.c.dim;
 
@@ -981,7 +985,7 @@ __global__ __launch_bounds__(256, prompt_per_cu(NQ, DP)) void attn_prompt_kernel
         none = (int)(__ballot(pg.hi < 0) >> u0 & 15);
         return u0 + wave;
     };
-    auto bytes_of = [&](int t0) { return min(last - t0 - wave * 16, 16) * dim * ES; };
+    auto bytes_of = [&](int n) { return __builtin_amdgcn_readfirstlane((SINKS ? max(min(in_sight(n) - n - wave * 16, 16), 0) : min(last - n - wave * 16, 16)) * dim * ES); };
     // brings the keys from t0 on to LDS; which of their four runs are in no page
     auto load = [&](int t0, int buf) {
         int none;
@@ -1039,6 +1043,7 @@ __global__ __launch_bounds__(256, prompt_per_cu(NQ, DP)) void attn_prompt_kernel
         load8(K8(), t0, u8);
         return none;
     };
+    auto some_hidden = [&](int t0) { return (t0 + PN > pos_lo + 1 || t0 < from_hi) && !(sinks_alone && t0 < a.kept); };   // of the step's keys, from some row
     // V of the step from t0 on, where some row does not see all of its keys: zeros for what none sees or must not be multiplied
     // by 0
     auto clean = [&](int t0, int buf) {
@@ -1117,7 +1122,7 @@ __global__ __launch_bounds__(256, prompt_per_cu(NQ, DP)) void attn_prompt_kernel
         } else {
             if (more) holes |= load(n0 + (NB - 1) * PN, buf == 0 ? NB - 1 : buf - 1) << 4 * (NB - 1);
         }
-        if (t0 + PN > pos_lo + 1 || t0 < from_hi) {
+        if (some_hidden(t0)) {
             clean(t0, buf);
             __syncthreads();
         }
@@ -1285,7 +1290,7 @@ __global__ __launch_bounds__(256, prompt_per_cu(NQ, DP)) void attn_prompt_kernel
     if (odd) {   // what was left out, for the keys of the steps that were looked through (an infinity or NaN, whatever its weight)
         for (int n = SINKS ? first : max(first, see_lo); n < last; n++) {
             const int t = at_key(n), t0 = t & ~(PN - 1);
-            if (!(t0 + PN > pos_lo + 1 || t0 < from_hi) || t > pos || (t < from && !(SINKS && t < a.sinks))) continue;
+            if (!some_hidden(t0) || t > pos || (t < from && !(SINKS && t < a.sinks))) continue;
             const int page = table[t >> a.c.shift];
             if (page < 0 || page >= a.c.npages) continue;
             const size_t at = a.c.row_at(page, head, t & ((1 << a.c.shift) - 1));
