@@ -881,8 +881,9 @@ __device__ u2 transposed(uint32_t lds) {
 }
 
 template <bool BF, int NQ, int DP, bool E8 = false, bool SINKS = false>
-__global__ __launch_bounds__(256, prompt_per_cu(NQ, DP)) void attn_prompt_kernel(AttnArgs a) {
+__global__ __launch_bounds__(256, E8 && NQ == 2 && DP == 64 ? 3 : prompt_per_cu(NQ, DP)) void attn_prompt_kernel(AttnArgs a) {
     constexpr bool UNSCALED = E8 && !BF;                     // (see below)
+    constexpr bool SHORT = E8 && NQ == 2;                    // of registers: what can be computed anew is not kept
     constexpr int NB = DP == 64 && !E8 ? 3 : 2;              // steps of keys in LDS
     constexpr int ES = E8 ? 1 : 2;                           // bytes of an element in the pools
     constexpr int KS = DP / 16, DT = DP / 32, CH = DP / 8;   // CH: pieces of a key
@@ -1000,10 +1001,9 @@ __global__ __launch_bounds__(256, prompt_per_cu(NQ, DP)) void attn_prompt_kernel
     };
     // 8 bits: the next step's keys wait in registers, 16 bytes of key n * ROWS8 + lane / CH8 in each, and are turned into 16 bits on their way
     // to LDS, where they lie as a 16-bit cache's do: at the beginning of a step, with the step after it asked for then; or, SHARED, K there and
-    // V at the end, in the same registers, with V asked for at the beginning and K at the end. us, so and SHARED, 4096 tokens, 32 heads over 8: of 128,
-    // bf16 156 and 162 (fp32 the same within 3%, a prompt's last 64 tokens 38.2 and 39.1), of 64 fp32 182 and 172, of 256 (2048 tokens), where both
-    // do not fit the registers, fp32 250 and 232, bf16 105 and 105.
-    constexpr bool SHARED = NQ == 2 && DP != 128;
+    // V at the end, in the same registers, with V asked for at the beginning and K at the end, where both do not fit. us, so and SHARED, fp32, 32 heads
+    // over 8: of 256, 2048 tokens, 207 and 181, of 128, 4096 tokens, 267 and 271.
+    constexpr bool SHARED = NQ == 2 && DP == 256;
     constexpr int CH8 = DP / 16, ROWS8 = 64 / CH8, R8 = E8 ? DP / 64 : 1;
     u4 x8[SHARED ? 1 : 2][R8];
     float scale8[SHARED ? 1 : 2];
@@ -1074,6 +1074,11 @@ __global__ __launch_bounds__(256, prompt_per_cu(NQ, DP)) void attn_prompt_kernel
     // reads: K piece (k * 2 + half) of key h * 32 + col; of V, as transposed() takes them, 4 elements of key u * 16 + r * 8 +
     // half * 4 + lane % 16 / 4
     constexpr int KA = KS < 8 ? KS : 8, VA = DT < 4 ? DT : 4;   // (addresses that are not another's at a constant distance)
+    // Reads of K, and fragments of V, under way ahead of the products: as the compiler left them, each product waited for its own. Where
+    // registers are SHORT, more than they have room for would be none (the compiler then drops the order): us with these and with none, 4096 tokens,
+    // heads of 128, 267 and 294, of 64 166 and 172, 2048 of 256 181 and 232, a prompt's last 64 of 8001 33.2 and 38.1. In a 16-bit cache's
+    // kernels, 8192 tokens: heads of 256, fp16 1330 and 1534, fp32 2017 and 2363; of 128 555 and 563.
+    constexpr int AHEAD_K = SHORT ? 4 : 6, AHEAD_V = !SHORT ? 4 : DP == 256 ? 1 : 2;
     uint32_t k_at[KA], v_at[VA];
 #pragma unroll
     for (int k = 0; k < KA; k++) k_at[k] = lds0 + col * DP * 2 + ((k * 2 + half) ^ k_turn<DP>(col)) * 16;
@@ -1088,8 +1093,9 @@ __global__ __launch_bounds__(256, prompt_per_cu(NQ, DP)) void attn_prompt_kernel
     if constexpr (E8) {
         if (first < last) {
             holes = load_k8(first);
+            if (!SHARED) load8(V8(), first, u8);
             settle(K8(), 0);
-            load8(V8(), first, u8);
+            if (SHARED) load8(V8(), first, u8);
             settle(V8(), 0);
             if (first + PN < last) {
                 holes |= load_k8(first + PN) << 4;
@@ -1127,16 +1133,18 @@ __global__ __launch_bounds__(256, prompt_per_cu(NQ, DP)) void attn_prompt_kernel
             __syncthreads();
         }
         if (!(idle || t0 > wpos_hi || (a.window && t0 + PN <= wpos_lo - a.window + 1 && !(SINKS && t0 < a.sinks)))) {
-            uint32_t k_now[KA], v_now[VA];   // (kept as they are, so that what is added to them goes into the instructions)
+            // (kept as they are, so that what is added to them goes into the instructions; where registers are short, each is the first with
+            // its piece's number exchanged into it)
+            uint32_t k_now[KA], v_now[VA];
 #pragma unroll
             for (int k = 0; k < KA; k++) {
-                k_now[k] = k_at[k] + buf * TILE;
-                asm volatile("" : "+v"(k_now[k]));
+                k_now[k] = SHORT ? (k_at[0] + buf * TILE) ^ k * 32 : k_at[k] + buf * TILE;
+                if constexpr (!SHORT) asm volatile("" : "+v"(k_now[k]));
             }
 #pragma unroll
             for (int j = 0; j < VA; j++) {
-                v_now[j] = v_at[j] + buf * TILE;
-                asm volatile("" : "+v"(v_now[j]));
+                v_now[j] = SHORT ? (v_at[0] + buf * TILE) ^ j * 64 : v_at[j] + buf * TILE;
+                if constexpr (!SHORT) asm volatile("" : "+v"(v_now[j]));
             }
             f16v s[2];
 #pragma unroll
@@ -1151,17 +1159,15 @@ __global__ __launch_bounds__(256, prompt_per_cu(NQ, DP)) void attn_prompt_kernel
 #pragma unroll
                     for (int t = 0; t < NQ; t++) s[h] = mfma32<BF>(kf, q[k][t], s[h]);
                 }
-            // Six reads of K under way, or (below) four fragments of V: as the compiler left it, each product waited for its
-            // own. With three terms the products are long enough. 8192 tokens, us, with and without: heads of 256, fp16 1330
-            // and 1534, fp32 2017 and 2363; of 128 555 and 563.
+            // (with three terms the products are long enough)
             if constexpr (NQ < 3) {
-                __builtin_amdgcn_sched_group_barrier(0x100, 6, 0);
+                __builtin_amdgcn_sched_group_barrier(0x100, AHEAD_K, 0);
 #pragma unroll
-                for (int i = 0; i < 2 * KS - 6; i++) {
+                for (int i = 0; i < 2 * KS - AHEAD_K; i++) {
                     __builtin_amdgcn_sched_group_barrier(0x8, NQ, 0);
                     __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
                 }
-                __builtin_amdgcn_sched_group_barrier(0x8, 6 * NQ, 0);
+                __builtin_amdgcn_sched_group_barrier(0x8, AHEAD_K * NQ, 0);
             }
             if (t0 + PN > wpos_lo + 1 || t0 < wfrom_hi) {
                 const int to = pos - t0 - half * 4, since = from - t0 - half * 4, sinks = SINKS ? a.sinks - t0 - half * 4 : 0;
@@ -1261,13 +1267,13 @@ __global__ __launch_bounds__(256, prompt_per_cu(NQ, DP)) void attn_prompt_kernel
                     for (int t = 0; t < NQ; t++) acc[j] = mfma32<BF>(vf, pt[u][t], acc[j]);
                 }
             if constexpr (NQ < 3) {
-                __builtin_amdgcn_sched_group_barrier(0x100, 8, 1);
+                __builtin_amdgcn_sched_group_barrier(0x100, 2 * AHEAD_V, 1);
 #pragma unroll
-                for (int i = 0; i < 4 * DT - 4; i++) {
+                for (int i = 0; i < 4 * DT - AHEAD_V; i++) {
                     __builtin_amdgcn_sched_group_barrier(0x8, NQ, 1);
                     __builtin_amdgcn_sched_group_barrier(0x100, 2, 1);
                 }
-                __builtin_amdgcn_sched_group_barrier(0x8, 4 * NQ, 1);
+                __builtin_amdgcn_sched_group_barrier(0x8, AHEAD_V * NQ, 1);
             }
         }
         holes >>= 4;
