@@ -333,6 +333,9 @@ __device__ float load_query(const uint8_t *row, bool valid, int g, int dim, floa
     }
 }
 
+// what a query's scores against a run of an 8-bit cache are multiplied by (never 0, as above)
+__device__ float times_scale(float cs, float ks) { return fmaxf(cs * ks, 1.17549435e-38f); }
+
 template <bool F32, bool BF> __device__ void store4(uint8_t *row, int d, const float (&x)[4]) {
     if constexpr (F32) {
         struct __attribute__((packed, aligned(4))) F4 { float x[4]; };
@@ -648,8 +651,8 @@ __global__ __launch_bounds__(256, DP == 64 && NQ < 3 ? 3 : decode_per_cu(DP, E8)
             }
             float cs[2] = {q_scale, q_scale};   // what the runs' scores are multiplied by
             if constexpr (UNSCALED) {
-                cs[0] *= ks[A][0];
-                cs[1] *= ks[A][1];
+                cs[0] = times_scale(q_scale, ks[A][0]);
+                cs[1] = times_scale(q_scale, ks[A][1]);
             }
             const bool ok0 = ok[A][0], ok1 = ok[A][1], more = n + AHEAD < steps;
             if (more) {
@@ -1195,7 +1198,7 @@ __global__ __launch_bounds__(256, E8 && NQ == 2 && DP == 64 ? 3 : prompt_per_cu(
                     float x = LOWEST;
 #pragma unroll
                     for (int i = 0; i < 8; i++) x = fmaxf(x, s[u >> 1][(u & 1) * 8 + i]);
-                    csr[u] = cs * k4[u];
+                    csr[u] = times_scale(cs, k4[u]);
                     x *= csr[u];
                     big = fmaxf(big, x);
                     big2 = fmaxf(big2, x + e4[u]);

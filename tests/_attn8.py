@@ -100,6 +100,13 @@ class Cache8:
             k, v = (VALUES[self.code[i][g, :, o]] * self.scale[i][g, :, o // RUN][..., None].astype(np.float64) for i in range(2))
         return k, v, ok
 
+    def v_scales(self, r):
+        """the scale of each of row r's V rows [len, heads] (0 where it has no page)"""
+        j = np.arange(int(self.len[r]))
+        g = self.table[r][j // self.page]
+        ok = (g >= 0) & (g < self.npages)
+        return np.where(ok[:, None], self.scale[1][np.where(ok, g, 0), :, j % self.page // RUN], 0.0)
+
     def upload(self, hip, seq=None):
         """(Kv, buffers to keep: K, V, table, lengths, scales of K and of V)"""
         keep = [hip.upload(x) for x in (*self.code, self.table, self.len, *self.scale)]
@@ -110,8 +117,12 @@ class Cache8:
 
 
 def attention(cache, starts, q, scale, window=0, sinks=0, seq=None):
-    """q [ntok, heads, dim] in 64 bits -> out, and per output the sum of |p v| (the scale of its rounding errors)"""
-    out, mag = np.zeros(q.shape), np.zeros(q.shape)
+    """q [ntok, heads, dim] in 64 bits -> out, per output the sum of |p v| (the scale of its rounding errors), and, of an 8-bit cache, what
+    weights below fp16's range may change in a prompt's row.
+
+    Those go into the products as p * (V's scale) relative to the row's largest such, which stands between 2^12 and 2^15; two terms of
+    fp16 (or one) are off by at most half of its smallest step, 2^-25, which is 2^-37 of the largest. n keys of numbers up to 448 add that up."""
+    out, mag, low = np.zeros(q.shape), np.zeros(q.shape), np.zeros(q.shape)
     G = q.shape[1] // cache.heads
     for b in range(len(starts) - 1):
         r = b if seq is None else seq[b]
@@ -132,4 +143,7 @@ def attention(cache, starts, q, scale, window=0, sinks=0, seq=None):
             p /= np.where(some, p.sum(1), 1.0)[:, None]
             out[starts[b]:starts[b + 1], h] = p @ V[:, h // G]
             mag[starts[b]:starts[b + 1], h] = p @ np.abs(V[:, h // G])
-    return out, mag
+            if isinstance(cache, Cache8):
+                largest = (p * np.where(any_sees[:, 0, 0], cache.v_scales(r)[:, h // G], 0.0)).max(1)
+                low[starts[b]:starts[b + 1], h] = (n * 448 * 2.0 ** -37 * largest)[:, None]
+    return out, mag, low

@@ -61,12 +61,19 @@ def run(hip, cache, starts, q, t, scale, window=0, sinks=0, seq=None, qpad=0, op
     return out
 
 
-def check(cache, starts, q, t, scale, got, window=0, sinks=0, seq=None):
+def allowed(cache, x, t, scale, mag, low, want, decode):
+    """_attn.tolerance, and what it does not count: weights below fp16's range in a prompt over 8 bits whose products are of fp16, and outputs
+    below fp16's smallest normal number, whose steps are 2^-24"""
+    tol = tolerance(cache, x, t, scale, mag, want)
+    return tol + (low if t != E.BF16 and not decode else 0) + (2.0 ** -25 if t == E.F16 else 0)
+
+
+def check(cache, starts, q, t, scale, got, window=0, sinks=0, seq=None, decode=False):
     x = from_bits(q, t)
     as_queries(cache, t)
-    want, mag = attention(cache, starts, x, scale, window, sinks, seq)
+    want, mag, low = attention(cache, starts, x, scale, window, sinks, seq)
     n = starts[-1]
-    tol = tolerance(cache, x, t, scale, mag, want)
+    tol = allowed(cache, x, t, scale, mag, low, want, decode)
     got = from_bits(got, t)[:n]
     err = np.abs(got - want[:n])
     bad = ~(err <= tol[:n])
@@ -77,7 +84,7 @@ def check(cache, starts, q, t, scale, got, window=0, sinks=0, seq=None):
 
 def both(hip, c, starts, q, t, scale, **k):
     got = run(hip, c, starts, q, t, scale, **k)
-    check(c, starts, q, t, scale, got, k.get("window", 0), k.get("sinks", 0), k.get("seq"))
+    check(c, starts, q, t, scale, got, k.get("window", 0), k.get("sinks", 0), k.get("seq"), k.get("decode", False))
     return got
 
 
@@ -311,6 +318,38 @@ def test_scales_far_apart(hip, types, decode):
 
 @pytest.mark.parametrize("decode", [True, False])
 @pytest.mark.parametrize("types", F8, ids=ids)
+def test_values(hip, types, decode):
+    """queries of zeros, tiny and huge, against runs of zeros (the least scale), of tiny and of huge keys; hidden keys stay hidden"""
+    t, ct = types
+    rng = np.random.default_rng(8)
+    n = 300
+    c = Cache8(1, 64, 16, [n] * 6, rng)
+    for r in range(6):
+        x = rng.standard_normal((2, n, 1, 64))
+        x[0, 16:64], x[1, 100:140] = 0, 0
+        x[0, 64:96] *= 2.0 ** -90
+        x[0, 128:160] *= 16
+        c.append(r, 0, x[0], x[1])
+    new = 1 if decode else 70
+    x = rng.standard_normal((6, new, 4, 64)).astype(np.float32)
+    x[0] = 0
+    x[1] *= 30
+    x[2] *= 1e-6 if t != E.F16 else 1e-4
+    x[3, :, :, ::2] *= 1e-4
+    x[4, :, :2] *= 200
+    x[5, :, 1] = 0
+    x = x.reshape(6 * new, 4, 64)
+    starts = list(range(0, 6 * new + 1, new))
+    both(hip, c, starts, to_bits(x, t), t, 0.125, decode=decode)
+    both(hip, c, starts, to_bits(x, t), t, 0.125, decode=decode, window=100, sinks=20)
+    if t != E.F16:   # beyond fp16's range either way: an fp32 row is scaled before it is split
+        both(hip, c, starts, to_bits(x * np.float32(1e-20), t), t, 1e19, decode=decode)
+        both(hip, c, starts, to_bits(x * np.float32(1e-20), t), t, 0.125, decode=decode, window=250, sinks=3)   # (hidden keys in a run of zeros)
+        both(hip, c, starts, to_bits(x * np.float32(1e20), t), t, 1e-21, decode=decode)
+
+
+@pytest.mark.parametrize("decode", [True, False])
+@pytest.mark.parametrize("types", F8, ids=ids)
 def test_batches_as_they_come(hip, types, decode):
     """by sequence numbers: padded, empty, lengths that are negative or past the table, holes and page numbers out of range"""
     t, ct = types
@@ -348,8 +387,8 @@ def test_nan_reaches_who_sees_it(hip, types, dim, window, sinks, n, new):
     scale, decode = dim ** -0.5, new == 1
     q = queries(rng, new, 4, dim, t)
     x = from_bits(q, t)
-    want, mag = attention(c, [0, new], x, scale, window, sinks)
-    tol = tolerance(c, x, t, scale, mag, want)
+    want, mag, low = attention(c, [0, new], x, scale, window, sinks)
+    tol = allowed(c, x, t, scale, mag, low, want, decode)
     pos = np.arange(n - new, n)
     sees = lambda j: (pos >= j) & ((pos < j + window) | (j < sinks) if window else True)
     at = lambda j: (c.table[0, j // 16], slice(None), j % 16)
