@@ -870,7 +870,8 @@ template <bool F32, bool BF> __global__ __launch_bounds__(256) void attn_decode_
 // fits, and the exponentials of one wave no longer pass under the products of another: 2.94 ms where this had 2.25. Tiles of
 // 256 rows in eight waves: within 2%.
 template <int DP> __device__ constexpr int k_turn(int t) { return DP == 64 ? t >> 1 & 7 : t & 15; }
-template <int DP> __device__ constexpr int v_turn(int t) { return DP == 64 ? (t >> 1 & 1) * 4 : (t & 3) * 4; }
+// (8 bits: the last bit too, for the writes to LDS, see settle)
+template <int DP, bool E8> __device__ constexpr int v_turn(int t) { return DP == 64 ? (t >> 1 & 1) * (E8 ? 5 : 4) : (t & 3) * 4 + (E8 ? t & 1 : 0); }
 
 // 64 pieces of 16 bytes from a run into LDS: lane i's, at `lane_offset` + `offset` from the run's first row, to lds + 16 i;
 // zeros past the run's end
@@ -974,7 +975,7 @@ __global__ __launch_bounds__(256, E8 && NQ == 2 && DP == 64 ? 3 : prompt_per_cu(
     }
 #pragma unroll
     for (int n = 0; n < VN; n++) {
-        const int t = n * ROWS + lane / CH, c = lane % CH ^ v_turn<DP>(t);
+        const int t = n * ROWS + lane / CH, c = lane % CH ^ v_turn<DP, E8>(t);
         v_from[n] = c * 8 < dim ? (t * dim + c * 8) * 2 : 0x40000000;
     }
     // the window of runs moved on to the one from t0 on: its number there; `holes` gets which of the step's four are in no page
@@ -1002,16 +1003,21 @@ __global__ __launch_bounds__(256, E8 && NQ == 2 && DP == 64 ? 3 : prompt_per_cu(
         for (int n = 0; n < NI; n++) run_to_lds(v, v_from[n % VN], n / VN * VN * ROWS * dim * 2, to + NB * TILE + n * 1024);
         return none;
     };
-    // 8 bits: the next step's keys wait in registers, 16 bytes of key n * ROWS8 + lane / CH8 in each, and are turned into 16 bits on their way
+    // 8 bits: the next step's keys wait in registers, 16 bytes of key n * ROWS8 + t8 in each, and are turned into 16 bits on their way
     // to LDS, where they lie as a 16-bit cache's do: at the beginning of a step, with the step after it asked for then; or, SHARED, K there and
     // V at the end, in the same registers, with V asked for at the beginning and K at the end, where both do not fit. us, so and SHARED, fp32, 32 heads
     // over 8: of 256, 2048 tokens, 207 and 181, of 128, 4096 tokens, 267 and 271.
     constexpr bool SHARED = NQ == 2 && DP == 256;
+    //
+    // A lane has 16 bytes, two pieces, of a key. Eight lanes in a row have 4 such of two keys whose pieces are exchanged differently in the last
+    // bit, so that their first pieces, and their second ones, fall on different banks.
     constexpr int CH8 = DP / 16, ROWS8 = 64 / CH8, R8 = E8 ? DP / 64 : 1;
+    const int c8 = DP == 64 ? lane & 3 : DP == 128 ? (lane & 3) + (lane >> 3 & 1) * 4 : (lane & 3) + (lane >> 3 & 3) * 4;
+    const int t8 = DP == 64 ? (lane >> 3 & 1) + (lane >> 2 & 1) * 2 + (lane >> 4) * 4 : DP == 128 ? (lane >> 2 & 1) + (lane >> 4) * 2 : (lane >> 2 & 1) + (lane >> 5) * 2;
     u4 x8[SHARED ? 1 : 2][R8];
     float scale8[SHARED ? 1 : 2];
     auto load8 = [&](auto is_v, int t0, int u) {
-        const int from = lane % CH8 * 16 < dim ? lane / CH8 * dim + lane % CH8 * 16 : 0x40000000;   // (elements past dim: past the run's end)
+        const int from = c8 * 16 < dim ? t8 * dim + c8 * 16 : 0x40000000;   // (elements past dim: past the run's end)
         const Run<false> r(is_v ? a.c.v : a.c.k, pg, u, bytes_of(t0));
         constexpr int W = !SHARED && is_v;
 #pragma unroll
@@ -1023,7 +1029,7 @@ __global__ __launch_bounds__(256, E8 && NQ == 2 && DP == 64 ? 3 : prompt_per_cu(
         const float scale = scale8[W];
 #pragma unroll
         for (int n = 0; n < R8; n++) {
-            const int t = n * ROWS8 + lane / CH8, c = lane % CH8 * 2, turn = is_v ? v_turn<DP>(t) : k_turn<DP>(t);
+            const int t = n * ROWS8 + t8, c = c8 * 2, turn = is_v ? v_turn<DP, E8>(t) : k_turn<DP>(t);
             uint8_t *key = lds + ((is_v ? NB : 0) + buf) * TILE + (wave * 16 + t) * DP * 2;
             *reinterpret_cast<u4 *>(key + (c ^ turn) * 16) = eight_of<BF>(x8[W][n][0], x8[W][n][1], scale);
             *reinterpret_cast<u4 *>(key + (c + 1 ^ turn) * 16) = eight_of<BF>(x8[W][n][2], x8[W][n][3], scale);
@@ -1088,7 +1094,7 @@ __global__ __launch_bounds__(256, E8 && NQ == 2 && DP == 64 ? 3 : prompt_per_cu(
 #pragma unroll
     for (int j = 0; j < VA; j++) {
         const int t = half * 4 + (lane & 15) / 4, e = j * 32 + (lane >> 4 & 1) * 16 + (lane & 3) * 4;
-        v_at[j] = lds0 + NB * TILE + t * DP * 2 + ((e / 8) ^ v_turn<DP>(t)) * 16 + e % 8 * 2;
+        v_at[j] = lds0 + NB * TILE + t * DP * 2 + ((e / 8) ^ v_turn<DP, E8>(t)) * 16 + e % 8 * 2;
     }
     if (tid == 0) odd = 0;
     __syncthreads();
