@@ -472,7 +472,7 @@ typedef struct {
 } es_hip_kv;
 /* An F8 cache. Its elements stand for the number times its 16 tokens' scale 2^e, -100 <= e <= 120, exactly; half the memory and
  * reads of a 16-bit cache, with elements off by at most 2^-4 of themselves, or 2^(e - 10) where they are small. Attention takes what they
- * stand for, as bf16. es_hip_kv_append_dev gives 16 tokens the least scale whose 448-fold is not less than any of their elements (infinities and
+ * stand for, unrounded. es_hip_kv_append_dev gives 16 tokens the least scale whose 448-fold is not less than any of their elements (infinities and
  * NaN, which become NaN, aside; from 2^-100 to 2^120, beyond which an element may stand for an infinity). Where some of the 16 were written by an
  * earlier call, those before the call's own stay, with no smaller a scale; should it grow, they are rounded to it once more: that loses
  * only bits below 2^(e - 9). No two sequences of a call may write to the same 16 tokens (a sequence named
@@ -493,8 +493,9 @@ int es_hip_kv_append_dev(const es_hip_kv *kv, int nseq, const int *start, int nt
  * same for out; aligned to their type. scale is positive and finite. A sequence without tokens gets zeros. Tokens that
  * a query does not see have no influence, whatever their rows hold; an infinity or NaN that it sees in V comes out as an infinity
  * or NaN in that element. fp32 q is carried to 22 bits or more through the matrix products, as are the weights p; with a 16-bit q,
- * decode carries p to 14 bits or more (F16: 20), which does not show beside out's rounding, and a prompt rounds p to the cache's
- * type: bring q as fp32 for more. Sums are fp32's: where a sum of |v| over the keys passes its range, which takes BF16, infinities
+ * decode carries p to 14 bits or more (F16 over F16: 20), which does not show beside out's rounding, and a prompt rounds p to q's
+ * type: bring q as fp32 for more. (An F8 cache's prompts with F32 or F16 q: a key whose p times V's scale is below 2^-37 of the row's
+ * largest such may count as none.) Sums are fp32's: where a sum of |v| over the keys passes its range, which takes BF16, infinities
  * or NaN come out. out may be q itself, with one stride, and overlaps nothing else that the call reads. Limits: 2^29 query rows
  * (tokens times heads), 2^23 sequences times heads, 2^31 blocks of 128 keys that the table rows could hold.
  * ws: the caller's device workspace of at least es_hip_attn_decode_workspace bytes (16-byte aligned; 0 bytes: may be NULL); its
