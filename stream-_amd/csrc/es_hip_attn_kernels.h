@@ -22,9 +22,9 @@
 // instruction turns two of them into either, exactly. bf16 queries take them with their scales, and all else is as over bf16. fp32 and fp16
 // queries (UNSCALED) take K as the numbers are, in fp16, so that fp32 needs two terms and not three; K's scales are factors of the scores. V is taken
 // with its scales, in bf16, by decode, whose weights are cut into two or three terms of bf16, and without, in fp16, by prompts, whose scales of
-// V become factors of the weights (see attn_prompt_kernel). The errors against 64 bits are those of 16-bit caches: fp32 1.9e-7 to 3.9e-7.
-// Half the bytes, and more instructions to a byte: 131072 tokens of one sequence, 4 heads of 128, 32.0 us (134 MB; over fp16 47.8), where decode's
-// 27 us at 5 TB/s are half instructions; 4096 prompt tokens, 32 heads of 128 over 8, bf16 154 us (over bf16 148), fp32 263 (over fp16 257).
+// V become factors of the weights (see attn_prompt_kernel). The errors against 64 bits of the cache's numbers: fp32 2.0e-7 to 3.9e-7.
+// Half the bytes, and more instructions to a byte: 131072 tokens of one sequence, 4 heads of 128, 32.0 us (134 MB; over bf16 48.1), where decode's
+// own kernel takes 27.3 (4.9 TB/s); 4096 prompt tokens, 32 heads of 128 over 8, bf16 157 us (over bf16 150), fp32 269 (over fp16 261).
 //
 // Sinks (SINKS). A window leaves the first `sinks` tokens of a sequence in sight. Keys are numbered without those between: the sinks rounded up to 64
 // (a.kept), then the window's steps, so that chunks, blocks and steps go over both without a gap.
