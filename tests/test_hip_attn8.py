@@ -606,6 +606,44 @@ def test_captured_calls_follow_the_lengths(hip, ct, prompt):
     assert rt.L.hipStreamDestroy(s) == 0
 
 
+@pytest.mark.parametrize("ct", [E.F8, E.F16], ids=lambda t: NAMES[t])
+def test_two_streams_at_once(hip, ct):
+    """decode and a prompt over one cache, sinks and none, on two streams with workspaces of their own: the bits of each call alone"""
+    rt, rng = Hip(), np.random.default_rng(33)
+    c = cache_of(ct, 2, 128, 16, [3000, 1700, 9], rng)
+    c.fill(rng)
+    kv, keep = c.upload(hip)
+    starts = [0, 64, 100, 103]
+    n, ds = starts[-1], hip.upload(np.array(starts, np.int32))
+    q = hip.upload(queries(rng, n, 8, 128, E.F32).astype(np.float32))
+    sizes = hip.attn_decode_workspace(kv, 3, 8), hip.attn_prompt_workspace(kv, 3, n, 8, E.F32)
+    assert all(sizes)
+    ws, rows, streams = [hip.alloc(b) for b in sizes], (3, n), [rt.stream() for _ in range(2)]
+
+    def call(i, window, sinks, o, s):
+        if i:
+            hip.attn_prompt_sinks_dev(kv, 3, ds, n, 8, E.F32, q, 0, 0.1, window, sinks, o, 0, ws[1], sizes[1], s.value)
+        else:
+            hip.attn_decode_sinks_dev(kv, 3, 8, E.F32, q, 0, 0.1, window, sinks, o, 0, ws[0], sizes[0], s.value)
+
+    for window, sinks in ((0, 0), (900, 70)):
+        outs = [[hip.alloc(m * 1024 * 4) for _ in range(9)] for m in rows]
+        for i in range(2):
+            call(i, window, sinks, outs[i][8], streams[0])
+            hip.synchronize()
+        for k in range(8):
+            for i in range(2):
+                call(i, window, sinks, outs[i][k], streams[i])
+        hip.synchronize()
+        for i, m in enumerate(rows):
+            alone = hip.download(outs[i][8], np.zeros(m * 1024, np.float32))
+            assert np.isfinite(alone).all()
+            for k in range(8):
+                assert np.array_equal(hip.download(outs[i][k], np.zeros(m * 1024, np.float32)), alone), (i, k)
+    for s in streams:
+        assert rt.L.hipStreamDestroy(s) == 0
+
+
 @pytest.mark.parametrize("dim", [64, 128, 256])
 @pytest.mark.parametrize("types", ALL, ids=ids)
 def test_nothing_outside_the_buffers(hip, types, dim):
