@@ -494,8 +494,9 @@ int es_hip_kv_append_dev(const es_hip_kv *kv, int nseq, const int *start, int nt
  * a query does not see have no influence, whatever their rows hold; an infinity or NaN that it sees in V comes out as an infinity
  * or NaN in that element. fp32 q is carried to 22 bits or more through the matrix products, as are the weights p; with a 16-bit q,
  * decode carries p to 14 bits or more (F16 over F16: 20), which does not show beside out's rounding, and a prompt rounds p to q's
- * type: bring q as fp32 for more. (An F8 cache's prompts with F32 or F16 q: a key whose p times V's scale is below 2^-37 of the row's
- * largest such may count as none.) Sums are fp32's: where a sum of |v| over the keys passes its range, which takes BF16, infinities
+ * type: bring q as fp32 for more. Where a type's range ends, a key may count as none, whatever its V: one whose p is below 2^-126 of the row's
+ * largest, in prompts over BF16, and over F8 with BF16 q, below 2^-118 (F32 q: 2^-123), over F16 below 2^-37; in an F8 cache's prompts with
+ * F32 or F16 q, one whose p times V's scale is below 2^-37 of the row's largest such. Sums are fp32's: where a sum of |v| over the keys passes its range, which takes BF16, infinities
  * or NaN come out. out may be q itself, with one stride, and overlaps nothing else that the call reads. Limits: 2^29 query rows
  * (tokens times heads), 2^23 sequences times heads, 2^31 blocks of 128 keys that the table rows could hold.
  * ws: the caller's device workspace of at least es_hip_attn_decode_workspace bytes (16-byte aligned; 0 bytes: may be NULL); its

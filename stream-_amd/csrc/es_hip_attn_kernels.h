@@ -1234,16 +1234,34 @@ __global__ __launch_bounds__(256, E8 && NQ == 2 && DP == 64 ? 3 : prompt_per_cu(
                         for (int i = 0; i < 16; i++) acc[j][i] *= f;
                 }
                 const float ref = reference(m);
+                // Below a `by` of 2^100, p's that fp32 has lost would be less than 2^-26 as weights, below fp16's range. Above it none is over
+                // 2^-85, which l does not show, and as fp32 may have lost what is to be a large weight, the exponents take the power of two.
+                float by[4];
+#pragma unroll
+                for (int u = 0; u < 4; u++) by[u] = by_scale * v4[u];
+                if (__any(fmaxf(fmaxf(by[0], by[1]), fmaxf(by[2], by[3])) > 0x1p100f)) {
+#pragma unroll
+                    for (int u = 0; u < 4; u++) {
+                        const bool far = by[u] > 0x1p100f;
+                        const float up = e4[u] + (BY - 100 + (ref - reference(m2)));
+#pragma unroll
+                        for (int i = 0; i < 8; i++) {
+                            const float x = s[u >> 1][(u & 1) * 8 + i];
+                            s[u >> 1][(u & 1) * 8 + i] = far ? __builtin_fmaf(x, csr[u], up) : x;
+                        }
+                        csr[u] = far ? 1.0f : csr[u];
+                        by[u] = far ? 0x1p100f : by[u];
+                    }
+                }
 #pragma unroll
                 for (int u = 0; u < 4; u++) {
-                    const float by = fminf(by_scale * v4[u], 0x1p126f);   // (a weight that this is too little for has underflowed)
                     h8 v, w;
 #pragma unroll
                     for (int i = 0; i < 8; i++) {
                         const float x = __builtin_amdgcn_exp2f(__builtin_fmaf(s[u >> 1][(u & 1) * 8 + i], csr[u], -ref));
                         l += x;
-                        v[i] = static_cast<_Float16>(__builtin_fmaf(x, by, 0.0f));
-                        if constexpr (NQ == 2) w[i] = static_cast<_Float16>(__builtin_fmaf(x, by, -static_cast<float>(v[i])));
+                        v[i] = static_cast<_Float16>(__builtin_fmaf(x, by[u], 0.0f));
+                        if constexpr (NQ == 2) w[i] = static_cast<_Float16>(__builtin_fmaf(x, by[u], -static_cast<float>(v[i])));
                     }
                     pt[u][0] = __builtin_bit_cast(u4, v);
                     if constexpr (NQ == 2) pt[u][1] = __builtin_bit_cast(u4, w);

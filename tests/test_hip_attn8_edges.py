@@ -1,0 +1,70 @@
+"""GPU tests of attention over the key-value cache in 8 bits where fp32's and fp16's ranges end, against the formula in 64 bits
+(tests/_attn8.py), with the tolerance derived in _attn.tolerance."""
+import numpy as np
+import pytest
+
+import es_hip_quant as E
+from _attn import from_bits, to_bits
+from _attn8 import RUN, Cache8, attention
+from test_hip_attn8 import F8, allowed, as_queries, ids, run
+
+pytestmark = pytest.mark.gpu
+
+LN2 = np.float32(0.6931472)   # as a call's scale: scores are exponents of 2
+
+
+def scored(c, scores, v):
+    """row 0's tokens, whole runs of one score (a negative whole number) and one V each: q = (1, 1, 0, ...) sees the scores. K's elements are a
+    multiple of 8 and the rest, which 8 bits hold exactly."""
+    n = len(scores) * RUN
+    k = np.zeros((n, 1, c.dim))
+    k[:, 0, 0] = np.repeat([s // 8 * 8 for s in scores], RUN)
+    k[:, 0, 1] = np.repeat([s % 8 for s in scores], RUN)
+    c.append(0, 0, k, v)
+    assert np.array_equal(c.rows(0)[0], k)
+
+
+def lost(c, x, scale):
+    """What keys whose p is below 2^-118 of the row's largest add to it [ntok, heads, 1..]: a prompt with bf16 queries keeps weights as 2^-8 p in
+    fp32 (so that no sum passes the range of its V's), whose least normal number is 2^-126; what is below may count as none."""
+    k, v, _ = c.rows(0)
+    pos = np.arange(len(k) - len(x), len(k))
+    out = np.zeros(x.shape)
+    for h in range(x.shape[1]):
+        s = np.where(np.arange(len(k)) <= pos[:, None], scale * (x[:, h] @ k[:, 0].T), -np.inf)
+        p = np.exp(s - s.max(1, keepdims=True))
+        out[:, h] = np.where(p < 2.0 ** -118, p, 0.0) / p.sum(1, keepdims=True) @ np.abs(v[:, 0])
+    return out
+
+
+@pytest.mark.parametrize("first", ["largest score first", "largest sum first"])
+@pytest.mark.parametrize("dim", [64, 128, 208])
+@pytest.mark.parametrize("types", F8, ids=ids)
+def test_prompt_scores_and_scales_far_apart(hip, types, dim, first):
+    """Keys whose score lies 80 to 125 powers of two below the row's largest, where p is a normal number of fp32 yet, with V as many above that
+    of the largest's: they are most of the sum, and of ordinary size."""
+    t, ct = types
+    rng = np.random.default_rng(dim)
+    below = [0, 80, 101, 112, 115, 118, 121, 123, 125]
+    for near in (0.0, 1e-3, 1.0):   # V of the largest score
+        order = below if first == "largest score first" else below[::-1]
+        c = Cache8(1, dim, 16, [len(order) * RUN], rng)
+        v = rng.standard_normal((len(order) * RUN, 1, dim))
+        for i, b in enumerate(order):
+            v[i * RUN:(i + 1) * RUN] *= 2.0 ** b if b else near
+        scored(c, [-b for b in order], v)
+        x = np.zeros((100, 4, dim), np.float32)
+        x[:, :, :2] = 1
+        x[:, 1, :2] = 0.5      # a row whose scores lie half as far apart: V's largest outweigh all
+        x[::3, 2, :2] = 0.9375
+        if t != E.F32:         # (fp16: outputs of up to 2^60 are infinities, which the check knows)
+            x[:, 1] = x[:, 0]
+        q = to_bits(x, t)
+        got = from_bits(run(hip, c, [0, 100], q, t, LN2), t)
+        as_queries(c, t)
+        want, mag, low = attention(c, [0, 100], x.astype(float), LN2)
+        tol = allowed(c, x.astype(float), t, LN2, mag, low, want, False) + (lost(c, x.astype(float), LN2) if t == E.BF16 else 0)
+        good = np.abs(got - want) <= tol
+        if t == E.F16:   # (what lies within the tolerance from 65520 on, on either side of 0, is an infinity of fp16)
+            good |= np.isinf(got) & (np.sign(got) * want + tol >= 65520)
+        assert good.all(), (np.argwhere(~good)[:5], got[~good][:5], want[~good][:5], tol[~good][:5])
