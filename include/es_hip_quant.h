@@ -516,7 +516,8 @@ int es_hip_attn_prompt_dev(const es_hip_kv *kv, int nseq, const int *start, int 
                            size_t qstride, float scale, int window, void *out, size_t ostride, void *ws, size_t ws_bytes,
                            void *stream);
 /* The same through a window that leaves the first `sinks` tokens of the sequence in sight: position pos sees tokens j <= pos with
- * j < sinks or j > pos - window (window 0: all). 0 sinks: the calls above. The same workspace. What lies between is not read. */
+ * j < sinks or j > pos - window (window 0: all). 0 sinks: the calls above. The same workspace. Of what lies between no more is read than
+ * the tokens in the same 64 as the last sink or the window's first, and nothing hangs on what they, their pages or their scales hold. */
 int es_hip_attn_decode_sinks_dev(const es_hip_kv *kv, int nseq, int heads, uint32_t type, const void *q, size_t qstride, float scale,
                                  int window, int sinks, void *out, size_t ostride, void *ws, size_t ws_bytes, void *stream);
 int es_hip_attn_prompt_sinks_dev(const es_hip_kv *kv, int nseq, const int *start, int ntok, int heads, uint32_t type, const void *q,

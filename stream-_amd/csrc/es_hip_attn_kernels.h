@@ -365,20 +365,22 @@ template <bool F32, bool BF> __device__ void store4(uint8_t *row, int d, const f
 }
 
 // Where runs of 16 keys of a sequence and head begin, one run per lane, in bytes from a pool's start; the upper half is negative
-// where the run is in no page, or not asked for. An 8-bit cache's have their scales with them.
+// where the run is in no page, or not asked for. An 8-bit cache's have their scales with them; the scale of a run that nobody sees, which shares
+// a step with those that are seen, is 1: its page may be another's by now, and hold a scale that nobody has written.
 template <bool E8> struct Runs {
     int lo, hi;
     float ks, vs;
-    __device__ Runs(const KvView &c, const int *table, int head, int run, bool asked) {
+    __device__ Runs(const KvView &c, const int *table, int head, int run, bool asked, bool seen) {
         const int page = asked ? table[run >> (c.shift - 4)] : -1;
         const bool none = page < 0 || page >= c.npages;
         const size_t row = c.row_at(page, head, (run & ((1 << (c.shift - 4)) - 1)) << 4), at = row * c.dim * (E8 ? 1 : 2);
         lo = (int)(uint32_t)at;
         hi = none ? -1 : (int)(at >> 32);
         if constexpr (E8) {
-            const size_t i = none ? 0 : row >> 4;
-            ks = none ? 1.0f : c.ks[i];
-            vs = none ? 1.0f : c.vs[i];
+            const bool known = seen && !none;
+            const size_t i = known ? row >> 4 : 0;
+            ks = known ? c.ks[i] : 1.0f;
+            vs = known ? c.vs[i] : 1.0f;
         }
     }
     __device__ bool none(int lane) const { return __builtin_amdgcn_readlane(hi, lane) < 0; }
@@ -572,7 +574,8 @@ __global__ __launch_bounds__(256, DP == 64 && NQ < 3 ? 3 : decode_per_cu(DP, E8)
         // step 32 s + i begins, of the 32 steps at hand and of the 32 after them.
         auto fetch = [&](int n) {
             const int run = (first >> 4) + ((n + (lane >> 1)) * 4 + wave) * 2 + (lane & 1);
-            return Runs<E8>(a.c, table, head, SINKS && run * 16 >= a.kept ? run + (base >> 4) : run, run * 16 < last);
+            return Runs<E8>(a.c, table, head, SINKS && run * 16 >= a.kept ? run + (base >> 4) : run, run * 16 < last,
+                            run * 16 + 16 > lo || (SINKS && run * 16 < a.sinks));
         };
         Runs<E8> pg = fetch(0), pgn = fetch(32);
         u4 q[KS][NQ];
@@ -971,7 +974,10 @@ __global__ __launch_bounds__(256, E8 && NQ == 2 && DP == 64 ? 3 : prompt_per_cu(
     float m2 = LOWEST, by_scale = 1 << (BY & 31);
 
     // where 64 runs of 16 keys from run `pb` on begin, one per lane, and the 64 after them
-    auto fetch = [&](int u) { return Runs<E8>(a.c, table, head, at_key(u * 16) >> 4, u * 16 < last); };
+    auto fetch = [&](int u) {
+        const int t = at_key(u * 16);
+        return Runs<E8>(a.c, table, head, t >> 4, u * 16 < last, t + 16 > see_lo || (SINKS && t < a.sinks));
+    };
     int pb = first >> 4;
     Runs<E8> pg = fetch(pb + lane), pgn = fetch(pb + 64 + lane);
 

@@ -6,7 +6,8 @@ import pytest
 import es_hip_quant as E
 from _attn import from_bits, to_bits
 from _attn8 import RUN, Cache8, attention
-from test_hip_attn8 import F8, allowed, as_queries, ids, run
+from test_hip_attn import queries
+from test_hip_attn8 import F8, allowed, as_queries, both, ids, run
 
 pytestmark = pytest.mark.gpu
 
@@ -68,3 +69,38 @@ def test_prompt_scores_and_scales_far_apart(hip, types, dim, first):
         if t == E.F16:   # (what lies within the tolerance from 65520 on, on either side of 0, is an infinity of fp16)
             good |= np.isinf(got) & (np.sign(got) * want + tol >= 65520)
         assert good.all(), (np.argwhere(~good)[:5], got[~good][:5], want[~good][:5], tol[~good][:5])
+
+
+def hide(c, starts, window, sinks, garbage):
+    """Runs of 16 tokens that no query of the call sees, their table entries as they are, hold NaN codes and these scales in turn; how many
+    of them share 64 tokens with what some query sees"""
+    near = 0
+    for r in range(len(c.len)):
+        n, f = int(c.len[r]), starts[r + 1] - starts[r]
+        since = max(0, n - f - window + 1)   # the first token that the first query's window shows
+        for u in range(-(-sinks // RUN), since // RUN):
+            g, o = c.table[r, u * RUN // c.page], u * RUN % c.page
+            for i in range(2):
+                c.code[i][g, :, o:o + RUN] = 0x7F
+                c.scale[i][g, :, o // RUN] = garbage[(u + i) % len(garbage)]
+            near += u // 4 == since // 64 or (sinks > 0 and u // 4 == (sinks - 1) // 4 // RUN)
+    return near
+
+
+@pytest.mark.parametrize("window,sinks", [(17, 0), (100, 0), (333, 0), (31, 4), (65, 70), (300, 17), (129, 130)])
+@pytest.mark.parametrize("dim", [64, 128, 208])
+@pytest.mark.parametrize("types", F8, ids=ids)
+def test_scales_of_hidden_runs(hip, types, dim, window, sinks):
+    """pages between sinks and window that are others' by now, and hold scales that nobody has written: no influence"""
+    t, ct = types
+    for decode in (True, False):
+        rng = np.random.default_rng(window + sinks + dim)
+        lens = [640, 705, 1000, 399, 260, 1800]
+        new = [1] * 6 if decode else [1, 37, 70, 20, 5, 130]
+        starts = [0] + np.cumsum(new).tolist()
+        c = Cache8(2, dim, 32, lens, rng)
+        c.fill(rng)
+        q = queries(rng, starts[-1], 4, dim, t)
+        before = both(hip, c, starts, q, t, dim ** -0.5, window=window, sinks=sinks, decode=decode)
+        assert hide(c, starts, window, sinks, [np.inf, np.nan, -np.inf, 0.0, -3.0]) >= 4
+        assert np.array_equal(before, run(hip, c, starts, q, t, dim ** -0.5, window, sinks, decode=decode))
