@@ -912,8 +912,8 @@ __global__ __launch_bounds__(256, E8 && NQ == 2 && DP == 64 ? 3 : prompt_per_cu(
     constexpr int BY = SHIFT<BF> - LAG<BF, NQ>;              // weights are 2^BY p
     __shared__ __attribute__((aligned(1024))) uint8_t lds[2 * NB * TILE];   // K of NB steps, V of them
     __shared__ int odd;                                      // elements of V were left out
-    // UNSCALED: of each step's four runs the scales of K and of V, and the exponents of the latter
-    __shared__ f4 run_ks[UNSCALED ? NB : 1], run_vs[UNSCALED ? NB : 1], run_ve[UNSCALED ? NB : 1];
+    // UNSCALED: of each step's four runs the scales of K and of V, and the exponents of the latter (a wave writes its run's)
+    __shared__ __attribute__((aligned(16))) float run_ks[UNSCALED ? NB : 1][4], run_vs[UNSCALED ? NB : 1][4], run_ve[UNSCALED ? NB : 1][4];
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int col = lane & 31, half = lane >> 5;
     const int head = blockIdx.x % a.c.heads, item = blockIdx.x / a.c.heads;
@@ -1214,7 +1214,8 @@ __global__ __launch_bounds__(256, E8 && NQ == 2 && DP == 64 ? 3 : prompt_per_cu(
             }
             u4 pt[4][NQ];
             if constexpr (UNSCALED) {
-                const f4 k4 = run_ks[buf], v4 = run_vs[buf], e4 = run_ve[buf];
+                auto four = [&](const float (&x)[4]) { return *reinterpret_cast<const f4 *>(x); };
+                const f4 k4 = four(run_ks[buf]), v4 = four(run_vs[buf]), e4 = four(run_ve[buf]);
                 float big = LOWEST, big2 = LOWEST, csr[4];
 #pragma unroll
                 for (int u = 0; u < 4; u++) {
