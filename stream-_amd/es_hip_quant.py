@@ -557,37 +557,43 @@ class Lib:
         self._check(self._L.es_hip_route_softmax_dev(int(logits), lstride, ntok, n_exp, k, int(norm_topk), int(sel), int(w),
                                                      kmax, stream))
 
-    # ---- paged key-value cache and attention (kv: a Kv; device pointers as DevBuf / ints) ----
+    # ---- paged key-value cache and attention (kv: a Kv, of an F8 cache a Kv8; device pointers as DevBuf / ints) ----
+    @staticmethod
+    def _kv(kv):
+        if kv.type == F8 and not isinstance(kv, Kv8):   # (the library would read the scales' addresses from behind it)
+            raise ValueError("an F8 cache is a Kv8, whose scales follow the other fields")
+        return C.byref(kv)
+
     def kv_append_dev(self, kv, nseq, start, ntok, src_type, k, kstride, v, vstride, stream=None):
         """start None: one token per sequence"""
-        self._check(self._L.es_hip_kv_append_dev(C.byref(kv), nseq, self._ptr(start), ntok, src_type, self._ptr(k), kstride,
+        self._check(self._L.es_hip_kv_append_dev(self._kv(kv), nseq, self._ptr(start), ntok, src_type, self._ptr(k), kstride,
                                                  self._ptr(v), vstride, stream))
 
     def attn_decode_workspace(self, kv, nseq, heads) -> int:
-        return self._L.es_hip_attn_decode_workspace(C.byref(kv), nseq, heads)
+        return self._L.es_hip_attn_decode_workspace(self._kv(kv), nseq, heads)
 
     def attn_prompt_workspace(self, kv, nseq, ntok, heads, t) -> int:
-        return self._L.es_hip_attn_prompt_workspace(C.byref(kv), nseq, ntok, heads, t)
+        return self._L.es_hip_attn_prompt_workspace(self._kv(kv), nseq, ntok, heads, t)
 
     def attn_workspace_upto(self, kv, nseq, ntok, heads) -> int:
         """for every decode and prompt call of up to nseq sequences and ntok tokens"""
-        return self._L.es_hip_attn_workspace_upto(C.byref(kv), nseq, ntok, heads)
+        return self._L.es_hip_attn_workspace_upto(self._kv(kv), nseq, ntok, heads)
 
     def attn_decode_dev(self, kv, nseq, heads, t, q, qstride, scale, window, out, ostride, ws, ws_bytes, stream=None):
-        self._check(self._L.es_hip_attn_decode_dev(C.byref(kv), nseq, heads, t, self._ptr(q), qstride, scale, window,
+        self._check(self._L.es_hip_attn_decode_dev(self._kv(kv), nseq, heads, t, self._ptr(q), qstride, scale, window,
                                                    self._ptr(out), ostride, self._ptr(ws), ws_bytes, stream))
 
     def attn_prompt_dev(self, kv, nseq, start, ntok, heads, t, q, qstride, scale, window, out, ostride, ws, ws_bytes, stream=None):
-        self._check(self._L.es_hip_attn_prompt_dev(C.byref(kv), nseq, self._ptr(start), ntok, heads, t, self._ptr(q), qstride,
+        self._check(self._L.es_hip_attn_prompt_dev(self._kv(kv), nseq, self._ptr(start), ntok, heads, t, self._ptr(q), qstride,
                                                    scale, window, self._ptr(out), ostride, self._ptr(ws), ws_bytes, stream))
 
     def attn_decode_sinks_dev(self, kv, nseq, heads, t, q, qstride, scale, window, sinks, out, ostride, ws, ws_bytes, stream=None):
-        self._check(self._L.es_hip_attn_decode_sinks_dev(C.byref(kv), nseq, heads, t, self._ptr(q), qstride, scale, window, sinks,
+        self._check(self._L.es_hip_attn_decode_sinks_dev(self._kv(kv), nseq, heads, t, self._ptr(q), qstride, scale, window, sinks,
                                                          self._ptr(out), ostride, self._ptr(ws), ws_bytes, stream))
 
     def attn_prompt_sinks_dev(self, kv, nseq, start, ntok, heads, t, q, qstride, scale, window, sinks, out, ostride, ws, ws_bytes,
                               stream=None):
-        self._check(self._L.es_hip_attn_prompt_sinks_dev(C.byref(kv), nseq, self._ptr(start), ntok, heads, t, self._ptr(q), qstride,
+        self._check(self._L.es_hip_attn_prompt_sinks_dev(self._kv(kv), nseq, self._ptr(start), ntok, heads, t, self._ptr(q), qstride,
                                                          scale, window, sinks, self._ptr(out), ostride, self._ptr(ws), ws_bytes, stream))
 
     def kv_copy_pages_dev(self, kv, nlayers, layer_bytes, src, dst, stream=None):
@@ -595,7 +601,7 @@ class Lib:
         if len(src) != len(dst):
             raise ValueError("src and dst have different lengths")
         s, d = np.ascontiguousarray(src, np.int32), np.ascontiguousarray(dst, np.int32)
-        self._check(self._L.es_hip_kv_copy_pages_dev(C.byref(kv), nlayers, layer_bytes, s.ctypes.data, d.ctypes.data, len(s), stream))
+        self._check(self._L.es_hip_kv_copy_pages_dev(self._kv(kv), nlayers, layer_bytes, s.ctypes.data, d.ctypes.data, len(s), stream))
 
     # ---- activation preparation on the device (device pointers as DevBuf / ints; None for an output not wanted) ----
     @staticmethod
