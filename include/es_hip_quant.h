@@ -481,7 +481,8 @@ typedef struct {
  * call's sequence b brings rows start[b] to start[b + 1] - 1 of k and v, which are its last tokens: those at len - n to len - 1
  * (start: device, nseq + 1 entries, not decreasing; NULL: one token per sequence, ntok = nseq). Rows from start[nseq] on are
  * not read; nothing is written for rows whose token would lie before the first or in no page. src_type: ES_HIP_F32 or the
- * cache's own type (an F8 cache: F32, F16 or BF16; at most 2^26 runs of 16 tokens times heads); token t's heads * dim elements at k + t * kstride elements (0: packed), the same for v; aligned to their
+ * cache's own type (an F8 cache: F32, F16 or BF16; (ntok / 16 + 2 * nseq + 1) * heads, or nseq * heads without start, is at most 2^26 - 4);
+ * token t's heads * dim elements at k + t * kstride elements (0: packed), the same for v; aligned to their
  * type. A page that several rows of the table share is written through whichever asks (where two tokens of one call have the same
  * place, it holds elements of either): see es_hip_kv_seq_extend for private copies. */
 int es_hip_kv_append_dev(const es_hip_kv *kv, int nseq, const int *start, int ntok, uint32_t src_type, const void *k,

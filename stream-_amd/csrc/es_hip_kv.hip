@@ -618,7 +618,8 @@ int es_hip_kv_append_dev(const es_hip_kv *kv, int nseq, const int *start, int nt
         e.nseq = nseq;
         e.ntok = ntok;
         const long long slots = start ? (long long)ntok / 16 + 2LL * nseq + 1 : nseq, waves = slots * kv->heads;
-        if (waves >= 1LL << 26) return host_fail(ES_HIP_EINVAL, "more than 2^26 runs of 16 tokens times heads");   // (a launch holds 2^24 workgroups of 256)
+        // (four waves a workgroup, and a launch has less than 2^32 threads)
+        if (waves > (1LL << 26) - 4) return host_fail(ES_HIP_EINVAL, "an F8 cache: (ntok / 16 + 2 nseq + 1) heads, or nseq heads without start, exceed 2^26 - 4");
         e.slots = (int)slots;
         const int dp = kv->dim <= 64 ? 0 : kv->dim <= 128 ? 1 : 2;
         static constexpr void (*kernels[3][3])(AppendArgs8) = {
