@@ -344,8 +344,8 @@ __device__ float load_query(const uint8_t *row, bool valid, int g, int dim, floa
     }
 }
 
-// what a query's scores against a run of an 8-bit cache are multiplied by (never 0, as above)
-__device__ float times_scale(float cs, float ks) { return fmaxf(cs * ks, 1.17549435e-38f); }
+// what a query's scores against a run of an 8-bit cache are multiplied by (never 0, as above, nor infinite, which would turn a score of 0 into NaN)
+__device__ float times_scale(float cs, float ks) { return __builtin_amdgcn_fmed3f(cs * ks, 1.17549435e-38f, 3.40282347e38f); }
 
 template <bool F32, bool BF> __device__ void store4(uint8_t *row, int d, const float (&x)[4]) {
     if constexpr (F32) {

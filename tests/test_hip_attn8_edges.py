@@ -104,3 +104,28 @@ def test_scales_of_hidden_runs(hip, types, dim, window, sinks):
         before = both(hip, c, starts, q, t, dim ** -0.5, window=window, sinks=sinks, decode=decode)
         assert hide(c, starts, window, sinks, [np.inf, np.nan, -np.inf, 0.0, -3.0]) >= 4
         assert np.array_equal(before, run(hip, c, starts, q, t, dim ** -0.5, window, sinks, decode=decode))
+
+
+@pytest.mark.parametrize("decode", [True, False])
+@pytest.mark.parametrize("types", F8, ids=ids)
+def test_scores_of_0_under_large_scales(hip, types, decode):
+    """queries that are 0 where keys are huge, and huge where keys are 0: every score is 0, and the output V's mean"""
+    t, ct = types
+    rng = np.random.default_rng(6)
+    c = Cache8(1, 64, 16, [80], rng)
+    x = rng.standard_normal((2, 80, 1, 64))
+    x[0, :, :, 32:] = 0
+    x[0, 16:48] *= 2.0 ** 100
+    c.append(0, 0, x[0], x[1])
+    new = 1 if decode else 40
+    q = np.zeros((new, 4, 64), np.float32)
+    q[:, :, 32:] = rng.standard_normal((new, 4, 32))
+    for size, scale in ((2.0 ** 60, 1.0), (1.0, 2.0 ** 60), (2.0 ** 40, 2.0 ** 20)):
+        if t == E.F16 and size > 1:
+            continue
+        y = to_bits(q * np.float32(size), t)
+        got = from_bits(run(hip, c, [0, new], y, t, scale, decode=decode), t)
+        as_queries(c, t)
+        want, mag, low = attention(c, [0, new], from_bits(y, t), scale)
+        none = np.zeros_like(want)   # (no products but with 0: the scores are exact)
+        assert (np.abs(got - want) <= allowed(c, none, t, 1.0, mag, low, want, decode)).all()
