@@ -1,5 +1,5 @@
 """GPU tests of attention over the key-value cache in 8 bits where fp32's and fp16's ranges end, against the formula in 64 bits
-(tests/_attn8.py), with the tolerance derived in _attn.tolerance."""
+(tests/_attn8.py) with the tolerance derived in _attn.tolerance, and of tokens that no query sees, over 8 and 16 bits, whatever they hold."""
 import numpy as np
 import pytest
 
@@ -7,7 +7,7 @@ import es_hip_quant as E
 from _attn import from_bits, to_bits
 from _attn8 import RUN, Cache8, attention
 from test_hip_attn import queries
-from test_hip_attn8 import F8, allowed, as_queries, both, ids, run
+from test_hip_attn8 import ALL, F8, allowed, as_queries, both, cache_of, ids, run
 
 pytestmark = pytest.mark.gpu
 
@@ -129,3 +129,26 @@ def test_scores_of_0_under_large_scales(hip, types, decode):
         want, mag, low = attention(c, [0, new], from_bits(y, t), scale)
         none = np.zeros_like(want)   # (no products but with 0: the scores are exact)
         assert (np.abs(got - want) <= allowed(c, none, t, 1.0, mag, low, want, decode)).all()
+
+
+@pytest.mark.parametrize("window,sinks", [(100, 0), (31, 4), (65, 70), (300, 17), (129, 130)])
+@pytest.mark.parametrize("dim", [64, 128, 208])
+@pytest.mark.parametrize("types", ALL[3:], ids=ids)
+def test_hidden_tokens_of_16_bits(hip, types, dim, window, sinks):
+    """the same over 16-bit caches: tokens that no query sees hold NaN and infinities, one by one"""
+    t, ct = types
+    for decode in (True, False):
+        rng = np.random.default_rng(window + sinks + dim)
+        lens = [640, 705, 1000, 399, 260, 1800]
+        new = [1] * 6 if decode else [1, 37, 70, 20, 5, 130]
+        starts = [0] + np.cumsum(new).tolist()
+        c = cache_of(ct, 2, dim, 32, lens, rng)
+        c.fill(rng)
+        q = queries(rng, starts[-1], 4, dim, t)
+        before = both(hip, c, starts, q, t, dim ** -0.5, window=window, sinks=sinks, decode=decode)
+        bad = to_bits(np.array([np.nan, np.inf, -np.inf], np.float32), ct)
+        for r, (n, f) in enumerate(zip(lens, new)):
+            j = np.arange(sinks, max(sinks, n - f - window + 1))
+            g, o = c.table[r, j // 32], j % 32
+            c.k[g, :, o], c.v[g, :, o] = bad[j % 3, None, None], bad[(j + 1) % 3, None, None]
+        assert np.array_equal(before, run(hip, c, starts, q, t, dim ** -0.5, window, sinks, decode=decode))
