@@ -475,7 +475,8 @@ typedef struct {
  * stand for, unrounded. es_hip_kv_append_dev gives 16 tokens the least scale whose 448-fold is not less than any of their elements (infinities and
  * NaN, which become NaN, aside; from 2^-100 to 2^120, beyond which an element may stand for an infinity). Where some of the 16 were written by an
  * earlier call, those before the call's own stay, with no smaller a scale; should it grow, they are rounded to it once more: that loses
- * only bits below 2^(e - 9). No two sequences of a call may write to the same 16 tokens (a sequence named
+ * only bits below 2^(e - 9). (So a call that reads those tokens comes before or after the append, not beside it; and what nobody has written there
+ * counts as written, with whatever scale the pool holds.) No two sequences of a call may write to the same 16 tokens (a sequence named
  * twice, pages shared without es_hip_kv_seq_extend's copies): what they then hold is undefined. */
 /* The rows of ntok new tokens into their pages, rounded to the cache's type (nearest even; fp16 overflows to infinity). The
  * call's sequence b brings rows start[b] to start[b + 1] - 1 of k and v, which are its last tokens: those at len - n to len - 1

@@ -450,7 +450,8 @@ constexpr int DECODE_PARTS = 512;   // parts of a tile that can be joined, and s
 constexpr int decode_per_cu(int dim, bool eight) { return eight && dim <= 64 ? 3 : dim <= 128 ? 2 : 1; }
 // Workgroups, all heads together: as many as fit the device at once and bring it to the memory's rate; half of that for one
 // sequence, whose tiles have the more parts to join: 20000 and 131072 tokens of 8 heads of 128, us, 21 and 87 with 256,
-// 23 and 90 with 512.
+// 23 and 90 with 512. 8 bits, fp32 queries, 5000, 20000 and 131072 tokens, with 256 and with 512: 8 heads of 64 11.2 and 11.9, 14.8 and 15.7, 41.1 and
+// 33.2 (the longest would gain); 4 of 128 11.8 and 11.7, 15.1 and 16.5, 32.2 and 33.7; 8 of 256 17.3 and 21.8, 25.5 and 34.6, 91.4 and 100.5.
 constexpr int decode_groups(int dim, int nseq, bool eight) { return nseq > 1 ? 256 * decode_per_cu(dim, eight) : 256; }
 
 // the sequences' blocks: lane i has those of sequence g + i, and `extra` more for each of its tiles
@@ -477,7 +478,11 @@ __device__ Blocks blocks_from(const AttnArgs &a, int g, int tiles, int extra) {
 // Every workgroup's way to its blocks: lane i holds those of the sequences `group` + i, of which there are `before` before. Blocks are dealt out
 // evenly, `each` to a workgroup. 8 bits (a.weigh): beginning another tile costs a workgroup about what a block does (its pages, its query and its keys
 // are waited for, its sums joined), which shows where a workgroup's share would hold three of the shortest tiles: then every tile counts `extra` = 1
-// block more, ahead of its own. us, without and with: 32 sequences of 77 to 8192 tokens, 4 heads of 128, 27.1 and 23.6.
+// block more, ahead of its own. us, without and with, where that is so: 32 sequences of 77 to 8192 tokens, 4 heads of 128, 27.3 and 23.7; 64 of 300
+// to 6000 38.8 and 37.2; 16 of 200 to 20000, 8 heads of 128, 40.0 and 37.8, 256 of 600 72.4 and 72.7; 64 of 100 to 1500, 8 of 64, 22.2 and 20.6. Where
+// it is not: 32 of 4096, 8 of 128, 50.2 and 51.9, 100 of 600 36.8 and 36.9; but 160 of 600 53.4 and 50.7, 16 of 300 to 6000, 4 of 128, 19.7 and
+// 17.8, 16 of 1000 to 9000, 4 of 256, 36.7 and 34.3, which would gain. To look for the shortest tile takes 0.2 us for up to 64 sequences, 0.9 for 100,
+// 1.6 for 256, 7 for 512.
 template <bool WEIGH> struct Deal {
     Blocks bl;
     uint32_t total, each, before = 0;
@@ -518,7 +523,8 @@ template <bool WEIGH> struct Deal {
 
 // AHEAD: steps of a wave's keys on their way. One is enough where other workgroups' are on theirs, and leaves more registers; with 8 bits, a
 // step of heads of 64, or one workgroup to a CU, two are better (decode_ahead). us with one and two, fp32: 131072 tokens of one sequence, 4 heads
-// of 128, 33.7 and 32.0; 32 sequences of 77 to 8192 27.1 and 28.6; 64 sequences of 1000 to 9000, 8 heads of 64, 64.6 and 60.3.
+// of 128, 33.9 and 32.2 (20000 14.6 and 15.1; 20000 and 131072 of 8 heads of 256 23.6 and 25.5, 89.2 and 91.3: one would do there); 32 sequences of 77 to
+// 8192 27.1 and 28.6; 64 sequences of 1000 to 9000, 8 heads of 64, 64.6 and 60.3.
 constexpr int decode_ahead(int dim, int nseq) { return dim <= 64 || nseq == 1 ? 2 : 1; }
 template <bool BF, int NQ, int DP, bool E8 = false, bool SINKS = false, int AHEAD = 1>
 __global__ __launch_bounds__(256, DP == 64 && NQ < 3 ? 3 : decode_per_cu(DP, E8)) void attn_decode_kernel(AttnArgs a) {
